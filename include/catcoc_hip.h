@@ -278,6 +278,44 @@ CATCOC_API uint32_t catcoc_pipelined_round_count(int commType, const CocTilingPa
 CATCOC_API void catcoc_reduce_add(void *stream, uint8_t *dst, uint8_t *src, uint64_t elementCount, uint32_t splitkFactor,
                                   uint32_t outDataType);
 
+/* ----------------------------------------------------------------------- */
+/* 8-bit floating point with block scales; rows that come in groups          */
+/* ----------------------------------------------------------------------- */
+
+/* No counterpart in the reference; beside its W8A8 and float products.  k and n are below 2^22, rows below 2^31, any of them odd; any alignment of
+ * the element type serves, rows that start on 4 bytes run the fast kernels.  A call with rows == 0 is accepted and writes nothing (a weight gradient:
+ * zeros).  Nothing needs a workspace, no sum depends on the order in which workgroups run, and every sum is held in fp32 and rounded once.
+ *
+ * Quantizer to e4m3 (OCP: finite values up to 448, and NaN).  scale = max(largest magnitude of the block, 2^-40) / 448, code = x / scale, rounded to
+ * nearest even.  blockRows 1: a scale for each 128 values of a row, scale [ceil(cols/128), rows] (a product's tile finds its rows' scales of a block
+ * together); blockRows 128: one for each 128x128 block, scale [ceil(rows/128), ceil(cols/128)].  gated (blockRows 1): x is [rows, 2 cols], a row holds
+ * gate and up beside each other, and silu(gate) * up is what is quantized.  dataType: FP16, BF16 or 0 (fp32).  A block that holds a NaN has a scale of
+ * NaN, one that holds an infinity a scale of infinity: products with it are NaN, as those of the values would be (or infinite). */
+CATCOC_API void catcoc_quantize_fp8(void *stream, const void *x, uint8_t *q, float *scale, uint32_t rows, uint32_t cols, uint32_t blockRows,
+                                    uint32_t gated, uint32_t dataType);
+
+/* c[m,n] = sum over blocks b of 128 values of k of scale_x1[b, i] * scale_x2[j / 128, b] * (x1[i, b] . x2[j, b]), plus the other ranks' fp32 partials in slot order
+ * (symmetricPtr: a CatcocSymmetricDesc of which rankIdx, rankSize, peers, peerLd and peerRowOffset count; NULL: one rank), rounded once to outDataType
+ * (FP16, BF16).  x1 [m,k] and x2 [n,k] (a weight matrix stored output-major) e4m3, scale_x1 [ceil(k/128), m], scale_x2 [ceil(n/128), ceil(k/128)]. */
+CATCOC_API void catcoc_fp8_matmul_allreduce(void *stream, const uint8_t *x1, const uint8_t *x2, const float *scale_x1, const float *scale_x2, void *c,
+                                            uint8_t *symmetricPtr, uint32_t m, uint32_t n, uint32_t k, uint32_t outDataType);
+
+/* out[i] = x[i] w[e] for rows i of group e, [groupEnds[e-1], groupEnds[e]) (groupEnds [groups] int32 on the GPU, ascending; values outside [0, rows] count
+ * as the nearer end).  x [rows,k], w [groups,k,n] or, transB, [groups,n,k], out [rows,n], all FP16 or all BF16 (dataType).  Rows past the last group
+ * are written as zeros.  The gradient of x is the same call on dy with the other transB. */
+CATCOC_API void catcoc_grouped_matmul(void *stream, uint32_t dataType, const void *x, const void *w, const int32_t *groupEnds, void *out, uint32_t rows,
+                                      uint32_t n, uint32_t k, uint32_t groups, uint32_t transB);
+
+/* The weight gradient: dw[e] = sum over the group's rows of x[i]^T dy[i], [groups,k,n] or, transB, [groups,n,k]; groups without rows get zeros.  x [rows,k],
+ * dy [rows,n] FP16 or BF16, dw outDataType: the same, the other, or 0 (fp32). */
+CATCOC_API void catcoc_grouped_matmul_dw(void *stream, uint32_t dataType, const void *x, const void *dy, const int32_t *groupEnds, void *dw, uint32_t rows,
+                                         uint32_t n, uint32_t k, uint32_t groups, uint32_t transB, uint32_t outDataType);
+
+/* catcoc_grouped_matmul on e4m3: x [rows,k] with scale_x [ceil(k/128), rows], w [groups,n,k] with scale_w [groups, ceil(n/128), ceil(k/128)]. */
+CATCOC_API void catcoc_grouped_fp8_matmul(void *stream, const uint8_t *x, const uint8_t *w, const float *scale_x, const float *scale_w,
+                                          const int32_t *groupEnds, void *out, uint32_t rows, uint32_t n, uint32_t k, uint32_t groups,
+                                          uint32_t outDataType);
+
 /* The reference's accuracy gate (examples/utils/verify_result.py:26-43,88-117 with the tolerances of
  * examples/utils/utils.py:44-52) on host arrays: every element |out - gold| <= rtol * max(1, |gold|) with
  * rtol = 2^-8 (fp16) / 2^-7 (bf16) for computeTimes < 2048 and twice that otherwise, and
@@ -450,7 +488,9 @@ enum {
     CATCOC_KERNEL_ALIGNED = 2,   /* 128x256 and 256x256 tiles of whole or ragged problems */
     CATCOC_KERNEL_FLEXIBLE = 3,  /* 64x256 and 128x256 tiles over any rows */
     CATCOC_KERNEL_SMALL = 4,     /* 32x32 to 192x128 tiles; 256x256: mixed with 128x128 ones */
-    CATCOC_KERNEL_STREAMING = 5  /* explicit kept rows: 128x128 tiles in k slices, 32 columns over the whole k */
+    CATCOC_KERNEL_STREAMING = 5, /* explicit kept rows: 128x128 tiles in k slices, 32 columns over the whole k */
+    CATCOC_KERNEL_RAGGED = 6,    /* e4m3 and grouped products: tiles fed by copies straight to LDS */
+    CATCOC_KERNEL_RAGGED_CHECKED = 7 /* the same on 64x64 tiles with every load checked */
 };
 typedef struct CatcocLaunchInfo {
     uint32_t kernel;             /* CATCOC_KERNEL_* */

@@ -12,6 +12,7 @@
 #include <new>
 #include <vector>
 
+#include "api_status.h"
 #include "catcoc_hip.h"
 #include "comm_reduce.h"
 #include "gemm_args.h"
@@ -92,8 +93,6 @@ void ok()
     g_err[0] = 0;
     g_status = 0;
 }
-
-enum { E_NULL = 1, E_DESC = 2, E_SHAPE = 3, E_RANK = 4, E_TILING = 5, E_DTYPE = 6, E_WORKSPACE = 7, E_LAUNCH = 8 };
 
 void launched(int e)
 {
@@ -1524,6 +1523,23 @@ void *scratch_for_current_device()
 }
 
 }  // namespace
+
+namespace catcoc {
+
+int api_fail(int code, const char *fmt, ...)
+{
+    va_list ap;
+    va_start(ap, fmt);
+    vsnprintf(g_err, sizeof(g_err), fmt, ap);
+    va_end(ap);
+    return g_status = code;
+}
+
+void api_launched(int e) { launched(e); }
+
+void api_launch_info(const CatcocLaunchInfo &info) { g_launch = info; }
+
+}  // namespace catcoc
 
 extern "C" {
 

@@ -1,0 +1,184 @@
+// Quantizer: rows of 16- or 32-bit values to e4m3 with one fp32 scale per 128 values of a row, or per 128x128 block.
+//
+// scale = max(largest magnitude, 2^-40) / 448, code = value / scale rounded to nearest even: both divisions are the correctly rounded ones.
+#include <hip/hip_runtime.h>
+
+#include "ragged.h"
+
+namespace catcoc {
+
+namespace {
+
+struct Eight {
+    float v[8];
+};
+
+// Values [at, at + 8) of a row of `size`; zeros past its end.
+template <uint32_t DT>
+__device__ __forceinline__ Eight load8(const void *x, size_t row, uint32_t pitch, uint32_t at, uint32_t size)
+{
+    constexpr uint32_t ES = DT == 0 ? 4u : 2u;
+    const unsigned char *p = (const unsigned char *)x + (row * pitch + at) * ES;
+    uint32_t raw[ES * 2];
+    if (at + 8u <= size) {
+        __builtin_memcpy(raw, p, sizeof raw);
+    } else {
+#pragma unroll
+        for (uint32_t i = 0; i < ES * 2u; ++i) raw[i] = 0;
+#pragma unroll
+        for (uint32_t i = 0; i < 7u; ++i) {
+            if (at + i >= size) continue;
+            if constexpr (DT == 0) __builtin_memcpy(&raw[i], p + 4u * i, 4);
+            else {
+                unsigned short h;
+                __builtin_memcpy(&h, p + 2u * i, 2);
+                raw[i >> 1] |= (uint32_t)h << (16u * (i & 1u));
+            }
+        }
+    }
+    Eight e;
+#pragma unroll
+    for (uint32_t i = 0; i < 8u; ++i) {
+        if constexpr (DT == 0) e.v[i] = __builtin_bit_cast(float, raw[i]);
+        else {
+            const uint32_t h = (raw[i >> 1] >> (16u * (i & 1u))) & 0xffffu;
+            if constexpr (DT == DT_BF16) e.v[i] = __builtin_bit_cast(float, h << 16);
+            else e.v[i] = (float)__builtin_bit_cast(_Float16, (unsigned short)h);
+        }
+    }
+    return e;
+}
+
+// silu(g) * u = g / (1 + e^-g) * u.  e^-g = 2^t, t = -g log2 e with the product's low part kept: |g| up to 88 would else cost the result 2^-18.
+__device__ __forceinline__ float silu_times(float g, float u)
+{
+    const float hi = -g * 1.44269504f;
+    const float lo = __builtin_fmaf(-g, 1.44269504f, -hi) + -g * 1.92596299e-8f;   // (log2 e less its fp32 value)
+    const float e = __builtin_amdgcn_exp2f(hi);
+    const float p = __builtin_isinf(e) || __builtin_isinf(hi) ? e : __builtin_fmaf(e, lo * 0.693147181f, e);
+    return g / (1.f + p) * u;
+}
+
+__device__ __forceinline__ uint32_t magnitude(float v) { return __builtin_bit_cast(uint32_t, v) & 0x7fffffffu; }   // (as an integer: a NaN is the largest)
+
+__device__ __forceinline__ float scale_of(uint32_t top)
+{
+    const float t = __builtin_bit_cast(float, top);
+    return (t < kScaleFloor ? kScaleFloor : t) / kE4m3Top;   // (NaN stays)
+}
+
+__device__ __forceinline__ v2i codes8(const Eight &e, float scale)
+{
+    float q[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) q[i] = e.v[i] / scale;
+    int a = 0, b = 0;
+    a = __builtin_amdgcn_cvt_pk_fp8_f32(q[0], q[1], a, false);
+    a = __builtin_amdgcn_cvt_pk_fp8_f32(q[2], q[3], a, true);
+    b = __builtin_amdgcn_cvt_pk_fp8_f32(q[4], q[5], b, false);
+    b = __builtin_amdgcn_cvt_pk_fp8_f32(q[6], q[7], b, true);
+    return v2i{a, b};
+}
+
+__device__ __forceinline__ void store8(unsigned char *q, size_t row, uint32_t pitch, uint32_t at, uint32_t size, v2i v)
+{
+    unsigned char *p = q + row * pitch + at;
+    if (at + 8u <= size) {
+        __builtin_memcpy(p, &v, 8);
+    } else {
+#pragma unroll
+        for (uint32_t i = 0; i < 7u; ++i)
+            if (at + i < size) p[i] = (unsigned char)((uint32_t)v[i >> 2] >> (8u * (i & 3u)));
+    }
+}
+
+// The largest of 16 consecutive lanes' values, in all of them.
+__device__ __forceinline__ uint32_t max16(uint32_t v)
+{
+    v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x128, 0xf, 0xf, false));   // row_ror:8, 4, 2, 1
+    v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x124, 0xf, 0xf, false));
+    v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x122, 0xf, 0xf, false));
+    v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x121, 0xf, 0xf, false));
+    return v;
+}
+
+}  // namespace
+
+// One scale per 128 values of a row: 16 lanes share a block, a wave takes the same block of four consecutive rows at a time.
+template <uint32_t DT, bool GATED>
+__global__ void __launch_bounds__(256) quantize_rows_kernel(const QuantArgs args)
+{
+    const uint32_t lane = threadIdx.x & 63u, blocks = (args.cols + kScaleBlock - 1u) / kScaleBlock;
+    const uint32_t quads = (args.rows + 3u) / 4u;
+    const uint64_t at = (uint64_t)blockIdx.x * 4u + (threadIdx.x >> 6);
+    if (at >= (uint64_t)quads * blocks) return;
+    const uint32_t quad = (uint32_t)(at / blocks), block = (uint32_t)(at - (uint64_t)quad * blocks);
+    const uint32_t row = 4u * quad + (lane >> 4), col = block * kScaleBlock + (lane & 15u) * 8u;
+    if (row >= args.rows) return;   // (whole groups of 16 lanes)
+    const uint32_t pitch = GATED ? 2u * args.cols : args.cols;
+    Eight e = load8<DT>(args.x, row, pitch, col, args.cols);
+    if constexpr (GATED) {
+        // (the upper half's values lie `cols` further on; where fewer than eight are left nothing is read)
+        const Eight u = load8<DT>((const unsigned char *)args.x + (size_t)args.cols * (DT == 0 ? 4u : 2u), row, pitch, col, args.cols);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) e.v[i] = silu_times(e.v[i], u.v[i]);
+    }
+    uint32_t top = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) top = max(top, magnitude(e.v[i]));
+    const float scale = scale_of(max16(top));
+    if ((lane & 15u) == 0) args.scale[(size_t)block * args.rows + row] = scale;
+    if (col < args.cols) store8(args.q, row, args.cols, col, args.cols, codes8(e, scale));
+}
+
+// One scale per 128x128 block: a workgroup holds the block in registers.
+template <uint32_t DT>
+__global__ void __launch_bounds__(256) quantize_blocks_kernel(const QuantArgs args)
+{
+    __shared__ uint32_t tops[4];
+    const uint32_t blocks = (args.cols + kScaleBlock - 1u) / kScaleBlock, rb = blockIdx.x / blocks, cb = blockIdx.x - rb * blocks;
+    const uint32_t col = cb * kScaleBlock + (threadIdx.x & 15u) * 8u, row0 = rb * kScaleBlock + (threadIdx.x >> 4);
+    Eight e[8];
+    uint32_t top = 0;
+#pragma unroll
+    for (uint32_t j = 0; j < 8u; ++j) {
+        if (row0 + 16u * j < args.rows) e[j] = load8<DT>(args.x, row0 + 16u * j, args.cols, col, args.cols);
+        else e[j] = Eight{};
+#pragma unroll
+        for (int i = 0; i < 8; ++i) top = max(top, magnitude(e[j].v[i]));
+    }
+    top = max16(top);
+    top = max(top, (uint32_t)__shfl_xor((int)top, 16));
+    top = max(top, (uint32_t)__shfl_xor((int)top, 32));
+    if ((threadIdx.x & 63u) == 0) tops[threadIdx.x >> 6] = top;
+    __syncthreads();
+    const float scale = scale_of(max(max(tops[0], tops[1]), max(tops[2], tops[3])));
+    if (threadIdx.x == 0) args.scale[blockIdx.x] = scale;
+    if (col >= args.cols) return;
+#pragma unroll
+    for (uint32_t j = 0; j < 8u; ++j)
+        if (row0 + 16u * j < args.rows) store8(args.q, row0 + 16u * j, args.cols, col, args.cols, codes8(e[j], scale));
+}
+
+template <uint32_t DT>
+static int launch_dt(const QuantArgs &a, bool blocks, bool gated, hipStream_t stream)
+{
+    const uint64_t cb = (a.cols + kScaleBlock - 1u) / kScaleBlock;
+    if (blocks) {
+        hipLaunchKernelGGL((quantize_blocks_kernel<DT>), dim3((uint32_t)((a.rows + kScaleBlock - 1u) / kScaleBlock * cb)), dim3(256), 0, stream, a);
+    } else {
+        const dim3 grid((uint32_t)(((a.rows + 3ull) / 4u * cb + 3u) / 4u));
+        if (gated) hipLaunchKernelGGL((quantize_rows_kernel<DT, true>), grid, dim3(256), 0, stream, a);
+        else hipLaunchKernelGGL((quantize_rows_kernel<DT, false>), grid, dim3(256), 0, stream, a);
+    }
+    return (int)hipGetLastError();
+}
+
+int launch_quantize(uint32_t dtype, const QuantArgs &a, bool blocks, bool gated, void *stream)
+{
+    if (dtype == DT_F16) return launch_dt<DT_F16>(a, blocks, gated, (hipStream_t)stream);
+    if (dtype == DT_BF16) return launch_dt<DT_BF16>(a, blocks, gated, (hipStream_t)stream);
+    return launch_dt<0>(a, blocks, gated, (hipStream_t)stream);
+}
+
+}  // namespace catcoc

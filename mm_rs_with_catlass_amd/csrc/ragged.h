@@ -1,0 +1,198 @@
+// Device code that the kernels of ragged products share: which tile a workgroup computes, the MFMAs of one step of k, rounding and stores.
+//
+// A step is 128 BYTES of k (64 values of 16 bits, 128 of e4m3: one scale block).  The first MFMA operand is the matrix (its columns become the result's
+// registers), the second the rows: a lane then holds four consecutive columns, 4 * (lane >> 4) + r of a 16-column block, of ONE row, lane & 15.  So a
+// row's scale is one value per lane, and a lane's results are 8 or 16 consecutive bytes of the output.
+#pragma once
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include "gemm_dma_kernel.h"
+#include "ragged_args.h"
+
+namespace catcoc {
+
+typedef int v8i __attribute__((ext_vector_type(8)));
+
+// A read of 16 bytes at any address.
+__device__ __forceinline__ v4i load16_any(const unsigned char *p)
+{
+    v4i v;
+    __builtin_memcpy(&v, p, 16);
+    return v;
+}
+
+// Inclusive sums over the lanes of a wave.
+__device__ __forceinline__ uint32_t wave_prefix(uint32_t v)
+{
+    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x111, 0xf, 0xf, false);   // row_shr:1, 2, 4, 8
+    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x112, 0xf, 0xf, false);
+    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x114, 0xf, 0xf, false);
+    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x118, 0xf, 0xf, false);
+    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x142, 0xa, 0xf, false);   // row_bcast:15 and 31
+    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x143, 0xc, 0xf, false);
+    return v;
+}
+
+// Position `wg` of a launch of `total` tiles that go round-robin to the eight XCDs: each of them gets a run of consecutive tiles, which share rows and
+// matrices in its L2.  Returns total or more past the end.
+__device__ __forceinline__ uint32_t xcd_run(uint32_t wg, uint32_t total)
+{
+    const uint32_t x = wg & 7u, at = wg >> 3, each = total >> 3, rest = total & 7u;
+    return at < each + (x < rest ? 1u : 0u) ? x * each + umin(x, rest) + at : 0xffffffffu;
+}
+
+// Rows of group e, kept inside [0, rows) and never of negative length whatever `ends` says; e == groups: the rows past the last group, whose results
+// are zero.
+__device__ __forceinline__ void group_rows(const RaggedArgs &args, uint32_t e, uint32_t &begin, uint32_t &end)
+{
+    if (args.ends == nullptr) {
+        begin = e == 0 ? 0u : args.rows;
+        end = args.rows;
+        return;
+    }
+    const int32_t b = e == 0 ? 0 : args.ends[umin(e, args.groups) - 1u];
+    const int32_t t = e < args.groups ? args.ends[e] : (int32_t)args.rows;
+    begin = (uint32_t)min(max(b, 0), (int32_t)args.rows);
+    end = (uint32_t)max(min(t, (int32_t)args.rows), (int32_t)begin);
+}
+
+// A tile of y: `rows` rows from `row` on, all of `group` (group == args.groups: zeros), column tile `colTile`.
+struct RaggedTile {
+    uint32_t group, row, rows, colTile;
+};
+
+// Tile of workgroup `wg` where a group's rows are cut into tiles of at most BX rows of about the same height (whole `unit`s), nt column tiles.  A group's tiles follow each
+// other, eight row tiles to a band and column by column within it: the tiles that run on an XCD at a time share few rows and columns.  Every wave
+// works it out by itself, 64 groups at a time.  False: no tile left.
+template <uint32_t BX>
+__device__ __forceinline__ bool ragged_tile(const RaggedArgs &args, uint32_t wg, uint32_t nt, uint32_t unit, RaggedTile &t)
+{
+    const uint32_t lane = threadIdx.x & 63u;
+    uint32_t first = 0, count, begin, end, local;   // the group's first row tile and how many it has
+    if (args.ends == nullptr) {
+        count = (args.rows + BX - 1u) / BX;
+        local = xcd_run(wg, count * nt);
+        if (local >= count * nt) return false;
+        t.group = 0;
+        begin = 0;
+        end = args.rows;
+    } else {
+        uint32_t total = 0, b = 0, e = 0, tiles = 0, upTo = 0;
+        const uint32_t chunks = args.groups / 64u + 1u;   // (one group more than there are: the rows past the last one)
+        for (uint32_t c = 0; c < chunks; ++c) {
+            const uint32_t g = c * 64u + lane;
+            group_rows(args, umin(g, args.groups), b, e);
+            tiles = g <= args.groups ? (e - b + BX - 1u) / BX : 0u;
+            upTo = wave_prefix(tiles);
+            total += (uint32_t)__builtin_amdgcn_readlane((int)upTo, 63);
+        }
+        const uint32_t at = xcd_run(wg, total * nt);
+        if (at >= total * nt) return false;
+        uint32_t before = 0;
+        for (uint32_t c = 0;; ++c) {
+            if (chunks > 1u) {
+                const uint32_t g = c * 64u + lane;
+                group_rows(args, umin(g, args.groups), b, e);
+                tiles = g <= args.groups ? (e - b + BX - 1u) / BX : 0u;
+                upTo = wave_prefix(tiles);
+            }
+            const uint64_t past = __ballot((before + upTo) * nt > at);
+            if (past != 0 || c + 1u == chunks) {
+                const int l = past != 0 ? __builtin_ctzll(past) : 63;
+                t.group = c * 64u + (uint32_t)l;
+                begin = (uint32_t)__builtin_amdgcn_readlane((int)b, l);
+                end = (uint32_t)__builtin_amdgcn_readlane((int)e, l);
+                count = (uint32_t)__builtin_amdgcn_readlane((int)tiles, l);
+                first = before + (uint32_t)__builtin_amdgcn_readlane((int)upTo, l) - count;
+                break;
+            }
+            before += (uint32_t)__builtin_amdgcn_readlane((int)upTo, 63);
+        }
+        local = at - first * nt;
+    }
+    const uint32_t band = local / (8u * nt), in = local - band * 8u * nt, wide = umin(8u, count - 8u * band);
+    t.colTile = in / wide;
+    const uint32_t r = 8u * band + in - t.colTile * wide;
+    const uint32_t units = (end - begin + unit - 1u) / unit, each = units / count, rest = units - each * count;
+    const uint32_t u0 = r * each + umin(r, rest);
+    t.row = begin + u0 * unit;
+    t.rows = umin((each + (r < rest ? 1u : 0u)) * unit, end - t.row);
+    t.group = (uint32_t)__builtin_amdgcn_readfirstlane((int)t.group);
+    t.row = (uint32_t)__builtin_amdgcn_readfirstlane((int)t.row);
+    t.rows = (uint32_t)__builtin_amdgcn_readfirstlane((int)t.rows);
+    t.colTile = (uint32_t)__builtin_amdgcn_readfirstlane((int)t.colTile);
+    return true;
+}
+
+// A step's 128 bytes of k of 16 rows or columns: the lane's two 16-byte pieces.
+struct Frag {
+    v4i lo, hi;
+};
+
+// acc += w x over a step.  e4m3: one MFMA over the whole step from zero, then acc += s * its result in fp32: the scales of a block are outside its sum.
+template <uint32_t DT>
+__device__ __forceinline__ void step_mfma(const Frag &w, const Frag &x, v4f &acc, float s)
+{
+    if constexpr (DT == DT_F8) {
+        const v8i a = __builtin_shufflevector(w.lo, w.hi, 0, 1, 2, 3, 4, 5, 6, 7), b = __builtin_shufflevector(x.lo, x.hi, 0, 1, 2, 3, 4, 5, 6, 7);
+        const v4f d = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, v4f{0.f, 0.f, 0.f, 0.f}, 0, 0, 0, 0, 0, 0);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) acc[r] = __builtin_fmaf(s, d[r], acc[r]);
+    } else {
+        acc = mfma16<DT>(w.lo, x.lo, acc);
+        acc = mfma16<DT>(w.hi, x.hi, acc);
+    }
+}
+
+// Two values rounded to the output's 16-bit type, to nearest even.
+__device__ __forceinline__ uint32_t round2(float a, float b, uint32_t type)
+{
+    typedef __bf16 v2bf __attribute__((ext_vector_type(2)));
+    typedef _Float16 v2h __attribute__((ext_vector_type(2)));
+    if (type == DT_BF16) return __builtin_bit_cast(uint32_t, v2bf{(__bf16)a, (__bf16)b});
+    return __builtin_bit_cast(uint32_t, v2h{(_Float16)a, (_Float16)b});
+}
+
+// Four consecutive values of one output row, `have` of them inside it.
+__device__ __forceinline__ void store4(const RaggedArgs &args, size_t at, v4f v, uint32_t have)
+{
+    if (args.outType == 0) {
+        float *p = (float *)args.out + at;
+        if (have >= 4u) __builtin_memcpy(p, &v, 16);
+        else {
+#pragma unroll
+            for (uint32_t r = 0; r < 3u; ++r)
+                if (r < have) p[r] = v[r];
+        }
+    } else {
+        unsigned short *p = (unsigned short *)args.out + at;
+        const v2i u = {(int)round2(v[0], v[1], args.outType), (int)round2(v[2], v[3], args.outType)};
+        if (have >= 4u) __builtin_memcpy(p, &u, 8);
+        else {
+#pragma unroll
+            for (uint32_t r = 0; r < 3u; ++r)
+                if (r < have) p[r] = (unsigned short)((uint32_t)u[r >> 1] >> (16u * (r & 1u)));
+        }
+    }
+}
+
+// The other ranks' partials of those values, added in slot order.
+__device__ __forceinline__ void add_peers4(const RaggedArgs &args, uint32_t row, uint32_t col, v4f &v, uint32_t have)
+{
+    for (uint32_t p = 0; p < args.nPeers; ++p) {
+        const float *q = args.peers[p] + (int64_t)row * args.peerLd + col;
+        if (have >= 4u) {
+            v4f u;
+            __builtin_memcpy(&u, q, 16);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) v[r] += u[r];
+        } else {
+#pragma unroll
+            for (uint32_t r = 0; r < 3u; ++r)
+                if (r < have) v[r] += q[r];
+        }
+    }
+}
+
+}  // namespace catcoc

@@ -53,7 +53,7 @@ class CatcocSymmetricDesc(C.Structure):
     ]
 
 
-KERNEL_GENERAL, KERNEL_ALIGNED, KERNEL_FLEXIBLE, KERNEL_SMALL, KERNEL_STREAMING = 1, 2, 3, 4, 5
+KERNEL_GENERAL, KERNEL_ALIGNED, KERNEL_FLEXIBLE, KERNEL_SMALL, KERNEL_STREAMING, KERNEL_RAGGED, KERNEL_RAGGED_CHECKED = 1, 2, 3, 4, 5, 6, 7
 
 
 class CatcocLaunchInfo(C.Structure):
@@ -89,6 +89,7 @@ EXPORTS = [
     "catcoc_pipelined_quant_matmul_reduce_scatter", "catcoc_pipelined_matmul_reduce_scatter", "catcoc_reduce_add",
     "catcoc_verify", "catcoc_comm_block_idx_ex", "catcoc_comm_core_loop", "catcoc_task_tiles",
     "catcoc_pipelined_plan_create", "catcoc_pipelined_plan_destroy", "catcoc_pipelined_round_count",
+    "catcoc_quantize_fp8", "catcoc_fp8_matmul_allreduce", "catcoc_grouped_matmul", "catcoc_grouped_matmul_dw", "catcoc_grouped_fp8_matmul",
 ]
 
 _lib = None
@@ -211,6 +212,13 @@ def load():
     L.catcoc_pipelined_plan_destroy.restype = None
     L.catcoc_pipelined_round_count.argtypes = [C.c_int, C.POINTER(CocTilingParams), C.POINTER(CatcocSymmetricDesc)]
     L.catcoc_pipelined_round_count.restype = u32
+    L.catcoc_quantize_fp8.argtypes = [vp] * 4 + [u32] * 5
+    L.catcoc_fp8_matmul_allreduce.argtypes = [vp] * 7 + [u32] * 4
+    L.catcoc_grouped_matmul.argtypes = [vp, u32] + [vp] * 4 + [u32] * 5
+    L.catcoc_grouped_matmul_dw.argtypes = [vp, u32] + [vp] * 4 + [u32] * 6
+    L.catcoc_grouped_fp8_matmul.argtypes = [vp] * 7 + [u32] * 5
+    for n in ("catcoc_quantize_fp8", "catcoc_fp8_matmul_allreduce", "catcoc_grouped_matmul", "catcoc_grouped_matmul_dw", "catcoc_grouped_fp8_matmul"):
+        getattr(L, n).restype = None
     _lib = L
     return L
 

@@ -544,6 +544,153 @@ def reduce_add(src, out_dtype=None, out=None):
     return out
 
 
+SCALE_BLOCK = 128   # values of k that share a scale of the e4m3 operators, and columns of a weight matrix that do
+
+
+def _blocks(n):
+    return -(-n // SCALE_BLOCK)
+
+
+def _type16(dtype, name):
+    if dtype not in _TORCH_TO_DT:
+        _fail("%s must be float16 or bfloat16 (got %s)", name, dtype)
+    return _TORCH_TO_DT[dtype]
+
+
+def quantize_fp8(x, block_rows=1, gated=False, out=None, scale=None):
+    """x [rows, cols] fp16, bf16 or fp32 -> (codes e4m3 [rows, cols], scale fp32) with x ~ code * scale (catcoc_quantize_fp8).
+
+    block_rows 1 (activations): a scale for each 128 values of a row, scale [ceil(cols/128), rows]; 128 (weights): for each
+    128x128 block, scale [ceil(rows/128), ceil(cols/128)].  gated: x is [rows, 2 cols], gate and up beside each other, and
+    silu(gate) * up is quantized.  out, scale: tensors for the results."""
+    _want(x, "x", (torch.float16, torch.bfloat16, torch.float32), 2)
+    if block_rows not in (1, SCALE_BLOCK):
+        _fail("block_rows must be 1 or %d (got %s)", SCALE_BLOCK, block_rows)
+    rows, cols = x.shape
+    if gated:
+        if block_rows != 1:
+            _fail("gated rows are quantized with block_rows=1")
+        if cols % 2:
+            _fail("gated: x has %d columns, gate and up need the same number", cols)
+        cols //= 2
+    want = (_blocks(cols), rows) if block_rows == 1 else (_blocks(rows), _blocks(cols))
+    _want(out, "out", torch.float8_e4m3fn, 2, None, (rows, cols))
+    _want(scale, "scale", torch.float32, 2, None, want)
+    _check_dev(x, *(t for t in (out, scale) if t is not None))
+    if out is None:
+        out = torch.empty((rows, cols), dtype=torch.float8_e4m3fn, device=x.device)
+    if scale is None:
+        scale = torch.empty(want, dtype=torch.float32, device=x.device)
+    _l.load().catcoc_quantize_fp8(_stream(), x.data_ptr(), out.data_ptr(), scale.data_ptr(), rows, cols, block_rows, int(gated), _TORCH_TO_DT.get(x.dtype, 0))
+    _l.check()
+    return out, scale
+
+
+def fp8_matmul_allreduce(x1, x2, scale_x1, scale_x2, peers=(), rank=0, rank_size=1, out_dtype=torch.bfloat16, peer_row_offset=0, out=None):
+    """e4m3 matmul -> all-reduce share with a scale for each block of 128 values of k (catcoc_fp8_matmul_allreduce).
+
+    x1 [m,k] with scale_x1 [ceil(k/128), m], x2 [n,k] (a stored weight matrix) with scale_x2 [ceil(n/128), ceil(k/128)], as quantize_fp8() makes them.
+    peers: rank_size-1 staged fp32 partials [m,n], added in list order; one rank: the plain product.  Returns [m,n] in out_dtype."""
+    _check_rank(rank, rank_size)
+    _want(x1, "x1", torch.float8_e4m3fn, 2)
+    _want(x2, "x2", torch.float8_e4m3fn, 2)
+    m, k = x1.shape
+    n = x2.shape[0]
+    if x2.shape[1] != k:
+        _fail("x2 has shape %s: its k extent does not match x1's k = %d", tuple(x2.shape), k)
+    if peer_row_offset < 0:
+        _fail("peer_row_offset must be >= 0")
+    _want(scale_x1, "scale_x1", torch.float32, 2, None, (_blocks(k), m))
+    _want(scale_x2, "scale_x2", torch.float32, 2, None, (_blocks(n), _blocks(k)))
+    ptrs, peer_ld = _peer_ptrs(peers, rank_size - 1, torch.float32, peer_row_offset + m, n)
+    dt = _type16(out.dtype if out is not None else out_dtype, "out" if out is not None else "out_dtype")
+    _want(out, "out", None, 2, None, (m, n))
+    _check_dev(x1, x2, scale_x1, scale_x2, *peers, *(() if out is None else (out,)))
+    if out is None:
+        out = torch.empty((m, n), dtype=out_dtype, device=x1.device)
+    d = _l.make_desc(rank, rank_size, ptrs, peer_ld, peer_row_offset) if rank_size > 1 else None
+    _l.load().catcoc_fp8_matmul_allreduce(_stream(), x1.data_ptr(), x2.data_ptr(), scale_x1.data_ptr(), scale_x2.data_ptr(), out.data_ptr(),
+                                          None if d is None else C.addressof(d), m, n, k, dt)
+    _l.check()
+    return out
+
+
+def _want_groups(x, group_ends, groups):
+    _want(group_ends, "group_ends", torch.int32, 1, None, (groups,))
+    if groups < 1:
+        _fail("there must be at least one group")
+
+
+def grouped_matmul(x, w, group_ends, trans_b=False, out=None):
+    """Rows in groups, one matrix for each group (catcoc_grouped_matmul): out[i] = x[i] @ w[e] for the rows i of group e.
+
+    x [rows,k] fp16 or bf16, sorted by group; w [groups,k,n] ([groups,n,k] with trans_b); group_ends [groups] int32 on the GPU: group e is rows
+    [group_ends[e-1], group_ends[e]), any of them empty.  Rows past the last group come out as zeros.  Returns [rows,n].
+    The gradient of x is grouped_matmul(dy, w, group_ends, trans_b=not trans_b), that of w grouped_matmul_dw()."""
+    _want(x, "x", None, 2)
+    dt = _type16(x.dtype, "x")
+    _want(w, "w", x.dtype, 3)
+    rows, k = x.shape
+    groups, n = w.shape[0], w.shape[1 if trans_b else 2]
+    if w.shape[2 if trans_b else 1] != k:
+        _fail("w has shape %s: its k extent does not match x's k = %d", tuple(w.shape), k)
+    _want_groups(x, group_ends, groups)
+    _want(out, "out", x.dtype, 2, None, (rows, n))
+    _check_dev(x, w, group_ends, *(() if out is None else (out,)))
+    if out is None:
+        out = torch.empty((rows, n), dtype=x.dtype, device=x.device)
+    _l.load().catcoc_grouped_matmul(_stream(), dt, x.data_ptr(), w.data_ptr(), group_ends.data_ptr(), out.data_ptr(), rows, n, k, groups, int(trans_b))
+    _l.check()
+    return out
+
+
+def grouped_matmul_dw(x, dy, group_ends, out_dtype=None, trans_b=False, out=None):
+    """The weight gradient of grouped_matmul (catcoc_grouped_matmul_dw): [groups,k,n] ([groups,n,k] with trans_b), out_dtype fp16, bf16 or fp32
+    (None: x's type); groups without rows get zeros."""
+    _want(x, "x", None, 2)
+    dt = _type16(x.dtype, "x")
+    _want(dy, "dy", x.dtype, 2)
+    rows, k = x.shape
+    n = dy.shape[1]
+    if dy.shape[0] != rows:
+        _fail("dy has %d rows, x has %d", dy.shape[0], rows)
+    groups = group_ends.numel()
+    _want_groups(x, group_ends, groups)
+    od = out.dtype if out is not None else x.dtype if out_dtype is None else out_dtype
+    odt = 0 if od == torch.float32 else _type16(od, "out_dtype")
+    shape = (groups, n, k) if trans_b else (groups, k, n)
+    _want(out, "out", None, 3, None, shape)
+    _check_dev(x, dy, group_ends, *(() if out is None else (out,)))
+    if out is None:
+        out = torch.empty(shape, dtype=od, device=x.device)
+    _l.load().catcoc_grouped_matmul_dw(_stream(), dt, x.data_ptr(), dy.data_ptr(), group_ends.data_ptr(), out.data_ptr(), rows, n, k, groups, int(trans_b), odt)
+    _l.check()
+    return out
+
+
+def grouped_fp8_matmul(x, w, scale_x, scale_w, group_ends, out_dtype=torch.bfloat16, out=None):
+    """grouped_matmul on e4m3 (catcoc_grouped_fp8_matmul): x [rows,k] with scale_x [ceil(k/128), rows], w [groups,n,k] with
+    scale_w [groups, ceil(n/128), ceil(k/128)].  Returns [rows,n] in out_dtype."""
+    _want(x, "x", torch.float8_e4m3fn, 2)
+    _want(w, "w", torch.float8_e4m3fn, 3)
+    rows, k = x.shape
+    groups, n = w.shape[0], w.shape[1]
+    if w.shape[2] != k:
+        _fail("w has shape %s: its k extent does not match x's k = %d", tuple(w.shape), k)
+    _want(scale_x, "scale_x", torch.float32, 2, None, (_blocks(k), rows))
+    _want(scale_w, "scale_w", torch.float32, 3, None, (groups, _blocks(n), _blocks(k)))
+    _want_groups(x, group_ends, groups)
+    dt = _type16(out.dtype if out is not None else out_dtype, "out" if out is not None else "out_dtype")
+    _want(out, "out", None, 2, None, (rows, n))
+    _check_dev(x, w, scale_x, scale_w, group_ends, *(() if out is None else (out,)))
+    if out is None:
+        out = torch.empty((rows, n), dtype=out_dtype, device=x.device)
+    _l.load().catcoc_grouped_fp8_matmul(_stream(), x.data_ptr(), w.data_ptr(), scale_x.data_ptr(), scale_w.data_ptr(), group_ends.data_ptr(), out.data_ptr(),
+                                        rows, n, k, groups, dt)
+    _l.check()
+    return out
+
+
 def verify(out, gold, dtype, compute_times):
     """The reference's accuracy gate on host data (float32 numpy arrays or CPU tensors).  -> (passed, n_bad, mean_rel_err)."""
     import numpy as np
