@@ -130,13 +130,19 @@ struct Frag {
     v4i lo, hi;
 };
 
+// A step's product of e4m3 values, before its scale.
+__device__ __forceinline__ v4f step_mfma_f8(const Frag &w, const Frag &x)
+{
+    const v8i a = __builtin_shufflevector(w.lo, w.hi, 0, 1, 2, 3, 4, 5, 6, 7), b = __builtin_shufflevector(x.lo, x.hi, 0, 1, 2, 3, 4, 5, 6, 7);
+    return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, v4f{0.f, 0.f, 0.f, 0.f}, 0, 0, 0, 0, 0, 0);
+}
+
 // acc += w x over a step.  e4m3: one MFMA over the whole step from zero, then acc += s * its result in fp32: the scales of a block are outside its sum.
 template <uint32_t DT>
 __device__ __forceinline__ void step_mfma(const Frag &w, const Frag &x, v4f &acc, float s)
 {
     if constexpr (DT == DT_F8) {
-        const v8i a = __builtin_shufflevector(w.lo, w.hi, 0, 1, 2, 3, 4, 5, 6, 7), b = __builtin_shufflevector(x.lo, x.hi, 0, 1, 2, 3, 4, 5, 6, 7);
-        const v4f d = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, v4f{0.f, 0.f, 0.f, 0.f}, 0, 0, 0, 0, 0, 0);
+        const v4f d = step_mfma_f8(w, x);
 #pragma unroll
         for (int r = 0; r < 4; ++r) acc[r] = __builtin_fmaf(s, d[r], acc[r]);
     } else {
@@ -177,7 +183,20 @@ __device__ __forceinline__ void store4(const RaggedArgs &args, size_t at, v4f v,
     }
 }
 
-// The other ranks' partials of those values, added in slot order.
+// Eight consecutive values in 16 bits.
+__device__ __forceinline__ void store8_16bit(const RaggedArgs &args, size_t at, v4i v, uint32_t have)
+{
+    unsigned short *p = (unsigned short *)args.out + at;
+    if (have >= 8u) {
+        __builtin_memcpy(p, &v, 16);
+    } else {
+#pragma unroll
+        for (uint32_t r = 0; r < 7u; ++r)
+            if (r < have) p[r] = (unsigned short)((uint32_t)v[r >> 1] >> (16u * (r & 1u)));
+    }
+}
+
+// The other ranks' partials of four such values, added in slot order.
 __device__ __forceinline__ void add_peers4(const RaggedArgs &args, uint32_t row, uint32_t col, v4f &v, uint32_t have)
 {
     for (uint32_t p = 0; p < args.nPeers; ++p) {

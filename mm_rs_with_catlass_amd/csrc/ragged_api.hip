@@ -2,11 +2,14 @@
 // choice of kernel.
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
+
 #include "api_status.h"
 #include "ragged_args.h"
 
 namespace catcoc {
 int launch_quantize(uint32_t dtype, const QuantArgs &a, bool blocks, bool gated, void *stream);
+int launch_ragged_tile(uint32_t dtype, const RaggedArgs &a, bool kn, bool dw, uint32_t wgs, void *stream);
 int launch_ragged_checked(uint32_t dtype, const RaggedArgs &a, bool kn, bool dw, uint32_t wgs, void *stream);
 }
 
@@ -38,13 +41,22 @@ int check_sizes(uint64_t rows, uint32_t k, uint32_t n, uint32_t groups)
 
 bool is16(uint32_t dt) { return dt == FP16 || dt == BF16; }
 
+// Rows of both operands start on 4 bytes, as the copies that go straight to LDS need it.
+bool rows_on_words(uint32_t dtype, const RaggedArgs &a, bool kn, bool dw)
+{
+    const uint64_t es = dtype == DT_F8 ? 1 : 2;
+    return ((uintptr_t)a.x | (uintptr_t)a.w) % 4 == 0 && a.k * es % 4 == 0 && ((!kn && !dw) || a.n * es % 4 == 0);
+}
+
 void run(uint32_t dtype, const RaggedArgs &a, bool kn, bool dw, void *stream)
 {
-    const uint64_t nt = cdiv(a.n, 64);
-    const uint64_t wgs = dw ? a.groups * cdiv(a.k, 64) * nt : most_row_tiles(a, 64) * nt;
+    const bool tile = rows_on_words(dtype, a, kn, dw) && (dw || a.rows > 32ull * a.groups);
+    const uint64_t bx = tile ? 256 : 64, nt = cdiv(a.n, bx);
+    // weight gradient on large tiles: eighths of every group's tiles, dealt out to one workgroup a CU
+    const uint64_t wgs = dw && tile ? std::min<uint64_t>(256, a.groups * cdiv(cdiv(a.k, bx) * nt, 8) * 8) : dw ? a.groups * cdiv(a.k, bx) * nt : most_row_tiles(a, bx) * nt;
     if (wgs > kMaxWgs) { api_fail(E_SHAPE, "%llu tiles are more than one launch holds", (unsigned long long)wgs); return; }
-    api_launch_info({CATCOC_KERNEL_RAGGED_CHECKED, 64, 64, 1, 0, 0});
-    api_launched(launch_ragged_checked(dtype, a, kn, dw, (uint32_t)wgs, stream));
+    api_launch_info({tile ? (uint32_t)CATCOC_KERNEL_RAGGED : (uint32_t)CATCOC_KERNEL_RAGGED_CHECKED, (uint32_t)bx, (uint32_t)bx, 1, 0, 0});
+    api_launched((tile ? launch_ragged_tile : launch_ragged_checked)(dtype, a, kn, dw, (uint32_t)wgs, stream));
 }
 
 }  // namespace

@@ -25,26 +25,32 @@ __device__ __forceinline__ v4i load16_within(const unsigned char *row, uint32_t 
 __device__ __forceinline__ uint32_t k_rows_slot(uint32_t row) { return (row >> 1) & 7u; }
 __device__ __forceinline__ uint32_t k_major64_slot(uint32_t row) { return (((row >> 1) & 1u) << 1) | (((row >> 3) & 1u) << 2); }
 
-__device__ __forceinline__ Frag frag_k_rows(const unsigned char *stage, uint32_t row0, uint32_t lane)
+// LDS offsets of a lane's pieces in an operand of one step, and the reads.
+//   k contiguous: the lane's row `row`; 16 rows on is 2048 bytes on.
+//   else:         rows of `pitch` bytes, columns [col0, +16), col0 a multiple of 16; SLOT: where piece q of a row lies.  16 i columns on (i < 8, inside the same
+//                 aligned 128 or, SLOT's values below 8, 64 columns) is this ^ 32 i.  TURNED: the column quads in the order 0, 2, 1, 3.
+__device__ __forceinline__ uint32_t at_k_rows(uint32_t row, uint32_t lane) { return row * 128u + ((lane >> 4) ^ k_rows_slot(row)) * 16u; }
+
+template <bool TURNED, typename SLOT>
+__device__ __forceinline__ uint32_t at_k_major(uint32_t pitch, uint32_t col0, uint32_t lane, SLOT slot)
 {
-    const uint32_t row = row0 + (lane & 15u), c = (lane >> 4) ^ k_rows_slot(row);
-    const unsigned char *p = stage + row * 128u;
-    return {*(const v4i *)(p + c * 16u), *(const v4i *)(p + (c ^ 4u) * 16u)};
+    const uint32_t i = lane & 15u, q = col0 / 8u + (TURNED ? i & 1u : (i >> 1) & 1u), half = TURNED ? (i >> 1) & 1u : i & 1u;
+    const uint32_t row = 8u * (lane >> 4) + (i >> 2);   // (slot(row) is that of row + 4, row + 32 and row + 36 too)
+    return row * pitch + (q ^ slot(row)) * 16u + half * 8u;
 }
 
-// Columns [col0, +16) of a k-major stage of `pitch` bytes a row; SLOT: where piece q of a row lies.
-template <typename SLOT>
-__device__ __forceinline__ Frag frag_k_major(const unsigned char *stage, uint32_t pitch, uint32_t col0, uint32_t lane, SLOT slot)
+__device__ __forceinline__ Frag frag_k_rows(const unsigned char *smem, uint32_t at)
 {
-    const uint32_t i = lane & 15u, g = lane >> 4, q = col0 / 8u + ((i & 3u) >> 1);
+    return {*(const v4i *)(smem + at), *(const v4i *)(smem + (at ^ 64u))};
+}
+
+template <uint32_t PITCH>
+__device__ __forceinline__ Frag frag_k_major(const unsigned char *smem, uint32_t at)
+{
     v4s16 v[4];
 #pragma unroll
-    for (uint32_t h = 0; h < 2u; ++h)
-#pragma unroll
-        for (uint32_t u = 0; u < 2u; ++u) {
-            const uint32_t row = 32u * h + 8u * g + 4u * u + (i >> 2);
-            v[2 * h + u] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((CATCOC_LDS v4s16 *)(stage + row * pitch + (q ^ slot(row)) * 16u + (i & 1u) * 8u));
-        }
+    for (uint32_t u = 0; u < 4u; ++u)
+        v[u] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((CATCOC_LDS v4s16 *)(smem + at + (32u * (u >> 1) + 4u * (u & 1u)) * PITCH));
     Frag f;
     f.lo = __builtin_bit_cast(v4i, __builtin_shufflevector(v[0], v[1], 0, 1, 2, 3, 4, 5, 6, 7));
     f.hi = __builtin_bit_cast(v4i, __builtin_shufflevector(v[2], v[3], 0, 1, 2, 3, 4, 5, 6, 7));
@@ -133,10 +139,10 @@ __global__ void __launch_bounds__(256, 2) ragged_checked_kernel(const RaggedArgs
         Frag fx[2], fw[2];
 #pragma unroll
         for (uint32_t i = 0; i < 2u; ++i) {
-            if constexpr (XK) fx[i] = frag_k_major(p, 128u, wr + 16u * i, lane, k_major64_slot);
-            else fx[i] = frag_k_rows(p, wr + 16u * i, lane);
-            if constexpr (WK) fw[i] = frag_k_major(p + 8192u, 128u, wc + 16u * i, lane, k_major64_slot);
-            else fw[i] = frag_k_rows(p + 8192u, wc + 16u * i, lane);
+            if constexpr (XK) fx[i] = frag_k_major<128>(p, at_k_major<false>(128u, wr + 16u * i, lane, k_major64_slot));
+            else fx[i] = frag_k_rows(p, at_k_rows(wr + 16u * i + (lane & 15u), lane));
+            if constexpr (WK) fw[i] = frag_k_major<128>(p + 8192u, at_k_major<false>(128u, wc + 16u * i, lane, k_major64_slot));
+            else fw[i] = frag_k_rows(p + 8192u, at_k_rows(wc + 16u * i + (lane & 15u), lane));
         }
 #pragma unroll
         for (int i = 0; i < 2; ++i)

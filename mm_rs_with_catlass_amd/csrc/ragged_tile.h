@@ -1,0 +1,451 @@
+// Ragged products on large tiles fed by copies that go straight to LDS.
+#pragma once
+#include "ragged_checked.h"
+
+namespace catcoc {
+
+// 16 (4) bytes per lane to LDS: lane l lands at ldsAddr + 16 l (4 l).  A scalar base and 32-bit lane offsets: no 64-bit address per copy to keep and to advance.
+__device__ __forceinline__ void copy16(const unsigned char *base, uint32_t off, uint32_t ldsAddr)
+{
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" : : "v"(off), "s"(base), "s"(ldsAddr) : "memory", "m0");
+}
+__device__ __forceinline__ void copy4(const unsigned char *base, uint32_t off, uint32_t ldsAddr)
+{
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dword %0, %1" : : "v"(off), "s"(base), "s"(ldsAddr) : "memory", "m0");
+}
+
+// Scalar loads: the address is the same for every lane, the memory is not written while the kernel runs.
+__device__ __forceinline__ float load_uniform(const float *p) { return *(const __attribute__((address_space(4))) float *)p; }
+
+template <typename T>
+__device__ __forceinline__ T *uniform_ptr(T *p)
+{
+    const uint64_t u = (uint64_t)p;
+    const uint32_t lo = (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)u), hi = (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)(u >> 32));
+    return (T *)(((uint64_t)hi << 32) | lo);
+}
+
+// Where an operand's pieces of one step lie, in memory and in LDS, in sub-stages of 16 KiB: 128 rows of 128 bytes of k, or (KM) 64 rows of k of 128 columns.
+//   KM = false: piece p of row r at slot p ^ k_rows_slot(r).   KM = true: piece p of row r at slot p ^ b16_slot<2>(r).
+// UNIT: a sub-stage's two halves of 64 rows (columns) are `apart` rows (columns) of the tile apart.  Rows and columns past the tile's last one repeat it.
+template <bool KM, uint32_t SUBS, uint32_t ES, uint32_t WAVES>
+struct TileOperand {
+    static constexpr uint32_t COPIES = 16u / WAVES;   // of a wave and sub-stage, 1 KiB each
+    const unsigned char *base;   // the tile's first row and column, first step
+    uint32_t pitch, have, apart;
+    uint32_t off[SUBS][COPIES];
+
+    // The row (column) of the tile that row (column) q of sub-stage h holds.
+    __device__ __forceinline__ uint32_t of_tile(uint32_t h, uint32_t q) const { return (q >> 6) * apart + 64u * h + (q & 63u); }
+    // Byte of the tile's step that byte `in` of the 16-byte slot `slot` of LDS row `row` holds.
+    __device__ __forceinline__ uint32_t source(uint32_t h, uint32_t row, uint32_t slot, uint32_t in) const
+    {
+        if constexpr (KM) {
+            const uint32_t piece = of_tile(h, (slot ^ b16_slot<2>(row)) * 8u) / 8u;
+            return row * pitch + umin(piece, (have - 1u) / 8u) * 16u + in;
+        } else {
+            return umin(of_tile(h, row), have - 1u) * pitch + (slot ^ k_rows_slot(row)) * 16u + in;
+        }
+    }
+    __device__ __forceinline__ void init(const unsigned char *p, uint32_t pitch_, uint32_t have_, uint32_t apart_, uint32_t wave, uint32_t lane)
+    {
+        base = uniform_ptr(p);
+        pitch = pitch_;
+        have = have_;
+        apart = apart_;
+#pragma unroll
+        for (uint32_t h = 0; h < SUBS; ++h)
+#pragma unroll
+            for (uint32_t j = 0; j < COPIES; ++j) {
+                const uint32_t at = (wave + WAVES * j) * 64u + lane;
+                off[h][j] = source(h, KM ? at >> 4 : at >> 3, KM ? at & 15u : at & 7u, 0);
+            }
+    }
+    __device__ __forceinline__ const unsigned char *at_step(uint32_t s) const { return base + (size_t)s * (KM ? 64u * pitch : 128u); }
+    // (rows: sixteen of them that no wave reads are left out; eight waves only, where that is all of a wave's copies or none)
+    static __device__ __forceinline__ bool wanted(uint32_t h, uint32_t ni, uint32_t wave) { return KM || WAVES != 8u || 4u * h + (wave >> 1) < ni; }
+    __device__ __forceinline__ void issue(uint32_t h, uint32_t s, uint32_t lds, uint32_t wave) const
+    {
+        const unsigned char *const p = at_step(s);
+#pragma unroll
+        for (uint32_t j = 0; j < COPIES; ++j) copy16(p, off[h][j], lds + (wave + WAVES * j) * 1024u);
+    }
+    // The last step where it ends inside its 128 bytes of k or 64 rows of k, or where pieces of 16 bytes would end behind the matrix: copies of what is there (4
+    // bytes at a time where a row ends inside a piece), and zeros.  inRow: bytes of a row that are there, from the step's first (KM: the tile's first column) on;
+    // rows: rows of k (KM).
+    __device__ __forceinline__ void issue_part(uint32_t h, uint32_t s, unsigned char *stage, uint32_t lds, uint32_t inRow, uint32_t rows, uint32_t wave, uint32_t lane) const
+    {
+        if (inRow % 16u == 0) part<16>(h, s, stage, lds, inRow, rows, wave, lane);
+        else part<4>(h, s, stage, lds, inRow, rows, wave, lane);
+    }
+    template <uint32_t BYTES>
+    __device__ __forceinline__ void part(uint32_t h, uint32_t s, unsigned char *stage, uint32_t lds, uint32_t inRow, uint32_t rows, uint32_t wave, uint32_t lane) const
+    {
+        constexpr uint32_t PER = (KM ? 256u : 128u) / BYTES;   // copied pieces of a row
+        const unsigned char *const p = at_step(s);
+#pragma unroll 1
+        for (uint32_t c = wave; c < 256u / BYTES; c += WAVES) {
+            const uint32_t at = c * 64u + lane, row = at / PER, slot = (at % PER) * BYTES / 16u, in = at * BYTES % 16u;
+            const uint32_t byte = KM ? of_tile(h, (slot ^ b16_slot<2>(row)) * 8u) * 2u + in : (slot ^ k_rows_slot(row)) * 16u + in;
+            const bool there = byte < inRow && (!KM || row < rows);
+            if (there) {
+                if constexpr (BYTES == 16u) copy16(p, source(h, row, slot, in), lds + c * 1024u);
+                else copy4(p, source(h, row, slot, in), lds + c * 256u);
+            } else if constexpr (BYTES == 16u) {
+                *(v4i *)(stage + at * 16u) = v4i{0, 0, 0, 0};
+            } else {
+                *(uint32_t *)(stage + at * 4u) = 0u;
+            }
+        }
+    }
+};
+
+// Which column of its 16 a matrix fragment's lane m holds: 0-3, 8-11, 4-7, 12-15.  The results of lane groups 0 and 2 (1 and 3) are then eight consecutive
+// columns, and one exchange of half waves between two column blocks gives every lane 16 bytes of output.
+__device__ __forceinline__ uint32_t result_col(uint32_t m) { return ((m >> 2) & 1u) * 8u + ((m >> 3) & 1u) * 4u + (m & 3u); }
+
+// A tile of 32 NIMAX rows and 64 WY columns: 2 WY waves, two by WY, of up to 16 NIMAX rows and 64 columns each (NI row fragments, as many as the tile's rows
+// need; four of columns).  A wave keeps a step's column fragments in registers and streams its row fragments, two ahead of the MFMAs.
+//
+// Two stages of 128 bytes of k, three where a wave has at most four row fragments (their stages are smaller).  When the last read of a step is out, the
+// wave waits for the next stage's copies (issued a whole step before, or two) and for its own reads; the barrier behind that says both that the next stage
+// is complete and that this one may be overwritten: its next copies start there.  The last two row fragments' MFMAs then cover the first reads of the next
+// step, whose column fragments take the registers of those just used.
+template <uint32_t DT, bool XK, bool WK, int WY, int NIMAX>
+struct RaggedTileLoop {
+    static constexpr uint32_t ES = DT == DT_F8 ? 1u : 2u, KE = 128u / ES;
+    static constexpr uint32_t WAVES = 2u * WY, BX = 32u * NIMAX, BY = 64u * WY, SUB = 16384u;
+    static constexpr uint32_t XSUBS = BX / 128u, WSUBS = BY / 128u;
+    static constexpr uint32_t stages(int ni) { return NIMAX == 8 && ni <= 4 ? 3u : 2u; }
+    static constexpr uint32_t stage_bytes(int ni) { return ((ni <= 4 ? 1u : 2u) + WSUBS) * SUB; }
+    static constexpr uint32_t SX = XSUBS == 2u ? 3u * stage_bytes(4) : 2u * stage_bytes(4);   // e4m3: row scales behind the stages
+    static constexpr uint32_t SXB = BX * 4u;
+    static constexpr uint32_t LDS = SX + (DT == DT_F8 ? 3u * SXB : 0u);
+    TileOperand<XK, XSUBS, ES, WAVES> x;
+    TileOperand<WK, WSUBS, ES, WAVES> w;
+    v4f acc[NIMAX][4];
+
+    struct Problem {
+        uint32_t K, steps;          // values of k, steps of them
+        uint32_t rows, cols;        // of the tile
+        uint32_t ni;                // row fragments of a wave
+        uint32_t xLeft, wLeft;      // columns of the matrix from the tile's first on (operands that are rows of k)
+        bool partLast;              // the last step is no whole one (issue_part)
+        const float *sx, *sw;       // e4m3: scales of the tile's first row, and of this wave's block of columns
+        uint32_t sxPitch;
+    };
+
+    // Copies of step s into `stage`; TWO: of both halves of the rows.
+    template <bool TWO>
+    __device__ __forceinline__ void issue(const Problem &p, unsigned char *smem, uint32_t stage, uint32_t s, uint32_t wave, uint32_t lane)
+    {
+        const uint32_t lds0 = (uint32_t)(uintptr_t)(CATCOC_LDS unsigned char *)smem, ws = stage + (TWO ? 2u : 1u) * SUB;
+        if (p.partLast && s + 1u == p.steps) {
+            const uint32_t left = p.K - s * KE;
+#pragma unroll 1
+            for (uint32_t h = 0; h < WSUBS; ++h) w.issue_part(h, s, smem + ws + h * SUB, lds0 + ws + h * SUB, WK ? p.wLeft * 2u : left * ES, left, wave, lane);
+#pragma unroll 1
+            for (uint32_t h = 0; h < (TWO ? 2u : 1u); ++h) x.issue_part(h, s, smem + stage + h * SUB, lds0 + stage + h * SUB, XK ? p.xLeft * 2u : left * ES, left, wave, lane);
+        } else {
+#pragma unroll
+            for (uint32_t h = 0; h < WSUBS; ++h) w.issue(h, s, lds0 + ws + h * SUB, wave);
+#pragma unroll
+            for (uint32_t h = 0; h < (TWO ? 2u : 1u); ++h)
+                if (x.wanted(h, p.ni, wave)) x.issue(h, s, lds0 + stage + h * SUB, wave);
+        }
+        if constexpr (DT == DT_F8) {   // 64 rows' scales a wave (several waves fetch the same ones)
+            const uint32_t q = wave % (BX / 64u);
+            copy4((const unsigned char *)(p.sx + (size_t)s * p.sxPitch), umin(64u * q + lane, p.rows - 1u) * 4u, lds0 + SX + s % 3u * SXB + q * 256u);
+        }
+    }
+
+    // A tile's first copies.
+    __device__ __forceinline__ void begin(const Problem &p, unsigned char *smem, uint32_t wave, uint32_t lane)
+    {
+        if (XSUBS == 2u && p.ni > 4u) {
+            if constexpr (XSUBS == 2u) {
+#pragma unroll 1
+                for (uint32_t s = 0; s < 2u && s < p.steps; ++s) issue<true>(p, smem, s * stage_bytes(8), s, wave, lane);
+            }
+        } else {
+#pragma unroll 1
+            for (uint32_t s = 0; s < stages(4) && s < p.steps; ++s) issue<false>(p, smem, s * stage_bytes(4), s, wave, lane);
+        }
+    }
+
+    // All but this wave's copies of the last N steps are there where `whole` steps follow, else all; then everybody's are, and everybody's reads are done.
+    template <int N>
+    __device__ __forceinline__ void meet(bool whole, bool first, bool second)
+    {
+        constexpr int C = (int)(16u / WAVES), W = N * (C * (int)WSUBS + (DT == DT_F8 ? 1 : 0));
+        if (N == 0 || !whole) CATCOC_WAIT_VMCNT(0);
+        else if (second) CATCOC_WAIT_VMCNT(W + 2 * N * C);
+        else if (first) CATCOC_WAIT_VMCNT(W + N * C);
+        else CATCOC_WAIT_VMCNT(W);
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        barrier_keep_vmem();
+    }
+
+    template <int NI>
+    __device__ __forceinline__ void run(const Problem &p, unsigned char *smem, uint32_t wave, uint32_t lane)
+    {
+        static_assert(NI >= 2 && NI <= NIMAX, "row fragments of a wave");
+        constexpr bool TWO = NI > 4;   // (row fragments in two sub-stages)
+        constexpr uint32_t STAGES = stages(NI), STAGE = stage_bytes(NI);
+        const uint32_t wr = wave / WY, wc = wave % WY;
+#pragma unroll
+        for (int i = 0; i < NI; ++i)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) acc[i][j] = v4f{0.f, 0.f, 0.f, 0.f};
+        if (p.steps == 0) return;
+        const uint32_t full = p.steps - (p.partLast ? 1u : 0u);   // whole steps
+        const bool first = TWO || x.wanted(0, NI, wave), second = TWO && x.wanted(1, NI, wave);
+        meet<(int)STAGES - 1>(full >= STAGES, first, second);
+
+        const uint32_t xa = XK ? at_k_major<false>(256u, 64u * wr, lane, b16_slot<2>) : at_k_rows(64u * wr + (lane & 15u), lane);
+        const uint32_t wh = WSUBS == 2u ? wc % 2u : 0u, w64 = 64u * (WSUBS == 2u ? wc / 2u : wc);   // the wave's columns: sub-stage, half of it
+        const uint32_t wa = ((TWO ? 2u : 1u) + wh) * SUB + (WK ? at_k_major<true>(256u, w64, lane, b16_slot<2>) : at_k_rows(w64 + result_col(lane & 15u), lane));
+        auto read_x = [&](uint32_t stage, uint32_t i) {
+            if constexpr (XK) return frag_k_major<256>(smem, ((stage + xa) ^ (32u * (i & 3u))) + (i >> 2) * SUB);
+            else return frag_k_rows(smem, stage + xa + 2048u * (i & 3u) + (i >> 2) * SUB);
+        };
+        auto read_w = [&](uint32_t stage, uint32_t j) {
+            if constexpr (WK) return frag_k_major<256>(smem, (stage + wa) ^ (32u * j));
+            else return frag_k_rows(smem, stage + wa + 2048u * j);
+        };
+        const uint32_t sa = SX + (wr * 16u * NI + (lane & 15u)) * 4u;
+        auto row_scale = [&](uint32_t s, int i) { return *(const float *)(smem + sa + s % 3u * SXB + 64u * i); };
+
+        // Row fragments' registers: the first two of a step have their own, which are free when the last two run.
+        constexpr int SLOTS = NI == 8 ? 4 : NI >= 4 ? 5 : NI;
+        auto slot = [](int i) { return NI == 8 ? i & 3 : i < 2 || NI < 4 ? i : 2 + (i - 2) % 3; };
+        Frag fx[SLOTS], fw[4], ahead[2];
+        float fs[SLOTS], aheadS[2], sw = 0.f;   // e4m3: the fragments' row scales, the columns' scale
+        // e4m3: a result is scaled and added while the MFMA behind the next one runs
+        v4f late[2];
+        float lateS[2];
+        int li[2], lj[2], queued = 0;
+        auto settle = [&](int q) {
+#pragma unroll
+            for (int r = 0; r < 4; ++r) acc[li[q]][lj[q]][r] = __builtin_fmaf(lateS[q], late[q][r], acc[li[q]][lj[q]][r]);
+            asm volatile("" : "+v"(acc[li[q]][lj[q]]));   // (here, and not all of them together behind the next branch)
+        };
+        auto multiply = [&](int i, int j, const Frag &f, float scale) {
+            if constexpr (DT == DT_F8) {
+                const v4f d = step_mfma_f8(fw[j], f);
+                if (queued >= 2) settle(queued & 1);
+                late[queued & 1] = d;
+                lateS[queued & 1] = scale;
+                li[queued & 1] = i;
+                lj[queued & 1] = j;
+                ++queued;
+                __builtin_amdgcn_sched_barrier(0);
+            } else {
+                step_mfma<DT>(fw[j], f, acc[i][j], 0.f);
+            }
+        };
+#pragma unroll
+        for (int j = 0; j < 4; ++j) fw[j] = read_w(0, j);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            fx[i] = read_x(0, i);
+            if constexpr (DT == DT_F8) fs[i] = row_scale(0, i);
+        }
+        if constexpr (DT == DT_F8) sw = load_uniform(p.sw);
+        uint32_t cur = 0;   // this step's stage
+#pragma unroll 1
+        for (uint32_t s = 0; s < p.steps; ++s) {
+            const uint32_t next = cur == (STAGES - 1u) * STAGE ? 0u : cur + STAGE;
+            queued = 0;
+#pragma unroll
+            for (int i = 0; i < NI - 2; ++i) {
+                fx[slot(i + 2)] = read_x(cur, i + 2);
+                if constexpr (DT == DT_F8) fs[slot(i + 2)] = row_scale(s, i + 2);
+                const float scale = DT == DT_F8 ? fs[slot(i)] * sw : 0.f;
+#pragma unroll
+                for (int jj = 0; jj < 4; ++jj) multiply(i, snake16(i, jj, 4), fx[slot(i)], scale);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            float swNext = 0.f;
+            if constexpr (DT == DT_F8) swNext = load_uniform(p.sw + umin(s + 1u, p.steps - 1u));
+            meet<(int)STAGES - 2>(s + STAGES <= full, first, second);
+            if (s + STAGES < p.steps) issue<TWO>(p, smem, cur, s + STAGES, wave, lane);
+            // (behind the last step nobody looks at what is read here)
+            const float s0 = DT == DT_F8 ? fs[slot(NI - 2)] * sw : 0.f, s1 = DT == DT_F8 ? fs[slot(NI - 1)] * sw : 0.f;
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                Frag &to = NI >= 4 ? fx[i] : ahead[i];
+                to = read_x(next, i);
+                if constexpr (DT == DT_F8) (NI >= 4 ? fs[i] : aheadS[i]) = row_scale(s + 1u, i);
+            }
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                multiply(NI - 2, j, fx[slot(NI - 2)], s0);
+                multiply(NI - 1, j, fx[slot(NI - 1)], s1);
+                fw[j] = read_w(next, j);
+            }
+            if constexpr (DT == DT_F8) {
+                settle(queued & 1);
+                settle((queued & 1) ^ 1);
+                sw = swNext;
+            }
+            if constexpr (NI < 4) {
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    fx[i] = ahead[i];
+                    if constexpr (DT == DT_F8) fs[i] = aheadS[i];
+                }
+            }
+            cur = next;
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    }
+
+    template <int NI = NIMAX>
+    __device__ __forceinline__ void run_rows(const Problem &p, unsigned char *smem, uint32_t wave, uint32_t lane)
+    {
+        if (p.ni == (uint32_t)NI || NI == 2) run<NI>(p, smem, wave, lane);
+        else if constexpr (NI > 2) run_rows<NI - 1>(p, smem, wave, lane);
+    }
+};
+
+// DW: x and w are rows of k (the group's rows), the result is the group's [k, n] matrix.  KN: w is [k, n].
+// A weight gradient's workgroups walk several tiles: few rows make few steps, and a tile's first copies are on their way while the one before is stored.
+template <uint32_t DT, bool KN, bool DW, int WY, int NIMAX>
+__global__ void __launch_bounds__(128 * WY, 2) ragged_tile_kernel(const RaggedArgs args)
+{
+    using Loop = RaggedTileLoop<DT, DW, KN || DW, WY, NIMAX>;
+    constexpr uint32_t ES = Loop::ES, BX = Loop::BX, BY = Loop::BY;
+    __shared__ __attribute__((aligned(16))) unsigned char smem[Loop::LDS];
+
+    const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(tid >> 6));
+    const uint32_t nt = (args.n + BY - 1u) / BY;
+    Loop loop;
+    typename Loop::Problem p;
+
+    // Tile `at` of this launch; DW: t.group's rows are the sum, t.row and t.rows rows of the result.
+    uint32_t sumBegin = 0, sumEnd = 0;
+    auto find = [&](uint32_t &at, RaggedTile &t) {
+        if constexpr (DW) {
+            // every XCD gets an eighth of each group's tiles: they cost what the group has rows
+            const uint32_t pt = (args.k + BX - 1u) / BX, tiles = pt * nt, share = (tiles + 7u) / 8u;
+            uint32_t in;
+            do {
+                const uint32_t j = at >> 3;
+                if (j >= args.groups * share) return false;
+                t.group = j / share;
+                in = ((at + t.group) & 7u) * share + j - t.group * share;
+                if (in >= tiles) at += gridDim.x;
+            } while (in >= tiles);
+            t.colTile = in / pt;
+            t.row = BX * (in - t.colTile * pt);
+            t.rows = umin(BX, args.k - t.row);
+            t.group = (uint32_t)__builtin_amdgcn_readfirstlane((int)t.group);
+            t.colTile = (uint32_t)__builtin_amdgcn_readfirstlane((int)t.colTile);
+            t.row = (uint32_t)__builtin_amdgcn_readfirstlane((int)t.row);
+            t.rows = (uint32_t)__builtin_amdgcn_readfirstlane((int)t.rows);
+            group_rows(args, t.group, sumBegin, sumEnd);
+            sumBegin = (uint32_t)__builtin_amdgcn_readfirstlane((int)sumBegin);
+            sumEnd = (uint32_t)__builtin_amdgcn_readfirstlane((int)sumEnd);
+            return true;
+        } else {
+            return ragged_tile<BX>(args, at, nt, 32u, t);
+        }
+    };
+    auto set = [&](const RaggedTile &t) {
+        const uint32_t col0 = BY * t.colTile;
+        p.wLeft = args.n - col0;
+        p.rows = t.rows;
+        p.cols = umin(BY, p.wLeft);
+        p.ni = DW ? (uint32_t)NIMAX : max((t.rows + 31u) / 32u, 2u);
+        if constexpr (DW) {
+            p.K = sumEnd - sumBegin;
+            p.xLeft = args.k - t.row;
+            p.partLast = p.K % 64u != 0 || args.k % 8u != 0 || args.n % 8u != 0;
+            loop.x.init((const unsigned char *)args.x + ((size_t)sumBegin * args.k + t.row) * 2u, args.k * 2u, t.rows, 16u * NIMAX, wave, lane);
+            loop.w.init((const unsigned char *)args.w + ((size_t)sumBegin * args.n + col0) * 2u, args.n * 2u, p.cols, BY / 2u, wave, lane);
+        } else {
+            const uint32_t g = umin(t.group, args.groups - 1u);
+            p.K = t.group < args.groups ? args.k : 0u;
+            const uint32_t wPitch = KN ? args.n * ES : args.k * ES;
+            p.xLeft = 0;
+            p.partLast = p.K % Loop::KE != 0 || (KN && args.n % 8u != 0);
+            loop.x.init((const unsigned char *)args.x + (size_t)t.row * args.k * ES, args.k * ES, t.rows, 16u * p.ni, wave, lane);
+            loop.w.init((const unsigned char *)args.w + (size_t)g * args.n * args.k * ES + (size_t)col0 * (KN ? ES : wPitch), wPitch, p.cols, BY / 2u, wave, lane);
+            if constexpr (DT == DT_F8) {
+                const uint32_t kb = (args.k + kScaleBlock - 1u) / kScaleBlock, nb = (args.n + kScaleBlock - 1u) / kScaleBlock;
+                p.sx = uniform_ptr(args.sx + t.row);
+                p.sxPitch = args.rows;
+                p.sw = uniform_ptr(args.sw + ((size_t)g * nb + umin((col0 + (wave % WY) * 64u) / kScaleBlock, nb - 1u)) * kb);
+            }
+        }
+        p.steps = (p.K + Loop::KE - 1u) / Loop::KE;
+    };
+
+    uint32_t at = blockIdx.x;
+    RaggedTile t;
+    if (!find(at, t)) return;
+    set(t);
+    loop.begin(p, smem, wave, lane);
+    for (;;) {
+        // DW: a workgroup's next tile is looked up while this one's first copies are on their way, and its own start before this one's results are stored
+        RaggedTile after;
+        bool more = false;
+        const size_t outRow = (DW ? (size_t)t.group * args.k : (size_t)0) + t.row;
+        const uint32_t ni = p.ni;
+        if constexpr (DW) {
+            at += gridDim.x;
+            more = find(at, after);
+            loop.template run<NIMAX>(p, smem, wave, lane);
+        } else {
+            loop.run_rows(p, smem, wave, lane);
+        }
+        const uint32_t rows = t.rows, row0 = t.row, col0 = BY * t.colTile, cols = p.cols;
+        if (more) {
+            t = after;
+            set(t);
+            loop.begin(p, smem, wave, lane);
+        }
+
+        // ---- output: rows [wr, +16 ni) and columns [wc, +64) of the tile are this wave's
+        const uint32_t wr = (wave / WY) * 16u * ni, wc = (wave % WY) * 64u, lr = lane & 15u;
+        if (DW && args.outType == 0) {
+#pragma unroll
+            for (uint32_t i = 0; i < (uint32_t)NIMAX; ++i) {
+                const uint32_t r = wr + 16u * i + lr;
+                if (i >= ni || r >= rows) continue;
+#pragma unroll
+                for (uint32_t j = 0; j < 4u; ++j) {
+                    const uint32_t c = wc + 16u * j + result_col((lane >> 4) * 4u);
+                    if (c < cols) store4(args, (outRow + r) * args.n + col0 + c, loop.acc[i][j], umin(4u, cols - c));
+                }
+            }
+        } else {
+#pragma unroll
+            for (uint32_t i = 0; i < (uint32_t)NIMAX; ++i) {
+                const uint32_t r = wr + 16u * i + lr;
+                if (i >= ni) continue;
+                if constexpr (DT == DT_F8) {
+                    if (args.nPeers && r < rows) {
+#pragma unroll
+                        for (uint32_t j = 0; j < 4u; ++j) {
+                            const uint32_t c = wc + 16u * j + result_col((lane >> 4) * 4u);
+                            if (c < cols) add_peers4(args, row0 + r, col0 + c, loop.acc[i][j], umin(4u, cols - c));
+                        }
+                    }
+                }
+#pragma unroll
+                for (uint32_t j = 0; j < 4u; j += 2u) {   // lanes 0-31: block j, lanes 32-63: block j + 1, eight columns each
+                    const v4f a = loop.acc[i][j], b = loop.acc[i][j + 1u];
+                    const auto lo = __builtin_amdgcn_permlane32_swap(round2(a[0], a[1], args.outType), round2(b[0], b[1], args.outType), false, false);
+                    const auto hi = __builtin_amdgcn_permlane32_swap(round2(a[2], a[3], args.outType), round2(b[2], b[3], args.outType), false, false);
+                    const uint32_t c = wc + 16u * (j + (lane >> 5)) + 8u * ((lane >> 4) & 1u);
+                    if (r < rows && c < cols) store8_16bit(args, (outRow + r) * args.n + col0 + c, v4i{(int)lo[0], (int)hi[0], (int)lo[1], (int)hi[1]}, umin(8u, cols - c));
+                }
+            }
+        }
+        if (!more) return;
+    }
+}
+
+}  // namespace catcoc

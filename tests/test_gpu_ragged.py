@@ -389,3 +389,50 @@ def test_calls_say_what_they_ran():
     ops.fp8_matmul_allreduce(x, w, sx, sw)
     info = L.last_launch()
     assert (info.kernel, info.tileRows, info.tileCols) == (L.KERNEL_RAGGED_CHECKED, 64, 64)
+
+
+LARGE = {"uneven": [513, 0, 31, 900, 260, 1], "one_group": [1300], "full": [512, 256]}
+
+
+@pytest.mark.parametrize("name", sorted(LARGE))
+@pytest.mark.parametrize("k,n", [(1024, 512), (1096, 776), (514, 1030), (66, 2)])
+@pytest.mark.parametrize("trans_b", [False, True])
+def test_large_tiles(name, k, n, trans_b):
+    counts = LARGE[name]
+    g = gen(k * n)
+    rows, groups = sum(counts), len(counts)
+    ends = ends_of(counts)
+    x, dy = randn(g, rows + 40, k, dtype=torch.bfloat16), randn(g, rows + 40, n, dtype=torch.bfloat16)
+    x[rows:], dy[rows:] = float("nan"), float("nan")
+    w = randn(g, groups, n, k, dtype=torch.bfloat16) if trans_b else randn(g, groups, k, n, dtype=torch.bfloat16)
+    out = ops.grouped_matmul(x, w, ends, trans_b=trans_b)
+    assert (L.last_launch().kernel, L.last_launch().tileRows) == (L.KERNEL_RAGGED, 256)
+    dw = ops.grouped_matmul_dw(x, dy, ends, out_dtype=torch.float32, trans_b=trans_b)
+    assert (L.last_launch().kernel, L.last_launch().tileRows) == (L.KERNEL_RAGGED, 256)
+    half = ops.grouped_matmul_dw(x, dy, ends, out_dtype=torch.float16, trans_b=trans_b)
+    for e, (i, j) in enumerate(ranges(counts)):
+        a, b, d = x[i:j].double(), w[e].double(), dy[i:j].double()
+        b = b.t() if trans_b else b
+        close(out[i:j], a @ b, a.abs() @ b.abs(), k, torch.bfloat16)
+        want, mag = a.t() @ d, a.abs().t() @ d.abs()
+        close(dw[e].t() if trans_b else dw[e], want, mag, j - i, torch.float32)
+        close(half[e].t() if trans_b else half[e], want, mag, j - i, torch.float16)
+    assert (out[rows:] == 0).all()
+
+
+@pytest.mark.parametrize("name", sorted(LARGE))
+@pytest.mark.parametrize("k,n", [(1024, 512), (1100, 777), (516, 1030), (132, 3)])
+def test_large_fp8_tiles(name, k, n):
+    counts = LARGE[name]
+    g = gen(k * n + 1)
+    rows, groups = sum(counts), len(counts)
+    x, sx = fp8_operand(g, rows + 3, k, 1)
+    sx *= 0.05 / 60
+    w = (randn(g, groups, n, k) * 60).clamp(-448, 448).to(F8)
+    sw = torch.rand((groups, blocks(n), blocks(k)), device=DEV, generator=g) + 0.5
+    out = ops.grouped_fp8_matmul(x, w, sx, sw, ends_of(counts))
+    assert (L.last_launch().kernel, L.last_launch().tileRows) == (L.KERNEL_RAGGED, 256)
+    for e, (i, j) in enumerate(ranges(counts)):
+        a, b = x[i:j].double() * spread(sx[:, i:j].t(), j - i, k, 1), w[e].double() * spread(sw[e], n, k, 128)
+        close(out[i:j], a @ b.t(), a.abs() @ b.abs().t(), k, torch.bfloat16, norm2(a, b))
+    assert (out[rows:] == 0).all()
