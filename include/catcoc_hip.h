@@ -282,9 +282,18 @@ CATCOC_API void catcoc_reduce_add(void *stream, uint8_t *dst, uint8_t *src, uint
 /* 8-bit floating point with block scales; rows that come in groups          */
 /* ----------------------------------------------------------------------- */
 
+typedef struct CatcocTile {
+    uint32_t rows, cols, teams;
+} CatcocTile;
+
 /* No counterpart in the reference; beside its W8A8 and float products.  k and n are below 2^22, rows below 2^31, any of them odd; any alignment of
  * the element type serves, rows that start on 4 bytes run the fast kernels.  A call with rows == 0 is accepted and writes nothing (a weight gradient:
  * zeros).  Nothing needs a workspace, no sum depends on the order in which workgroups run, and every sum is held in fp32 and rounded once.
+ *
+ * `tile` of the products: the kernel's tile, for tests and tuning as m0 and n0 of CocTilingParams; NULL or zeros let the library choose.  Any product: 64x64 with one team
+ * (every load checked, any alignment); rows that start on 4 bytes: 256x256 and 128x128 with one, and, weight gradients apart, 64x128 and 128x128 with two teams of waves that
+ * share a tile's steps of k, and with four 16x32 and 32x32 (w as [n,k]) or 16x64, 32x64 and 64x64 (as [k,n]).  Anything else is rejected.  Sums are added in an order that
+ * depends on the tile alone.
  *
  * Quantizer to e4m3 (OCP: finite values up to 448, and NaN).  scale = max(largest magnitude of the block, 2^-40) / 448, code = x / scale, rounded to
  * nearest even.  blockRows 1: a scale for each 128 values of a row, scale [ceil(cols/128), rows] (a product's tile finds its rows' scales of a block
@@ -298,23 +307,24 @@ CATCOC_API void catcoc_quantize_fp8(void *stream, const void *x, uint8_t *q, flo
  * (symmetricPtr: a CatcocSymmetricDesc of which rankIdx, rankSize, peers, peerLd and peerRowOffset count; NULL: one rank), rounded once to outDataType
  * (FP16, BF16).  x1 [m,k] and x2 [n,k] (a weight matrix stored output-major) e4m3, scale_x1 [ceil(k/128), m], scale_x2 [ceil(n/128), ceil(k/128)]. */
 CATCOC_API void catcoc_fp8_matmul_allreduce(void *stream, const uint8_t *x1, const uint8_t *x2, const float *scale_x1, const float *scale_x2, void *c,
-                                            uint8_t *symmetricPtr, uint32_t m, uint32_t n, uint32_t k, uint32_t outDataType);
+                                            uint8_t *symmetricPtr, uint32_t m, uint32_t n, uint32_t k, uint32_t outDataType,
+                                            const CatcocTile *tile);
 
 /* out[i] = x[i] w[e] for rows i of group e, [groupEnds[e-1], groupEnds[e]) (groupEnds [groups] int32 on the GPU, ascending; values outside [0, rows] count
  * as the nearer end).  x [rows,k], w [groups,k,n] or, transB, [groups,n,k], out [rows,n], all FP16 or all BF16 (dataType).  Rows past the last group
  * are written as zeros.  The gradient of x is the same call on dy with the other transB. */
 CATCOC_API void catcoc_grouped_matmul(void *stream, uint32_t dataType, const void *x, const void *w, const int32_t *groupEnds, void *out, uint32_t rows,
-                                      uint32_t n, uint32_t k, uint32_t groups, uint32_t transB);
+                                      uint32_t n, uint32_t k, uint32_t groups, uint32_t transB, const CatcocTile *tile);
 
 /* The weight gradient: dw[e] = sum over the group's rows of x[i]^T dy[i], [groups,k,n] or, transB, [groups,n,k]; groups without rows get zeros.  x [rows,k],
  * dy [rows,n] FP16 or BF16, dw outDataType: the same, the other, or 0 (fp32). */
 CATCOC_API void catcoc_grouped_matmul_dw(void *stream, uint32_t dataType, const void *x, const void *dy, const int32_t *groupEnds, void *dw, uint32_t rows,
-                                         uint32_t n, uint32_t k, uint32_t groups, uint32_t transB, uint32_t outDataType);
+                                         uint32_t n, uint32_t k, uint32_t groups, uint32_t transB, uint32_t outDataType, const CatcocTile *tile);
 
 /* catcoc_grouped_matmul on e4m3: x [rows,k] with scale_x [ceil(k/128), rows], w [groups,n,k] with scale_w [groups, ceil(n/128), ceil(k/128)]. */
 CATCOC_API void catcoc_grouped_fp8_matmul(void *stream, const uint8_t *x, const uint8_t *w, const float *scale_x, const float *scale_w,
                                           const int32_t *groupEnds, void *out, uint32_t rows, uint32_t n, uint32_t k, uint32_t groups,
-                                          uint32_t outDataType);
+                                          uint32_t outDataType, const CatcocTile *tile);
 
 /* The reference's accuracy gate (examples/utils/verify_result.py:26-43,88-117 with the tolerances of
  * examples/utils/utils.py:44-52) on host arrays: every element |out - gold| <= rtol * max(1, |gold|) with
@@ -495,7 +505,7 @@ enum {
 typedef struct CatcocLaunchInfo {
     uint32_t kernel;             /* CATCOC_KERNEL_* */
     uint32_t tileRows, tileCols;
-    uint32_t kSlices;            /* 1 = none */
+    uint32_t kSlices;            /* 1 = none; CATCOC_KERNEL_RAGGED: teams of a workgroup */
     uint32_t dealt;              /* small tiles of 128 columns: a reduce-scatter's kept rows are dealt out to all row tiles */
     uint32_t largeTiles;         /* mixed tiles: how many are 256x256 */
 } CatcocLaunchInfo;

@@ -62,16 +62,15 @@ struct RaggedTile {
     uint32_t group, row, rows, colTile;
 };
 
-// Tile of workgroup `wg` where a group's rows are cut into tiles of at most BX rows of about the same height (whole `unit`s), nt column tiles.  A group's tiles follow each
+// Tile of workgroup `wg` where a group's rows are cut into tiles of at most bx rows of about the same height (whole `unit`s), nt column tiles.  A group's tiles follow each
 // other, eight row tiles to a band and column by column within it: the tiles that run on an XCD at a time share few rows and columns.  Every wave
 // works it out by itself, 64 groups at a time.  False: no tile left.
-template <uint32_t BX>
-__device__ __forceinline__ bool ragged_tile(const RaggedArgs &args, uint32_t wg, uint32_t nt, uint32_t unit, RaggedTile &t)
+__device__ __forceinline__ bool ragged_tile(const RaggedArgs &args, uint32_t wg, uint32_t bx, uint32_t nt, uint32_t unit, RaggedTile &t)
 {
     const uint32_t lane = threadIdx.x & 63u;
     uint32_t first = 0, count, begin, end, local;   // the group's first row tile and how many it has
     if (args.ends == nullptr) {
-        count = (args.rows + BX - 1u) / BX;
+        count = (args.rows + bx - 1u) / bx;
         local = xcd_run(wg, count * nt);
         if (local >= count * nt) return false;
         t.group = 0;
@@ -83,7 +82,7 @@ __device__ __forceinline__ bool ragged_tile(const RaggedArgs &args, uint32_t wg,
         for (uint32_t c = 0; c < chunks; ++c) {
             const uint32_t g = c * 64u + lane;
             group_rows(args, umin(g, args.groups), b, e);
-            tiles = g <= args.groups ? (e - b + BX - 1u) / BX : 0u;
+            tiles = g <= args.groups ? (e - b + bx - 1u) / bx : 0u;
             upTo = wave_prefix(tiles);
             total += (uint32_t)__builtin_amdgcn_readlane((int)upTo, 63);
         }
@@ -94,7 +93,7 @@ __device__ __forceinline__ bool ragged_tile(const RaggedArgs &args, uint32_t wg,
             if (chunks > 1u) {
                 const uint32_t g = c * 64u + lane;
                 group_rows(args, umin(g, args.groups), b, e);
-                tiles = g <= args.groups ? (e - b + BX - 1u) / BX : 0u;
+                tiles = g <= args.groups ? (e - b + bx - 1u) / bx : 0u;
                 upTo = wave_prefix(tiles);
             }
             const uint64_t past = __ballot((before + upTo) * nt > at);
@@ -196,22 +195,47 @@ __device__ __forceinline__ void store8_16bit(const RaggedArgs &args, size_t at, 
     }
 }
 
-// The other ranks' partials of four such values, added in slot order.
-__device__ __forceinline__ void add_peers4(const RaggedArgs &args, uint32_t row, uint32_t col, v4f &v, uint32_t have)
+// The other ranks' partials of four consecutive values of a row: `BATCH` of them from slot `first` on, asked for together ...
+template <int BATCH>
+__device__ __forceinline__ void load_peers4(const RaggedArgs &args, uint32_t first, uint32_t row, uint32_t col, uint32_t have, v4f (&u)[BATCH])
 {
-    for (uint32_t p = 0; p < args.nPeers; ++p) {
-        const float *q = args.peers[p] + (int64_t)row * args.peerLd + col;
-        if (have >= 4u) {
-            v4f u;
-            __builtin_memcpy(&u, q, 16);
 #pragma unroll
-            for (int r = 0; r < 4; ++r) v[r] += u[r];
+    for (uint32_t p = 0; p < (uint32_t)BATCH; ++p) {
+        u[p] = v4f{0.f, 0.f, 0.f, 0.f};
+        if (first + p >= args.nPeers || have == 0u) continue;
+        const float *q = args.peers[first + p] + (int64_t)row * args.peerLd + col;
+        if (have >= 4u) {
+            __builtin_memcpy(&u[p], q, 16);
         } else {
 #pragma unroll
             for (uint32_t r = 0; r < 3u; ++r)
-                if (r < have) v[r] += q[r];
+                if (r < have) u[p][r] = q[r];
         }
     }
+}
+
+// ... and all of them added in slot order, the first `BATCH` from `u`.
+template <int BATCH>
+__device__ __forceinline__ void add_peers4(const RaggedArgs &args, uint32_t row, uint32_t col, v4f &v, uint32_t have, v4f (&u)[BATCH])
+{
+    for (uint32_t first = 0; first < args.nPeers; first += BATCH) {
+        if (first != 0) load_peers4<BATCH>(args, first, row, col, have, u);
+#pragma unroll
+        for (uint32_t p = 0; p < (uint32_t)BATCH; ++p)
+            if (first + p < args.nPeers) {
+#pragma unroll
+                for (int r = 0; r < 4; ++r) v[r] += u[p][r];
+            }
+    }
+}
+
+// The same where nothing was asked for yet.
+__device__ __forceinline__ void add_peers4(const RaggedArgs &args, uint32_t row, uint32_t col, v4f &v, uint32_t have)
+{
+    if (args.nPeers == 0) return;
+    v4f u[4];
+    load_peers4<4>(args, 0, row, col, have, u);
+    add_peers4<4>(args, row, col, v, have, u);
 }
 
 }  // namespace catcoc

@@ -2,6 +2,8 @@
 // choice of kernel.
 #include <hip/hip_runtime.h>
 
+#include <math.h>
+
 #include <algorithm>
 
 #include "api_status.h"
@@ -9,7 +11,8 @@
 
 namespace catcoc {
 int launch_quantize(uint32_t dtype, const QuantArgs &a, bool blocks, bool gated, void *stream);
-int launch_ragged_tile(uint32_t dtype, const RaggedArgs &a, bool kn, bool dw, uint32_t wgs, void *stream);
+int launch_ragged_tile(uint32_t dtype, const RaggedArgs &a, bool kn, bool dw, uint32_t cols, uint32_t teams, uint32_t wgs, void *stream);
+int launch_ragged_small(uint32_t dtype, const RaggedArgs &a, bool kn, uint32_t rows, uint32_t wgs, void *stream);
 int launch_ragged_checked(uint32_t dtype, const RaggedArgs &a, bool kn, bool dw, uint32_t wgs, void *stream);
 }
 
@@ -48,15 +51,114 @@ bool rows_on_words(uint32_t dtype, const RaggedArgs &a, bool kn, bool dw)
     return ((uintptr_t)a.x | (uintptr_t)a.w) % 4 == 0 && a.k * es % 4 == 0 && ((!kn && !dw) || a.n * es % 4 == 0);
 }
 
-void run(uint32_t dtype, const RaggedArgs &a, bool kn, bool dw, void *stream)
+// The kernels that a product can run on: their tiles, and how many teams of a workgroup's waves share a tile's steps of k.
+struct Choice {
+    enum Kind { SMALL, TILE, CHECKED } kind;
+    uint32_t rows, cols, teams;
+};
+constexpr Choice kChecked{Choice::CHECKED, 64, 64, 1};
+constexpr Choice kSmallNk[] = {{Choice::SMALL, 16, 32, 4}, {Choice::SMALL, 32, 32, 4}};
+constexpr Choice kSmallKn[] = {{Choice::SMALL, 16, 64, 4}, {Choice::SMALL, 32, 64, 4}, {Choice::SMALL, 64, 64, 4}};
+constexpr Choice kTeams64{Choice::TILE, 64, 128, 2}, kTeams128{Choice::TILE, 128, 128, 2}, kTile128{Choice::TILE, 128, 128, 1}, kTile256{Choice::TILE, 256, 256, 1};
+
+// By what a launch is estimated to take, in us: the larger of what memory needs for each byte once (5.7 GB/ms; `reach`: over what a kernel reaches of it) and of its
+// rounds of workgroups, a quarter of the smaller, and a start.  A round costs its steps of 128 bytes of k, `step` us each with the GPU full, `few` of that with
+// at most one workgroup a CU.  Fitted to, and compared on, 47 sizes that ran on all of these kernels (1 to 8192 rows of e4m3 against 2048 to 8192 columns and
+// k; 16 to 4096 rows in 8 to 64 groups of 4096x1792, 16 bits either way and e4m3): for 41 of them the choice is within 6 % of the fastest, the worst 1.22 of
+// it.  How the rows of groups lie is not known here: half a tile more than the mean is assumed.
+Choice choose(uint32_t dtype, const RaggedArgs &a, bool kn)
 {
-    const bool tile = rows_on_words(dtype, a, kn, dw) && (dw || a.rows > 32ull * a.groups);
-    const uint64_t bx = tile ? 256 : 64, nt = cdiv(a.n, bx);
-    // weight gradient on large tiles: eighths of every group's tiles, dealt out to one workgroup a CU
-    const uint64_t wgs = dw && tile ? std::min<uint64_t>(256, a.groups * cdiv(cdiv(a.k, bx) * nt, 8) * 8) : dw ? a.groups * cdiv(a.k, bx) * nt : most_row_tiles(a, bx) * nt;
+    const bool f8 = dtype == DT_F8;
+    const double es = f8 ? 1 : 2, steps = (double)cdiv(a.k * (uint64_t)es, 128);
+    const double active = a.ends ? std::min(a.groups, a.rows) : 1, mean = a.rows / active;
+    const double mem = (active * a.k * a.n * es + a.rows * (double)a.k * es + a.rows * (double)a.n * (2.0 + 4.0 * a.nPeers)) / 5.7e6;
+    Choice best = kTile256;
+    double least = 0;
+    auto row_tiles = [&](uint32_t rows) { return a.ends ? active * std::max(1.0, mean / rows + 0.5) : (double)cdiv(a.rows, rows); };
+    auto offer = [&](const Choice &c, double start, double slots, double step, double few, double reach) {
+        const double tiles = row_tiles(c.rows) * (double)cdiv(a.n, c.cols);
+        double rounds = tiles / slots;
+        rounds = a.ends || rounds > 4 ? std::max(1.0, rounds + 0.3) : std::ceil(rounds);
+        const double work = (tiles <= 256 ? few : 1.0) * step * steps * rounds, m = mem * reach;
+        const double t = start + std::max(m, work) + 0.25 * std::min(m, work);
+        if (least == 0 || t < least) { least = t; best = c; }
+    };
+    if (kn) {
+        offer(kSmallKn[0], 5, 512, 0.2, 1, 1);
+        offer(kSmallKn[1], 5, 256, 0.17, 1, 1);
+        offer(kSmallKn[2], 5, 256, 0.24, 1, 1);
+    } else {
+        offer(kSmallNk[0], 5, 512, f8 ? 0.156 : 0.106, 0.83, 1);
+        offer(kSmallNk[1], 5, 512, f8 ? 0.21 : 0.16, 0.7, 1);
+    }
+    offer(kTeams64, 6, 256, f8 ? 0.43 : 0.41, 1, 1.2);
+    offer(kTeams128, 6, 256, f8 ? 0.6 : 0.55, 1, 1.2);
+    offer(kTile128, 6, 512, f8 ? 1.05 : 1.09, 0.65, 1.05);
+    const double height = std::min(8.0, std::max(2.0, std::ceil(a.rows / row_tiles(256) / 32)));   // in 32 rows
+    offer(kTile256, 8, 256, f8 ? 0.35 + 0.19 * height : 0.45 + 0.125 * height, 1, f8 ? 1.2 : 0.98);
+    return best;
+}
+
+// Weight gradients: rounds of 256 (512) workgroups, each a start and its steps.  Measured (us, fp32 results, 256x256 / 128x128 tiles): 8 groups of 512 rows,
+// 512x512 22.5 / 10.4; 64 of 256, 512x512 38.9 / 27.9; 8 of 128, 2048x2048 38.0 / 34.6; 16 of 256, 1024x1024 25.5 / 25.4; 8 of 2048, 1024x2048 71 / 78;
+// 16 of 512, 4096x1792 227 / 273; one of 4096, 4096x4096 117 / 156.
+Choice choose_dw(const RaggedArgs &a)
+{
+    const double steps = std::ceil((double)a.rows / a.groups / 64);
+    const double large = std::ceil(a.groups * (double)(cdiv(a.k, 256) * cdiv(a.n, 256)) / 256) * (9 + 1.5 * steps);
+    const double small = std::ceil(a.groups * (double)(cdiv(a.k, 128) * cdiv(a.n, 128)) / 512) * (3.5 + steps);
+    return small < large ? kTile128 : kTile256;
+}
+
+// What the caller asks for, where a product can run on it.
+const Choice *asked_for(const CatcocTile &tile, bool kn, bool dw, bool words)
+{
+    auto is = [&](const Choice &c) { return c.rows == tile.rows && c.cols == tile.cols && c.teams == tile.teams; };
+    if (is(kChecked)) return &kChecked;
+    if (!words) return nullptr;
+    for (const Choice *c : {&kTile256, &kTile128})
+        if (is(*c)) return c;
+    if (dw) return nullptr;
+    for (const Choice *c : {&kTeams64, &kTeams128})
+        if (is(*c)) return c;
+    if (kn) {
+        for (const Choice &c : kSmallKn)
+            if (is(c)) return &c;
+    } else {
+        for (const Choice &c : kSmallNk)
+            if (is(c)) return &c;
+    }
+    return nullptr;
+}
+
+void run(uint32_t dtype, const RaggedArgs &args, bool kn, bool dw, const CatcocTile *tile, void *stream)
+{
+    RaggedArgs a = args;
+    const bool words = rows_on_words(dtype, a, kn, dw);
+    Choice c = kChecked;
+    if (tile != nullptr && (tile->rows || tile->cols || tile->teams)) {
+        const Choice *asked = asked_for(*tile, kn, dw, words);
+        if (asked == nullptr) {
+            api_fail(E_TILING, "no kernel of %ux%u tiles and %u team(s) for this product%s", tile->rows, tile->cols, tile->teams, words ? "" : " (rows that do not start on 4 bytes run 64x64 tiles, 1 team)");
+            return;
+        }
+        c = *asked;
+    } else if (words) {
+        c = dw ? choose_dw(a) : choose(dtype, a, kn);
+    }
+    a.tileRows = c.rows;
+    const uint64_t nt = cdiv(a.n, c.cols);
+    uint64_t wgs = most_row_tiles(a, c.rows) * nt;
+    if (dw) {
+        wgs = a.groups * cdiv(a.k, c.rows) * nt;
+        if (c.kind == Choice::TILE)   // eighths of every group's tiles, dealt out to one workgroup a CU (two of 128 columns)
+            wgs = std::min<uint64_t>(65536 / c.cols, a.groups * cdiv(cdiv(a.k, c.rows) * nt, 8) * 8);
+    }
     if (wgs > kMaxWgs) { api_fail(E_SHAPE, "%llu tiles are more than one launch holds", (unsigned long long)wgs); return; }
-    api_launch_info({tile ? (uint32_t)CATCOC_KERNEL_RAGGED : (uint32_t)CATCOC_KERNEL_RAGGED_CHECKED, (uint32_t)bx, (uint32_t)bx, 1, 0, 0});
-    api_launched((tile ? launch_ragged_tile : launch_ragged_checked)(dtype, a, kn, dw, (uint32_t)wgs, stream));
+    api_launch_info({c.kind == Choice::CHECKED ? (uint32_t)CATCOC_KERNEL_RAGGED_CHECKED : (uint32_t)CATCOC_KERNEL_RAGGED, c.rows, c.cols, c.teams, 0, 0});
+    if (c.kind == Choice::SMALL) api_launched(launch_ragged_small(dtype, a, kn, c.rows, (uint32_t)wgs, stream));
+    else if (c.kind == Choice::TILE) api_launched(launch_ragged_tile(dtype, a, kn, dw, c.cols, c.teams, (uint32_t)wgs, stream));
+    else api_launched(launch_ragged_checked(dtype, a, kn, dw, (uint32_t)wgs, stream));
 }
 
 }  // namespace
@@ -78,7 +180,7 @@ void catcoc_quantize_fp8(void *stream, const void *x, uint8_t *q, float *scale, 
 }
 
 void catcoc_fp8_matmul_allreduce(void *stream, const uint8_t *x1, const uint8_t *x2, const float *scale_x1, const float *scale_x2, void *c,
-                                 uint8_t *symmetricPtr, uint32_t m, uint32_t n, uint32_t k, uint32_t outDataType)
+                                 uint8_t *symmetricPtr, uint32_t m, uint32_t n, uint32_t k, uint32_t outDataType, const CatcocTile *tile)
 {
     if (!is16(outDataType)) { api_fail(E_DTYPE, "outDataType %u must be FP16 (1) or BF16 (27)", outDataType); return; }
     if (check_sizes(m, k, n, 1)) return;
@@ -110,11 +212,11 @@ void catcoc_fp8_matmul_allreduce(void *stream, const uint8_t *x1, const uint8_t 
     a.n = n;
     a.groups = 1;
     a.outType = outDataType;
-    run(DT_F8, a, false, false, stream);
+    run(DT_F8, a, false, false, tile, stream);
 }
 
 void catcoc_grouped_matmul(void *stream, uint32_t dataType, const void *x, const void *w, const int32_t *groupEnds, void *out, uint32_t rows, uint32_t n,
-                           uint32_t k, uint32_t groups, uint32_t transB)
+                           uint32_t k, uint32_t groups, uint32_t transB, const CatcocTile *tile)
 {
     if (!is16(dataType)) { api_fail(E_DTYPE, "dataType %u must be FP16 (1) or BF16 (27)", dataType); return; }
     if (check_sizes(rows, k, n, groups)) return;
@@ -130,11 +232,12 @@ void catcoc_grouped_matmul(void *stream, uint32_t dataType, const void *x, const
     a.n = n;
     a.groups = groups;
     a.outType = dataType;
-    run(dataType, a, transB == 0, false, stream);
+    run(dataType, a, transB == 0, false, tile, stream);
 }
 
 void catcoc_grouped_matmul_dw(void *stream, uint32_t dataType, const void *x, const void *dy, const int32_t *groupEnds, void *dw, uint32_t rows, uint32_t n,
-                              uint32_t k, uint32_t groups, uint32_t transB, uint32_t outDataType)
+                              uint32_t k, uint32_t groups, uint32_t transB, uint32_t outDataType,
+                              const CatcocTile *tile)
 {
     if (!is16(dataType)) { api_fail(E_DTYPE, "dataType %u must be FP16 (1) or BF16 (27)", dataType); return; }
     if (outDataType != 0 && !is16(outDataType)) { api_fail(E_DTYPE, "outDataType %u must be 0 (fp32), FP16 or BF16", outDataType); return; }
@@ -150,11 +253,12 @@ void catcoc_grouped_matmul_dw(void *stream, uint32_t dataType, const void *x, co
     a.n = transB ? k : n;
     a.groups = groups;
     a.outType = outDataType;
-    run(dataType, a, false, true, stream);
+    run(dataType, a, false, true, tile, stream);
 }
 
 void catcoc_grouped_fp8_matmul(void *stream, const uint8_t *x, const uint8_t *w, const float *scale_x, const float *scale_w, const int32_t *groupEnds,
-                               void *out, uint32_t rows, uint32_t n, uint32_t k, uint32_t groups, uint32_t outDataType)
+                               void *out, uint32_t rows, uint32_t n, uint32_t k, uint32_t groups, uint32_t outDataType,
+                               const CatcocTile *tile)
 {
     if (!is16(outDataType)) { api_fail(E_DTYPE, "outDataType %u must be FP16 (1) or BF16 (27)", outDataType); return; }
     if (check_sizes(rows, k, n, groups)) return;
@@ -172,7 +276,7 @@ void catcoc_grouped_fp8_matmul(void *stream, const uint8_t *x, const uint8_t *w,
     a.n = n;
     a.groups = groups;
     a.outType = outDataType;
-    run(DT_F8, a, false, false, stream);
+    run(DT_F8, a, false, false, tile, stream);
 }
 
 }  // extern "C"

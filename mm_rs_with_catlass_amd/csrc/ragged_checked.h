@@ -87,7 +87,7 @@ __global__ void __launch_bounds__(256, 2) ragged_checked_kernel(const RaggedArgs
         X = (const unsigned char *)args.x + ((size_t)b * args.k + t.row) * 2u;
         W = (const unsigned char *)args.w + ((size_t)b * args.n + 64u * t.colTile) * 2u;
     } else {
-        if (!ragged_tile<64>(args, blockIdx.x, nt, 64u, t)) return;
+        if (!ragged_tile(args, blockIdx.x, 64u, nt, 64u, t)) return;
         group = t.group;
         K = group < args.groups ? args.k : 0u;
         X = (const unsigned char *)args.x + (size_t)t.row * args.k * ES;

@@ -107,26 +107,31 @@ __device__ __forceinline__ uint32_t result_col(uint32_t m) { return ((m >> 2) & 
 // A tile of 32 NIMAX rows and 64 WY columns: 2 WY waves, two by WY, of up to 16 NIMAX rows and 64 columns each (NI row fragments, as many as the tile's rows
 // need; four of columns).  A wave keeps a step's column fragments in registers and streams its row fragments, two ahead of the MFMAs.
 //
-// Two stages of 128 bytes of k, three where a wave has at most four row fragments (their stages are smaller).  When the last read of a step is out, the
-// wave waits for the next stage's copies (issued a whole step before, or two) and for its own reads; the barrier behind that says both that the next stage
+// Two stages of 128 bytes of k, three with eight waves and at most four row fragments each (their stages are smaller).  When the last read of a step is out, the
+// wave waits for the next stage's copies (issued a whole step before, or several) and for its own reads; the barrier behind that says both that the next stage
 // is complete and that this one may be overwritten: its next copies start there.  The last two row fragments' MFMAs then cover the first reads of the next
 // step, whose column fragments take the registers of those just used.
-template <uint32_t DT, bool XK, bool WK, int WY, int NIMAX>
+//
+// KG = 2: two teams of 2 WY waves multiply every other step of the same tile, each through stages of its own, and add their sums at the end (team 0's first).
+// A launch of at most one tile per CU else has one wave on a SIMD, which pays for barrier, LDS and issue one after the other.
+template <uint32_t DT, bool XK, bool WK, int WY, int NIMAX, int KG>
 struct RaggedTileLoop {
     static constexpr uint32_t ES = DT == DT_F8 ? 1u : 2u, KE = 128u / ES;
     static constexpr uint32_t WAVES = 2u * WY, BX = 32u * NIMAX, BY = 64u * WY, SUB = 16384u;
     static constexpr uint32_t XSUBS = BX / 128u, WSUBS = BY / 128u;
     static constexpr uint32_t stages(int ni) { return NIMAX == 8 && ni <= 4 ? 3u : 2u; }
     static constexpr uint32_t stage_bytes(int ni) { return ((ni <= 4 ? 1u : 2u) + WSUBS) * SUB; }
-    static constexpr uint32_t SX = XSUBS == 2u ? 3u * stage_bytes(4) : 2u * stage_bytes(4);   // e4m3: row scales behind the stages
-    static constexpr uint32_t SXB = BX * 4u;
-    static constexpr uint32_t LDS = SX + (DT == DT_F8 ? 3u * SXB : 0u);
+    static constexpr uint32_t SX = stages(4) * stage_bytes(4);   // e4m3: row scales behind the stages
+    static constexpr uint32_t SXB = BX * 4u, SXN = stages(4);
+    static constexpr uint32_t LDS = SX + (DT == DT_F8 ? SXN * SXB : 0u);   // of a team
+    static_assert(KG == 1 || (KG == 2 && NIMAX * WAVES * 2048u <= SX), "two teams: half of a team's sums fit its stages");
     TileOperand<XK, XSUBS, ES, WAVES> x;
     TileOperand<WK, WSUBS, ES, WAVES> w;
     v4f acc[NIMAX][4];
 
     struct Problem {
-        uint32_t K, steps;          // values of k, steps of them
+        uint32_t K, steps;          // values of k, this team's steps of them
+        uint32_t rounds, team;      // steps of the team that has most; which one this is
         uint32_t rows, cols;        // of the tile
         uint32_t ni;                // row fragments of a wave
         uint32_t xLeft, wLeft;      // columns of the matrix from the tile's first on (operands that are rows of k)
@@ -135,27 +140,29 @@ struct RaggedTileLoop {
         uint32_t sxPitch;
     };
 
-    // Copies of step s into `stage`; TWO: of both halves of the rows.
+    static __device__ __forceinline__ uint32_t of_all(const Problem &p, uint32_t s) { return KG * s + (KG > 1 ? p.team : 0u); }
+
+    // Copies of the team's step s into `stage`; TWO: of both halves of the rows.
     template <bool TWO>
     __device__ __forceinline__ void issue(const Problem &p, unsigned char *smem, uint32_t stage, uint32_t s, uint32_t wave, uint32_t lane)
     {
         const uint32_t lds0 = (uint32_t)(uintptr_t)(CATCOC_LDS unsigned char *)smem, ws = stage + (TWO ? 2u : 1u) * SUB;
         if (p.partLast && s + 1u == p.steps) {
-            const uint32_t left = p.K - s * KE;
+            const uint32_t left = p.K - of_all(p, s) * KE;
 #pragma unroll 1
-            for (uint32_t h = 0; h < WSUBS; ++h) w.issue_part(h, s, smem + ws + h * SUB, lds0 + ws + h * SUB, WK ? p.wLeft * 2u : left * ES, left, wave, lane);
+            for (uint32_t h = 0; h < WSUBS; ++h) w.issue_part(h, of_all(p, s), smem + ws + h * SUB, lds0 + ws + h * SUB, WK ? p.wLeft * 2u : left * ES, left, wave, lane);
 #pragma unroll 1
-            for (uint32_t h = 0; h < (TWO ? 2u : 1u); ++h) x.issue_part(h, s, smem + stage + h * SUB, lds0 + stage + h * SUB, XK ? p.xLeft * 2u : left * ES, left, wave, lane);
+            for (uint32_t h = 0; h < (TWO ? 2u : 1u); ++h) x.issue_part(h, of_all(p, s), smem + stage + h * SUB, lds0 + stage + h * SUB, XK ? p.xLeft * 2u : left * ES, left, wave, lane);
         } else {
 #pragma unroll
-            for (uint32_t h = 0; h < WSUBS; ++h) w.issue(h, s, lds0 + ws + h * SUB, wave);
+            for (uint32_t h = 0; h < WSUBS; ++h) w.issue(h, of_all(p, s), lds0 + ws + h * SUB, wave);
 #pragma unroll
             for (uint32_t h = 0; h < (TWO ? 2u : 1u); ++h)
-                if (x.wanted(h, p.ni, wave)) x.issue(h, s, lds0 + stage + h * SUB, wave);
+                if (x.wanted(h, p.ni, wave)) x.issue(h, of_all(p, s), lds0 + stage + h * SUB, wave);
         }
         if constexpr (DT == DT_F8) {   // 64 rows' scales a wave (several waves fetch the same ones)
             const uint32_t q = wave % (BX / 64u);
-            copy4((const unsigned char *)(p.sx + (size_t)s * p.sxPitch), umin(64u * q + lane, p.rows - 1u) * 4u, lds0 + SX + s % 3u * SXB + q * 256u);
+            copy4((const unsigned char *)(p.sx + (size_t)of_all(p, s) * p.sxPitch), umin(64u * q + lane, p.rows - 1u) * 4u, lds0 + SX + s % SXN * SXB + q * 256u);
         }
     }
 
@@ -197,24 +204,27 @@ struct RaggedTileLoop {
         for (int i = 0; i < NI; ++i)
 #pragma unroll
             for (int j = 0; j < 4; ++j) acc[i][j] = v4f{0.f, 0.f, 0.f, 0.f};
-        if (p.steps == 0) return;
+        if (p.rounds == 0) return;
         const uint32_t full = p.steps - (p.partLast ? 1u : 0u);   // whole steps
         const bool first = TWO || x.wanted(0, NI, wave), second = TWO && x.wanted(1, NI, wave);
         meet<(int)STAGES - 1>(full >= STAGES, first, second);
 
         const uint32_t xa = XK ? at_k_major<false>(256u, 64u * wr, lane, b16_slot<2>) : at_k_rows(64u * wr + (lane & 15u), lane);
         const uint32_t wh = WSUBS == 2u ? wc % 2u : 0u, w64 = 64u * (WSUBS == 2u ? wc / 2u : wc);   // the wave's columns: sub-stage, half of it
-        const uint32_t wa = ((TWO ? 2u : 1u) + wh) * SUB + (WK ? at_k_major<true>(256u, w64, lane, b16_slot<2>) : at_k_rows(w64 + result_col(lane & 15u), lane));
+        uint32_t wa = ((TWO ? 2u : 1u) + wh) * SUB + (WK ? at_k_major<true>(256u, w64, lane, b16_slot<2>) : at_k_rows(w64 + result_col(lane & 15u), lane));
+        // Two teams: team 1 has its column blocks in the order 2, 3, 0, 1, so that 0 and 1 are those that either team stores.
+        if (KG > 1 && p.team) wa ^= WK ? 64u : 4096u;
         auto read_x = [&](uint32_t stage, uint32_t i) {
             if constexpr (XK) return frag_k_major<256>(smem, ((stage + xa) ^ (32u * (i & 3u))) + (i >> 2) * SUB);
             else return frag_k_rows(smem, stage + xa + 2048u * (i & 3u) + (i >> 2) * SUB);
         };
         auto read_w = [&](uint32_t stage, uint32_t j) {
             if constexpr (WK) return frag_k_major<256>(smem, (stage + wa) ^ (32u * j));
+            else if constexpr (KG > 1) return frag_k_rows(smem, ((stage + wa) ^ (j / 2u * 4096u)) + 2048u * (j % 2u));
             else return frag_k_rows(smem, stage + wa + 2048u * j);
         };
         const uint32_t sa = SX + (wr * 16u * NI + (lane & 15u)) * 4u;
-        auto row_scale = [&](uint32_t s, int i) { return *(const float *)(smem + sa + s % 3u * SXB + 64u * i); };
+        auto row_scale = [&](uint32_t s, int i) { return *(const float *)(smem + sa + s % SXN * SXB + 64u * i); };
 
         // Row fragments' registers: the first two of a step have their own, which are free when the last two run.
         constexpr int SLOTS = NI == 8 ? 4 : NI >= 4 ? 5 : NI;
@@ -251,12 +261,21 @@ struct RaggedTileLoop {
             fx[i] = read_x(0, i);
             if constexpr (DT == DT_F8) fs[i] = row_scale(0, i);
         }
-        if constexpr (DT == DT_F8) sw = load_uniform(p.sw);
+        if constexpr (DT == DT_F8) sw = load_uniform(p.sw + (KG > 1 ? min(p.team, (p.K - 1u) / KE) : 0u));
         uint32_t cur = 0;   // this step's stage
 #pragma unroll 1
-        for (uint32_t s = 0; s < p.steps; ++s) {
+        for (uint32_t s = 0; s < p.rounds; ++s) {
+            if (KG > 1 && s >= p.steps) {   // (the other team has one more)
+                meet<0>(false, first, second);
+                break;
+            }
             const uint32_t next = cur == (STAGES - 1u) * STAGE ? 0u : cur + STAGE;
             queued = 0;
+            float swNext = 0.f;
+            if constexpr (DT == DT_F8) {   // (asked for here: its wait is the one for the step's reads)
+                swNext = load_uniform(p.sw + umin(of_all(p, s + 1u), (p.K - 1u) / KE));
+                __builtin_amdgcn_sched_barrier(0);
+            }
 #pragma unroll
             for (int i = 0; i < NI - 2; ++i) {
                 fx[slot(i + 2)] = read_x(cur, i + 2);
@@ -266,8 +285,6 @@ struct RaggedTileLoop {
                 for (int jj = 0; jj < 4; ++jj) multiply(i, snake16(i, jj, 4), fx[slot(i)], scale);
                 __builtin_amdgcn_sched_barrier(0);
             }
-            float swNext = 0.f;
-            if constexpr (DT == DT_F8) swNext = load_uniform(p.sw + umin(s + 1u, p.steps - 1u));
             meet<(int)STAGES - 2>(s + STAGES <= full, first, second);
             if (s + STAGES < p.steps) issue<TWO>(p, smem, cur, s + STAGES, wave, lane);
             // (behind the last step nobody looks at what is read here)
@@ -301,6 +318,30 @@ struct RaggedTileLoop {
         }
     }
 
+    // Two teams: each gets the other's sums of the columns that it stores.
+    __device__ __forceinline__ void join(const Problem &p, unsigned char *all, uint32_t wave, uint32_t lane)
+    {
+        // (all reads of the stages were before the last barrier)
+        unsigned char *const to = all + p.team * LDS + wave * (NIMAX * 2048u) + lane * 16u, *const from = all + (1u - p.team) * LDS + wave * (NIMAX * 2048u) + lane * 16u;
+#pragma unroll
+        for (uint32_t i = 0; i < (uint32_t)NIMAX; ++i)
+            if (i < p.ni) {
+                *(v4f *)(to + 2048u * i) = acc[i][2];
+                *(v4f *)(to + 2048u * i + 1024u) = acc[i][3];
+            }
+        __syncthreads();
+#pragma unroll
+        for (uint32_t i = 0; i < (uint32_t)NIMAX; ++i)
+            if (i < p.ni) {
+                const v4f a = *(const v4f *)(from + 2048u * i), b = *(const v4f *)(from + 2048u * i + 1024u);
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    acc[i][0][r] += a[r];
+                    acc[i][1][r] += b[r];
+                }
+            }
+    }
+
     template <int NI = NIMAX>
     __device__ __forceinline__ void run_rows(const Problem &p, unsigned char *smem, uint32_t wave, uint32_t lane)
     {
@@ -311,14 +352,17 @@ struct RaggedTileLoop {
 
 // DW: x and w are rows of k (the group's rows), the result is the group's [k, n] matrix.  KN: w is [k, n].
 // A weight gradient's workgroups walk several tiles: few rows make few steps, and a tile's first copies are on their way while the one before is stored.
-template <uint32_t DT, bool KN, bool DW, int WY, int NIMAX>
-__global__ void __launch_bounds__(128 * WY, 2) ragged_tile_kernel(const RaggedArgs args)
+template <uint32_t DT, bool KN, bool DW, int WY, int NIMAX, int KG>
+__global__ void __launch_bounds__(128 * WY * KG, 2) ragged_tile_kernel(const RaggedArgs args)
 {
-    using Loop = RaggedTileLoop<DT, DW, KN || DW, WY, NIMAX>;
+    using Loop = RaggedTileLoop<DT, DW, KN || DW, WY, NIMAX, KG>;
     constexpr uint32_t ES = Loop::ES, BX = Loop::BX, BY = Loop::BY;
-    __shared__ __attribute__((aligned(16))) unsigned char smem[Loop::LDS];
+    static_assert(!DW || KG == 1, "a weight gradient's tiles have one team");
+    __shared__ __attribute__((aligned(16))) unsigned char lds[KG * Loop::LDS];
 
-    const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(tid >> 6));
+    const uint32_t tid = threadIdx.x, lane = tid & 63u, waves = (uint32_t)__builtin_amdgcn_readfirstlane((int)(tid >> 6));
+    const uint32_t wave = waves % Loop::WAVES, team = waves / Loop::WAVES;
+    unsigned char *const smem = lds + team * Loop::LDS;
     const uint32_t nt = (args.n + BY - 1u) / BY;
     Loop loop;
     typename Loop::Problem p;
@@ -349,7 +393,7 @@ __global__ void __launch_bounds__(128 * WY, 2) ragged_tile_kernel(const RaggedAr
             sumEnd = (uint32_t)__builtin_amdgcn_readfirstlane((int)sumEnd);
             return true;
         } else {
-            return ragged_tile<BX>(args, at, nt, 32u, t);
+            return ragged_tile(args, at, args.tileRows, nt, 32u, t);
         }
     };
     auto set = [&](const RaggedTile &t) {
@@ -380,6 +424,12 @@ __global__ void __launch_bounds__(128 * WY, 2) ragged_tile_kernel(const RaggedAr
             }
         }
         p.steps = (p.K + Loop::KE - 1u) / Loop::KE;
+        p.rounds = (p.steps + KG - 1u) / KG;
+        p.team = team;
+        if constexpr (KG > 1) {
+            p.partLast = p.partLast && (p.steps - 1u) % KG == team;
+            p.steps = p.steps > team ? (p.steps - team + KG - 1u) / KG : 0u;
+        }
     };
 
     uint32_t at = blockIdx.x;
@@ -399,6 +449,7 @@ __global__ void __launch_bounds__(128 * WY, 2) ragged_tile_kernel(const RaggedAr
             loop.template run<NIMAX>(p, smem, wave, lane);
         } else {
             loop.run_rows(p, smem, wave, lane);
+            if constexpr (KG > 1) loop.join(p, lds, wave, lane);
         }
         const uint32_t rows = t.rows, row0 = t.row, col0 = BY * t.colTile, cols = p.cols;
         if (more) {
@@ -407,15 +458,16 @@ __global__ void __launch_bounds__(128 * WY, 2) ragged_tile_kernel(const RaggedAr
             loop.begin(p, smem, wave, lane);
         }
 
-        // ---- output: rows [wr, +16 ni) and columns [wc, +64) of the tile are this wave's
-        const uint32_t wr = (wave / WY) * 16u * ni, wc = (wave % WY) * 64u, lr = lane & 15u;
+        // ---- output: rows [wr, +16 ni) and columns [wc, +64) of the tile are this wave's (two teams: half of the columns each)
+        constexpr uint32_t NJ = KG == 1 ? 4u : 2u;   // column blocks that this wave stores
+        const uint32_t wr = (wave / WY) * 16u * ni, wc = (wave % WY) * 64u + 32u * team, lr = lane & 15u;
         if (DW && args.outType == 0) {
 #pragma unroll
             for (uint32_t i = 0; i < (uint32_t)NIMAX; ++i) {
                 const uint32_t r = wr + 16u * i + lr;
                 if (i >= ni || r >= rows) continue;
 #pragma unroll
-                for (uint32_t j = 0; j < 4u; ++j) {
+                for (uint32_t j = 0; j < NJ; ++j) {
                     const uint32_t c = wc + 16u * j + result_col((lane >> 4) * 4u);
                     if (c < cols) store4(args, (outRow + r) * args.n + col0 + c, loop.acc[i][j], umin(4u, cols - c));
                 }
@@ -428,14 +480,14 @@ __global__ void __launch_bounds__(128 * WY, 2) ragged_tile_kernel(const RaggedAr
                 if constexpr (DT == DT_F8) {
                     if (args.nPeers && r < rows) {
 #pragma unroll
-                        for (uint32_t j = 0; j < 4u; ++j) {
+                        for (uint32_t j = 0; j < NJ; ++j) {
                             const uint32_t c = wc + 16u * j + result_col((lane >> 4) * 4u);
                             if (c < cols) add_peers4(args, row0 + r, col0 + c, loop.acc[i][j], umin(4u, cols - c));
                         }
                     }
                 }
 #pragma unroll
-                for (uint32_t j = 0; j < 4u; j += 2u) {   // lanes 0-31: block j, lanes 32-63: block j + 1, eight columns each
+                for (uint32_t j = 0; j < NJ; j += 2u) {   // lanes 0-31: block j, lanes 32-63: block j + 1, eight columns each
                     const v4f a = loop.acc[i][j], b = loop.acc[i][j + 1u];
                     const auto lo = __builtin_amdgcn_permlane32_swap(round2(a[0], a[1], args.outType), round2(b[0], b[1], args.outType), false, false);
                     const auto hi = __builtin_amdgcn_permlane32_swap(round2(a[2], a[3], args.outType), round2(b[2], b[3], args.outType), false, false);

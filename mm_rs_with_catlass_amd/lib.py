@@ -60,6 +60,10 @@ class CatcocLaunchInfo(C.Structure):
     _fields_ = [(n, C.c_uint32) for n in ("kernel", "tileRows", "tileCols", "kSlices", "dealt", "largeTiles")]
 
 
+class CatcocTile(C.Structure):
+    _fields_ = [(n, C.c_uint32) for n in ("rows", "cols", "teams")]
+
+
 _DESC = struct.Struct("=11I4x%dQqq7Q" % MAX_RANKS)   # CatcocSymmetricDesc's fields in order
 assert _DESC.size == C.sizeof(CatcocSymmetricDesc)
 _NO_PEERS = (0,) * MAX_RANKS
@@ -213,10 +217,10 @@ def load():
     L.catcoc_pipelined_round_count.argtypes = [C.c_int, C.POINTER(CocTilingParams), C.POINTER(CatcocSymmetricDesc)]
     L.catcoc_pipelined_round_count.restype = u32
     L.catcoc_quantize_fp8.argtypes = [vp] * 4 + [u32] * 5
-    L.catcoc_fp8_matmul_allreduce.argtypes = [vp] * 7 + [u32] * 4
-    L.catcoc_grouped_matmul.argtypes = [vp, u32] + [vp] * 4 + [u32] * 5
-    L.catcoc_grouped_matmul_dw.argtypes = [vp, u32] + [vp] * 4 + [u32] * 6
-    L.catcoc_grouped_fp8_matmul.argtypes = [vp] * 7 + [u32] * 5
+    L.catcoc_fp8_matmul_allreduce.argtypes = [vp] * 7 + [u32] * 4 + [vp]
+    L.catcoc_grouped_matmul.argtypes = [vp, u32] + [vp] * 4 + [u32] * 5 + [vp]
+    L.catcoc_grouped_matmul_dw.argtypes = [vp, u32] + [vp] * 4 + [u32] * 6 + [vp]
+    L.catcoc_grouped_fp8_matmul.argtypes = [vp] * 7 + [u32] * 5 + [vp]
     for n in ("catcoc_quantize_fp8", "catcoc_fp8_matmul_allreduce", "catcoc_grouped_matmul", "catcoc_grouped_matmul_dw", "catcoc_grouped_fp8_matmul"):
         getattr(L, n).restype = None
     _lib = L

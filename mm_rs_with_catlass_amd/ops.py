@@ -557,6 +557,11 @@ def _type16(dtype, name):
     return _TORCH_TO_DT[dtype]
 
 
+def _tile(tile):
+    """(rows, cols, teams) of the kernel's tile (catcoc_hip.h says which exist), None: the library's choice."""
+    return None if tile is None else C.byref(_l.CatcocTile(*tile))
+
+
 def quantize_fp8(x, block_rows=1, gated=False, out=None, scale=None):
     """x [rows, cols] fp16, bf16 or fp32 -> (codes e4m3 [rows, cols], scale fp32) with x ~ code * scale (catcoc_quantize_fp8).
 
@@ -586,11 +591,12 @@ def quantize_fp8(x, block_rows=1, gated=False, out=None, scale=None):
     return out, scale
 
 
-def fp8_matmul_allreduce(x1, x2, scale_x1, scale_x2, peers=(), rank=0, rank_size=1, out_dtype=torch.bfloat16, peer_row_offset=0, out=None):
+def fp8_matmul_allreduce(x1, x2, scale_x1, scale_x2, peers=(), rank=0, rank_size=1, out_dtype=torch.bfloat16, peer_row_offset=0, out=None, tile=None):
     """e4m3 matmul -> all-reduce share with a scale for each block of 128 values of k (catcoc_fp8_matmul_allreduce).
 
     x1 [m,k] with scale_x1 [ceil(k/128), m], x2 [n,k] (a stored weight matrix) with scale_x2 [ceil(n/128), ceil(k/128)], as quantize_fp8() makes them.
-    peers: rank_size-1 staged fp32 partials [m,n], added in list order; one rank: the plain product.  Returns [m,n] in out_dtype."""
+    peers: rank_size-1 staged fp32 partials [m,n], added in list order; one rank: the plain product.  tile: (rows, cols, teams) of the
+    kernel's tile, None = the library's choice.  Returns [m,n] in out_dtype."""
     _check_rank(rank, rank_size)
     _want(x1, "x1", torch.float8_e4m3fn, 2)
     _want(x2, "x2", torch.float8_e4m3fn, 2)
@@ -610,7 +616,7 @@ def fp8_matmul_allreduce(x1, x2, scale_x1, scale_x2, peers=(), rank=0, rank_size
         out = torch.empty((m, n), dtype=out_dtype, device=x1.device)
     d = _l.make_desc(rank, rank_size, ptrs, peer_ld, peer_row_offset) if rank_size > 1 else None
     _l.load().catcoc_fp8_matmul_allreduce(_stream(), x1.data_ptr(), x2.data_ptr(), scale_x1.data_ptr(), scale_x2.data_ptr(), out.data_ptr(),
-                                          None if d is None else C.addressof(d), m, n, k, dt)
+                                          None if d is None else C.addressof(d), m, n, k, dt, _tile(tile))
     _l.check()
     return out
 
@@ -621,7 +627,7 @@ def _want_groups(x, group_ends, groups):
         _fail("there must be at least one group")
 
 
-def grouped_matmul(x, w, group_ends, trans_b=False, out=None):
+def grouped_matmul(x, w, group_ends, trans_b=False, out=None, tile=None):
     """Rows in groups, one matrix for each group (catcoc_grouped_matmul): out[i] = x[i] @ w[e] for the rows i of group e.
 
     x [rows,k] fp16 or bf16, sorted by group; w [groups,k,n] ([groups,n,k] with trans_b); group_ends [groups] int32 on the GPU: group e is rows
@@ -639,12 +645,12 @@ def grouped_matmul(x, w, group_ends, trans_b=False, out=None):
     _check_dev(x, w, group_ends, *(() if out is None else (out,)))
     if out is None:
         out = torch.empty((rows, n), dtype=x.dtype, device=x.device)
-    _l.load().catcoc_grouped_matmul(_stream(), dt, x.data_ptr(), w.data_ptr(), group_ends.data_ptr(), out.data_ptr(), rows, n, k, groups, int(trans_b))
+    _l.load().catcoc_grouped_matmul(_stream(), dt, x.data_ptr(), w.data_ptr(), group_ends.data_ptr(), out.data_ptr(), rows, n, k, groups, int(trans_b), _tile(tile))
     _l.check()
     return out
 
 
-def grouped_matmul_dw(x, dy, group_ends, out_dtype=None, trans_b=False, out=None):
+def grouped_matmul_dw(x, dy, group_ends, out_dtype=None, trans_b=False, out=None, tile=None):
     """The weight gradient of grouped_matmul (catcoc_grouped_matmul_dw): [groups,k,n] ([groups,n,k] with trans_b), out_dtype fp16, bf16 or fp32
     (None: x's type); groups without rows get zeros."""
     _want(x, "x", None, 2)
@@ -663,12 +669,12 @@ def grouped_matmul_dw(x, dy, group_ends, out_dtype=None, trans_b=False, out=None
     _check_dev(x, dy, group_ends, *(() if out is None else (out,)))
     if out is None:
         out = torch.empty(shape, dtype=od, device=x.device)
-    _l.load().catcoc_grouped_matmul_dw(_stream(), dt, x.data_ptr(), dy.data_ptr(), group_ends.data_ptr(), out.data_ptr(), rows, n, k, groups, int(trans_b), odt)
+    _l.load().catcoc_grouped_matmul_dw(_stream(), dt, x.data_ptr(), dy.data_ptr(), group_ends.data_ptr(), out.data_ptr(), rows, n, k, groups, int(trans_b), odt, _tile(tile))
     _l.check()
     return out
 
 
-def grouped_fp8_matmul(x, w, scale_x, scale_w, group_ends, out_dtype=torch.bfloat16, out=None):
+def grouped_fp8_matmul(x, w, scale_x, scale_w, group_ends, out_dtype=torch.bfloat16, out=None, tile=None):
     """grouped_matmul on e4m3 (catcoc_grouped_fp8_matmul): x [rows,k] with scale_x [ceil(k/128), rows], w [groups,n,k] with
     scale_w [groups, ceil(n/128), ceil(k/128)].  Returns [rows,n] in out_dtype."""
     _want(x, "x", torch.float8_e4m3fn, 2)
@@ -686,7 +692,7 @@ def grouped_fp8_matmul(x, w, scale_x, scale_w, group_ends, out_dtype=torch.bfloa
     if out is None:
         out = torch.empty((rows, n), dtype=out_dtype, device=x.device)
     _l.load().catcoc_grouped_fp8_matmul(_stream(), x.data_ptr(), w.data_ptr(), scale_x.data_ptr(), scale_w.data_ptr(), group_ends.data_ptr(), out.data_ptr(),
-                                        rows, n, k, groups, dt)
+                                        rows, n, k, groups, dt, _tile(tile))
     _l.check()
     return out
 

@@ -391,48 +391,113 @@ def test_calls_say_what_they_ran():
     assert (info.kernel, info.tileRows, info.tileCols) == (L.KERNEL_RAGGED_CHECKED, 64, 64)
 
 
-LARGE = {"uneven": [513, 0, 31, 900, 260, 1], "one_group": [1300], "full": [512, 256]}
+TILES = [(256, 256, 1), (128, 128, 1), (128, 128, 2), (64, 128, 2), (64, 64, 1)]
+SMALL_NK, SMALL_KN = [(16, 32, 4), (32, 32, 4)], [(16, 64, 4), (32, 64, 4), (64, 64, 4)]
+UNEVEN = {"large": [513, 0, 31, 900, 260, 1], "one_group": [1300], "full": [512, 256], "few": [1, 0, 15, 16, 17, 0, 40, 70, 129], "many": [(5 * i) % 23 for i in range(75)]}
 
 
-@pytest.mark.parametrize("name", sorted(LARGE))
-@pytest.mark.parametrize("k,n", [(1024, 512), (1096, 776), (514, 1030), (66, 2)])
-@pytest.mark.parametrize("trans_b", [False, True])
-def test_large_tiles(name, k, n, trans_b):
-    counts = LARGE[name]
+def ran(tile):
+    info = L.last_launch()
+    return (info.tileRows, info.tileCols, info.kSlices) == tile and info.kernel == (L.KERNEL_RAGGED_CHECKED if tile == (64, 64, 1) else L.KERNEL_RAGGED)
+
+
+@pytest.mark.parametrize("name", sorted(UNEVEN))
+@pytest.mark.parametrize("k,n", [(1024, 512), (1096, 776), (514, 1030), (66, 2), (64, 128), (192, 250), (2050, 130)])
+@pytest.mark.parametrize("tile,trans_b", [(t, b) for b in (False, True) for t in TILES + (SMALL_NK if b else SMALL_KN)])
+def test_every_tile_of_grouped_products(name, k, n, tile, trans_b):
+    counts = UNEVEN[name]
     g = gen(k * n)
     rows, groups = sum(counts), len(counts)
     ends = ends_of(counts)
-    x, dy = randn(g, rows + 40, k, dtype=torch.bfloat16), randn(g, rows + 40, n, dtype=torch.bfloat16)
-    x[rows:], dy[rows:] = float("nan"), float("nan")
+    x = randn(g, rows + 40, k, dtype=torch.bfloat16)
+    x[rows:] = float("nan")
     w = randn(g, groups, n, k, dtype=torch.bfloat16) if trans_b else randn(g, groups, k, n, dtype=torch.bfloat16)
-    out = ops.grouped_matmul(x, w, ends, trans_b=trans_b)
-    assert (L.last_launch().kernel, L.last_launch().tileRows) == (L.KERNEL_RAGGED, 256)
-    dw = ops.grouped_matmul_dw(x, dy, ends, out_dtype=torch.float32, trans_b=trans_b)
-    assert (L.last_launch().kernel, L.last_launch().tileRows) == (L.KERNEL_RAGGED, 256)
-    half = ops.grouped_matmul_dw(x, dy, ends, out_dtype=torch.float16, trans_b=trans_b)
+    out = ops.grouped_matmul(x, w, ends, trans_b=trans_b, tile=tile)
+    assert ran(tile)
     for e, (i, j) in enumerate(ranges(counts)):
-        a, b, d = x[i:j].double(), w[e].double(), dy[i:j].double()
+        a, b = x[i:j].double(), w[e].double()
         b = b.t() if trans_b else b
         close(out[i:j], a @ b, a.abs() @ b.abs(), k, torch.bfloat16)
-        want, mag = a.t() @ d, a.abs().t() @ d.abs()
-        close(dw[e].t() if trans_b else dw[e], want, mag, j - i, torch.float32)
-        close(half[e].t() if trans_b else half[e], want, mag, j - i, torch.float16)
     assert (out[rows:] == 0).all()
 
 
-@pytest.mark.parametrize("name", sorted(LARGE))
-@pytest.mark.parametrize("k,n", [(1024, 512), (1100, 777), (516, 1030), (132, 3)])
-def test_large_fp8_tiles(name, k, n):
-    counts = LARGE[name]
+@pytest.mark.parametrize("name", sorted(UNEVEN))
+@pytest.mark.parametrize("k,n", [(1024, 512), (1096, 776), (514, 1030), (66, 2), (256, 130)])
+@pytest.mark.parametrize("tile", [(256, 256, 1), (128, 128, 1), (64, 64, 1)])
+@pytest.mark.parametrize("out_dtype", [torch.float32, torch.float16])
+def test_every_tile_of_weight_gradients(name, k, n, tile, out_dtype):
+    counts = UNEVEN[name]
+    g = gen(k * n + 2)
+    rows = sum(counts)
+    ends = ends_of(counts)
+    x, dy = randn(g, rows + 40, k, dtype=torch.bfloat16), randn(g, rows + 40, n, dtype=torch.bfloat16)
+    x[rows:], dy[rows:] = float("nan"), float("nan")
+    for trans_b in (False, True):
+        dw = ops.grouped_matmul_dw(x, dy, ends, out_dtype=out_dtype, trans_b=trans_b, tile=tile)
+        assert ran(tile)
+        for e, (i, j) in enumerate(ranges(counts)):
+            a, d = x[i:j].double(), dy[i:j].double()
+            close(dw[e].t() if trans_b else dw[e], a.t() @ d, a.abs().t() @ d.abs(), j - i, out_dtype)
+
+
+@pytest.mark.parametrize("name", sorted(UNEVEN))
+@pytest.mark.parametrize("k,n", [(1024, 512), (1100, 777), (516, 1030), (132, 3), (128, 128), (260, 250), (4, 100)])
+@pytest.mark.parametrize("tile", TILES + SMALL_NK)
+def test_every_tile_of_fp8_products(name, k, n, tile):
+    counts = UNEVEN[name]
     g = gen(k * n + 1)
     rows, groups = sum(counts), len(counts)
     x, sx = fp8_operand(g, rows + 3, k, 1)
     sx *= 0.05 / 60
     w = (randn(g, groups, n, k) * 60).clamp(-448, 448).to(F8)
     sw = torch.rand((groups, blocks(n), blocks(k)), device=DEV, generator=g) + 0.5
-    out = ops.grouped_fp8_matmul(x, w, sx, sw, ends_of(counts))
-    assert (L.last_launch().kernel, L.last_launch().tileRows) == (L.KERNEL_RAGGED, 256)
+    out = ops.grouped_fp8_matmul(x, w, sx, sw, ends_of(counts), tile=tile)
+    assert ran(tile)
     for e, (i, j) in enumerate(ranges(counts)):
         a, b = x[i:j].double() * spread(sx[:, i:j].t(), j - i, k, 1), w[e].double() * spread(sw[e], n, k, 128)
         close(out[i:j], a @ b.t(), a.abs() @ b.abs().t(), k, torch.bfloat16, norm2(a, b))
     assert (out[rows:] == 0).all()
+
+
+@pytest.mark.parametrize("m,k,n", [(300, 1000, 390), (33, 384, 130), (1, 4100, 260), (129, 132, 65)])
+@pytest.mark.parametrize("tile", TILES + SMALL_NK)
+def test_every_tile_adds_its_peers(m, k, n, tile):
+    g = gen(m * k)
+    x, sx = fp8_operand(g, m, k, 1)
+    w, sw = fp8_operand(g, n, k, 128)
+    sx *= 0.05 / 60
+    peers = [randn(g, m, n) for _ in range(9)]
+    out = ops.fp8_matmul_allreduce(x, w, sx, sw, peers, rank=3, rank_size=10, out_dtype=torch.float16, tile=tile)
+    assert ran(tile)
+    a, b = x.double() * spread(sx.t(), m, k, 1), w.double() * spread(sw, n, k, 128)
+    want, mag = a @ b.t(), a.abs() @ b.abs().t()
+    for p in peers:
+        want, mag = want + p.double(), mag + p.double().abs()
+    close(out, want, mag, k + 10, torch.float16, norm2(a, b))
+
+
+@pytest.mark.parametrize("rows,groups,k,n", [(64, 64, 512, 512), (512, 8, 512, 512), (1024, 8, 512, 2048), (4096, 8, 512, 2048), (4096, 2, 256, 8192), (16384, 4, 128, 4096), (300, 4, 509, 640)])
+def test_the_choice_of_tiles_changes_no_more_than_the_order_of_sums(rows, groups, k, n):
+    g = gen(rows + k)
+    ends = ends_of([rows // groups] * groups)
+    x, w = randn(g, rows, k, dtype=torch.bfloat16), randn(g, groups, n, k, dtype=torch.bfloat16)
+    out = ops.grouped_matmul(x, w, ends, trans_b=True)
+    same = ops.grouped_matmul(x, w, ends, trans_b=True, tile=(64, 64, 1))
+    e = 1 % groups
+    i = slice(e * (rows // groups), e * (rows // groups) + min(7, rows // groups))
+    a, b = x[i].double(), w[e].double().t()
+    close(out[i], a @ b, a.abs() @ b.abs(), k, torch.bfloat16)
+    assert ((out.double() - same.double()).abs() <= 2.0 ** -7 * same.double().abs() + 1e-3).all()
+
+
+def test_tiles_that_do_not_exist_are_refused():
+    x, w, ends = torch.ones((8, 64), dtype=torch.bfloat16, device=DEV), torch.ones((2, 64, 32), dtype=torch.bfloat16, device=DEV), ends_of([3, 5])
+    dy = torch.ones((8, 32), dtype=torch.bfloat16, device=DEV)
+    for call in (lambda t: ops.grouped_matmul(x, w, ends, tile=t), lambda t: ops.grouped_matmul_dw(x, dy, ends, tile=t)):
+        for t in ((256, 128, 1), (16, 32, 4), (1, 1, 1), (64, 64, 2)):
+            with pytest.raises(L.CatcocError, match="no kernel of"):
+                call(t)
+    with pytest.raises(L.CatcocError, match="do not start on 4 bytes"):
+        ops.grouped_matmul(x[:, :63].contiguous(), w[:, :63].contiguous(), ends, tile=(128, 128, 1))
+    with pytest.raises(L.CatcocError, match="no kernel of"):
+        ops.grouped_matmul_dw(x, dy, ends, tile=(128, 128, 2))

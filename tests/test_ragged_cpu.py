@@ -94,22 +94,23 @@ def test_c_abi_refuses():
     says("non-NULL", so.catcoc_quantize_fp8, 16, None, 16, 4, 128, 1, 0, L.BF16)
     says("empty problem", so.catcoc_quantize_fp8, 16, 16, 16, 4, 0, 1, 0, L.BF16)
     f = so.catcoc_fp8_matmul_allreduce
-    says("outDataType", f, 16, 16, 16, 16, 16, None, 4, 4, 4, L.INT8)
-    says("must be below", f, 16, 16, 16, 16, 16, None, 4, 1 << 22, 4, L.BF16)
-    says("non-NULL", f, 16, 16, 16, None, 16, None, 4, 4, 4, L.BF16)
+    says("outDataType", f, 16, 16, 16, 16, 16, None, 4, 4, 4, L.INT8, None)
+    says("must be below", f, 16, 16, 16, 16, 16, None, 4, 1 << 22, 4, L.BF16, None)
+    says("non-NULL", f, 16, 16, 16, None, 16, None, 4, 4, 4, L.BF16, None)
     d = L.make_desc(0, 3, [16])
     d.peerLd = 4
-    says("peers[1] is NULL", f, 16, 16, 16, 16, 16, C.addressof(d), 4, 4, 4, L.BF16)
+    says("peers[1] is NULL", f, 16, 16, 16, 16, 16, C.addressof(d), 4, 4, 4, L.BF16, None)
     d.magic = 0
-    says("bad magic", f, 16, 16, 16, 16, 16, C.addressof(d), 4, 4, 4, L.BF16)
+    says("bad magic", f, 16, 16, 16, 16, 16, C.addressof(d), 4, 4, 4, L.BF16, None)
     g = so.catcoc_grouped_matmul
     for match, a in [("dataType", (L.INT8, 16, 16, 16, 16, 4, 4, 4, 2, 0)), ("groups out of range", (L.BF16, 16, 16, 16, 16, 4, 4, 4, 0, 0)),
                      ("non-NULL", (L.BF16, 16, 16, None, 16, 4, 4, 4, 2, 0)), ("empty problem", (L.BF16, 16, 16, 16, 16, 4, 0, 4, 2, 0)),
                      ("rows", (L.BF16, 16, 16, 16, 16, 1 << 31, 4, 4, 2, 0))]:
-        says(match, g, *a)
-    says("outDataType", so.catcoc_grouped_matmul_dw, L.BF16, 16, 16, 16, 16, 4, 4, 4, 2, 0, L.INT8)
-    says("non-NULL", so.catcoc_grouped_matmul_dw, L.BF16, 16, 16, 16, None, 4, 4, 4, 2, 0, 0)
-    says("non-NULL", so.catcoc_grouped_fp8_matmul, 16, 16, 16, 16, 16, None, 4, 4, 4, 2, L.BF16)
+        says(match, g, *a, None)
+    says("outDataType", so.catcoc_grouped_matmul_dw, L.BF16, 16, 16, 16, 16, 4, 4, 4, 2, 0, L.INT8, None)
+    says("non-NULL", so.catcoc_grouped_matmul_dw, L.BF16, 16, 16, 16, None, 4, 4, 4, 2, 0, 0, None)
+    says("non-NULL", so.catcoc_grouped_fp8_matmul, 16, 16, 16, 16, 16, None, 4, 4, 4, 2, L.BF16, None)
+    says("no kernel of 48x48", g, L.BF16, 16, 16, 16, 16, 4, 4, 4, 2, 0, C.byref(L.CatcocTile(48, 48, 1)))
     # no rows: accepted, nothing launched
-    g(None, L.BF16, None, None, None, None, 0, 4, 4, 2, 0)
+    g(None, L.BF16, None, None, None, None, 0, 4, 4, 2, 0, None)
     assert so.catcoc_last_status() == 0
