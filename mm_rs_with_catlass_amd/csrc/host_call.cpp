@@ -230,7 +230,235 @@ PyObject *call(PyObject *, PyObject *const *v, Py_ssize_t n)
     Py_RETURN_NONE;
 }
 
-PyMethodDef methods[] = {{"attach", (PyCFunction)(void *)attach, METH_FASTCALL, "addresses of the library's functions, CatcocError, CocTilingParams"},
+// ---- e4m3 and grouped operators: quantize_fp8() and its like below, of the same kind as call().
+decltype(&catcoc_quantize_fp8) quantizeFp8;
+decltype(&catcoc_fp8_matmul_allreduce) fp8Matmul;
+decltype(&catcoc_grouped_matmul) groupedMatmul;
+decltype(&catcoc_grouped_matmul_dw) groupedDw;
+decltype(&catcoc_grouped_fp8_matmul) groupedFp8;
+
+PyObject *attachRagged(PyObject *, PyObject *const *v, Py_ssize_t n)
+{
+    if (n != 5) return PyErr_Format(PyExc_TypeError, "attach_ragged takes five addresses");
+    void *p[5];
+    for (int i = 0; i < 5; ++i) {
+        p[i] = PyLong_AsVoidPtr(v[i]);
+        if (p[i] == nullptr) return PyErr_Occurred() ? nullptr : PyErr_Format(PyExc_ValueError, "address %d is null", i);
+    }
+    quantizeFp8 = (decltype(quantizeFp8))p[0];
+    fp8Matmul = (decltype(fp8Matmul))p[1];
+    groupedMatmul = (decltype(groupedMatmul))p[2];
+    groupedDw = (decltype(groupedDw))p[3];
+    groupedFp8 = (decltype(groupedFp8))p[4];
+    Py_RETURN_NONE;
+}
+
+constexpr int64_t BLOCK = 128, MOST = 0x7fffffff;
+constexpr at::ScalarType F8 = at::ScalarType::Float8_e4m3fn;
+
+int64_t blocks(int64_t n) { return (n + BLOCK - 1) / BLOCK; }
+
+// A tensor of exactly this shape, or, None, a new one.
+struct Result {
+    at::Tensor made;
+    const at::Tensor *t = &made;
+    PyObject *given = nullptr;
+
+    Result(PyObject *o, at::ScalarType type, at::IntArrayRef shape, const at::Tensor &like)
+    {
+        if (o == Py_None) {
+            made = at::empty(shape, like.options().dtype(type));
+            return;
+        }
+        t = &tensor(o, type, (int64_t)shape.size());
+        if (t->sizes() != shape) throw Other{};
+        given = o;
+    }
+    Result(const Result &) = delete;
+    uint8_t *at_() { return address(*t); }
+    PyObject *object()
+    {
+        if (given == nullptr) return THPVariable_Wrap(std::move(made));
+        Py_INCREF(given);
+        return given;
+    }
+};
+
+const at::Tensor &shaped(PyObject *o, at::ScalarType type, at::IntArrayRef shape)
+{
+    const at::Tensor &t = tensor(o, type, (int64_t)shape.size());
+    if (t.sizes() != shape) throw Other{};
+    return t;
+}
+
+uint32_t code(at::ScalarType t, bool floats = false)
+{
+    if (t == at::kHalf) return FP16;
+    if (t == at::kBFloat16) return BF16;
+    if (floats && t == at::kFloat) return 0;
+    throw Other{};
+}
+
+// The type of a result: that of `out`, else what is asked for.
+at::ScalarType resultType(PyObject *out, PyObject *dtype)
+{
+    if (out != Py_None) return THPVariable_CheckExact(out) ? THPVariable_Unpack(out).scalar_type() : throw Other{};
+    if (!THPDtype_Check(dtype)) throw Other{};
+    return ((THPDtype *)dtype)->scalar_type;
+}
+
+void *stream() { return (void *)c10::hip::getCurrentHIPStream().stream(); }
+
+template <typename F>
+PyObject *guarded(const char *name, Py_ssize_t n, Py_ssize_t wanted, F &&body)
+{
+    if (n != wanted || errorType == nullptr || groupedFp8 == nullptr) return PyErr_Format(PyExc_TypeError, "%s takes %zd arguments, after attach and attach_ragged", name, wanted);
+    try {
+        return body();
+    } catch (const Other &) {
+    } catch (const std::exception &) {
+        PyErr_Clear();
+    }
+    Py_RETURN_NONE;
+}
+
+// What the library answered: false where it refused (the error is set).
+bool accepted()
+{
+    if (lastStatus() == 0) return true;
+    PyErr_SetString(errorType, lastError());
+    return false;
+}
+
+PyObject *quantize(PyObject *, PyObject *const *v, Py_ssize_t n)   // x, block_rows, gated, out, scale
+{
+    return guarded("quantize_fp8", n, 5, [&]() -> PyObject * {
+        const at::Tensor &x = tensor(v[0], at::ScalarType::Undefined, 2);
+        const uint32_t type = code(x.scalar_type(), true);
+        const int64_t blockRows = number(v[1], BLOCK);
+        const bool gated = number(v[2], 1) != 0;
+        const int64_t rows = x.size(0), cols = gated ? x.size(1) / 2 : x.size(1);
+        if ((blockRows != 1 && blockRows != BLOCK) || (gated && (blockRows != 1 || x.size(1) % 2 != 0)) || rows > MOST || cols > MOST) throw Other{};
+        Result q(v[3], F8, {rows, cols}, x);
+        Result scale(v[4], at::kFloat, blockRows == 1 ? at::IntArrayRef({blocks(cols), rows}) : at::IntArrayRef({blocks(rows), blocks(cols)}), x);
+        uint8_t *const px = address(x), *const pq = q.at_();
+        float *const ps = (float *)scale.at_();
+        void *const s = stream();
+        Py_BEGIN_ALLOW_THREADS
+        quantizeFp8(s, px, pq, ps, (uint32_t)rows, (uint32_t)cols, (uint32_t)blockRows, gated, type);
+        Py_END_ALLOW_THREADS
+        if (!accepted()) return nullptr;
+        PyObject *a = q.object(), *b = scale.object(), *both = a && b ? PyTuple_Pack(2, a, b) : nullptr;
+        Py_XDECREF(a);
+        Py_XDECREF(b);
+        return both;
+    });
+}
+
+PyObject *fp8(PyObject *, PyObject *const *v, Py_ssize_t n)   // x1, x2, scale_x1, scale_x2, peers, rank, rank_size, out_dtype, peer_row_offset, out
+{
+    return guarded("fp8_matmul_allreduce", n, 10, [&]() -> PyObject * {
+        const at::Tensor &x = tensor(v[0], F8, 2), &w = tensor(v[1], F8, 2);
+        const int64_t m = x.size(0), k = x.size(1), cols = w.size(0);
+        if (w.size(1) != k || m > MOST || k > MOST || cols > MOST) throw Other{};
+        const at::Tensor &sx = shaped(v[2], at::kFloat, {blocks(k), m}), &sw = shaped(v[3], at::kFloat, {blocks(cols), blocks(k)});
+        const int64_t P = number(v[6], CATCOC_MAX_RANKS), rank = number(v[5], P - 1), peerRow = number(v[8], MOST);
+        const bool list = PyList_CheckExact(v[4]);
+        if ((!list && !PyTuple_CheckExact(v[4])) || (list ? PyList_GET_SIZE(v[4]) : PyTuple_GET_SIZE(v[4])) != P - 1) throw Other{};
+        CatcocSymmetricDesc d{};
+        d.magic = CATCOC_DESC_MAGIC;
+        d.rankIdx = (uint32_t)rank;
+        d.rankSize = (uint32_t)P;
+        d.peerRowOffset = peerRow;
+        for (Py_ssize_t i = 0; i < P - 1; ++i) {
+            const at::Tensor &p = tensor(list ? PyList_GET_ITEM(v[4], i) : PyTuple_GET_ITEM(v[4], i), at::kFloat, 2);
+            if (p.size(0) < peerRow + m || p.size(1) < cols || (i && p.size(1) != d.peerLd)) throw Other{};
+            d.peers[i] = address(p);
+            d.peerLd = p.size(1);
+        }
+        const at::ScalarType type = resultType(v[9], v[7]);
+        const uint32_t outType = code(type);
+        Result out(v[9], type, {m, cols}, x);
+        uint8_t *const px = address(x), *const pw = address(w), *const po = out.at_();
+        const float *const psx = (const float *)address(sx), *const psw = (const float *)address(sw);
+        void *const s = stream();
+        Py_BEGIN_ALLOW_THREADS
+        fp8Matmul(s, px, pw, psx, psw, po, (uint8_t *)&d, (uint32_t)m, (uint32_t)cols, (uint32_t)k, outType, nullptr);
+        Py_END_ALLOW_THREADS
+        return accepted() ? out.object() : nullptr;
+    });
+}
+
+PyObject *grouped(PyObject *, PyObject *const *v, Py_ssize_t n)   // x, w, group_ends, trans_b, out
+{
+    return guarded("grouped_matmul", n, 5, [&]() -> PyObject * {
+        const at::Tensor &x = tensor(v[0], at::ScalarType::Undefined, 2);
+        const uint32_t type = code(x.scalar_type());
+        const at::Tensor &w = tensor(v[1], x.scalar_type(), 3);
+        const bool transB = number(v[3], 1) != 0;
+        const int64_t rows = x.size(0), k = x.size(1), groups = w.size(0), cols = w.size(transB ? 1 : 2);
+        if (w.size(transB ? 2 : 1) != k || rows > MOST || k > MOST || cols > MOST || groups < 1 || groups > MOST) throw Other{};
+        const int32_t *const ends = (const int32_t *)address(shaped(v[2], at::kInt, {groups}));
+        Result out(v[4], x.scalar_type(), {rows, cols}, x);
+        uint8_t *const px = address(x), *const pw = address(w), *const po = out.at_();
+        void *const s = stream();
+        Py_BEGIN_ALLOW_THREADS
+        groupedMatmul(s, type, px, pw, ends, po, (uint32_t)rows, (uint32_t)cols, (uint32_t)k, (uint32_t)groups, transB, nullptr);
+        Py_END_ALLOW_THREADS
+        return accepted() ? out.object() : nullptr;
+    });
+}
+
+PyObject *dw(PyObject *, PyObject *const *v, Py_ssize_t n)   // x, dy, group_ends, out_dtype, trans_b, out
+{
+    return guarded("grouped_matmul_dw", n, 6, [&]() -> PyObject * {
+        const at::Tensor &x = tensor(v[0], at::ScalarType::Undefined, 2);
+        const uint32_t type = code(x.scalar_type());
+        const at::Tensor &dy = tensor(v[1], x.scalar_type(), 2), &e = tensor(v[2], at::kInt, 1);
+        const bool transB = number(v[4], 1) != 0;
+        const int64_t rows = x.size(0), k = x.size(1), groups = e.size(0), cols = dy.size(1);
+        if (dy.size(0) != rows || rows > MOST || k > MOST || cols > MOST || groups < 1 || groups > MOST) throw Other{};
+        const at::ScalarType made = v[5] == Py_None && v[3] == Py_None ? x.scalar_type() : resultType(v[5], v[3]);
+        const uint32_t outType = code(made, true);
+        Result out(v[5], made, transB ? at::IntArrayRef({groups, cols, k}) : at::IntArrayRef({groups, k, cols}), x);
+        uint8_t *const px = address(x), *const pd = address(dy), *const po = out.at_();
+        const int32_t *const ends = (const int32_t *)address(e);
+        void *const s = stream();
+        Py_BEGIN_ALLOW_THREADS
+        groupedDw(s, type, px, pd, ends, po, (uint32_t)rows, (uint32_t)cols, (uint32_t)k, (uint32_t)groups, transB, outType, nullptr);
+        Py_END_ALLOW_THREADS
+        return accepted() ? out.object() : nullptr;
+    });
+}
+
+PyObject *fp8Grouped(PyObject *, PyObject *const *v, Py_ssize_t n)   // x, w, scale_x, scale_w, group_ends, out_dtype, out
+{
+    return guarded("grouped_fp8_matmul", n, 7, [&]() -> PyObject * {
+        const at::Tensor &x = tensor(v[0], F8, 2), &w = tensor(v[1], F8, 3);
+        const int64_t rows = x.size(0), k = x.size(1), groups = w.size(0), cols = w.size(1);
+        if (w.size(2) != k || rows > MOST || k > MOST || cols > MOST || groups < 1 || groups > MOST) throw Other{};
+        const at::Tensor &sx = shaped(v[2], at::kFloat, {blocks(k), rows}), &sw = shaped(v[3], at::kFloat, {groups, blocks(cols), blocks(k)});
+        const int32_t *const ends = (const int32_t *)address(shaped(v[4], at::kInt, {groups}));
+        const at::ScalarType type = resultType(v[6], v[5]);
+        const uint32_t outType = code(type);
+        Result out(v[6], type, {rows, cols}, x);
+        uint8_t *const px = address(x), *const pw = address(w), *const po = out.at_();
+        const float *const psx = (const float *)address(sx), *const psw = (const float *)address(sw);
+        void *const s = stream();
+        Py_BEGIN_ALLOW_THREADS
+        groupedFp8(s, px, pw, psx, psw, ends, po, (uint32_t)rows, (uint32_t)cols, (uint32_t)k, (uint32_t)groups, outType, nullptr);
+        Py_END_ALLOW_THREADS
+        return accepted() ? out.object() : nullptr;
+    });
+}
+
+PyMethodDef methods[] = {{"attach_ragged", (PyCFunction)(void *)attachRagged, METH_FASTCALL, "addresses of the e4m3 and grouped operators' functions"},
+                         {"quantize_fp8", (PyCFunction)(void *)quantize, METH_FASTCALL, "one call: (codes, scale), or None for the Python path"},
+                         {"fp8_matmul_allreduce", (PyCFunction)(void *)fp8, METH_FASTCALL, "one call: the output, or None for the Python path"},
+                         {"grouped_matmul", (PyCFunction)(void *)grouped, METH_FASTCALL, "one call: the output, or None for the Python path"},
+                         {"grouped_matmul_dw", (PyCFunction)(void *)dw, METH_FASTCALL, "one call: the output, or None for the Python path"},
+                         {"grouped_fp8_matmul", (PyCFunction)(void *)fp8Grouped, METH_FASTCALL, "one call: the output, or None for the Python path"},
+                         {"attach", (PyCFunction)(void *)attach, METH_FASTCALL, "addresses of the library's functions, CatcocError, CocTilingParams"},
                          {"call", (PyCFunction)(void *)call, METH_FASTCALL, "one operator call: the output, or None for the Python path"},
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_host", nullptr, -1, methods};

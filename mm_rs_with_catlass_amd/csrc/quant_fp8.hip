@@ -1,6 +1,9 @@
 // Quantizer: rows of 16- or 32-bit values to e4m3 with one fp32 scale per 128 values of a row, or per 128x128 block.
 //
-// scale = max(largest magnitude, 2^-40) / 448, code = value / scale rounded to nearest even: both divisions are the correctly rounded ones.
+// scale = max(largest magnitude, 2^-40) / 448, code = value / scale rounded to nearest even: both divisions are the correctly rounded ones.  A block's values share their
+// divisor, so a quotient takes three operations instead of a division's ten: with r the correctly rounded 1 / s, q = x r and the remainder
+// x - q s (exact in one fused operation), fma(remainder, r, q) is the correctly rounded x / s (Markstein, IBM J. Res. Dev. 34, 1990).  It needs a remainder that is
+// representable, which the scale's floor sees to: a value whose code is not 0 is at least 2^-59.
 #include <hip/hip_runtime.h>
 
 #include "ragged.h"
@@ -56,7 +59,7 @@ __device__ __forceinline__ float silu_times(float g, float u)
     const float lo = __builtin_fmaf(-g, 1.44269504f, -hi) + -g * 1.92596299e-8f;   // (log2 e less its fp32 value)
     const float e = __builtin_amdgcn_exp2f(hi);
     const float p = __builtin_isinf(e) || __builtin_isinf(hi) ? e : __builtin_fmaf(e, lo * 0.693147181f, e);
-    return g / (1.f + p) * u;
+    return g * __builtin_amdgcn_rcpf(1.f + p) * u;
 }
 
 __device__ __forceinline__ uint32_t magnitude(float v) { return __builtin_bit_cast(uint32_t, v) & 0x7fffffffu; }   // (as an integer: a NaN is the largest)
@@ -70,8 +73,16 @@ __device__ __forceinline__ float scale_of(uint32_t top)
 __device__ __forceinline__ v2i codes8(const Eight &e, float scale)
 {
     float q[8];
+    const float r = 1.f / scale;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) q[i] = e.v[i] / scale;
+    for (int i = 0; i < 8; ++i) {
+        const float t = e.v[i] * r;
+        q[i] = __builtin_fmaf(__builtin_fmaf(-t, scale, e.v[i]), r, t);
+    }
+    if (!__builtin_isfinite(scale)) {   // (zeros and NaN)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) q[i] = e.v[i] / scale;
+    }
     int a = 0, b = 0;
     a = __builtin_amdgcn_cvt_pk_fp8_f32(q[0], q[1], a, false);
     a = __builtin_amdgcn_cvt_pk_fp8_f32(q[2], q[3], a, true);
@@ -104,31 +115,40 @@ __device__ __forceinline__ uint32_t max16(uint32_t v)
 
 }  // namespace
 
-// One scale per 128 values of a row: 16 lanes share a block, a wave takes the same block of four consecutive rows at a time.
-template <uint32_t DT, bool GATED>
+// One scale per 128 values of a row: 16 lanes share a block; a wave takes the same block of 4 QUADS consecutive rows, whose loads all go out first.
+template <uint32_t DT, bool GATED, int QUADS>
 __global__ void __launch_bounds__(256) quantize_rows_kernel(const QuantArgs args)
 {
     const uint32_t lane = threadIdx.x & 63u, blocks = (args.cols + kScaleBlock - 1u) / kScaleBlock;
-    const uint32_t quads = (args.rows + 3u) / 4u;
-    const uint64_t at = (uint64_t)blockIdx.x * 4u + (threadIdx.x >> 6);
-    if (at >= (uint64_t)quads * blocks) return;
-    const uint32_t quad = (uint32_t)(at / blocks), block = (uint32_t)(at - (uint64_t)quad * blocks);
-    const uint32_t row = 4u * quad + (lane >> 4), col = block * kScaleBlock + (lane & 15u) * 8u;
-    if (row >= args.rows) return;   // (whole groups of 16 lanes)
+    const uint32_t groups = (args.rows + 4u * QUADS - 1u) / (4u * QUADS);
+    const uint32_t at = blockIdx.x * 4u + (threadIdx.x >> 6);   // (fewer than 2^31 blocks of four rows, the host sees to it)
+    const uint32_t group = at / blocks, block = at - group * blocks;
+    if (group >= groups) return;
+    const uint32_t row0 = 4u * QUADS * group + (lane >> 4), col = block * kScaleBlock + (lane & 15u) * 8u;
     const uint32_t pitch = GATED ? 2u * args.cols : args.cols;
-    Eight e = load8<DT>(args.x, row, pitch, col, args.cols);
-    if constexpr (GATED) {
-        // (the upper half's values lie `cols` further on; where fewer than eight are left nothing is read)
-        const Eight u = load8<DT>((const unsigned char *)args.x + (size_t)args.cols * (DT == 0 ? 4u : 2u), row, pitch, col, args.cols);
+    // (the upper half's values lie `cols` further on; where fewer than eight are left nothing is read)
+    const void *const up = (const unsigned char *)args.x + (GATED ? (size_t)args.cols * (DT == 0 ? 4u : 2u) : (size_t)0);
+    Eight e[QUADS], u[GATED ? QUADS : 1];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) e.v[i] = silu_times(e.v[i], u.v[i]);
+    for (int j = 0; j < QUADS; ++j) {
+        const uint32_t row = umin(row0 + 4u * j, args.rows - 1u);   // (rows past the last one repeat it and are not stored)
+        e[j] = load8<DT>(args.x, row, pitch, col, args.cols);
+        if constexpr (GATED) u[j] = load8<DT>(up, row, pitch, col, args.cols);
     }
-    uint32_t top = 0;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) top = max(top, magnitude(e.v[i]));
-    const float scale = scale_of(max16(top));
-    if ((lane & 15u) == 0) args.scale[(size_t)block * args.rows + row] = scale;
-    if (col < args.cols) store8(args.q, row, args.cols, col, args.cols, codes8(e, scale));
+    for (int j = 0; j < QUADS; ++j) {
+        const uint32_t row = row0 + 4u * j;
+        uint32_t top = 0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            if constexpr (GATED) e[j].v[i] = silu_times(e[j].v[i], u[j].v[i]);
+            top = max(top, magnitude(e[j].v[i]));
+        }
+        const float scale = scale_of(max16(top));
+        if (row >= args.rows) continue;
+        if ((lane & 15u) == 0) args.scale[(size_t)block * args.rows + row] = scale;
+        if (col < args.cols) store8(args.q, row, args.cols, col, args.cols, codes8(e[j], scale));
+    }
 }
 
 // One scale per 128x128 block: a workgroup holds the block in registers.
@@ -167,9 +187,14 @@ static int launch_dt(const QuantArgs &a, bool blocks, bool gated, hipStream_t st
     if (blocks) {
         hipLaunchKernelGGL((quantize_blocks_kernel<DT>), dim3((uint32_t)((a.rows + kScaleBlock - 1u) / kScaleBlock * cb)), dim3(256), 0, stream, a);
     } else {
-        const dim3 grid((uint32_t)(((a.rows + 3ull) / 4u * cb + 3u) / 4u));
-        if (gated) hipLaunchKernelGGL((quantize_rows_kernel<DT, true>), grid, dim3(256), 0, stream, a);
-        else hipLaunchKernelGGL((quantize_rows_kernel<DT, false>), grid, dim3(256), 0, stream, a);
+        // four rows a wave where that leaves a CU fewer than 32 waves, else sixteen
+        const uint64_t fours = (a.rows + 3ull) / 4u * cb;
+        const bool many = fours >= 4u * 8192u;
+        const dim3 grid((uint32_t)(((many ? (a.rows + 15ull) / 16u * cb : fours) + 3u) / 4u));
+        if (gated && many) hipLaunchKernelGGL((quantize_rows_kernel<DT, true, 4>), grid, dim3(256), 0, stream, a);
+        else if (gated) hipLaunchKernelGGL((quantize_rows_kernel<DT, true, 1>), grid, dim3(256), 0, stream, a);
+        else if (many) hipLaunchKernelGGL((quantize_rows_kernel<DT, false, 4>), grid, dim3(256), 0, stream, a);
+        else hipLaunchKernelGGL((quantize_rows_kernel<DT, false, 1>), grid, dim3(256), 0, stream, a);
     }
     return (int)hipGetLastError();
 }

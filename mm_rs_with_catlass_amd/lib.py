@@ -237,6 +237,8 @@ def load_host():
     _host.attach(*(C.cast(getattr(L, n), C.c_void_p).value for n in (
         "catcoc_get_kernel", "catcoc_launch_quant_matmul_reduce_scatter", "catcoc_get_task_count", "catcoc_default_tiling", "catcoc_last_status", "catcoc_last_error")),
         CatcocError, CocTilingParams)
+    _host.attach_ragged(*(C.cast(getattr(L, n), C.c_void_p).value for n in (
+        "catcoc_quantize_fp8", "catcoc_fp8_matmul_allreduce", "catcoc_grouped_matmul", "catcoc_grouped_matmul_dw", "catcoc_grouped_fp8_matmul")))
     return _host
 
 

@@ -56,6 +56,15 @@ def _call(*args):
     return _call(*args)
 
 
+_host = None   # the module of csrc/host_call.cpp, whose functions of the e4m3 and grouped operators answer None where the code below them is meant
+
+
+def _compiled():
+    global _host
+    _host = _l.load_host()
+    return _host
+
+
 def _ptr(t):
     return None if t is None else t.data_ptr()
 
@@ -568,6 +577,9 @@ def quantize_fp8(x, block_rows=1, gated=False, out=None, scale=None):
     block_rows 1 (activations): a scale for each 128 values of a row, scale [ceil(cols/128), rows]; 128 (weights): for each
     128x128 block, scale [ceil(rows/128), ceil(cols/128)].  gated: x is [rows, 2 cols], gate and up beside each other, and
     silu(gate) * up is quantized.  out, scale: tensors for the results."""
+    done = (_host or _compiled()).quantize_fp8(x, block_rows, gated, out, scale)
+    if done is not None:
+        return done
     _want(x, "x", (torch.float16, torch.bfloat16, torch.float32), 2)
     if block_rows not in (1, SCALE_BLOCK):
         _fail("block_rows must be 1 or %d (got %s)", SCALE_BLOCK, block_rows)
@@ -597,6 +609,10 @@ def fp8_matmul_allreduce(x1, x2, scale_x1, scale_x2, peers=(), rank=0, rank_size
     x1 [m,k] with scale_x1 [ceil(k/128), m], x2 [n,k] (a stored weight matrix) with scale_x2 [ceil(n/128), ceil(k/128)], as quantize_fp8() makes them.
     peers: rank_size-1 staged fp32 partials [m,n], added in list order; one rank: the plain product.  tile: (rows, cols, teams) of the
     kernel's tile, None = the library's choice.  Returns [m,n] in out_dtype."""
+    if tile is None:
+        done = (_host or _compiled()).fp8_matmul_allreduce(x1, x2, scale_x1, scale_x2, peers, rank, rank_size, out_dtype, peer_row_offset, out)
+        if done is not None:
+            return done
     _check_rank(rank, rank_size)
     _want(x1, "x1", torch.float8_e4m3fn, 2)
     _want(x2, "x2", torch.float8_e4m3fn, 2)
@@ -633,6 +649,10 @@ def grouped_matmul(x, w, group_ends, trans_b=False, out=None, tile=None):
     x [rows,k] fp16 or bf16, sorted by group; w [groups,k,n] ([groups,n,k] with trans_b); group_ends [groups] int32 on the GPU: group e is rows
     [group_ends[e-1], group_ends[e]), any of them empty.  Rows past the last group come out as zeros.  Returns [rows,n].
     The gradient of x is grouped_matmul(dy, w, group_ends, trans_b=not trans_b), that of w grouped_matmul_dw()."""
+    if tile is None:
+        done = (_host or _compiled()).grouped_matmul(x, w, group_ends, trans_b, out)
+        if done is not None:
+            return done
     _want(x, "x", None, 2)
     dt = _type16(x.dtype, "x")
     _want(w, "w", x.dtype, 3)
@@ -653,6 +673,10 @@ def grouped_matmul(x, w, group_ends, trans_b=False, out=None, tile=None):
 def grouped_matmul_dw(x, dy, group_ends, out_dtype=None, trans_b=False, out=None, tile=None):
     """The weight gradient of grouped_matmul (catcoc_grouped_matmul_dw): [groups,k,n] ([groups,n,k] with trans_b), out_dtype fp16, bf16 or fp32
     (None: x's type); groups without rows get zeros."""
+    if tile is None:
+        done = (_host or _compiled()).grouped_matmul_dw(x, dy, group_ends, out_dtype, trans_b, out)
+        if done is not None:
+            return done
     _want(x, "x", None, 2)
     dt = _type16(x.dtype, "x")
     _want(dy, "dy", x.dtype, 2)
@@ -677,6 +701,10 @@ def grouped_matmul_dw(x, dy, group_ends, out_dtype=None, trans_b=False, out=None
 def grouped_fp8_matmul(x, w, scale_x, scale_w, group_ends, out_dtype=torch.bfloat16, out=None, tile=None):
     """grouped_matmul on e4m3 (catcoc_grouped_fp8_matmul): x [rows,k] with scale_x [ceil(k/128), rows], w [groups,n,k] with
     scale_w [groups, ceil(n/128), ceil(k/128)].  Returns [rows,n] in out_dtype."""
+    if tile is None:
+        done = (_host or _compiled()).grouped_fp8_matmul(x, w, scale_x, scale_w, group_ends, out_dtype, out)
+        if done is not None:
+            return done
     _want(x, "x", torch.float8_e4m3fn, 2)
     _want(w, "w", torch.float8_e4m3fn, 3)
     rows, k = x.shape
