@@ -59,13 +59,13 @@ struct Choice {
 constexpr Choice kChecked{Choice::CHECKED, 64, 64, 1};
 constexpr Choice kSmallNk[] = {{Choice::SMALL, 16, 32, 4}, {Choice::SMALL, 32, 32, 4}};
 constexpr Choice kSmallKn[] = {{Choice::SMALL, 16, 64, 4}, {Choice::SMALL, 32, 64, 4}, {Choice::SMALL, 64, 64, 4}};
-constexpr Choice kTeams64{Choice::TILE, 64, 128, 2}, kTeams128{Choice::TILE, 128, 128, 2}, kTile128{Choice::TILE, 128, 128, 1}, kTile256{Choice::TILE, 256, 256, 1};
+constexpr Choice kTeams64{Choice::TILE, 64, 128, 2}, kTeams128{Choice::TILE, 128, 128, 2}, kTile128{Choice::TILE, 128, 128, 1}, kTile160{Choice::TILE, 160, 256, 1}, kTile256{Choice::TILE, 256, 256, 1};
 
 // By what a launch is estimated to take, in us: the larger of what memory needs for each byte once (5.7 GB/ms; `reach`: over what a kernel reaches of it) and of its
 // rounds of workgroups, a quarter of the smaller, and a start.  A round costs its steps of 128 bytes of k, `step` us each with the GPU full, `few` of that with
-// at most one workgroup a CU.  Fitted to, and compared on, 47 sizes that ran on all of these kernels (1 to 8192 rows of e4m3 against 2048 to 8192 columns and
-// k; 16 to 4096 rows in 8 to 64 groups of 4096x1792, 16 bits either way and e4m3): for 41 of them the choice is within 6 % of the fastest, the worst 1.22 of
-// it.  How the rows of groups lie is not known here: half a tile more than the mean is assumed.
+// at most one workgroup a CU.  Fitted to, and compared on, 62 sizes that ran on all of these kernels (1 to 8192 rows of e4m3 against 2048 to 8192 columns and
+// k; 64 to 8000 rows in 8 to 128 groups of 4096x1792, uneven, 16 bits either way and e4m3): for 52 of them the choice is within 6 %
+// of the fastest, the worst 1.20 of it.  How the rows of groups lie is not known here: half a tile more than the mean is assumed.
 Choice choose(uint32_t dtype, const RaggedArgs &a, bool kn)
 {
     const bool f8 = dtype == DT_F8;
@@ -78,15 +78,15 @@ Choice choose(uint32_t dtype, const RaggedArgs &a, bool kn)
     auto offer = [&](const Choice &c, double start, double slots, double step, double few, double reach) {
         const double tiles = row_tiles(c.rows) * (double)cdiv(a.n, c.cols);
         double rounds = tiles / slots;
-        rounds = a.ends || rounds > 4 ? std::max(1.0, rounds + 0.3) : std::ceil(rounds);
+        rounds = rounds > (a.ends ? 3.0 : 4.0) ? rounds + 0.3 : std::ceil(rounds);
         const double work = (tiles <= 256 ? few : 1.0) * step * steps * rounds, m = mem * reach;
         const double t = start + std::max(m, work) + 0.25 * std::min(m, work);
         if (least == 0 || t < least) { least = t; best = c; }
     };
     if (kn) {
-        offer(kSmallKn[0], 5, 512, 0.2, 1, 1);
-        offer(kSmallKn[1], 5, 256, 0.17, 1, 1);
-        offer(kSmallKn[2], 5, 256, 0.24, 1, 1);
+        offer(kSmallKn[0], 5, 512, 0.2, 1, 1.12);
+        offer(kSmallKn[1], 5, 256, 0.17, 1, 1.12);
+        offer(kSmallKn[2], 5, 256, 0.24, 1, 1.12);
     } else {
         offer(kSmallNk[0], 5, 512, f8 ? 0.156 : 0.106, 0.83, 1);
         offer(kSmallNk[1], 5, 512, f8 ? 0.21 : 0.16, 0.7, 1);
@@ -94,8 +94,11 @@ Choice choose(uint32_t dtype, const RaggedArgs &a, bool kn)
     offer(kTeams64, 6, 256, f8 ? 0.43 : 0.41, 1, 1.2);
     offer(kTeams128, 6, 256, f8 ? 0.6 : 0.55, 1, 1.2);
     offer(kTile128, 6, 512, f8 ? 1.05 : 1.09, 0.65, 1.05);
-    const double height = std::min(8.0, std::max(2.0, std::ceil(a.rows / row_tiles(256) / 32)));   // in 32 rows
-    offer(kTile256, 8, 256, f8 ? 0.35 + 0.19 * height : 0.45 + 0.125 * height, 1, f8 ? 1.2 : 0.98);
+    for (const Choice *c : {&kTile160, &kTile256}) {
+        const double height = std::min(c->rows / 32.0, std::max(2.0, std::ceil(a.rows / row_tiles(c->rows) / 32)));   // in 32 rows; above five two stages instead of three
+        offer(*c, 8, 256, f8 ? 0.35 + 0.19 * height + (height > 5 ? 0.05 : 0) : height > 5 ? 0.65 + 0.11 * height : 0.45 + 0.115 * height, 1,
+              (f8 ? 1.15 : 0.98) + (c->rows > 160 ? 0.05 : 0));
+    }
     return best;
 }
 
@@ -119,7 +122,7 @@ const Choice *asked_for(const CatcocTile &tile, bool kn, bool dw, bool words)
     for (const Choice *c : {&kTile256, &kTile128})
         if (is(*c)) return c;
     if (dw) return nullptr;
-    for (const Choice *c : {&kTeams64, &kTeams128})
+    for (const Choice *c : {&kTeams64, &kTeams128, &kTile160})
         if (is(*c)) return c;
     if (kn) {
         for (const Choice &c : kSmallKn)

@@ -33,10 +33,17 @@ struct TileOperand {
     static constexpr uint32_t COPIES = 16u / WAVES;   // of a wave and sub-stage, 1 KiB each
     const unsigned char *base;   // the tile's first row and column, first step
     uint32_t pitch, have, apart;
+    bool packed;                 // of the second sub-stage only 16 rows of either half are there, 4 KiB
     uint32_t off[SUBS][COPIES];
 
     // The row (column) of the tile that row (column) q of sub-stage h holds.
-    __device__ __forceinline__ uint32_t of_tile(uint32_t h, uint32_t q) const { return (q >> 6) * apart + 64u * h + (q & 63u); }
+    __device__ __forceinline__ uint32_t of_tile(uint32_t h, uint32_t q) const
+    {
+        const uint32_t log = !KM && h == 1u && packed ? 4u : 6u;
+        return (q >> log) * apart + 64u * h + (q & ((1u << log) - 1u));
+    }
+    // Copies between a wave's first and second of a sub-stage.
+    __device__ __forceinline__ uint32_t stride(uint32_t h) const { return !KM && h == 1u && packed ? 2u : WAVES; }
     // Byte of the tile's step that byte `in` of the 16-byte slot `slot` of LDS row `row` holds.
     __device__ __forceinline__ uint32_t source(uint32_t h, uint32_t row, uint32_t slot, uint32_t in) const
     {
@@ -47,17 +54,18 @@ struct TileOperand {
             return umin(of_tile(h, row), have - 1u) * pitch + (slot ^ k_rows_slot(row)) * 16u + in;
         }
     }
-    __device__ __forceinline__ void init(const unsigned char *p, uint32_t pitch_, uint32_t have_, uint32_t apart_, uint32_t wave, uint32_t lane)
+    __device__ __forceinline__ void init(const unsigned char *p, uint32_t pitch_, uint32_t have_, uint32_t apart_, bool packed_, uint32_t wave, uint32_t lane)
     {
         base = uniform_ptr(p);
         pitch = pitch_;
         have = have_;
         apart = apart_;
+        packed = packed_;
 #pragma unroll
         for (uint32_t h = 0; h < SUBS; ++h)
 #pragma unroll
             for (uint32_t j = 0; j < COPIES; ++j) {
-                const uint32_t at = (wave + WAVES * j) * 64u + lane;
+                const uint32_t at = (wave + stride(h) * j) * 64u + lane;
                 off[h][j] = source(h, KM ? at >> 4 : at >> 3, KM ? at & 15u : at & 7u, 0);
             }
     }
@@ -68,7 +76,7 @@ struct TileOperand {
     {
         const unsigned char *const p = at_step(s);
 #pragma unroll
-        for (uint32_t j = 0; j < COPIES; ++j) copy16(p, off[h][j], lds + (wave + WAVES * j) * 1024u);
+        for (uint32_t j = 0; j < COPIES; ++j) copy16(p, off[h][j], lds + (wave + stride(h) * j) * 1024u);
     }
     // The last step where it ends inside its 128 bytes of k or 64 rows of k, or where pieces of 16 bytes would end behind the matrix: copies of what is there (4
     // bytes at a time where a row ends inside a piece), and zeros.  inRow: bytes of a row that are there, from the step's first (KM: the tile's first column) on;
@@ -84,7 +92,7 @@ struct TileOperand {
         constexpr uint32_t PER = (KM ? 256u : 128u) / BYTES;   // copied pieces of a row
         const unsigned char *const p = at_step(s);
 #pragma unroll 1
-        for (uint32_t c = wave; c < 256u / BYTES; c += WAVES) {
+        for (uint32_t c = wave; c < (!KM && h == 1u && packed ? 64u : 256u) / BYTES; c += WAVES) {
             const uint32_t at = c * 64u + lane, row = at / PER, slot = (at % PER) * BYTES / 16u, in = at * BYTES % 16u;
             const uint32_t byte = KM ? of_tile(h, (slot ^ b16_slot<2>(row)) * 8u) * 2u + in : (slot ^ k_rows_slot(row)) * 16u + in;
             const bool there = byte < inRow && (!KM || row < rows);
@@ -107,7 +115,7 @@ __device__ __forceinline__ uint32_t result_col(uint32_t m) { return ((m >> 2) & 
 // A tile of 32 NIMAX rows and 64 WY columns: 2 WY waves, two by WY, of up to 16 NIMAX rows and 64 columns each (NI row fragments, as many as the tile's rows
 // need; four of columns).  A wave keeps a step's column fragments in registers and streams its row fragments, two ahead of the MFMAs.
 //
-// Two stages of 128 bytes of k, three with eight waves and at most four row fragments each (their stages are smaller).  When the last read of a step is out, the
+// Two stages of 128 bytes of k, three with eight waves and at most five row fragments each (their stages are smaller).  When the last read of a step is out, the
 // wave waits for the next stage's copies (issued a whole step before, or several) and for its own reads; the barrier behind that says both that the next stage
 // is complete and that this one may be overwritten: its next copies start there.  The last two row fragments' MFMAs then cover the first reads of the next
 // step, whose column fragments take the registers of those just used.
@@ -119,10 +127,12 @@ struct RaggedTileLoop {
     static constexpr uint32_t ES = DT == DT_F8 ? 1u : 2u, KE = 128u / ES;
     static constexpr uint32_t WAVES = 2u * WY, BX = 32u * NIMAX, BY = 64u * WY, SUB = 16384u;
     static constexpr uint32_t XSUBS = BX / 128u, WSUBS = BY / 128u;
-    static constexpr uint32_t stages(int ni) { return NIMAX == 8 && ni <= 4 ? 3u : 2u; }
-    static constexpr uint32_t stage_bytes(int ni) { return ((ni <= 4 ? 1u : 2u) + WSUBS) * SUB; }
-    static constexpr uint32_t SX = stages(4) * stage_bytes(4);   // e4m3: row scales behind the stages
-    static constexpr uint32_t SXB = BX * 4u, SXN = stages(4);
+    static constexpr bool PACK = NIMAX == 8 && !XK;   // five row fragments a wave: the fifth ones packed, so that three stages fit
+    static constexpr uint32_t stages(int ni) { return NIMAX == 8 && ni <= (PACK ? 5 : 4) ? 3u : 2u; }
+    static constexpr uint32_t x_bytes(int ni) { return ni <= 4 ? SUB : PACK && ni == 5 ? SUB + 4096u : 2u * SUB; }
+    static constexpr uint32_t stage_bytes(int ni) { return x_bytes(ni) + WSUBS * SUB; }
+    static constexpr uint32_t SX = NIMAX == 8 ? (XK ? 2u * stage_bytes(8) : 3u * stage_bytes(5)) : 2u * stage_bytes(4);   // e4m3: row scales behind the stages
+    static constexpr uint32_t SXB = BX * 4u, SXN = NIMAX == 8 ? 3u : 2u;
     static constexpr uint32_t LDS = SX + (DT == DT_F8 ? SXN * SXB : 0u);   // of a team
     static_assert(KG == 1 || (KG == 2 && NIMAX * WAVES * 2048u <= SX), "two teams: half of a team's sums fit its stages");
     TileOperand<XK, XSUBS, ES, WAVES> x;
@@ -142,11 +152,12 @@ struct RaggedTileLoop {
 
     static __device__ __forceinline__ uint32_t of_all(const Problem &p, uint32_t s) { return KG * s + (KG > 1 ? p.team : 0u); }
 
-    // Copies of the team's step s into `stage`; TWO: of both halves of the rows.
-    template <bool TWO>
+    // Copies of the team's step s into `stage`.
+    template <int NI>
     __device__ __forceinline__ void issue(const Problem &p, unsigned char *smem, uint32_t stage, uint32_t s, uint32_t wave, uint32_t lane)
     {
-        const uint32_t lds0 = (uint32_t)(uintptr_t)(CATCOC_LDS unsigned char *)smem, ws = stage + (TWO ? 2u : 1u) * SUB;
+        const uint32_t lds0 = (uint32_t)(uintptr_t)(CATCOC_LDS unsigned char *)smem, ws = stage + x_bytes(NI);
+        constexpr bool TWO = NI > 4;
         if (p.partLast && s + 1u == p.steps) {
             const uint32_t left = p.K - of_all(p, s) * KE;
 #pragma unroll 1
@@ -167,17 +178,19 @@ struct RaggedTileLoop {
     }
 
     // A tile's first copies.
+    template <int NI>
+    __device__ __forceinline__ void first(const Problem &p, unsigned char *smem, uint32_t wave, uint32_t lane)
+    {
+#pragma unroll 1
+        for (uint32_t s = 0; s < stages(NI) && s < p.steps; ++s) issue<NI>(p, smem, s * stage_bytes(NI), s, wave, lane);
+    }
     __device__ __forceinline__ void begin(const Problem &p, unsigned char *smem, uint32_t wave, uint32_t lane)
     {
-        if (XSUBS == 2u && p.ni > 4u) {
-            if constexpr (XSUBS == 2u) {
-#pragma unroll 1
-                for (uint32_t s = 0; s < 2u && s < p.steps; ++s) issue<true>(p, smem, s * stage_bytes(8), s, wave, lane);
-            }
-        } else {
-#pragma unroll 1
-            for (uint32_t s = 0; s < stages(4) && s < p.steps; ++s) issue<false>(p, smem, s * stage_bytes(4), s, wave, lane);
+        if constexpr (NIMAX == 8) {
+            if (p.ni > 5u) return first<8>(p, smem, wave, lane);
+            if (p.ni == 5u) return first<5>(p, smem, wave, lane);
         }
+        first<4>(p, smem, wave, lane);
     }
 
     // All but this wave's copies of the last N steps are there where `whole` steps follow, else all; then everybody's are, and everybody's reads are done.
@@ -210,12 +223,14 @@ struct RaggedTileLoop {
         meet<(int)STAGES - 1>(full >= STAGES, first, second);
 
         const uint32_t xa = XK ? at_k_major<false>(256u, 64u * wr, lane, b16_slot<2>) : at_k_rows(64u * wr + (lane & 15u), lane);
+        const uint32_t x4 = SUB + at_k_rows(16u * wr + (lane & 15u), lane);   // (packed: the fifth row fragment)
         const uint32_t wh = WSUBS == 2u ? wc % 2u : 0u, w64 = 64u * (WSUBS == 2u ? wc / 2u : wc);   // the wave's columns: sub-stage, half of it
-        uint32_t wa = ((TWO ? 2u : 1u) + wh) * SUB + (WK ? at_k_major<true>(256u, w64, lane, b16_slot<2>) : at_k_rows(w64 + result_col(lane & 15u), lane));
+        uint32_t wa = x_bytes(NI) + wh * SUB + (WK ? at_k_major<true>(256u, w64, lane, b16_slot<2>) : at_k_rows(w64 + result_col(lane & 15u), lane));
         // Two teams: team 1 has its column blocks in the order 2, 3, 0, 1, so that 0 and 1 are those that either team stores.
         if (KG > 1 && p.team) wa ^= WK ? 64u : 4096u;
         auto read_x = [&](uint32_t stage, uint32_t i) {
             if constexpr (XK) return frag_k_major<256>(smem, ((stage + xa) ^ (32u * (i & 3u))) + (i >> 2) * SUB);
+            else if (PACK && NI == 5 && i == 4u) return frag_k_rows(smem, stage + x4);
             else return frag_k_rows(smem, stage + xa + 2048u * (i & 3u) + (i >> 2) * SUB);
         };
         auto read_w = [&](uint32_t stage, uint32_t j) {
@@ -231,10 +246,10 @@ struct RaggedTileLoop {
         auto slot = [](int i) { return NI == 8 ? i & 3 : i < 2 || NI < 4 ? i : 2 + (i - 2) % 3; };
         Frag fx[SLOTS], fw[4], ahead[2];
         float fs[SLOTS], aheadS[2], sw = 0.f;   // e4m3: the fragments' row scales, the columns' scale
-        // e4m3: a result is scaled and added while the MFMA behind the next one runs
-        v4f late[2];
-        float lateS[2];
-        int li[2], lj[2], queued = 0;
+        constexpr int LAG = 3;   // e4m3: a result is scaled and added while the MFMAs behind it run
+        v4f late[LAG];
+        float lateS[LAG];
+        int li[LAG], lj[LAG], queued = 0;
         auto settle = [&](int q) {
 #pragma unroll
             for (int r = 0; r < 4; ++r) acc[li[q]][lj[q]][r] = __builtin_fmaf(lateS[q], late[q][r], acc[li[q]][lj[q]][r]);
@@ -243,11 +258,11 @@ struct RaggedTileLoop {
         auto multiply = [&](int i, int j, const Frag &f, float scale) {
             if constexpr (DT == DT_F8) {
                 const v4f d = step_mfma_f8(fw[j], f);
-                if (queued >= 2) settle(queued & 1);
-                late[queued & 1] = d;
-                lateS[queued & 1] = scale;
-                li[queued & 1] = i;
-                lj[queued & 1] = j;
+                if (queued >= LAG) settle(queued % LAG);
+                late[queued % LAG] = d;
+                lateS[queued % LAG] = scale;
+                li[queued % LAG] = i;
+                lj[queued % LAG] = j;
                 ++queued;
                 __builtin_amdgcn_sched_barrier(0);
             } else {
@@ -262,6 +277,8 @@ struct RaggedTileLoop {
             if constexpr (DT == DT_F8) fs[i] = row_scale(0, i);
         }
         if constexpr (DT == DT_F8) sw = load_uniform(p.sw + (KG > 1 ? min(p.team, (p.K - 1u) / KE) : 0u));
+        // Of the two waves on a SIMD one starts its copies behind the barrier, the other at the next step's start: while copies wait for their issue the other one multiplies.
+        const bool early = WAVES != 8u || wave < WAVES / 2u;
         uint32_t cur = 0;   // this step's stage
 #pragma unroll 1
         for (uint32_t s = 0; s < p.rounds; ++s) {
@@ -271,6 +288,7 @@ struct RaggedTileLoop {
             }
             const uint32_t next = cur == (STAGES - 1u) * STAGE ? 0u : cur + STAGE;
             queued = 0;
+            if (!early && s > 0u && s + STAGES - 1u < p.steps) issue<NI>(p, smem, cur == 0u ? (STAGES - 1u) * STAGE : cur - STAGE, s + STAGES - 1u, wave, lane);
             float swNext = 0.f;
             if constexpr (DT == DT_F8) {   // (asked for here: its wait is the one for the step's reads)
                 swNext = load_uniform(p.sw + umin(of_all(p, s + 1u), (p.K - 1u) / KE));
@@ -286,7 +304,7 @@ struct RaggedTileLoop {
                 __builtin_amdgcn_sched_barrier(0);
             }
             meet<(int)STAGES - 2>(s + STAGES <= full, first, second);
-            if (s + STAGES < p.steps) issue<TWO>(p, smem, cur, s + STAGES, wave, lane);
+            if (early && s + STAGES < p.steps) issue<NI>(p, smem, cur, s + STAGES, wave, lane);
             // (behind the last step nobody looks at what is read here)
             const float s0 = DT == DT_F8 ? fs[slot(NI - 2)] * sw : 0.f, s1 = DT == DT_F8 ? fs[slot(NI - 1)] * sw : 0.f;
 #pragma unroll
@@ -302,8 +320,8 @@ struct RaggedTileLoop {
                 fw[j] = read_w(next, j);
             }
             if constexpr (DT == DT_F8) {
-                settle(queued & 1);
-                settle((queued & 1) ^ 1);
+#pragma unroll
+                for (int q = 0; q < LAG; ++q) settle((queued + q) % LAG);
                 sw = swNext;
             }
             if constexpr (NI < 4) {
@@ -406,16 +424,16 @@ __global__ void __launch_bounds__(128 * WY * KG, 2) ragged_tile_kernel(const Rag
             p.K = sumEnd - sumBegin;
             p.xLeft = args.k - t.row;
             p.partLast = p.K % 64u != 0 || args.k % 8u != 0 || args.n % 8u != 0;
-            loop.x.init((const unsigned char *)args.x + ((size_t)sumBegin * args.k + t.row) * 2u, args.k * 2u, t.rows, 16u * NIMAX, wave, lane);
-            loop.w.init((const unsigned char *)args.w + ((size_t)sumBegin * args.n + col0) * 2u, args.n * 2u, p.cols, BY / 2u, wave, lane);
+            loop.x.init((const unsigned char *)args.x + ((size_t)sumBegin * args.k + t.row) * 2u, args.k * 2u, t.rows, 16u * NIMAX, false, wave, lane);
+            loop.w.init((const unsigned char *)args.w + ((size_t)sumBegin * args.n + col0) * 2u, args.n * 2u, p.cols, BY / 2u, false, wave, lane);
         } else {
             const uint32_t g = umin(t.group, args.groups - 1u);
             p.K = t.group < args.groups ? args.k : 0u;
             const uint32_t wPitch = KN ? args.n * ES : args.k * ES;
             p.xLeft = 0;
             p.partLast = p.K % Loop::KE != 0 || (KN && args.n % 8u != 0);
-            loop.x.init((const unsigned char *)args.x + (size_t)t.row * args.k * ES, args.k * ES, t.rows, 16u * p.ni, wave, lane);
-            loop.w.init((const unsigned char *)args.w + (size_t)g * args.n * args.k * ES + (size_t)col0 * (KN ? ES : wPitch), wPitch, p.cols, BY / 2u, wave, lane);
+            loop.x.init((const unsigned char *)args.x + (size_t)t.row * args.k * ES, args.k * ES, t.rows, 16u * p.ni, Loop::PACK && p.ni == 5u, wave, lane);
+            loop.w.init((const unsigned char *)args.w + (size_t)g * args.n * args.k * ES + (size_t)col0 * (KN ? ES : wPitch), wPitch, p.cols, BY / 2u, false, wave, lane);
             if constexpr (DT == DT_F8) {
                 const uint32_t kb = (args.k + kScaleBlock - 1u) / kScaleBlock, nb = (args.n + kScaleBlock - 1u) / kScaleBlock;
                 p.sx = uniform_ptr(args.sx + t.row);

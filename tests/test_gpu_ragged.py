@@ -391,7 +391,7 @@ def test_calls_say_what_they_ran():
     assert (info.kernel, info.tileRows, info.tileCols) == (L.KERNEL_RAGGED_CHECKED, 64, 64)
 
 
-TILES = [(256, 256, 1), (128, 128, 1), (128, 128, 2), (64, 128, 2), (64, 64, 1)]
+TILES = [(256, 256, 1), (160, 256, 1), (128, 128, 1), (128, 128, 2), (64, 128, 2), (64, 64, 1)]
 SMALL_NK, SMALL_KN = [(16, 32, 4), (32, 32, 4)], [(16, 64, 4), (32, 64, 4), (64, 64, 4)]
 UNEVEN = {"large": [513, 0, 31, 900, 260, 1], "one_group": [1300], "full": [512, 256], "few": [1, 0, 15, 16, 17, 0, 40, 70, 129], "many": [(5 * i) % 23 for i in range(75)]}
 
