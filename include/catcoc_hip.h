@@ -291,7 +291,7 @@ typedef struct CatcocTile {
  * zeros).  Nothing needs a workspace, no sum depends on the order in which workgroups run, and every sum is held in fp32 and rounded once.
  *
  * `tile` of the products: the kernel's tile, for tests and tuning as m0 and n0 of CocTilingParams; NULL or zeros let the library choose.  Any product: 64x64 with one team
- * (every load checked, any alignment); rows that start on 4 bytes: 256x256 and 128x128 with one, and, weight gradients apart, 160x256 with one, 64x128 and 128x128 with two teams of waves that
+ * (every load checked, any alignment); rows that start on 4 bytes: 256x256 and 128x128 with one, and, weight gradients apart, 96x256 to 224x256 in steps of 32 rows with one, 64x128 and 128x128 with two teams of waves that
  * share a tile's steps of k, and with four 16x32 and 32x32 (w as [n,k]) or 16x64, 32x64 and 64x64 (as [k,n]).  Anything else is rejected.  Sums are added in an order that
  * depends on the tile alone.
  *

@@ -59,13 +59,15 @@ struct Choice {
 constexpr Choice kChecked{Choice::CHECKED, 64, 64, 1};
 constexpr Choice kSmallNk[] = {{Choice::SMALL, 16, 32, 4}, {Choice::SMALL, 32, 32, 4}};
 constexpr Choice kSmallKn[] = {{Choice::SMALL, 16, 64, 4}, {Choice::SMALL, 32, 64, 4}, {Choice::SMALL, 64, 64, 4}};
-constexpr Choice kTeams64{Choice::TILE, 64, 128, 2}, kTeams128{Choice::TILE, 128, 128, 2}, kTile128{Choice::TILE, 128, 128, 1}, kTile160{Choice::TILE, 160, 256, 1}, kTile256{Choice::TILE, 256, 256, 1};
+constexpr Choice kTeams64{Choice::TILE, 64, 128, 2}, kTeams128{Choice::TILE, 128, 128, 2}, kTile128{Choice::TILE, 128, 128, 1}, kTile256{Choice::TILE, 256, 256, 1};
+constexpr uint32_t kLeastRows = 96;   // tiles of 256 columns: 96 to 256 rows in steps of 32
 
-// By what a launch is estimated to take, in us: the larger of what memory needs for each byte once (5.7 GB/ms; `reach`: over what a kernel reaches of it) and of its
+// By what a launch is estimated to take, in us: the larger of what memory needs for each byte once (5.7 GB/ms; `reach`: over what a kernel reaches of it in several rounds) and of its
 // rounds of workgroups, a quarter of the smaller, and a start.  A round costs its steps of 128 bytes of k, `step` us each with the GPU full, `few` of that with
-// at most one workgroup a CU.  Fitted to, and compared on, 62 sizes that ran on all of these kernels (1 to 8192 rows of e4m3 against 2048 to 8192 columns and
-// k; 64 to 8000 rows in 8 to 128 groups of 4096x1792, uneven, 16 bits either way and e4m3): for 52 of them the choice is within 6 %
-// of the fastest, the worst 1.20 of it.  How the rows of groups lie is not known here: half a tile more than the mean is assumed.
+// at most one workgroup a CU.  Fitted to, and compared on, 84 sizes that ran on all of these kernels (1 to 8192 rows of e4m3 against 2048 to 8192 columns and
+// k; 64 to 16384 rows in 1 to 128 groups of 1792 to 4096 by 1792 to 8192, uneven, 16 bits either way and e4m3): for 74 of them the choice is within 7 % of the
+// fastest, the worst 1.17 of it.  Heights: 4096 rows in 16 groups of 4096x3584 take 195 us in tiles of at most 256 rows, 177 of 192, 153 of 160, 181 of 128;
+// 2400 in 8 groups of 2048x4096 49, 43, 65 and 57 (16 bits).
 Choice choose(uint32_t dtype, const RaggedArgs &a, bool kn)
 {
     const bool f8 = dtype == DT_F8;
@@ -74,12 +76,22 @@ Choice choose(uint32_t dtype, const RaggedArgs &a, bool kn)
     const double mem = (active * a.k * a.n * es + a.rows * (double)a.k * es + a.rows * (double)a.n * (2.0 + 4.0 * a.nPeers)) / 5.7e6;
     Choice best = kTile256;
     double least = 0;
-    auto row_tiles = [&](uint32_t rows) { return a.ends ? active * std::max(1.0, mean / rows + 0.5) : (double)cdiv(a.rows, rows); };
+    // Groups are taken to have 0.4, 0.6 .. 1.6 of the mean: how many tiles of at most `rows` that makes, and how high they are, in 32 rows (no less than two).
+    auto row_tiles = [&](uint32_t rows, double *height) {
+        double tiles = 0, high = 0;
+        for (int i = a.ends ? 2 : 5; i <= (a.ends ? 8 : 5); ++i) {
+            const double group = mean * 0.2 * i, t = std::max(1.0, std::ceil(group / rows));
+            tiles += t;
+            high += t * std::max(2.0, std::ceil(group / t / 32));
+        }
+        if (height) *height = a.ends ? 0.8 * high / tiles + 0.2 * std::min(rows / 32.0, std::max(2.0, std::ceil(mean * 1.6 / 32))) : high / tiles;   // (a round ends with its highest)
+        return a.ends ? active * tiles / 7 : tiles;
+    };
     auto offer = [&](const Choice &c, double start, double slots, double step, double few, double reach) {
-        const double tiles = row_tiles(c.rows) * (double)cdiv(a.n, c.cols);
+        const double tiles = row_tiles(c.rows, nullptr) * (double)cdiv(a.n, c.cols);
         double rounds = tiles / slots;
-        rounds = rounds > (a.ends ? 3.0 : 4.0) ? rounds + 0.3 : std::ceil(rounds);
-        const double work = (tiles <= 256 ? few : 1.0) * step * steps * rounds, m = mem * reach;
+        rounds = rounds > 4 ? rounds + 0.3 : std::ceil(rounds);
+        const double work = (tiles <= 256 ? few : 1.0) * step * steps * rounds, m = mem * (tiles <= slots ? std::min(reach, 1.0) : reach);
         const double t = start + std::max(m, work) + 0.25 * std::min(m, work);
         if (least == 0 || t < least) { least = t; best = c; }
     };
@@ -91,13 +103,14 @@ Choice choose(uint32_t dtype, const RaggedArgs &a, bool kn)
         offer(kSmallNk[0], 5, 512, f8 ? 0.156 : 0.106, 0.83, 1);
         offer(kSmallNk[1], 5, 512, f8 ? 0.21 : 0.16, 0.7, 1);
     }
-    offer(kTeams64, 6, 256, f8 ? 0.43 : 0.41, 1, 1.2);
-    offer(kTeams128, 6, 256, f8 ? 0.6 : 0.55, 1, 1.2);
-    offer(kTile128, 6, 512, f8 ? 1.05 : 1.09, 0.65, 1.05);
-    for (const Choice *c : {&kTile160, &kTile256}) {
-        const double height = std::min(c->rows / 32.0, std::max(2.0, std::ceil(a.rows / row_tiles(c->rows) / 32)));   // in 32 rows; above five two stages instead of three
-        offer(*c, 8, 256, f8 ? 0.35 + 0.19 * height + (height > 5 ? 0.05 : 0) : height > 5 ? 0.65 + 0.11 * height : 0.45 + 0.115 * height, 1,
-              (f8 ? 1.15 : 0.98) + (c->rows > 160 ? 0.05 : 0));
+    offer(kTeams64, 6, 256, f8 ? 0.43 : 0.41, f8 ? 1 : 0.85, 1.2);
+    offer(kTeams128, 6, 256, f8 ? 0.6 : 0.55, f8 ? 1 : 0.85, 1.2);
+    offer(kTile128, 6, 512, f8 ? 1.05 : 1.09, 0.65, f8 ? 1.15 : 1.05);
+    for (uint32_t rows = kLeastRows; rows <= kTile256.rows; rows += 32) {
+        double height;   // above five two stages instead of three
+        row_tiles(rows, &height);
+        offer({Choice::TILE, rows, 256, 1}, 8, 256, f8 ? 0.35 + 0.19 * height + (height > 5 ? 0.05 : 0) : height > 5 ? 0.65 + 0.11 * height : 0.45 + 0.115 * height, 1,
+              (f8 ? 1.15 : 0.98) + (rows > 160 ? 0.05 : 0));
     }
     return best;
 }
@@ -113,25 +126,17 @@ Choice choose_dw(const RaggedArgs &a)
     return small < large ? kTile128 : kTile256;
 }
 
-// What the caller asks for, where a product can run on it.
-const Choice *asked_for(const CatcocTile &tile, bool kn, bool dw, bool words)
+// Whether a product can run on what the caller asks for.
+bool can_run(const Choice &asked, bool kn, bool dw, bool words)
 {
-    auto is = [&](const Choice &c) { return c.rows == tile.rows && c.cols == tile.cols && c.teams == tile.teams; };
-    if (is(kChecked)) return &kChecked;
-    if (!words) return nullptr;
-    for (const Choice *c : {&kTile256, &kTile128})
-        if (is(*c)) return c;
-    if (dw) return nullptr;
-    for (const Choice *c : {&kTeams64, &kTeams128, &kTile160})
-        if (is(*c)) return c;
-    if (kn) {
-        for (const Choice &c : kSmallKn)
-            if (is(c)) return &c;
-    } else {
-        for (const Choice &c : kSmallNk)
-            if (is(c)) return &c;
-    }
-    return nullptr;
+    auto is = [&](const Choice &c) { return c.rows == asked.rows && c.cols == asked.cols && c.teams == asked.teams; };
+    if (!words) return false;
+    if (is(kTile256) || is(kTile128)) return true;
+    if (dw) return false;
+    if (is(kTeams64) || is(kTeams128)) return true;
+    if (asked.cols == 256 && asked.teams == 1) return asked.rows >= kLeastRows && asked.rows <= kTile256.rows && asked.rows % 32 == 0;
+    if (kn) return std::any_of(std::begin(kSmallKn), std::end(kSmallKn), is);
+    return std::any_of(std::begin(kSmallNk), std::end(kSmallNk), is);
 }
 
 void run(uint32_t dtype, const RaggedArgs &args, bool kn, bool dw, const CatcocTile *tile, void *stream)
@@ -140,12 +145,13 @@ void run(uint32_t dtype, const RaggedArgs &args, bool kn, bool dw, const CatcocT
     const bool words = rows_on_words(dtype, a, kn, dw);
     Choice c = kChecked;
     if (tile != nullptr && (tile->rows || tile->cols || tile->teams)) {
-        const Choice *asked = asked_for(*tile, kn, dw, words);
-        if (asked == nullptr) {
+        c = {tile->teams == 4 ? Choice::SMALL : Choice::TILE, tile->rows, tile->cols, tile->teams};
+        if (c.rows == kChecked.rows && c.cols == kChecked.cols && c.teams == kChecked.teams) {
+            c = kChecked;
+        } else if (!can_run(c, kn, dw, words)) {
             api_fail(E_TILING, "no kernel of %ux%u tiles and %u team(s) for this product%s", tile->rows, tile->cols, tile->teams, words ? "" : " (rows that do not start on 4 bytes run 64x64 tiles, 1 team)");
             return;
         }
-        c = *asked;
     } else if (words) {
         c = dw ? choose_dw(a) : choose(dtype, a, kn);
     }

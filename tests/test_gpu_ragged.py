@@ -391,7 +391,8 @@ def test_calls_say_what_they_ran():
     assert (info.kernel, info.tileRows, info.tileCols) == (L.KERNEL_RAGGED_CHECKED, 64, 64)
 
 
-TILES = [(256, 256, 1), (160, 256, 1), (128, 128, 1), (128, 128, 2), (64, 128, 2), (64, 64, 1)]
+TILES = [(256, 256, 1), (224, 256, 1), (160, 256, 1), (96, 256, 1), (128, 128, 1), (128, 128, 2), (64, 128, 2), (64, 64, 1)]
+TILES_DW = [(256, 256, 1), (128, 128, 1), (64, 64, 1)]
 SMALL_NK, SMALL_KN = [(16, 32, 4), (32, 32, 4)], [(16, 64, 4), (32, 64, 4), (64, 64, 4)]
 UNEVEN = {"large": [513, 0, 31, 900, 260, 1], "one_group": [1300], "full": [512, 256], "few": [1, 0, 15, 16, 17, 0, 40, 70, 129], "many": [(5 * i) % 23 for i in range(75)]}
 
@@ -423,7 +424,7 @@ def test_every_tile_of_grouped_products(name, k, n, tile, trans_b):
 
 @pytest.mark.parametrize("name", sorted(UNEVEN))
 @pytest.mark.parametrize("k,n", [(1024, 512), (1096, 776), (514, 1030), (66, 2), (256, 130)])
-@pytest.mark.parametrize("tile", [(256, 256, 1), (128, 128, 1), (64, 64, 1)])
+@pytest.mark.parametrize("tile", TILES_DW)
 @pytest.mark.parametrize("out_dtype", [torch.float32, torch.float16])
 def test_every_tile_of_weight_gradients(name, k, n, tile, out_dtype):
     counts = UNEVEN[name]
@@ -438,6 +439,21 @@ def test_every_tile_of_weight_gradients(name, k, n, tile, out_dtype):
         for e, (i, j) in enumerate(ranges(counts)):
             a, d = x[i:j].double(), dy[i:j].double()
             close(dw[e].t() if trans_b else dw[e], a.t() @ d, a.abs().t() @ d.abs(), j - i, out_dtype)
+
+
+# Several tiles for each workgroup, with every number of steps, of rows in the last one and of tiles without rows between them.
+@pytest.mark.parametrize("tile", TILES_DW)
+@pytest.mark.parametrize("k,n", [(1024, 768), (1030, 700), (896, 1032)])
+@pytest.mark.parametrize("out_dtype", [torch.float32, torch.bfloat16])
+def test_weight_gradients_of_many_tiles(k, n, tile, out_dtype):
+    counts = [0, 0] + [(131 * i * i + 64 * i) % 450 if i % 7 else 0 for i in range(34)] + [64, 128, 192, 256, 320, 63, 65, 1, 0]
+    g = gen(k + n)
+    x, dy = randn(g, sum(counts), k, dtype=torch.float16), randn(g, sum(counts), n, dtype=torch.float16)
+    dw = ops.grouped_matmul_dw(x, dy, ends_of(counts), out_dtype=out_dtype, tile=tile)
+    assert ran(tile)
+    for e, (i, j) in enumerate(ranges(counts)):
+        a, d = x[i:j].double(), dy[i:j].double()
+        close(dw[e], a.t() @ d, a.abs().t() @ d.abs(), j - i, out_dtype)
 
 
 @pytest.mark.parametrize("name", sorted(UNEVEN))
