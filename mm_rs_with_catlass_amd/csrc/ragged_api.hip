@@ -80,7 +80,7 @@ Choice choose(uint32_t dtype, const RaggedArgs &a, bool kn)
     auto row_tiles = [&](uint32_t rows, double *height) {
         double tiles = 0, high = 0;
         for (int i = a.ends ? 2 : 5; i <= (a.ends ? 8 : 5); ++i) {
-            const double group = mean * 0.2 * i, t = std::max(1.0, std::ceil(group / rows));
+            const double group = mean * i / 5, t = std::max(1.0, std::ceil(group / rows));
             tiles += t;
             high += t * std::max(2.0, std::ceil(group / t / 32));
         }
