@@ -4,6 +4,9 @@
 // divisor, so a quotient takes three operations instead of a division's ten: with r the correctly rounded 1 / s, q = x r and the remainder
 // x - q s (exact in one fused operation), fma(remainder, r, q) is the correctly rounded x / s (Markstein, IBM J. Res. Dev. 34, 1990).  It needs a remainder that is
 // representable, which the scale's floor sees to: a value whose code is not 0 is at least 2^-59.
+//
+// Bound by memory where there are many rows: 16384 rows of 1792 gated values, bf16, 30.5 us, 4.8 TB/s (a copy reaches 4.9), 39.6 us with a division a value and four rows a wave; blocks of
+// 4096x4096 bf16 10.4 us; 16 rows of 1024 5.6 us, the launch.
 #include <hip/hip_runtime.h>
 
 #include "ragged.h"

@@ -3,6 +3,8 @@
 // Four waves of 32x32; a step's pieces of both operands are fetched into registers while the one before is multiplied, and written to the other half of
 // a double buffer in LDS.  A piece is 16 bytes wherever that many belong to its row, read at whatever address it has, else its values one by one and
 // zeros behind them.  It serves rows that do not start on 4 bytes (the copies that go straight to LDS need that).
+// Bound by its small tile's loads through registers: 4096 rows in 16 groups of 4096x3584, bf16, 279 us against 148 on the tiles of aligned rows; e4m3 512x4096x4096 24
+// against 20.
 #pragma once
 #include "ragged.h"
 

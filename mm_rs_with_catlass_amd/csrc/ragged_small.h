@@ -7,6 +7,9 @@ namespace catcoc {
 // A tile of 16 NI rows and 16 NJ columns on four waves that deal a tile's steps of 128 bytes of k out among themselves: wave w multiplies steps w, w + 4, ...
 // through a ring of its own in LDS, NS stages deep, and meets nobody until the four sums are added, in the order of the waves.  So no wave ever waits for another
 // one's copies, and what is in flight per CU (two workgroups, where their rings fit) is 64 KiB and more, what memory needs to stream.
+// Bound by the matrix's bytes: one row of e4m3 times 8192x8192 and seven peers 12.2 us (5.5 TB/s), 16 rows in 14 of 64 groups of 4096x3584 in bf16 72 us (5.7 TB/s),
+// 256 rows in 60 of them in e4m3 148 us (5.9 TB/s), where reads alone reach 6.1 TB/s.  Narrow tiles, since a decode launch has no more columns to fill 256 CUs with:
+// on 128x128 tiles the first takes 40 us.
 template <uint32_t DT, bool KN, int NI, int NJ, int NS>
 struct RaggedSmall {
     static constexpr uint32_t ES = DT == DT_F8 ? 1u : 2u, KE = 128u / ES, WAVES = 4u;

@@ -325,6 +325,69 @@ def test_gradients_against_differences():
         assert abs(float(dw[e, i, j]) - d) <= 1e-5 * (1 + abs(d))
 
 
+FAR_TILES = [None, (256, 256, 1), (128, 128, 1), (64, 128, 2), (64, 64, 1)]
+
+
+@pytest.mark.parametrize("trans_b", [False, True])
+def test_matrices_past_4_gib(trans_b):
+    groups, k, n, rows = 34, 8192, 8192, 11
+    w = torch.zeros((groups, n, k) if trans_b else (groups, k, n), dtype=torch.bfloat16, device=DEV)
+    assert w[-1].data_ptr() - w.data_ptr() > 2 ** 32
+    g = gen(21)
+    w[-1] = randn(g, *w.shape[1:])
+    x = randn(g, rows, k, dtype=torch.bfloat16)
+    counts = [4] + [0] * (groups - 2) + [7]
+    b = w[-1].double().t() if trans_b else w[-1].double()
+    for tile in FAR_TILES + (SMALL_NK if trans_b else SMALL_KN):
+        out = ops.grouped_matmul(x, w, ends_of(counts), trans_b=trans_b, tile=tile)
+        assert (out[:4] == 0).all()
+        close(out[4:], x[4:].double() @ b, x[4:].double().abs() @ b.abs(), k, torch.bfloat16)
+
+
+def test_rows_past_4_gib():
+    rows, k, n, last = 2 ** 18 + 300, 8192, 136, 150
+    x, dy = torch.zeros((rows, k), dtype=torch.bfloat16, device=DEV), torch.zeros((rows, n), dtype=torch.bfloat16, device=DEV)
+    assert x[-last].data_ptr() - x.data_ptr() > 2 ** 32
+    g = gen(22)
+    x[-last:], dy[-last:] = randn(g, last, k), randn(g, last, n)
+    w = randn(g, 2, k, n, dtype=torch.bfloat16)
+    ends = ends_of([rows - last, last])
+    a, d = x[-last:].double(), dy[-last:].double()
+    for tile in FAR_TILES:
+        out = ops.grouped_matmul(x, w, ends, tile=tile)
+        assert (out[:-last] == 0).all()
+        close(out[-last:], a @ w[1].double(), a.abs() @ w[1].double().abs(), k, torch.bfloat16)
+    back = torch.zeros((rows, k), dtype=torch.bfloat16, device=DEV)   # (results past 4 GiB)
+    ops.grouped_matmul(dy, w, ends, trans_b=True, out=back)
+    assert (back[:-last] == 0).all()
+    close(back[-last:], d @ w[1].double().t(), d.abs() @ w[1].double().abs().t(), n, torch.bfloat16)
+    for tile in (None, (256, 256, 1), (128, 128, 1), (64, 64, 1)):
+        dw = ops.grouped_matmul_dw(x, dy, ends, out_dtype=torch.float32, tile=tile)
+        assert (dw[0] == 0).all()
+        close(dw[1], a.t() @ d, a.abs().t() @ d.abs(), last, torch.float32)
+    for br in (1, 128):
+        q, sx = ops.quantize_fp8(x, block_rows=br)
+        first = rows - rows % 128 - 128
+        want, scale = plain_quantize(x[first:].float().cpu().numpy(), br)
+        assert (q[first:].float().cpu().numpy() == torch.from_numpy(want).to(F8).float().numpy()).all()
+        got = sx[:, first:] if br == 1 else sx[first // 128:]
+        assert (got.cpu().numpy() == scale).all()
+
+
+def test_fp8_rows_past_4_gib():
+    rows, k, n, last = 2 ** 19 + 300, 8192, 130, 150
+    x = torch.zeros((rows, k), dtype=torch.uint8, device=DEV).view(F8)
+    sx = torch.ones((blocks(k), rows), device=DEV)
+    g = gen(23)
+    x[-last:], sx[:, -last:] = fp8_operand(g, last, k, 1)
+    w, sw = fp8_operand(g, n, k, 128)
+    a, b = x[-last:].double() * spread(sx[:, -last:].t().contiguous(), last, k, 1), w.double() * spread(sw, n, k, 128)
+    for tile in FAR_TILES:
+        out = ops.fp8_matmul_allreduce(x, w, sx, sw, tile=tile)
+        assert (out[:-last] == 0).all()
+        close(out[-last:], a @ b.t(), a.abs() @ b.abs().t(), k + 1, torch.bfloat16, norm2(a, b))
+
+
 def test_no_rows():
     ends = torch.zeros(3, dtype=torch.int32, device=DEV)
     x, dy = torch.empty((0, 64), dtype=torch.bfloat16, device=DEV), torch.empty((0, 32), dtype=torch.bfloat16, device=DEV)
