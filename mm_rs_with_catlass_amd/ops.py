@@ -637,10 +637,14 @@ def fp8_matmul_allreduce(x1, x2, scale_x1, scale_x2, peers=(), rank=0, rank_size
     return out
 
 
-def _want_groups(x, group_ends, groups):
-    _want(group_ends, "group_ends", torch.int32, 1, None, (groups,))
-    if groups < 1:
+def _want_groups(group_ends, groups=None):
+    """How many groups there are (groups: how many there must be)."""
+    if not isinstance(group_ends, torch.Tensor):
+        _fail("group_ends must be an int32 tensor on the GPU (got %s)", type(group_ends).__name__)
+    _want(group_ends, "group_ends", torch.int32, 1, None, None if groups is None else (groups,))
+    if group_ends.numel() < 1:
         _fail("there must be at least one group")
+    return group_ends.numel()
 
 
 def grouped_matmul(x, w, group_ends, trans_b=False, out=None, tile=None):
@@ -660,7 +664,7 @@ def grouped_matmul(x, w, group_ends, trans_b=False, out=None, tile=None):
     groups, n = w.shape[0], w.shape[1 if trans_b else 2]
     if w.shape[2 if trans_b else 1] != k:
         _fail("w has shape %s: its k extent does not match x's k = %d", tuple(w.shape), k)
-    _want_groups(x, group_ends, groups)
+    _want_groups(group_ends, groups)
     _want(out, "out", x.dtype, 2, None, (rows, n))
     _check_dev(x, w, group_ends, *(() if out is None else (out,)))
     if out is None:
@@ -684,8 +688,7 @@ def grouped_matmul_dw(x, dy, group_ends, out_dtype=None, trans_b=False, out=None
     n = dy.shape[1]
     if dy.shape[0] != rows:
         _fail("dy has %d rows, x has %d", dy.shape[0], rows)
-    groups = group_ends.numel()
-    _want_groups(x, group_ends, groups)
+    groups = _want_groups(group_ends)
     od = out.dtype if out is not None else x.dtype if out_dtype is None else out_dtype
     odt = 0 if od == torch.float32 else _type16(od, "out_dtype")
     shape = (groups, n, k) if trans_b else (groups, k, n)
@@ -713,7 +716,7 @@ def grouped_fp8_matmul(x, w, scale_x, scale_w, group_ends, out_dtype=torch.bfloa
         _fail("w has shape %s: its k extent does not match x's k = %d", tuple(w.shape), k)
     _want(scale_x, "scale_x", torch.float32, 2, None, (_blocks(k), rows))
     _want(scale_w, "scale_w", torch.float32, 3, None, (groups, _blocks(n), _blocks(k)))
-    _want_groups(x, group_ends, groups)
+    _want_groups(group_ends, groups)
     dt = _type16(out.dtype if out is not None else out_dtype, "out" if out is not None else "out_dtype")
     _want(out, "out", None, 2, None, (rows, n))
     _check_dev(x, w, scale_x, scale_w, group_ends, *(() if out is None else (out,)))

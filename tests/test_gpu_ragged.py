@@ -580,3 +580,62 @@ def test_tiles_that_do_not_exist_are_refused():
         ops.grouped_matmul(x[:, :63].contiguous(), w[:, :63].contiguous(), ends, tile=(128, 128, 1))
     with pytest.raises(L.CatcocError, match="no kernel of"):
         ops.grouped_matmul_dw(x, dy, ends, tile=(128, 128, 2))
+
+
+class Nothing:
+    """In the place of the compiled calls: leaves every call to the Python path."""
+
+    def __getattr__(self, name):
+        return lambda *a: None
+
+
+def both_calls(monkeypatch, fn, *a, **kw):
+    """What the compiled and the Python path make of a call: results, or the error's text."""
+    seen = []
+    for host in (None, Nothing()):
+        with monkeypatch.context() as m:
+            if host is not None:
+                m.setattr(ops, "_host", host)
+            try:
+                r = fn(*a, **kw)
+                seen.append([t.clone().view(torch.uint8) if t.dtype == F8 else t.clone() for t in (r if isinstance(r, tuple) else (r,))])
+            except L.CatcocError as e:
+                seen.append(str(e))
+    assert type(seen[0]) is type(seen[1])
+    if isinstance(seen[0], str):
+        assert seen[0] == seen[1]
+        return False
+    assert all(torch.equal(p, q) for p, q in zip(*seen))
+    return True
+
+
+def test_the_compiled_call_and_the_python_path_answer_alike(monkeypatch):
+    g = gen(31)
+    rows, k, n, groups = 20, 256, 130, 3
+    x, dy = randn(g, rows, k, dtype=torch.bfloat16), randn(g, rows, n, dtype=torch.bfloat16)
+    w, ends = randn(g, groups, n, k, dtype=torch.bfloat16), ends_of([4, 0, 16])
+    (x8, sx), (w8, sw) = ops.quantize_fp8(x), ops.quantize_fp8(w[0], block_rows=128)
+    ws8, ssw = torch.stack([w8.view(torch.uint8)] * groups).view(F8), torch.stack([sw] * groups)
+    peers = [randn(g, rows + 3, n + 2) for _ in range(2)]
+    wide = randn(g, rows, 2 * k, dtype=torch.bfloat16)
+    q, f, m, d, e = ops.quantize_fp8, ops.fp8_matmul_allreduce, ops.grouped_matmul, ops.grouped_matmul_dw, ops.grouped_fp8_matmul
+
+    def alike(fn, *a, **kw):
+        return both_calls(monkeypatch, fn, *a, **kw)
+    for fn, a, kw in ((q, (x,), {}), (q, (x.float(), 128), {}), (q, (wide,), {"gated": True}), (q, (torch.nn.Parameter(x),), {}),
+                      (q, (x,), {"out": torch.empty_like(x8), "scale": torch.empty_like(sx)}),
+                      (f, (x8, w8, sx, sw), {}), (f, (x8, w8, sx, sw, peers, 1, 3, torch.float16, 2), {}), (f, (x8, w8, sx, sw, tuple(peers)), {"rank_size": 3}),
+                      (f, (x8, w8, sx, sw), {"out": torch.empty((rows, n), dtype=torch.float16, device=DEV)}),
+                      (m, (x, w, ends), {"trans_b": True}), (m, (dy, w, ends), {}), (d, (x, dy, ends), {}), (d, (x, dy, ends, torch.float32, True), {}),
+                      (d, (x, dy, ends), {"out": torch.empty((groups, k, n), device=DEV)}), (e, (x8, ws8, sx, ssw, ends), {}), (e, (x8, ws8, sx, ssw, ends, torch.float16), {})):
+        assert alike(fn, *a, **kw), (fn.__name__, kw)
+    for fn, a, kw in ((q, (x.int(),), {}), (q, (wide[:, ::2],), {}), (q, (x, 64), {}), (q, (x, 128, True), {}), (q, (x,), {"out": x}), (q, (x,), {"scale": sx[:, 1:]}),
+                      (q, (x.cpu(),), {}), (q, (x[0],), {}),
+                      (f, (x8, w8, sx.cpu(), sw), {}), (f, (x8, w8[:, 1:], sx, sw), {}), (f, (x8, w8, sx, sw, peers), {}), (f, (x8, w8, sx, sw, peers, 3, 3), {}),
+                      (f, (x8, w8, sx, sw, peers, 0, 3, torch.bfloat16, 4), {}), (f, (x8, w8, sx, sw, [peers[0], peers[1].half()], 0, 3), {}),
+                      (f, (x8, w8, sx, sw), {"out_dtype": torch.float32}), (f, (x8, w8, sx, sw), {"out": torch.empty((rows, n), device=DEV)}),
+                      (m, (x, w, ends), {}), (m, (x, w.half(), ends, True), {}), (m, (x, w, ends.long(), True), {}), (m, (x, w, ends[:2], True), {}),
+                      (m, (x, w, ends, True), {"out": torch.empty((rows, n), device=DEV)}), (m, (x[:, ::2], w[:, :, ::2], ends, True), {}),
+                      (d, (x, dy[1:], ends), {}), (d, (x, dy, ends, torch.float64), {}), (d, (x, dy, ends.cpu()), {}), (d, (x, dy, [4, 4, 20]), {}),
+                      (e, (x8, ws8, sx, sw, ends), {}), (e, (x8, ws8, sx, ssw, ends, torch.float32), {}), (e, (x, ws8, sx, ssw, ends), {})):
+        assert not alike(fn, *a, **kw), (fn.__name__, kw)

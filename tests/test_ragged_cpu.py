@@ -70,6 +70,7 @@ def test_grouped_operators_refuse():
     refuses("out_dtype must be", d, x, dy, ends, out_dtype=torch.float64)
     refuses("out must have shape", d, x, dy, ends, out=torch.empty((groups, n, k), dtype=torch.float32))
     refuses("group_ends must be", d, x, dy, ends.float())
+    refuses("group_ends must be", d, x, dy, [1, 2, 10])
     refuses("must live on the GPU", d, x, dy, ends)
     q = ops.grouped_fp8_matmul
     x8, w8 = torch.zeros((rows, k), dtype=F8), torch.zeros((groups, n, k), dtype=F8)
