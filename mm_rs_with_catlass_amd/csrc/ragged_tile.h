@@ -394,18 +394,32 @@ __global__ void __launch_bounds__(128 * WY * KG, 2) ragged_tile_kernel(const Rag
     Loop loop;
     typename Loop::Problem p;
 
+    uint32_t order = 0;   // DW: lane i's group is the i-th of up to 64, those with most rows first
+    if constexpr (DW) {
+        if (args.groups <= 64u) {
+            uint32_t b = 0, e = 0, rank = lane;
+            if (lane < args.groups) group_rows(args, lane, b, e);
+            if (lane < args.groups) rank = 0;
+            for (uint32_t g = 0; g < args.groups; ++g) {
+                const uint32_t rows = (uint32_t)__builtin_amdgcn_readlane((int)(e - b), (int)g);
+                if (lane < args.groups) rank += rows > e - b || (rows == e - b && g < lane) ? 1u : 0u;
+            }
+            order = (uint32_t)__builtin_amdgcn_ds_permute((int)(rank * 4u), (int)lane);
+        }
+    }
     // Tile `at` of this launch; DW: t.group's rows are the sum, t.row and t.rows rows of the result.
     uint32_t sumBegin = 0, sumEnd = 0;
     auto find = [&](uint32_t &at, RaggedTile &t) {
         if constexpr (DW) {
-            // every XCD gets an eighth of each group's tiles: they cost what the group has rows
+            // every XCD gets an eighth of each group's tiles: they cost what the group has rows; its workgroups take them in turns, forth and back
             const uint32_t pt = (args.k + BX - 1u) / BX, tiles = pt * nt, share = (tiles + 7u) / 8u;
             uint32_t in;
             do {
-                const uint32_t j = at >> 3;
+                const uint32_t per = gridDim.x >> 3, turn = (at >> 3) / per, place = (at >> 3) - turn * per, j = turn * per + (turn & 1u ? per - 1u - place : place);
                 if (j >= args.groups * share) return false;
                 t.group = j / share;
                 in = ((at + t.group) & 7u) * share + j - t.group * share;
+                if (args.groups <= 64u) t.group = (uint32_t)__builtin_amdgcn_readlane((int)order, (int)__builtin_amdgcn_readfirstlane((int)t.group));
                 if (in >= tiles) at += gridDim.x;
             } while (in >= tiles);
             t.colTile = in / pt;
