@@ -62,6 +62,43 @@ struct RaggedTile {
     uint32_t group, row, rows, colTile;
 };
 
+// Which of up to 64 groups (or the rows past the last one) workgroup `wg` works for where every XCD gets an eighth of each group's tiles, the highest first;
+// count: the group's row tiles, local: which of its tiles.  False: none.
+__device__ __forceinline__ bool dealt_group(const RaggedArgs &args, uint32_t wg, uint32_t bx, uint32_t nt, uint32_t &group, uint32_t &begin, uint32_t &end, uint32_t &count, uint32_t &local)
+{
+    const uint32_t lane = threadIdx.x & 63u;
+    uint32_t b, e;
+    group_rows(args, umin(lane, args.groups - 1u), b, e);
+    const uint32_t mine = lane < args.groups ? (e - b + bx - 1u) / bx : 0u, height = mine ? (e - b + 32u * mine - 1u) / (32u * mine) : 0u;
+    uint32_t rank = 0, before = 0;   // by height, at most 256 / 32
+#pragma unroll
+    for (uint32_t h = 9; h-- > 0u;) {
+        const uint64_t same = __ballot(height == h);
+        if (height == h) rank = before + (uint32_t)__builtin_popcountll(same & ((1ull << lane) - 1ull));
+        before += (uint32_t)__builtin_popcountll(same);
+    }
+    const uint32_t order = (uint32_t)__builtin_amdgcn_ds_permute((int)(rank * 4u), (int)lane);
+    // lane i: the i-th group's tiles, and those of them that this XCD gets; what is left of a division by eight goes to the XCDs in turn
+    const uint32_t tiles = (uint32_t)__builtin_amdgcn_ds_permute((int)(rank * 4u), (int)(mine * nt)), each = tiles >> 3, rest = tiles & 7u;
+    const uint32_t place = (wg - (wave_prefix(rest) - rest)) & 7u, part = each + (place < rest ? 1u : 0u), upTo = wave_prefix(part), j = wg >> 3;
+    const uint64_t past = __ballot(upTo > j);
+    if (past == 0) {   // rows past the last group
+        group = args.groups;
+        begin = (uint32_t)__builtin_amdgcn_readlane((int)e, 63);
+        end = args.rows;
+        count = (end - begin + bx - 1u) / bx;
+        local = 8u * (j - (uint32_t)__builtin_amdgcn_readlane((int)upTo, 63)) + (wg & 7u);
+        return local < count * nt;
+    }
+    const int l = __builtin_ctzll(past);
+    local = (uint32_t)__builtin_amdgcn_readlane((int)(place * each + umin(place, rest) + j + part - upTo), l);
+    group = (uint32_t)__builtin_amdgcn_readlane((int)order, l);
+    begin = (uint32_t)__builtin_amdgcn_readlane((int)b, (int)group);
+    end = (uint32_t)__builtin_amdgcn_readlane((int)e, (int)group);
+    count = (uint32_t)__builtin_amdgcn_readlane((int)mine, (int)group);
+    return true;
+}
+
 // Tile of workgroup `wg` where a group's rows are cut into tiles of at most bx rows of about the same height (whole `unit`s), nt column tiles.  A group's tiles follow each
 // other, eight row tiles to a band and column by column within it: the tiles that run on an XCD at a time share few rows and columns.  Every wave
 // works it out by itself, 64 groups at a time.  False: no tile left.
@@ -76,6 +113,8 @@ __device__ __forceinline__ bool ragged_tile(const RaggedArgs &args, uint32_t wg,
         t.group = 0;
         begin = 0;
         end = args.rows;
+    } else if (args.dealt) {
+        if (!dealt_group(args, wg, bx, nt, t.group, begin, end, count, local)) return false;
     } else {
         uint32_t total = 0, b = 0, e = 0, tiles = 0, upTo = 0;
         const uint32_t chunks = args.groups / 64u + 1u;   // (one group more than there are: the rows past the last one)

@@ -62,6 +62,12 @@ constexpr Choice kSmallKn[] = {{Choice::SMALL, 16, 64, 4}, {Choice::SMALL, 32, 6
 constexpr Choice kTeams64{Choice::TILE, 64, 128, 2}, kTeams128{Choice::TILE, 128, 128, 2}, kTile128{Choice::TILE, 128, 128, 1}, kTile256{Choice::TILE, 256, 256, 1};
 constexpr uint32_t kLeastRows = 96;   // tiles of 256 columns: 96 to 256 rows in steps of 32
 
+// Whether each group's tiles are dealt out to all XCDs, the highest first, or every XCD gets a run of all tiles: dealt out they end together, but every XCD reads
+// every group's rows, which has to be less than the matrices; runs of many groups end together by themselves.  Measured (us, run / dealt, tiles of at most 256
+// rows, 16 bits): 15 groups of together 4099 rows, 3584x4096, 192 / 173; 16 of 4096, 4096x3584, 177 / 160; 24 of 6000, 4096x3584, 251 / 224; 48 of 12000, 2048x2048,
+// 164 / 147; 62 of 16384, 4096x3584, 575 / 581 (160 rows); and where the rows are more than the matrices 16 of 12000, 4096x1792, 197 / 210 and 8 of 4096 59 / 65 (128 rows).
+bool deal(const RaggedArgs &a) { return a.ends && a.groups <= 48 && 8ull * a.rows <= (uint64_t)std::min(a.groups, a.rows) * a.n; }
+
 // By what a launch is estimated to take, in us: the larger of what memory needs for each byte once (5.7 GB/ms; `reach`: over what a kernel reaches of it in several rounds) and of its
 // rounds of workgroups, a quarter of the smaller, and a start.  A round costs its steps of 128 bytes of k, `step` us each with the GPU full, `few` of that with
 // at most one workgroup a CU.  Fitted to, and compared on, 84 sizes that ran on all of these kernels (1 to 8192 rows of e4m3 against 2048 to 8192 columns and
@@ -74,6 +80,7 @@ Choice choose(uint32_t dtype, const RaggedArgs &a, bool kn)
     const double es = f8 ? 1 : 2, steps = (double)cdiv(a.k * (uint64_t)es, 128);
     const double active = a.ends ? std::min(a.groups, a.rows) : 1, mean = a.rows / active;
     const double mem = (active * a.k * a.n * es + a.rows * (double)a.k * es + a.rows * (double)a.n * (2.0 + 4.0 * a.nPeers)) / 5.7e6;
+    const bool dealt = deal(a);
     Choice best = kTile256;
     double least = 0;
     // Groups are taken to have 0.4, 0.6 .. 1.6 of the mean: how many tiles of at most `rows` that makes, and how high they are, in 32 rows (no less than two).
@@ -84,7 +91,7 @@ Choice choose(uint32_t dtype, const RaggedArgs &a, bool kn)
             tiles += t;
             high += t * std::max(2.0, std::ceil(group / t / 32));
         }
-        if (height) *height = a.ends ? 0.8 * high / tiles + 0.2 * std::min(rows / 32.0, std::max(2.0, std::ceil(mean * 1.6 / 32))) : high / tiles;   // (a round ends with its highest)
+        if (height) *height = a.ends && !dealt ? 0.8 * high / tiles + 0.2 * std::min(rows / 32.0, std::max(2.0, std::ceil(mean * 1.6 / 32))) : high / tiles;   // (a round ends with its highest)
         return a.ends ? active * tiles / 7 : tiles;
     };
     auto offer = [&](const Choice &c, double start, double slots, double step, double few, double reach) {
@@ -110,7 +117,7 @@ Choice choose(uint32_t dtype, const RaggedArgs &a, bool kn)
         double height;   // above five two stages instead of three
         row_tiles(rows, &height);
         offer({Choice::TILE, rows, 256, 1}, 8, 256, f8 ? 0.35 + 0.19 * height + (height > 5 ? 0.05 : 0) : height > 5 ? 0.65 + 0.11 * height : 0.45 + 0.115 * height, 1,
-              (f8 ? 1.15 : 0.98) + (rows > 160 ? 0.05 : 0));
+              (f8 ? 1.15 : 0.98) + (rows > 160 && !dealt ? 0.05 : 0));
     }
     return best;
 }
@@ -158,6 +165,8 @@ void run(uint32_t dtype, const RaggedArgs &args, bool kn, bool dw, const CatcocT
     a.tileRows = c.rows;
     const uint64_t nt = cdiv(a.n, c.cols);
     uint64_t wgs = most_row_tiles(a, c.rows) * nt;
+    a.dealt = c.kind == Choice::TILE && !dw && deal(a);
+    if (a.dealt) wgs = cdiv(wgs, 8) * 8 + 8;   // (an XCD's eighths of the groups and of the rows behind them are rounded by themselves)
     if (dw) {
         wgs = a.groups * cdiv(a.k, c.rows) * nt;
         if (c.kind == Choice::TILE)   // eighths of every group's tiles, dealt out to one workgroup a CU (two of 128 columns)

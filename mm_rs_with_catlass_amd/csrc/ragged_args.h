@@ -26,6 +26,7 @@ struct RaggedArgs {
     uint32_t nPeers;
     uint32_t rows, k, n, groups;
     uint32_t outType;          // 0 (fp32), DT_F16, DT_BF16
+    uint32_t dealt;            // groups' tiles are dealt out to the XCDs (dealt_group), not a run of them to each
     uint32_t tileRows;         // large tiles: at most so many rows each, a multiple of 32 and no more than the kernel's
 };
 

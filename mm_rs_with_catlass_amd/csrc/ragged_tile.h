@@ -1,8 +1,9 @@
 // Ragged products on large tiles fed by copies that go straight to LDS.
 //
 // What bounds them: a step of a 256x256 tile multiplies 64 KiB that come from the L2 at 56 to 72 GB/s a CU, about as long as its MFMAs take in 16 bits and e4m3
-// alike (a step is 128 bytes of k).  So tiles are as large as registers allow, and a copy has a whole step or two to arrive.  Measured: e4m3 8192x27392x4096 750 us (2.45 PFLOP/s; a library product of 8192^3 reaches 2.73), 16384 rows in 62 groups of 4096x3584 in 16 bits
-// 565 us (850 TFLOP/s, 3.6 TB/s), in e4m3 318 us (1.5 PFLOP/s), weight gradients of 8 groups of 2048 rows, 4096x1792, 240 us (1.0 PFLOP/s).
+// alike (a step is 128 bytes of k).  So tiles are as large as registers allow, and a copy has a whole step or two to arrive.  Measured: e4m3 8192x27392x4096 750 us
+// (2.45 PFLOP/s; a library product of 8192^3 reaches 2.73), 16384 rows in 62 groups of 4096x3584 in 16 bits 570 us (840 TFLOP/s, 3.6 TB/s), in e4m3 320 us (1.5
+// PFLOP/s), weight gradients of 8 uneven groups of together 16384 rows, 4096x1792, 226 us (1.07 PFLOP/s; 240 with the groups in their own order).
 #pragma once
 #include "ragged_checked.h"
 
@@ -376,7 +377,7 @@ struct RaggedTileLoop {
 
 // DW: x and w are rows of k (the group's rows), the result is the group's [k, n] matrix.  KN: w is [k, n].
 // A weight gradient's workgroups walk several tiles: few rows make few steps, and a tile's first copies are on their way while the one before is stored.
-// 4099 rows in 15 groups, 4096x3584 in fp32, 330 us: 150 without the stores, and the stores alone take 176 in this order (881 MB, 5.0 TB/s).  They do not overlap:
+// 4099 rows in 15 groups, 4096x3584 in fp32, 325 us: 150 without the stores, and the stores alone take 176 in this order (881 MB, 5.0 TB/s).  They do not overlap:
 // 128x256 tiles that store a tile piece by piece between the next one's steps took 373 us, five stages of 32 rows that leave 2.5 us of work in LDS 326 (and
 // the long sums of 8 groups of 2048 rows 271 instead of 240).
 template <uint32_t DT, bool KN, bool DW, int WY, int NIMAX, int KG>

@@ -504,6 +504,25 @@ def test_every_tile_of_weight_gradients(name, k, n, tile, out_dtype):
             close(dw[e].t() if trans_b else dw[e], a.t() @ d, a.abs().t() @ d.abs(), j - i, out_dtype)
 
 
+# Groups of very different heights, rows past the last one, more row tiles than a band has: each group's tiles go to all XCDs (fewer rows than matrices) ...
+@pytest.mark.parametrize("tile,trans_b", [(t, b) for b in (False, True) for t in TILES + (SMALL_NK if b else SMALL_KN) + [None]])
+@pytest.mark.parametrize("groups", [28, 48, 64])   # (... but not with 64)
+def test_tiles_of_uneven_groups(groups, tile, trans_b):
+    k, n = 192, 776
+    counts = [900, 0, 3, 64] + [0] * (groups - 8) + [130, 131, 1, 259]
+    g = gen(groups)
+    rows = sum(counts)
+    x = randn(g, rows + 333, k, dtype=torch.bfloat16)
+    x[rows:] = float("nan")
+    w = randn(g, groups, n, k, dtype=torch.bfloat16) if trans_b else randn(g, groups, k, n, dtype=torch.bfloat16)
+    out = ops.grouped_matmul(x, w, ends_of(counts), trans_b=trans_b, tile=tile)
+    for e, (i, j) in enumerate(ranges(counts)):
+        a, b = x[i:j].double(), w[e].double()
+        b = b.t() if trans_b else b
+        close(out[i:j], a @ b, a.abs() @ b.abs(), k, torch.bfloat16)
+    assert (out[rows:] == 0).all()
+
+
 # Several tiles for each workgroup, with every number of steps, of rows in the last one and of tiles without rows between them.
 @pytest.mark.parametrize("tile", TILES_DW)
 @pytest.mark.parametrize("k,n", [(1024, 768), (1030, 700), (896, 1032)])
