@@ -12,20 +12,40 @@ from . import ops
 
 
 class GroupedLinear(torch.autograd.Function):
-    """y[i] = w[e] x[i] for the rows i of group e; w [groups, out, in].  Both gradients are grouped products as well."""
+    """y[i] = w[e] x[i] for the rows i of group e; w [groups, out, in] ([groups, in, out] without trans_b).  Both gradients are grouped
+    products as well, and differentiable in their turn."""
 
     @staticmethod
-    def forward(ctx, x, w, ends):
+    def forward(ctx, x, w, ends, trans_b=True):
         ctx.save_for_backward(x, w, ends)
-        return ops.grouped_matmul(x, w, ends, trans_b=True)
+        ctx.trans_b = trans_b
+        return ops.grouped_matmul(x, w, ends, trans_b=trans_b)
 
     @staticmethod
     def backward(ctx, dy):
         x, w, ends = ctx.saved_tensors
         dy = dy.contiguous()
-        dx = ops.grouped_matmul(dy, w, ends) if ctx.needs_input_grad[0] else None
-        dw = ops.grouped_matmul_dw(x, dy, ends, out_dtype=w.dtype, trans_b=True) if ctx.needs_input_grad[1] else None
-        return dx, dw, None
+        dx = GroupedLinear.apply(dy, w, ends, not ctx.trans_b) if ctx.needs_input_grad[0] else None
+        dw = GroupedOuter.apply(x, dy, ends, ctx.trans_b) if ctx.needs_input_grad[1] else None
+        return dx, dw, None, None
+
+
+class GroupedOuter(torch.autograd.Function):
+    """The weight gradient of GroupedLinear: dw[e] = sum over the rows i of group e of dy[i] x[i]^T (of x[i] dy[i]^T without trans_b)."""
+
+    @staticmethod
+    def forward(ctx, x, dy, ends, trans_b):
+        ctx.save_for_backward(x, dy, ends)
+        ctx.trans_b = trans_b
+        return ops.grouped_matmul_dw(x, dy, ends, trans_b=trans_b)
+
+    @staticmethod
+    def backward(ctx, g):
+        x, dy, ends = ctx.saved_tensors
+        g = g.contiguous()
+        dx = GroupedLinear.apply(dy, g, ends, not ctx.trans_b) if ctx.needs_input_grad[0] else None
+        ddy = GroupedLinear.apply(x, g, ends, ctx.trans_b) if ctx.needs_input_grad[1] else None
+        return dx, ddy, None, None
 
 
 def sort_by_expert(choice, experts):

@@ -1,0 +1,75 @@
+"""The layer of experts without a GPU: plain products stand in for the grouped operators.  As the kernels' do, their results carry no graph."""
+import pytest
+import torch
+
+from mm_rs_with_catlass_amd import experts as E
+
+
+def groups_of(ends, rows):
+    begin = 0
+    for e, end in enumerate(ends.tolist()):
+        yield e, begin, end
+        begin = end
+    assert begin <= rows
+
+
+@torch.no_grad()
+def grouped_matmul(x, w, ends, trans_b=False):
+    y = x.new_zeros((x.shape[0], w.shape[1 if trans_b else 2]))
+    for e, i, j in groups_of(ends, x.shape[0]):
+        y[i:j] = x[i:j] @ (w[e].t() if trans_b else w[e])
+    return y
+
+
+@torch.no_grad()
+def grouped_matmul_dw(x, dy, ends, out_dtype=None, trans_b=False):
+    a, b = (dy, x) if trans_b else (x, dy)
+    dw = a.new_zeros((ends.numel(), a.shape[1], b.shape[1]), dtype=out_dtype or x.dtype)
+    for e, i, j in groups_of(ends, x.shape[0]):
+        dw[e] = a[i:j].t() @ b[i:j]
+    return dw
+
+
+@pytest.fixture(autouse=True)
+def stand_in(monkeypatch):
+    monkeypatch.setattr(E.ops, "grouped_matmul", grouped_matmul)
+    monkeypatch.setattr(E.ops, "grouped_matmul_dw", grouped_matmul_dw)
+
+
+def randn(seed, *shape, dtype=torch.float64):
+    return torch.randn(shape, generator=torch.Generator().manual_seed(seed), dtype=dtype)
+
+
+def test_first_and_second_gradients_of_a_grouped_product_against_differences():
+    ends = torch.tensor([2, 2, 5], dtype=torch.int32)     # (one group without rows, two rows of no group)
+    x, w = randn(1, 7, 4).requires_grad_(), randn(2, 3, 5, 4).requires_grad_()
+
+    def f(a, b):
+        return E.GroupedLinear.apply(a, b, ends)
+    assert torch.autograd.gradcheck(f, (x, w))
+    assert torch.autograd.gradgradcheck(f, (x, w))
+
+
+def plain_experts(x, w_gate_up, w_down, choice, share):
+    rows = []
+    for t in range(x.shape[0]):
+        row = torch.zeros_like(x[t])
+        for j in range(choice.shape[1]):
+            gate, up = (w_gate_up[choice[t, j]] @ x[t]).chunk(2)
+            row = row + share[t, j] * (w_down[choice[t, j]] @ (torch.nn.functional.silu(gate) * up))
+        rows.append(row)
+    return torch.stack(rows)
+
+
+def test_a_penalty_on_first_gradients_reaches_all_operands():
+    # everything in fp32 against 64 bits: sums of at most 12 x 16 products, five of them behind each other
+    tokens, hidden, inter, count, top = 6, 12, 8, 4, 2
+    choice = torch.stack([torch.randperm(count, generator=torch.Generator().manual_seed(t))[:top] for t in range(tokens)])
+    values = [randn(11, tokens, hidden), 0.5 * randn(12, count, 2 * inter, hidden), 0.5 * randn(13, count, hidden, inter), randn(14, tokens, top).abs()]
+    results = []
+    for layer, dtype in ((E.experts, torch.float32), (plain_experts, torch.float64)):
+        x, w1, w2, share = leaves = [v.to(dtype).requires_grad_() for v in values]
+        first = torch.autograd.grad(layer(x, w1, w2, choice, share).square().sum(), leaves, create_graph=True)
+        results.append(torch.autograd.grad(sum(g.square().sum() for g in first), leaves))
+    for got, want in zip(*results):
+        assert (got.double() - want).norm() <= 1e-4 * want.norm()

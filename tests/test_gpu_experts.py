@@ -143,3 +143,29 @@ def test_command(capsys):
     losses = [float(s.split()[-1]) for s in lines[:-1]]
     assert losses[-1] < 0.5 * losses[0]
     assert float(lines[-1].split("%")[0].split()[-1]) <= 10.5
+
+
+def test_second_gradients():
+    """L = <c, dx> + <d, dw> of a grouped product's first gradients: each of L's gradients is one or two products of given values."""
+    from mm_rs_with_catlass_amd.experts import GroupedLinear
+    dtype, counts, k, n = torch.bfloat16, [5, 0, 70, 33], 72, 136
+    g = torch.Generator().manual_seed(8)
+    rows, groups = sum(counts) + 4, len(counts)           # (four rows of no group)
+    x, dy, c = (torch.randn(rows, width, generator=g).to(dtype) for width in (k, n, k))
+    w, d = (torch.randn(groups, n, k, generator=g).to(dtype) for _ in range(2))
+    ends = torch.tensor(counts).cumsum(0).to(torch.int32).cuda()
+    x1, w1, dy1 = (t.cuda().requires_grad_() for t in (x, w, dy))
+    dx, dw = torch.autograd.grad(GroupedLinear.apply(x1, w1, ends), (x1, w1), dy1, create_graph=True)
+    got = torch.autograd.grad((dx.float() * c.cuda().float()).sum() + (dw.float() * d.cuda().float()).sum(), (x1, w1, dy1))
+    at = 0
+    for e, count in enumerate(counts):
+        i = slice(at, at + count)
+        at += count
+        if count == 0:
+            assert not got[1][e].any()
+            continue
+        xs, ys, cs, ws, ds = (Near(t.double()) for t in (x[i], dy[i], c[i], w[e], d[e]))
+        (ys @ ds).rounded(dtype).holds(got[0][i], "the gradient of x")
+        (ys.t() @ cs).rounded(dtype).holds(got[1][e], "the gradient of w")
+        ((cs @ ws.t()).rounded(dtype) + (xs @ ds.t()).rounded(dtype)).rounded(dtype).holds(got[2][i], "the gradient of dy")
+    assert not got[0][at:].any() and not got[2][at:].any()
