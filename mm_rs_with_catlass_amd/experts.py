@@ -50,11 +50,13 @@ class GroupedOuter(torch.autograd.Function):
 
 def sort_by_expert(choice, experts):
     """choice [tokens, top], each token's experts -> (order, back, ends): row i of the sorted rows is choice order[i] of the flattened ones,
-    back undoes it, group_ends for the operators.  Nothing is read back to the host."""
-    flat = choice.reshape(-1)
+    back undoes it, group_ends for the operators.  Nothing is read back to the host.  Choices below 0 or past the last expert (a dropped token) are
+    sorted behind the last group: rows of no group, whose results and gradients are zeros."""
+    flat = choice.reshape(-1).long()
+    flat = torch.where(flat < 0, experts, flat)
     order = torch.argsort(flat, stable=True)
     back = torch.empty_like(order).scatter_(0, order, torch.arange(order.numel(), device=order.device))
-    ends = torch.searchsorted(flat[order], torch.arange(experts, device=flat.device, dtype=flat.dtype), right=True).to(torch.int32)
+    ends = torch.searchsorted(flat[order], torch.arange(experts, device=flat.device), right=True).to(torch.int32)
     return order, back, ends
 
 
@@ -70,7 +72,7 @@ def gather(y, share, back):
 
 def experts(x, w_gate_up, w_down, choice, share):
     """x [tokens, hidden] fp16 or bf16, w_gate_up [experts, 2 inter, hidden], w_down [experts, hidden, inter], choice and share [tokens, top]:
-    each token's experts and their weights.  Returns [tokens, hidden]; differentiable in x, both weights and share."""
+    each token's experts (none: -1) and their weights.  Returns [tokens, hidden]; differentiable in x, both weights and share."""
     order, back, ends = sort_by_expert(choice, w_gate_up.shape[0])
     h = GroupedLinear.apply(spread(x, choice.shape[1], order), w_gate_up, ends)
     gate, up = h.float().chunk(2, 1)

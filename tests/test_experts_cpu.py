@@ -73,3 +73,26 @@ def test_a_penalty_on_first_gradients_reaches_all_operands():
         results.append(torch.autograd.grad(sum(g.square().sum() for g in first), leaves))
     for got, want in zip(*results):
         assert (got.double() - want).norm() <= 1e-4 * want.norm()
+
+
+@pytest.mark.parametrize("dtype", [torch.int64, torch.int32, torch.int16])
+def test_choices_of_no_expert_take_part_in_nothing(dtype):
+    choice = torch.tensor([[3, -1], [1, 5], [-7, 9], [0, 3]], dtype=dtype)
+    order, back, ends = E.sort_by_expert(choice, 4)
+    assert ends.tolist() == [1, 2, 2, 4] and ends.dtype == torch.int32
+    few = torch.tensor([[127], [-1], [0]], dtype=torch.int8)       # (as many experts as the type has)
+    assert E.sort_by_expert(few, 128)[2].tolist() == [1] * 127 + [2]
+    assert choice.flatten()[order[:4]].tolist() == [0, 1, 3, 3] and order[back].tolist() == list(range(8))
+
+    tokens, hidden, inter = 4, 6, 5
+    values = [randn(21, tokens, hidden), randn(22, 4, 2 * inter, hidden), randn(23, 4, hidden, inter), randn(24, tokens, 2).abs()]
+    dropped = (choice < 0) | (choice >= 4)
+    results = []
+    for mine in (choice, torch.where(dropped, 0, choice)):     # (as expert 0's with no weight)
+        leaves = [v.float().requires_grad_() for v in values]
+        x, w1, w2, share = leaves
+        out = E.experts(x, w1, w2, mine, torch.where(dropped, 0, share) if mine is not choice else share)
+        results.append([out, *torch.autograd.grad(out.square().sum(), leaves)])
+    for got, want in zip(*results):
+        assert torch.allclose(got, want, rtol=1e-5, atol=1e-5)      # sums of the same values, in another order
+    assert not results[0][0][2].any()

@@ -169,3 +169,20 @@ def test_second_gradients():
         (ys.t() @ cs).rounded(dtype).holds(got[1][e], "the gradient of w")
         ((cs @ ws.t()).rounded(dtype) + (xs @ ds.t()).rounded(dtype)).rounded(dtype).holds(got[2][i], "the gradient of dy")
     assert not got[0][at:].any() and not got[2][at:].any()
+
+
+def test_tokens_without_an_expert():
+    from mm_rs_with_catlass_amd.experts import ServedExperts, experts
+    x, w1, w2, choice, share = (t.cuda() for t in layer(9, 50, 256, 128, 5, 2, torch.bfloat16))
+    whole = experts(x, w1, w2, choice, share), ServedExperts(w1, w2)(x, choice, share)
+    choice[7], choice[20, 1], choice[21, 0] = -1, -1, 5
+    kept = torch.where((choice >= 0) & (choice < 5), share, 0)       # the same with no weight, which changes no product
+    same = torch.where((choice >= 0) & (choice < 5), choice, 0)
+    for got, want, before in zip((experts(x, w1, w2, choice, share), ServedExperts(w1, w2)(x, choice, share)),
+                                 (experts(x, w1, w2, same, kept), ServedExperts(w1, w2)(x, same, kept)), whole):
+        # (the choice of a tile, and with it the order of a sum in fp32, may differ: a rounding of each sum, and of what is added up)
+        assert ((got.double() - want.double()).abs() <= 4 * U[torch.bfloat16] * before.double().abs().amax()).all()
+        assert not got[7].any()
+        rest = torch.ones(50, dtype=torch.bool)
+        rest[[7, 20, 21]] = False
+        assert ((got[rest].double() - before[rest].double()).abs() <= 4 * U[torch.bfloat16] * before.double().abs().amax()).all()
