@@ -67,7 +67,7 @@ def spread(x, top, order):
 
 def gather(y, share, back):
     """The experts' rows back at their tokens, weighted (summed in fp32, rounded once)."""
-    return (y[back].view(*share.shape, -1).float() * share.float().unsqueeze(-1)).sum(1).to(y.dtype)
+    return (y[back].view(*share.shape, y.shape[1]).float() * share.float().unsqueeze(-1)).sum(1).to(y.dtype)
 
 
 def experts(x, w_gate_up, w_down, choice, share):

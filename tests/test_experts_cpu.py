@@ -96,3 +96,12 @@ def test_choices_of_no_expert_take_part_in_nothing(dtype):
     for got, want in zip(*results):
         assert torch.allclose(got, want, rtol=1e-5, atol=1e-5)      # sums of the same values, in another order
     assert not results[0][0][2].any()
+
+
+def test_no_tokens():
+    x, w1, w2 = randn(31, 0, 6).float(), randn(32, 3, 8, 6).float(), randn(33, 3, 6, 4).float()
+    leaves = [t.requires_grad_() for t in (x, w1, w2, torch.zeros(0, 2))]
+    out = E.experts(*leaves[:3], torch.zeros((0, 2), dtype=torch.int64), leaves[3])
+    assert out.shape == (0, 6)
+    for grad, leaf in zip(torch.autograd.grad(out.sum(), leaves), leaves):
+        assert grad.shape == leaf.shape and not grad.any()

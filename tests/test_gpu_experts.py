@@ -186,3 +186,16 @@ def test_tokens_without_an_expert():
         rest = torch.ones(50, dtype=torch.bool)
         rest[[7, 20, 21]] = False
         assert ((got[rest].double() - before[rest].double()).abs() <= 4 * U[torch.bfloat16] * before.double().abs().amax()).all()
+
+
+@pytest.mark.parametrize("shared", [False, True])
+def test_no_tokens(shared):
+    from mm_rs_with_catlass_amd.experts import ServedExperts, experts
+    x, w1, w2, choice, share = (t.cuda() for t in layer(10, 3, 256, 128, 4, 2, torch.float16))
+    leaves = [t.requires_grad_() for t in (x[:0].clone(), w1, w2, share[:0].clone())]
+    out = experts(*leaves[:3], choice[:0], leaves[3])
+    assert out.shape == (0, 256)
+    for grad, leaf in zip(torch.autograd.grad(out.sum(), leaves), leaves):
+        assert grad.shape == leaf.shape and not grad.any()
+    served = ServedExperts(w1.detach(), w2.detach(), *((w1[0].detach(), w2[0].detach()) if shared else ()))
+    assert served(x[:0], choice[:0], share[:0]).shape == (0, 256)
