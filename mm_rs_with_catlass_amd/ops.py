@@ -566,6 +566,13 @@ def _type16(dtype, name):
     return _TORCH_TO_DT[dtype]
 
 
+def _fits(name, **sizes):
+    """Sizes go through the C ABI in 32 bits, and ctypes keeps no more of a number than that; which of the smaller ones are served is the library's to say."""
+    for what, size in sizes.items():
+        if size >= 2 ** 31:
+            _fail("%s has %d %s: fewer than 2^31 are supported", name, size, what)
+
+
 def _tile(tile):
     """(rows, cols, teams) of the kernel's tile (catcoc_hip.h says which exist), None: the library's choice."""
     return None if tile is None else C.byref(_l.CatcocTile(*tile))
@@ -590,6 +597,7 @@ def quantize_fp8(x, block_rows=1, gated=False, out=None, scale=None):
         if cols % 2:
             _fail("gated: x has %d columns, gate and up need the same number", cols)
         cols //= 2
+    _fits("x", rows=rows, columns=cols)
     want = (_blocks(cols), rows) if block_rows == 1 else (_blocks(rows), _blocks(cols))
     _want(out, "out", torch.float8_e4m3fn, 2, None, (rows, cols))
     _want(scale, "scale", torch.float32, 2, None, want)
@@ -620,6 +628,8 @@ def fp8_matmul_allreduce(x1, x2, scale_x1, scale_x2, peers=(), rank=0, rank_size
     n = x2.shape[0]
     if x2.shape[1] != k:
         _fail("x2 has shape %s: its k extent does not match x1's k = %d", tuple(x2.shape), k)
+    _fits("x1", rows=m, columns=k)
+    _fits("x2", rows=n)
     if peer_row_offset < 0:
         _fail("peer_row_offset must be >= 0")
     _want(scale_x1, "scale_x1", torch.float32, 2, None, (_blocks(k), m))
@@ -664,6 +674,8 @@ def grouped_matmul(x, w, group_ends, trans_b=False, out=None, tile=None):
     groups, n = w.shape[0], w.shape[1 if trans_b else 2]
     if w.shape[2 if trans_b else 1] != k:
         _fail("w has shape %s: its k extent does not match x's k = %d", tuple(w.shape), k)
+    _fits("x", rows=rows, columns=k)
+    _fits("w", groups=groups, **{"rows" if trans_b else "columns": n})
     _want_groups(group_ends, groups)
     _want(out, "out", x.dtype, 2, None, (rows, n))
     _check_dev(x, w, group_ends, *(() if out is None else (out,)))
@@ -689,6 +701,9 @@ def grouped_matmul_dw(x, dy, group_ends, out_dtype=None, trans_b=False, out=None
     if dy.shape[0] != rows:
         _fail("dy has %d rows, x has %d", dy.shape[0], rows)
     groups = _want_groups(group_ends)
+    _fits("x", rows=rows, columns=k)
+    _fits("dy", columns=n)
+    _fits("group_ends", groups=groups)
     od = out.dtype if out is not None else x.dtype if out_dtype is None else out_dtype
     odt = 0 if od == torch.float32 else _type16(od, "out_dtype")
     shape = (groups, n, k) if trans_b else (groups, k, n)
@@ -714,6 +729,8 @@ def grouped_fp8_matmul(x, w, scale_x, scale_w, group_ends, out_dtype=torch.bfloa
     groups, n = w.shape[0], w.shape[1]
     if w.shape[2] != k:
         _fail("w has shape %s: its k extent does not match x's k = %d", tuple(w.shape), k)
+    _fits("x", rows=rows, columns=k)
+    _fits("w", groups=groups, rows=n)
     _want(scale_x, "scale_x", torch.float32, 2, None, (_blocks(k), rows))
     _want(scale_w, "scale_w", torch.float32, 3, None, (groups, _blocks(n), _blocks(k)))
     _want_groups(group_ends, groups)

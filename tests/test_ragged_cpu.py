@@ -115,3 +115,30 @@ def test_c_abi_refuses():
     # no rows: accepted, nothing launched
     g(None, L.BF16, None, None, None, None, 0, 4, 4, 2, 0, None)
     assert so.catcoc_last_status() == 0
+
+
+def test_sizes_past_32_bits_are_refused():
+    """The C ABI has 32-bit sizes: 2^32 + 5 rows must not become five."""
+    def wide(*shape, dtype=F8):
+        return torch.zeros((1,) * len(shape), dtype=dtype).expand(*shape)
+    far, h = 2 ** 32 + 5, torch.float16
+    ends = torch.ones(1, dtype=torch.int32)
+    refuses("x has 4294967301 rows", ops.quantize_fp8, wide(far, 1, dtype=h))
+    refuses("x has 4294967301 columns", ops.quantize_fp8, wide(1, far, dtype=h))
+    refuses("x has 4294967301 columns", ops.quantize_fp8, wide(1, 2 * far, dtype=h), gated=True)
+    f = ops.fp8_matmul_allreduce
+    refuses("x1 has 4294967301 rows", f, wide(far, 1), wide(4, 1), wide(1, far, dtype=torch.float32), wide(1, 1, dtype=torch.float32))
+    refuses("x2 has 4294967301 rows", f, wide(4, 1), wide(far, 1), wide(1, 4, dtype=torch.float32), wide(-(-far // 128), 1, dtype=torch.float32))
+    refuses("x1 has 4294967301 columns", f, wide(4, far), wide(4, far), wide(-(-far // 128), 4, dtype=torch.float32), wide(1, -(-far // 128), dtype=torch.float32))
+    m, d, e = ops.grouped_matmul, ops.grouped_matmul_dw, ops.grouped_fp8_matmul
+    refuses("x has 4294967301 rows", m, wide(far, 1, dtype=h), wide(1, 1, 1, dtype=h), ends)
+    refuses("x has 4294967301 columns", m, wide(1, far, dtype=h), wide(1, far, 1, dtype=h), ends)
+    refuses("w has 4294967301 columns", m, wide(1, 1, dtype=h), wide(1, 1, far, dtype=h), ends)
+    refuses("w has 4294967301 rows", m, wide(1, 1, dtype=h), wide(1, far, 1, dtype=h), ends, trans_b=True)
+    refuses("w has 4294967301 groups", m, wide(1, 1, dtype=h), wide(far, 1, 1, dtype=h), wide(far, dtype=torch.int32))
+    refuses("x has 4294967301 rows", d, wide(far, 1, dtype=h), wide(far, 1, dtype=h), ends)
+    refuses("x has 4294967301 columns", d, wide(1, far, dtype=h), wide(1, 1, dtype=h), ends)
+    refuses("dy has 4294967301 columns", d, wide(1, 1, dtype=h), wide(1, far, dtype=h), ends)
+    refuses("group_ends has 4294967301 groups", d, wide(1, 1, dtype=h), wide(1, 1, dtype=h), wide(far, dtype=torch.int32))
+    refuses("x has 4294967301 rows", e, wide(far, 1), wide(1, 1, 1), wide(1, far, dtype=torch.float32), wide(1, 1, 1, dtype=torch.float32), ends)
+    refuses("w has 4294967301 rows", e, wide(1, 1), wide(1, far, 1), wide(1, 1, dtype=torch.float32), wide(1, -(-far // 128), 1, dtype=torch.float32), ends)
