@@ -124,7 +124,7 @@ __global__ void __launch_bounds__(256) quantize_rows_kernel(const QuantArgs args
 {
     const uint32_t lane = threadIdx.x & 63u, blocks = (args.cols + kScaleBlock - 1u) / kScaleBlock;
     const uint32_t groups = (args.rows + 4u * QUADS - 1u) / (4u * QUADS);
-    const uint32_t at = blockIdx.x * 4u + (threadIdx.x >> 6);   // (fewer than 2^31 blocks of four rows, the host sees to it)
+    const uint32_t at = workgroup() * 4u + (threadIdx.x >> 6);   // (fewer than 2^31 blocks of four rows, the host sees to it)
     const uint32_t group = at / blocks, block = at - group * blocks;
     if (group >= groups) return;
     const uint32_t row0 = 4u * QUADS * group + (lane >> 4), col = block * kScaleBlock + (lane & 15u) * 8u;
@@ -159,7 +159,8 @@ template <uint32_t DT>
 __global__ void __launch_bounds__(256) quantize_blocks_kernel(const QuantArgs args)
 {
     __shared__ uint32_t tops[4];
-    const uint32_t blocks = (args.cols + kScaleBlock - 1u) / kScaleBlock, rb = blockIdx.x / blocks, cb = blockIdx.x - rb * blocks;
+    const uint32_t at = workgroup(), blocks = (args.cols + kScaleBlock - 1u) / kScaleBlock, rb = at / blocks, cb = at - rb * blocks;
+    if (rb >= (args.rows + kScaleBlock - 1u) / kScaleBlock) return;
     const uint32_t col = cb * kScaleBlock + (threadIdx.x & 15u) * 8u, row0 = rb * kScaleBlock + (threadIdx.x >> 4);
     Eight e[8];
     uint32_t top = 0;
@@ -176,7 +177,7 @@ __global__ void __launch_bounds__(256) quantize_blocks_kernel(const QuantArgs ar
     if ((threadIdx.x & 63u) == 0) tops[threadIdx.x >> 6] = top;
     __syncthreads();
     const float scale = scale_of(max(max(tops[0], tops[1]), max(tops[2], tops[3])));
-    if (threadIdx.x == 0) args.scale[blockIdx.x] = scale;
+    if (threadIdx.x == 0) args.scale[at] = scale;
     if (col >= args.cols) return;
 #pragma unroll
     for (uint32_t j = 0; j < 8u; ++j)
@@ -188,12 +189,12 @@ static int launch_dt(const QuantArgs &a, bool blocks, bool gated, hipStream_t st
 {
     const uint64_t cb = (a.cols + kScaleBlock - 1u) / kScaleBlock;
     if (blocks) {
-        hipLaunchKernelGGL((quantize_blocks_kernel<DT>), dim3((uint32_t)((a.rows + kScaleBlock - 1u) / kScaleBlock * cb)), dim3(256), 0, stream, a);
+        hipLaunchKernelGGL((quantize_blocks_kernel<DT>), grid_of((a.rows + kScaleBlock - 1u) / kScaleBlock * cb, 256), dim3(256), 0, stream, a);
     } else {
         // four rows a wave where that leaves a CU fewer than 32 waves, else sixteen
         const uint64_t fours = (a.rows + 3ull) / 4u * cb;
         const bool many = fours >= 4u * 8192u;
-        const dim3 grid((uint32_t)(((many ? (a.rows + 15ull) / 16u * cb : fours) + 3u) / 4u));
+        const dim3 grid = grid_of(((many ? (a.rows + 15ull) / 16u * cb : fours) + 3u) / 4u, 256);
         if (gated && many) hipLaunchKernelGGL((quantize_rows_kernel<DT, true, 4>), grid, dim3(256), 0, stream, a);
         else if (gated) hipLaunchKernelGGL((quantize_rows_kernel<DT, true, 1>), grid, dim3(256), 0, stream, a);
         else if (many) hipLaunchKernelGGL((quantize_rows_kernel<DT, false, 4>), grid, dim3(256), 0, stream, a);

@@ -21,7 +21,7 @@ using namespace catcoc;
 namespace {
 
 constexpr uint32_t kMaxWidth = 1u << 22;   // a tile's rows are addressed with 32-bit byte offsets
-constexpr uint64_t kMaxWgs = 0x7fffffffull;
+constexpr uint64_t kMaxWgs = 0x7fffffffull;       // of a launch in two dimensions (checked products, the quantizer)
 
 uint64_t cdiv(uint64_t a, uint64_t b) { return (a + b - 1) / b; }
 
@@ -62,11 +62,21 @@ constexpr Choice kSmallKn[] = {{Choice::SMALL, 16, 64, 4}, {Choice::SMALL, 32, 6
 constexpr Choice kTeams64{Choice::TILE, 64, 128, 2}, kTeams128{Choice::TILE, 128, 128, 2}, kTile128{Choice::TILE, 128, 128, 1}, kTile256{Choice::TILE, 256, 256, 1};
 constexpr uint32_t kLeastRows = 96;   // tiles of 256 columns: 96 to 256 rows in steps of 32
 
+// Most workgroups of a launch on kernel c: its tiles other than the checked ones lie in one dimension, which holds fewer than 2^32 threads.
+uint64_t most_wgs(const Choice &c) { return c.kind == Choice::CHECKED ? kMaxWgs : 0xffffffffull / (c.kind == Choice::TILE && (c.cols == 256 || c.teams == 2) ? 512 : 256); }
+
 // Whether each group's tiles are dealt out to all XCDs, the highest first, or every XCD gets a run of all tiles: dealt out they end together, but every XCD reads
 // every group's rows, which has to be less than the matrices; runs of many groups end together by themselves.  Measured (us, run / dealt, tiles of at most 256
 // rows, 16 bits): 15 groups of together 4099 rows, 3584x4096, 192 / 173; 16 of 4096, 4096x3584, 177 / 160; 24 of 6000, 4096x3584, 251 / 224; 48 of 12000, 2048x2048,
 // 164 / 147; 62 of 16384, 4096x3584, 575 / 581 (160 rows); and where the rows are more than the matrices 16 of 12000, 4096x1792, 197 / 210 and 8 of 4096 59 / 65 (128 rows).
 bool deal(const RaggedArgs &a) { return a.ends && a.groups <= 48 && 8ull * a.rows <= (uint64_t)std::min(a.groups, a.rows) * a.n; }
+
+// Workgroups of a product on kernel c.
+uint64_t count_wgs(const RaggedArgs &a, const Choice &c)
+{
+    const uint64_t wgs = most_row_tiles(a, c.rows) * cdiv(a.n, c.cols);
+    return c.kind == Choice::TILE && deal(a) ? cdiv(wgs, 8) * 8 + 8 : wgs;   // (dealt out, an XCD's eighths of the groups and of the rows behind them are rounded by themselves)
+}
 
 // By what a launch is estimated to take, in us: the larger of what memory needs for each byte once (5.7 GB/ms; `reach`: over what a kernel reaches of it in several rounds) and of its
 // rounds of workgroups, a quarter of the smaller, and a start.  A round costs its steps of 128 bytes of k, `step` us each with the GPU full, `few` of that with
@@ -81,8 +91,9 @@ Choice choose(uint32_t dtype, const RaggedArgs &a, bool kn)
     const double active = a.ends ? std::min(a.groups, a.rows) : 1, mean = a.rows / active;
     const double mem = (active * a.k * a.n * es + a.rows * (double)a.k * es + a.rows * (double)a.n * (2.0 + 4.0 * a.nPeers)) / 5.7e6;
     const bool dealt = deal(a);
-    Choice best = kTile256;
+    Choice best = kChecked;   // (whose launches hold more tiles than the others')
     double least = 0;
+    const bool many = (a.rows / 16.0 + a.groups + 2) * (a.n / 32.0 + 1) > 4e6;   // more tiles of 16x32 than this: each kernel's own are counted
     // Groups are taken to have 0.4, 0.6 .. 1.6 of the mean: how many tiles of at most `rows` that makes, and how high they are, in 32 rows (no less than two).
     auto row_tiles = [&](uint32_t rows, double *height) {
         double tiles = 0, high = 0;
@@ -95,6 +106,7 @@ Choice choose(uint32_t dtype, const RaggedArgs &a, bool kn)
         return a.ends ? active * tiles / 7 : tiles;
     };
     auto offer = [&](const Choice &c, double start, double slots, double step, double few, double reach) {
+        if (many && count_wgs(a, c) > most_wgs(c)) return;
         const double tiles = row_tiles(c.rows, nullptr) * (double)cdiv(a.n, c.cols);
         double rounds = tiles / slots;
         rounds = rounds > 4 ? rounds + 0.3 : std::ceil(rounds);
@@ -163,16 +175,17 @@ void run(uint32_t dtype, const RaggedArgs &args, bool kn, bool dw, const CatcocT
         c = dw ? choose_dw(a) : choose(dtype, a, kn);
     }
     a.tileRows = c.rows;
-    const uint64_t nt = cdiv(a.n, c.cols);
-    uint64_t wgs = most_row_tiles(a, c.rows) * nt;
     a.dealt = c.kind == Choice::TILE && !dw && deal(a);
-    if (a.dealt) wgs = cdiv(wgs, 8) * 8 + 8;   // (an XCD's eighths of the groups and of the rows behind them are rounded by themselves)
-    if (dw) {
-        wgs = a.groups * cdiv(a.k, c.rows) * nt;
+    uint64_t wgs;
+    if (!dw) {
+        wgs = count_wgs(a, c);
+    } else {
+        const uint64_t tiles = cdiv(a.k, c.rows) * cdiv(a.n, c.cols);
+        wgs = a.groups * tiles;
         if (c.kind == Choice::TILE)   // eighths of every group's tiles, dealt out to one workgroup a CU (two of 128 columns)
-            wgs = std::min<uint64_t>(65536 / c.cols, a.groups * cdiv(cdiv(a.k, c.rows) * nt, 8) * 8);
+            wgs = std::min<uint64_t>(65536 / c.cols, a.groups * cdiv(tiles, 8) * 8);
     }
-    if (wgs > kMaxWgs) { api_fail(E_SHAPE, "%llu tiles are more than one launch holds", (unsigned long long)wgs); return; }
+    if (wgs > most_wgs(c)) { api_fail(E_SHAPE, "%llu tiles are more than one launch holds", (unsigned long long)wgs); return; }
     api_launch_info({c.kind == Choice::CHECKED ? (uint32_t)CATCOC_KERNEL_RAGGED_CHECKED : (uint32_t)CATCOC_KERNEL_RAGGED, c.rows, c.cols, c.teams, 0, 0});
     if (c.kind == Choice::SMALL) api_launched(launch_ragged_small(dtype, a, kn, c.rows, (uint32_t)wgs, stream));
     else if (c.kind == Choice::TILE) api_launched(launch_ragged_tile(dtype, a, kn, dw, c.cols, c.teams, (uint32_t)wgs, stream));

@@ -74,7 +74,7 @@ __global__ void __launch_bounds__(256, 2) ragged_checked_kernel(const RaggedArgs
     const unsigned char *X, *W;
     uint32_t group = 0;
     if constexpr (DW) {
-        const uint32_t pt = (args.k + 63u) / 64u, total = args.groups * pt * nt, at = xcd_run(blockIdx.x, total);
+        const uint32_t pt = (args.k + 63u) / 64u, total = args.groups * pt * nt, at = xcd_run(workgroup(), total);
         if (at >= total) return;
         group = at / (pt * nt);
         const uint32_t in = at - group * (pt * nt);
@@ -89,7 +89,7 @@ __global__ void __launch_bounds__(256, 2) ragged_checked_kernel(const RaggedArgs
         X = (const unsigned char *)args.x + ((size_t)b * args.k + t.row) * 2u;
         W = (const unsigned char *)args.w + ((size_t)b * args.n + 64u * t.colTile) * 2u;
     } else {
-        if (!ragged_tile(args, blockIdx.x, 64u, nt, 64u, t)) return;
+        if (!ragged_tile(args, workgroup(), 64u, nt, 64u, t)) return;
         group = t.group;
         K = group < args.groups ? args.k : 0u;
         X = (const unsigned char *)args.x + (size_t)t.row * args.k * ES;

@@ -658,3 +658,58 @@ def test_the_compiled_call_and_the_python_path_answer_alike(monkeypatch):
                       (d, (x, dy[1:], ends), {}), (d, (x, dy, ends, torch.float64), {}), (d, (x, dy, ends.cpu()), {}), (d, (x, dy, [4, 4, 20]), {}),
                       (e, (x8, ws8, sx, sw, ends), {}), (e, (x8, ws8, sx, ssw, ends, torch.float32), {}), (e, (x, ws8, sx, ssw, ends), {})):
         assert not alike(fn, *a, **kw), (fn.__name__, kw)
+
+
+# ---- launches of more workgroups than one dimension of a grid holds (2^32 threads) --------------------------------------------------
+
+@pytest.mark.parametrize("br", [1, 128])
+def test_quantize_as_many_rows_as_there_can_be(br):
+    rows = 2 ** 31 - 1
+    x = torch.empty((rows, 1), dtype=torch.bfloat16, device=DEV).normal_(generator=gen(41)).clamp_(2.0 ** -10)
+    q, s = ops.quantize_fp8(x, block_rows=br)
+    if br == 1:
+        # a block of one value: its code is the largest one
+        assert all(bool((part == 0x7e).all()) for part in q.view(torch.uint8).split(2 ** 28))
+    for first in (0, 2 ** 28 - 128, 2 ** 30 - 256, rows - rows % 128 - 256):
+        part = slice(first, min(first + 1024, rows))
+        want, scale = plain_quantize(x[part].float().cpu().numpy(), br)
+        assert torch.equal(q[part].cpu().view(torch.uint8), torch.from_numpy(want).to(F8).view(torch.uint8))
+        got = s[:, part] if br == 1 else s[first // 128:first // 128 + scale.shape[0]]
+        assert np.array_equal(got.cpu().numpy(), scale)
+
+
+def test_grouped_products_of_as_many_rows_as_there_can_be():
+    rows, groups = 2 ** 31 - 1, 3
+    g = gen(42)
+    table = torch.randint(-2, 3, (2 ** 20, 2), device=DEV, generator=g).to(torch.bfloat16)      # (small whole numbers: every product and sum is exact)
+    x = table.repeat(2 ** 11, 1)[:rows]
+    w = torch.randint(-2, 3, (groups, 2, 2), device=DEV, generator=g).to(torch.bfloat16)
+    ends = [2 ** 30 + 5, 2 ** 30 + 5, rows - 7]
+    for tile in ((16, 64, 4), (128, 128, 1), (256, 256, 1)):       # (each one or more tiles too many)
+        with pytest.raises(L.CatcocError, match="tiles are more than one launch holds"):
+            ops.grouped_matmul(x, w, torch.tensor(ends, dtype=torch.int32, device=DEV), tile=tile)
+    for tile in (None, (64, 64, 1)):
+        out = ops.grouped_matmul(x, w, torch.tensor(ends, dtype=torch.int32, device=DEV), tile=tile)
+        assert ran((64, 64, 1))
+        for first in range(0, rows, 2 ** 27):
+            last = min(first + 2 ** 27, rows)
+            for begin, end, e in ((0, ends[0], 0), (ends[0], ends[2], 2)):
+                i, j = max(first, begin), min(last, end)
+                if i < j:
+                    want = x[i:j, :1] * w[e, 0] + x[i:j, 1:] * w[e, 1]
+                    assert torch.equal(out[i:j], want), (tile, i, j)
+        assert not out[ends[2]:].any()
+        del out
+    fewer = 2 ** 31 - 2 ** 20        # whole tiles of 128 rows that one launch holds
+    ops.grouped_matmul(x[:fewer], w, torch.tensor(ends, dtype=torch.int32, device=DEV).clamp_(max=fewer))
+    assert L.last_launch().tileCols >= 128
+
+
+def test_weight_gradients_of_as_many_groups_as_there_can_be():
+    groups, k = 65536, 64 * 256 + 1
+    g = gen(43)
+    x, dy = randn(g, groups, k, dtype=torch.float16), randn(g, groups, 1, dtype=torch.float16)
+    dw = ops.grouped_matmul_dw(x, dy, torch.arange(1, groups + 1, dtype=torch.int32, device=DEV))
+    assert ran((64, 64, 1))
+    for i in range(0, groups, 4096):
+        assert torch.equal(dw[i:i + 4096, :, 0], (x[i:i + 4096].float() * dy[i:i + 4096].float()).half())      # (one row a group: one rounding)
