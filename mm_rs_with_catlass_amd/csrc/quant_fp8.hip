@@ -55,14 +55,36 @@ __device__ __forceinline__ Eight load8(const void *x, size_t row, uint32_t pitch
     return e;
 }
 
-// silu(g) * u = g / (1 + e^-g) * u.  e^-g = 2^t, t = -g log2 e with the product's low part kept: |g| up to 88 would else cost the result 2^-18.
+// silu(g) * u = g / (1 + e^-g) * u, where e^-g and its reciprocal are far inside fp32's range.  e^-g = 2^t e^r, t = -g log2 e and r what its rounding leaves: it would
+// else cost the result 2^-18.
 __device__ __forceinline__ float silu_times(float g, float u)
 {
-    const float hi = -g * 1.44269504f;
-    const float lo = __builtin_fmaf(-g, 1.44269504f, -hi) + -g * 1.92596299e-8f;   // (log2 e less its fp32 value)
-    const float e = __builtin_amdgcn_exp2f(hi);
-    const float p = __builtin_isinf(e) || __builtin_isinf(hi) ? e : __builtin_fmaf(e, lo * 0.693147181f, e);
-    return g * __builtin_amdgcn_rcpf(1.f + p) * u;
+    const float t = g * -1.44269504f, r = __builtin_fmaf(t, -0.693147181f, -g), e = __builtin_amdgcn_exp2f(t);
+    return g * __builtin_amdgcn_rcpf(1.f + __builtin_fmaf(e, r, e)) * u;
+}
+
+// The same for any gate, as g u / (1 + h^2) with h = e^(-|g|/2), times h^2 where g < 0, one h before u and one behind it: g h is below 1 and nothing leaves fp32's
+// range that the result does not leave (e^-g does from g = -88 on, where a large u still makes something of silu).  From |g| = 175 on h is 0.
+__device__ __forceinline__ float silu_times_far(float g, float u)
+{
+    const float a = __builtin_amdgcn_fmed3f(__builtin_fabsf(g), 0.f, 200.f);   // (an infinity would leave no remainder; a NaN is in g still)
+    const float t = a * -0.721347520f, r = __builtin_fmaf(t, -0.693147181f, a * -0.5f), h0 = __builtin_amdgcn_exp2f(t), h = __builtin_fmaf(h0, r, h0);
+    const float s = __builtin_amdgcn_rcpf(__builtin_fmaf(h, h, 1.f)), f = g < 0.f ? h : 1.f;
+    return g * (f * s) * u * f;
+}
+
+__device__ __forceinline__ void silu_times8(Eight &g, const Eight &u)
+{
+    float top = 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) top = __builtin_fmaxf(top, __builtin_fabsf(g.v[i]));   // (a NaN stays one on either way)
+    if (top < 64.f) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) g.v[i] = silu_times(g.v[i], u.v[i]);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) g.v[i] = silu_times_far(g.v[i], u.v[i]);
+    }
 }
 
 __device__ __forceinline__ uint32_t magnitude(float v) { return __builtin_bit_cast(uint32_t, v) & 0x7fffffffu; }   // (as an integer: a NaN is the largest)
@@ -141,12 +163,10 @@ __global__ void __launch_bounds__(256) quantize_rows_kernel(const QuantArgs args
 #pragma unroll
     for (int j = 0; j < QUADS; ++j) {
         const uint32_t row = row0 + 4u * j;
+        if constexpr (GATED) silu_times8(e[j], u[j]);
         uint32_t top = 0;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            if constexpr (GATED) e[j].v[i] = silu_times(e[j].v[i], u[j].v[i]);
-            top = max(top, magnitude(e[j].v[i]));
-        }
+        for (int i = 0; i < 8; ++i) top = max(top, magnitude(e[j].v[i]));
         const float scale = scale_of(max16(top));
         if (row >= args.rows) continue;
         if ((lane & 15u) == 0) args.scale[(size_t)block * args.rows + row] = scale;

@@ -713,3 +713,58 @@ def test_weight_gradients_of_as_many_groups_as_there_can_be():
     assert ran((64, 64, 1))
     for i in range(0, groups, 4096):
         assert torch.equal(dw[i:i + 4096, :, 0], (x[i:i + 4096].float() * dy[i:i + 4096].float()).half())      # (one row a group: one rounding)
+
+
+# ---- gated rows at the ends of the range --------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_quantize_gated_where_the_gate_is_nearly_shut(dtype):
+    """silu(g) = g e^g / (1 + e^g) of gates down to -180 is far below fp32's range, times a large value it is not.  One value a row: its scale says it."""
+    g = gen(51)
+    gates = torch.tensor([-80.0, -86.0, -87.0, -87.25, -87.5, -88.0, -88.5, -89.0, -92.0, -100.0, -104.0, -120.0, -150.0, 0.0, -1e-30, 1e-30, 30.0, 100.0], device=DEV)
+    gates = torch.cat([gates, torch.rand(2000, device=DEV, generator=g) * 300 - 180])
+    ups = torch.tensor([1.0, 1e10, -1e30, 3e38], device=DEV)
+    x = torch.cartesian_prod(gates, torch.cat([ups, torch.exp2(torch.rand(20, device=DEV, generator=g) * 190 - 64)])).to(dtype)
+    v = x.double()
+    v = v[:, 0] * torch.sigmoid(v[:, 0]) * v[:, 1]
+    x, v = x[v.abs() < 3.4e38], v[v.abs() < 3.4e38]
+    q, s = ops.quantize_fp8(x.contiguous(), gated=True)
+    # (a dozen fp32 operations, each off by a few 2^-24, two of them counted twice)
+    want = v.abs().clamp_min(2.0 ** -40) / 448
+    assert ((s[0].double() - want).abs() <= 2.0 ** -20 * want).all()
+    t = v / want
+    step = torch.exp2(torch.floor(torch.log2(t.abs().clamp_min(2.0 ** -6))) - 3)
+    assert ((q[:, 0].double() - t).abs() <= step / 2 + 2.0 ** -19 * t.abs() + 2.0 ** -30).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+def test_quantize_gated_values_that_are_not_finite(dtype):
+    inf, nan = float("inf"), float("nan")
+    pairs = [(inf, 1.0), (inf, -2.0), (-inf, 1.0), (nan, 1.0), (1.0, inf), (-1.0, inf), (-100.0, inf), (1.0, nan), (0.0, inf), (inf, 0.0), (inf, inf), (-100.0, nan)]
+    x = torch.zeros((len(pairs) + 1, 2 * 130), device=DEV)
+    x[:, :130], x[:, 130:] = 1.0, 2.0
+    for i, (gate, up) in enumerate(pairs):
+        x[i, 7], x[i, 137] = gate, up
+    q, s = ops.quantize_fp8(x.to(dtype), gated=True)
+    for i, (gate, up) in enumerate(pairs):
+        want = torch.tensor(gate).double() * torch.sigmoid(torch.tensor(gate).double()) * up      # what the definition makes of it: an infinity or NaN
+        assert not want.isfinite()
+        assert s[0, i].isnan() if want.isnan() else s[0, i].isinf(), (gate, up)
+        assert q[i, 7].float().isnan()
+        assert (q[i, :128].float()[torch.arange(128) != 7] == 0).all() if want.isinf() else q[i, :128].float().isnan().all()
+    assert torch.equal(s[1], s[1, -1:].expand(len(pairs) + 1)) and torch.equal(q[:, 128:].view(torch.uint8), q[-1:, 128:].view(torch.uint8).expand(len(pairs) + 1, -1))
+    assert s[0, -1].isfinite()
+
+
+@pytest.mark.parametrize("rows,cols", [(3, 8), (130, 264), (1000, 1792)])
+def test_quantize_gated_small_and_large_gates_beside_each_other(rows, cols):
+    x = randn(gen(52 + rows), rows, 2 * cols)
+    x[:, :cols] *= 60
+    q, s = ops.quantize_fp8(x, gated=True)
+    v = x.double()
+    v = v[:, :cols] * torch.sigmoid(v[:, :cols]) * v[:, cols:]
+    want = torch.nn.functional.pad(v.abs(), (0, blocks(cols) * 128 - cols)).view(rows, -1, 128).amax(2).clamp_min(2.0 ** -40).t() / 448
+    assert ((s.double() - want).abs() <= 2.0 ** -20 * want).all()
+    t = v / spread(s.t(), rows, cols, 1)
+    step = torch.exp2(torch.floor(torch.log2(t.abs().clamp_min(2.0 ** -6))) - 3)
+    assert ((q.double() - t).abs() <= step / 2 + 2.0 ** -19 * t.abs() + 2.0 ** -30).all()
