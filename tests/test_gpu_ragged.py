@@ -768,3 +768,35 @@ def test_quantize_gated_small_and_large_gates_beside_each_other(rows, cols):
     t = v / spread(s.t(), rows, cols, 1)
     step = torch.exp2(torch.floor(torch.log2(t.abs().clamp_min(2.0 ** -6))) - 3)
     assert ((q.double() - t).abs() <= step / 2 + 2.0 ** -19 * t.abs() + 2.0 ** -30).all()
+
+
+@pytest.mark.parametrize("k", [128, 1000])
+@pytest.mark.parametrize("tile", [(64, 64, 1), (16, 32, 4), (32, 32, 4), (64, 128, 2), (128, 128, 1), (256, 256, 1)])
+def test_fp8_products_that_cancel_keep_what_the_instruction_promises(k, tile):
+    """Of eight adjacent products 13 bits below the leading one of the largest are kept: each is off by less than 2^-13 of the largest.  Eights without a large
+    product lose nothing by another's; all else is fp32."""
+    g = gen(61 + k)
+    m, n = 40, 300
+    x = torch.randint(-8, 9, (m, k), device=DEV, generator=g).float() / 8
+    w = torch.randint(-8, 9, (n, k), device=DEV, generator=g).float() / 8
+    at = torch.stack([torch.randperm(k, device=DEV, generator=g)[:2] for _ in range(m)])
+    at[::4, 1] = at[::4, 0] ^ 1           # the same eight, another one, another block
+    at.clamp_(max=k - 1)
+    i = torch.arange(m, device=DEV)
+    x[i, at[:, 0]], x[i, at[:, 1]] = 128.0, -128.0
+    w[: n // 2, :] = torch.where(torch.rand(n // 2, k, device=DEV, generator=g) < 0.5, 128.0, w[: n // 2])     # (2^14 less 2^14 in some of the results)
+    x8, w8 = x.to(F8), w.to(F8)
+    assert torch.equal(x8.float(), x) and torch.equal(w8.float(), w)
+    out = ops.fp8_matmul_allreduce(x8, w8, torch.ones((blocks(k), m), device=DEV), torch.ones((blocks(n), blocks(k)), device=DEV), tile=tile)
+    want, lost = torch.zeros((m, n), dtype=torch.float64, device=DEV), torch.zeros((m, n), dtype=torch.float64, device=DEV)
+    mag = torch.zeros((m, n), dtype=torch.float64, device=DEV)
+    for j in range(0, k, 8):
+        p = x[:, None, j:j + 8].double() * w[None, :, j:j + 8].double()
+        want += p.sum(2)
+        mag += p.abs().sum(2)
+        top = torch.exp2(torch.floor(torch.log2(p.abs().amax(2).clamp_min(2.0 ** -20))))
+        lost += (torch.frac(p / top[:, :, None] * 2.0 ** 13) != 0).sum(2) * top * 2.0 ** -13
+    bound = lost + k * 2.0 ** -23 * mag + ROUND[torch.bfloat16] * (want.abs() + lost)
+    off = (out.double() - want).abs()
+    assert (off <= bound).all(), float((off / bound).max())
+    assert (want.abs() < 2.0 ** -10 * mag).any()       # (some results are what is left of large products)
