@@ -314,7 +314,8 @@ CATCOC_API void catcoc_fp8_matmul_allreduce(void *stream, const uint8_t *x1, con
                                             const CatcocTile *tile);
 
 /* out[i] = x[i] w[e] for rows i of group e, [groupEnds[e-1], groupEnds[e]) (groupEnds [groups] int32 on the GPU, ascending; values outside [0, rows] count
- * as the nearer end).  x [rows,k], w [groups,k,n] or, transB, [groups,n,k], out [rows,n], all FP16 or all BF16 (dataType).  Rows past the last group
+ * as the nearer end; where they descend nothing outside the operands is read or written, but rows that several groups claim may hold either one's result, or
+ * none).  x [rows,k], w [groups,k,n] or, transB, [groups,n,k], out [rows,n], all FP16 or all BF16 (dataType).  Rows past the last group
  * are written as zeros.  The gradient of x is the same call on dy with the other transB. */
 CATCOC_API void catcoc_grouped_matmul(void *stream, uint32_t dataType, const void *x, const void *w, const int32_t *groupEnds, void *out, uint32_t rows,
                                       uint32_t n, uint32_t k, uint32_t groups, uint32_t transB, const CatcocTile *tile);

@@ -199,3 +199,26 @@ def test_no_tokens(shared):
         assert grad.shape == leaf.shape and not grad.any()
     served = ServedExperts(w1.detach(), w2.detach(), *((w1[0].detach(), w2[0].detach()) if shared else ()))
     assert served(x[:0], choice[:0], share[:0]).shape == (0, 256)
+
+
+@pytest.mark.parametrize("served", [False, True])
+def test_the_layer_in_a_captured_graph(served):
+    from mm_rs_with_catlass_amd.experts import ServedExperts, experts
+    x, w1, w2, choice, share = (t.cuda() for t in layer(11, 90, 256, 128, 6, 2, torch.bfloat16))
+    whole = ServedExperts(w1, w2, w1[0], w2[0])
+
+    def call():
+        return whole(x, choice, share) if served else experts(x, w1, w2, choice, share)
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        call()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = call()
+    for i in range(6):                                  # other tokens, other experts for them
+        for to, values in zip((x, choice, share), (layer(20 + i, 90, 256, 128, 6, 2, torch.bfloat16)[j] for j in (0, 3, 4))):
+            to.copy_(values)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, call()), i

@@ -800,3 +800,149 @@ def test_fp8_products_that_cancel_keep_what_the_instruction_promises(k, tile):
     off = (out.double() - want).abs()
     assert (off <= bound).all(), float((off / bound).max())
     assert (want.abs() < 2.0 ** -10 * mag).any()       # (some results are what is left of large products)
+
+
+# ---- streams and graphs: every operator ----------------------------------------------------------------------------------------------
+
+class Everything:
+    """One call of each operator on the same few operands, with results of their own."""
+
+    def __init__(self, seed):
+        g = self.g = gen(seed)
+        self.counts, self.k, self.n = [100, 0, 300, 57], 512, 384
+        rows = sum(self.counts)
+        self.x, self.dy = randn(g, rows, self.k, dtype=torch.bfloat16), randn(g, rows, self.n, dtype=torch.bfloat16)
+        self.w, self.ends = randn(g, 4, self.n, self.k, dtype=torch.bfloat16), ends_of(self.counts)
+        self.x8, self.sx = fp8_operand(g, rows, self.k, 1)
+        self.w8 = (randn(g, 4, self.n, self.k) * 60).clamp(-448, 448).to(F8)
+        self.sw = torch.rand((4, blocks(self.n), blocks(self.k)), device=DEV, generator=g) + 0.5
+        self.peers = [randn(g, rows, self.n) for _ in range(2)]
+
+    def inputs(self):
+        return [self.x, self.dy, self.x8, self.sx, self.ends, *self.peers]
+
+    def others(self):
+        """Other values for the same operands, other groups among them."""
+        v = Everything.__new__(Everything)
+        Everything.__init__(v, 71)
+        v.ends = ends_of([57, 300, 100, 0])
+        return v
+
+    def run(self):
+        return [*ops.quantize_fp8(self.x), ops.quantize_fp8(self.x, gated=True)[0], ops.quantize_fp8(self.dy, block_rows=128)[0],
+                ops.fp8_matmul_allreduce(self.x8, self.w8[1], self.sx, self.sw[1], self.peers, 1, 3), ops.grouped_matmul(self.x, self.w, self.ends, trans_b=True),
+                ops.grouped_matmul(self.dy, self.w, self.ends), ops.grouped_matmul_dw(self.x, self.dy, self.ends, out_dtype=torch.float32),
+                ops.grouped_fp8_matmul(self.x8, self.w8, self.sx, self.sw, self.ends)]
+
+
+def same(a, b):
+    return all(torch.equal(p.view(torch.uint8), q.view(torch.uint8)) for p, q in zip(a, b))
+
+
+def test_every_operator_waits_for_its_streams_work():
+    now = Everything(70)
+    then = now.others()
+    then.w, then.w8, then.sw = now.w, now.w8, now.sw
+    before, want = now.run(), then.run()
+    assert not any(torch.equal(p.view(torch.uint8), q.view(torch.uint8)) for p, q in zip(before, want))
+    long = torch.zeros((8192, 8192), dtype=torch.float16, device=DEV)
+    torch.cuda.synchronize()
+    side, done = torch.cuda.Stream(), torch.cuda.Event()
+    with torch.cuda.stream(side):
+        for _ in range(20):
+            long = long @ long                      # (20 ms and more before the operands get their values)
+        for a, b in zip(now.inputs(), then.inputs()):
+            a.copy_(b)
+        got = now.run()
+        done.record()
+    assert not done.query()                         # nothing so far has waited for it
+    side.synchronize()
+    assert same(got, want)
+
+
+def test_every_operator_in_a_captured_graph():
+    now = Everything(72)
+    then = now.others()
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        now.run()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = now.run()
+    for i in range(6):
+        for a, b in zip(now.inputs(), then.inputs()):
+            keep = a.clone()
+            a.copy_(b)
+            b.copy_(keep)
+        for t in out:
+            t.view(torch.uint8).fill_(0xff)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert same(out, now.run()), i
+
+
+# ---- ends that descend or lie outside the rows ---------------------------------------------------------------------------------------
+
+ODD_ENDS = {"descending": [5, 3, 600, 400], "outside": [-7, 20, 2000, 100], "none": [0, 0, 0, 0], "all_in_the_first": [700, 700, 700, 700], "turning": [700, 0, 700, 0],
+            "extremes": [2 ** 31 - 1, -2 ** 31, 300, 2 ** 31 - 1], "one_step_back": [100, 350, 349, 700], "many": [(37 * i) % 700 for i in range(90)],
+            "as_many_as_are_dealt": [(53 * i) % 700 for i in range(48)]}
+
+
+def claims(ends, rows):
+    """The rows of every group as the operators bound them, and which rows are one group's alone."""
+    mine, times, at = [], np.zeros(rows, int), 0
+    for e, end in enumerate(list(ends) + [rows]):
+        begin = min(max(ends[e - 1], 0), rows) if e else 0
+        mine.append((begin, max(min(end, rows), begin)))
+        times[mine[-1][0]:mine[-1][1]] += 1
+    return mine, times == 1
+
+
+@pytest.mark.parametrize("name", sorted(ODD_ENDS))
+@pytest.mark.parametrize("kind,tile", [(kind, t) for kind in ("kn", "nk", "f8") for t in [None] + TILES + (SMALL_KN if kind == "kn" else SMALL_NK)])
+def test_odd_ends_on_every_tile(name, kind, tile):
+    ends, rows, k, n = ODD_ENDS[name], 700, 128, 2600 if name == "as_many_as_are_dealt" else 136
+    groups = len(ends)
+    g = gen(groups)
+    room = torch.full((rows + 8, n), 7.0, dtype=torch.bfloat16, device=DEV)
+    on_gpu = torch.tensor(ends, dtype=torch.int32, device=DEV)
+    if kind == "f8":
+        x, sx = fp8_operand(g, rows, k, 1)
+        w = (randn(g, groups, n, k) * 60).clamp(-448, 448).to(F8)
+        sw = torch.rand((groups, blocks(n), blocks(k)), device=DEV, generator=g) + 0.5
+        ops.grouped_fp8_matmul(x, w, sx, sw, on_gpu, out=room[4:-4], tile=tile)
+        a, b = x.double() * spread(sx.t(), rows, k, 1), torch.stack([(w[e].double() * spread(sw[e], n, k, 128)).t() for e in range(groups)])
+    else:
+        x = randn(g, rows, k, dtype=torch.bfloat16)
+        w = randn(g, groups, n, k, dtype=torch.bfloat16) if kind == "nk" else randn(g, groups, k, n, dtype=torch.bfloat16)
+        ops.grouped_matmul(x, w, on_gpu, trans_b=kind == "nk", out=room[4:-4], tile=tile)
+        a, b = x.double(), w.double().transpose(1, 2) if kind == "nk" else w.double()
+    assert (room[:4] == 7).all() and (room[-4:] == 7).all()
+    mine, alone = claims(ends, rows)
+    height = (tile or (16,))[0]
+    most = (rows - groups - 1) // height + groups + 1       # (row tiles of a launch: as many as ascending ends can have)
+    if sum(-(-(j - i) // height) for i, j in mine) > most:
+        return
+    alone, out = torch.from_numpy(alone).to(DEV), room[4:-4]
+    for e, (i, j) in enumerate(mine):
+        keep = alone[i:j]
+        if e == groups:
+            assert (out[i:j][keep] == 0).all()
+        elif keep.any():
+            p, q = a[i:j][keep], b[e]
+            close(out[i:j][keep], p @ q, p.abs() @ q.abs(), k, torch.bfloat16, norm2(p, q.t()) if kind == "f8" else None)
+
+
+@pytest.mark.parametrize("name", sorted(ODD_ENDS))
+@pytest.mark.parametrize("tile", [None] + TILES_DW)
+def test_odd_ends_of_weight_gradients(name, tile):
+    ends, rows, k, n = ODD_ENDS[name], 700, 130, 136
+    g = gen(len(ends) + 1)
+    x, dy = randn(g, rows, k, dtype=torch.bfloat16), randn(g, rows, n, dtype=torch.bfloat16)
+    room = torch.full((len(ends) + 2, k, n), 7.0, device=DEV)
+    ops.grouped_matmul_dw(x, dy, torch.tensor(ends, dtype=torch.int32, device=DEV), out=room[1:-1], tile=tile)
+    assert (room[0] == 7).all() and (room[-1] == 7).all()
+    for e, (i, j) in enumerate(claims(ends, rows)[0][:-1]):      # (a gradient's groups may share rows)
+        a, d = x[i:j].double().t(), dy[i:j].double()
+        close(room[1 + e], a @ d, a.abs() @ d.abs(), j - i, torch.float32)
