@@ -377,7 +377,9 @@ struct RaggedTileLoop {
 
 // DW: x and w are rows of k (the group's rows), the result is the group's [k, n] matrix.  KN: w is [k, n].
 // A weight gradient's workgroups walk several tiles: few rows make few steps, and a tile's first copies are on their way while the one before is stored.
-// 4099 rows in 15 groups, 4096x3584 in fp32, 325 us: 150 without the stores, and the stores alone take 176 in this order (881 MB, 5.0 TB/s).  They do not overlap:
+// 4099 rows in 16 groups (one without rows), 4096x3584 in fp32, 327 us: 150 without the stores, and the stores alone take 178 in this order (940 MB, 5.3 TB/s).
+// They hardly overlap: vmcnt counts copies and stores in their order, so the wait for a tile's first step, whose copies are older than the stores, lets 24 of a
+// wave's 32 stores finish too, and directly behind it five of the 11 registers that this kernel spills come back one after the other, each behind all that is under way.
 // 128x256 tiles that store a tile piece by piece between the next one's steps took 373 us, five stages of 32 rows that leave 2.5 us of work in LDS 326 (and
 // the long sums of 8 groups of 2048 rows 271 instead of 240).
 template <uint32_t DT, bool KN, bool DW, int WY, int NIMAX, int KG>
