@@ -83,8 +83,8 @@ uint64_t count_wgs(const RaggedArgs &a, const Choice &c)
 // at most one workgroup a CU.  Fitted to, and compared on, 84 sizes that ran on all of these kernels (1 to 8192 rows of e4m3 against 2048 to 8192 columns and
 // k; 64 to 16384 rows in 1 to 128 groups of 1792 to 4096 by 1792 to 8192, uneven, 16 bits either way and e4m3): for 74 of them the choice is within 7 % of the
 // fastest, the worst 1.17 of it.  The constants have no other reason than that fit.  Of 48 sizes that it has not seen (1 to 12000 rows, 1 to 128 groups, k and n 512 to 6000)
-// the choice is within 7 % of the fastest for 41.  The others are e4m3 with few rows a group and a short k, where a small tile's start counts for more than the estimate
-// has it (453 rows in 128 groups of 4480x512 130 us on 16x32, 67 on 128x128; 257 in 48 of 2688x512 24.5 and 16.6; 91 in 128 of 5376x1408 128 and 104), and 16 bits with k = 512
+// the choice is within 7 % of the fastest for 41.  The others are e4m3 with few rows a group, the further off the shorter k is, as a small tile's start counts for more than
+// the estimate has it (453 rows in 128 groups of 4480x512 130 us on 16x32, 67 on 128x128; 257 in 48 of 2688x512 24.5 and 16.6; 91 in 128 of 5376x1408 128 and 104), and 16 bits with k = 512
 // (11096 rows in 48 groups of 1792x512 46.6 us on 128x256, 36.3 on 256x256).  Heights: 4096 rows in 16 groups of 4096x3584 take 195 us in tiles of at most 256 rows, 177 of 192, 153 of 160, 181 of 128;
 // 2400 in 8 groups of 2048x4096 49, 43, 65 and 57 (16 bits).
 Choice choose(uint32_t dtype, const RaggedArgs &a, bool kn)

@@ -25,9 +25,15 @@ class GroupedLinear(torch.autograd.Function):
     def backward(ctx, dy):
         x, w, ends = ctx.saved_tensors
         dy = dy.contiguous()
-        dx = GroupedLinear.apply(dy, w, ends, not ctx.trans_b) if ctx.needs_input_grad[0] else None
-        dw = GroupedOuter.apply(x, dy, ends, ctx.trans_b) if ctx.needs_input_grad[1] else None
+        # (a gradient that nobody differentiates needs no function of its own: 64 tokens' forward and backward 480 us, 550 with one)
+        linear, outer = (GroupedLinear.apply, GroupedOuter.apply) if torch.is_grad_enabled() else (ops.grouped_matmul, _outer)
+        dx = linear(dy, w, ends, not ctx.trans_b) if ctx.needs_input_grad[0] else None
+        dw = outer(x, dy, ends, ctx.trans_b) if ctx.needs_input_grad[1] else None
         return dx, dw, None, None
+
+
+def _outer(x, dy, ends, trans_b):
+    return ops.grouped_matmul_dw(x, dy, ends, trans_b=trans_b)
 
 
 class GroupedOuter(torch.autograd.Function):
@@ -37,7 +43,7 @@ class GroupedOuter(torch.autograd.Function):
     def forward(ctx, x, dy, ends, trans_b):
         ctx.save_for_backward(x, dy, ends)
         ctx.trans_b = trans_b
-        return ops.grouped_matmul_dw(x, dy, ends, trans_b=trans_b)
+        return _outer(x, dy, ends, trans_b)
 
     @staticmethod
     def backward(ctx, g):
@@ -52,11 +58,10 @@ def sort_by_expert(choice, experts):
     """choice [tokens, top], each token's experts -> (order, back, ends): row i of the sorted rows is choice order[i] of the flattened ones,
     back undoes it, group_ends for the operators.  Nothing is read back to the host.  Choices below 0 or past the last expert (a dropped token) are
     sorted behind the last group: rows of no group, whose results and gradients are zeros."""
-    flat = choice.reshape(-1).long()
-    flat = torch.where(flat < 0, experts, flat)
-    order = torch.argsort(flat, stable=True)
+    flat = choice.reshape(-1).long() & (2 ** 63 - 1)     # (a negative number without its sign is larger than any expert's)
+    flat, order = torch.sort(flat, stable=True)
     back = torch.empty_like(order).scatter_(0, order, torch.arange(order.numel(), device=order.device))
-    ends = torch.searchsorted(flat[order], torch.arange(experts, device=flat.device), right=True).to(torch.int32)
+    ends = torch.searchsorted(flat, torch.arange(experts, device=flat.device), right=True, out_int32=True)
     return order, back, ends
 
 

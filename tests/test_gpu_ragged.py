@@ -846,10 +846,13 @@ def test_every_operator_waits_for_its_streams_work():
     before, want = now.run(), then.run()
     assert not any(torch.equal(p.view(torch.uint8), q.view(torch.uint8)) for p, q in zip(before, want))
     long = torch.zeros((8192, 8192), dtype=torch.float16, device=DEV)
-    torch.cuda.synchronize()
     side, done = torch.cuda.Stream(), torch.cuda.Event()
+    with torch.cuda.stream(side):                   # (memory for all results: allocating may wait for the GPU)
+        room = [now.run(), long @ long, long @ long]
+    torch.cuda.synchronize()
+    del room
     with torch.cuda.stream(side):
-        for _ in range(20):
+        for _ in range(40):
             long = long @ long                      # (20 ms and more before the operands get their values)
         for a, b in zip(now.inputs(), then.inputs()):
             a.copy_(b)
