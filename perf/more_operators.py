@@ -103,7 +103,7 @@ def draw(rng):
         experts, groups = rng.choice([8, 16, 32, 60, 64, 128, 160, 256]), 1
         if experts >= 60 and rng.random() < 0.4:
             groups = 4 if experts == 60 else 8
-        top = min(rng.choice([1, 2, 4, 6, 8]), experts // 2)
+        top = min(rng.choice([1, 2, 4, 6, 8] if op == "route" else [2, 4, 6, 8]), experts // 2)    # (one share of its own sum is 1: no gradient)
         tokens = _log(rng, 1, 16384)
         c = _route("", op, tokens, experts, top, rng.choice(["bf16", "fp16", "fp32", "fp32"]), rng.choice(["softmax", "sigmoid"]), rng.random() < 0.5, groups,
                    max(1, groups // 2), rng.choice([1, 2]) if groups > 1 else 1, rng.random() < 0.6, rng.choice([1.0, 1.0, 2.5]), rng.choice([0, 0, tokens // 8]))
