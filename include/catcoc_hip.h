@@ -330,6 +330,66 @@ CATCOC_API void catcoc_grouped_fp8_matmul(void *stream, const uint8_t *x, const 
                                           const int32_t *groupEnds, void *out, uint32_t rows, uint32_t n, uint32_t k, uint32_t groups,
                                           uint32_t outDataType, const CatcocTile *tile);
 
+/* ----------------------------------------------------------------------- */
+/* Around a layer of experts: norm, router, rows to their experts and back   */
+/* ----------------------------------------------------------------------- */
+
+/* No counterpart in the reference; beside the e4m3 and grouped operators.  Any alignment of the element type serves.  A call without rows or tokens is accepted and
+ * writes nothing (dw, ends: zeros).  Sums are held in fp32 and rounded once, in an order that the sizes alone decide; nothing is added by atomics that come out in
+ * another order on another run.  dataType: FP16, BF16 or 0 (fp32); other types of a call are that or 0.
+ *
+ * Root-mean-square norm of rows: s = x + residual, rounded to residualType and kept in `sum` (which may be `residual`), y = s / sqrt(mean(s^2) + eps) * weight of what is
+ * kept.  residual and sum NULL: s = x.  y goes to out (which may be x) in x's type, and, or, to e4m3 codes q with scale [ceil(cols/128), rows] as catcoc_quantize_fp8 makes
+ * them, each rounded from fp32 by itself; NULL: not wanted.  x, residual, sum, out, q [rows,cols], at most 16384 columns; weight [cols]. */
+CATCOC_API void catcoc_rms_norm(void *stream, const void *x, const void *residual, const void *weight, void *out, void *sum, uint8_t *q, float *scale,
+                                uint32_t rows, uint32_t cols, float eps, uint32_t dataType, uint32_t residualType, uint32_t weightType);
+
+/* Its gradients, from dy (dataType) and what was normalised: x (`sum` where there was a residual), sumType.  With r = 1 / sqrt(mean(x^2) + eps), n = x r, g = dy weight:
+ * dx = r (g - n mean(g n)) + dsum, in sumType; it is the gradient of the residual too.  dsum: NULL or what else flows into the sum, sumType (dx may be dsum).  dw [cols] =
+ * sum over the rows of dy n, in weightType.  workspace: catcoc_rms_norm_backward_workspace_size() bytes, of any content. */
+CATCOC_API uint64_t catcoc_rms_norm_backward_workspace_size(uint32_t rows, uint32_t cols);
+CATCOC_API void catcoc_rms_norm_backward(void *stream, const void *dy, const void *x, const void *weight, const void *dsum, void *dx, void *dw, void *workspace,
+                                         uint64_t workspaceBytes, uint32_t rows, uint32_t cols, float eps, uint32_t dataType, uint32_t sumType,
+                                         uint32_t weightType);
+
+enum { CATCOC_SCORE_SOFTMAX = 0, CATCOC_SCORE_SIGMOID = 1 };
+typedef struct CatcocRouting {
+    uint32_t score;              /* CATCOC_SCORE_*: what a logit becomes */
+    uint32_t groups;             /* experts come in so many groups of consecutive ones (0: 1) ... */
+    uint32_t topGroups;          /* ... of which so many are chosen from (0: all) ... */
+    uint32_t groupTop;           /* ... by the sum of the best one or two of a group (0: 1) */
+    uint32_t renormalize;        /* shares of the chosen scores' sum, not the scores themselves */
+    float scale;                 /* of the shares */
+} CatcocRouting;
+
+/* choice[t] = the `top` (at most 64) experts of token t, the best first, by score + bias (fp32 [experts]; NULL: none; it does not enter the shares), of equal ones the lower
+ * index; share[t] = their scores, of their sum where renormalised, times scale.  Scores with a bias or in groups by sums are compared in 64 bits to 42 bits behind the leading one, others
+ * exactly.  logits [tokens, experts], at most 1024 experts in at most 64 groups.  An expert whose logit or bias is -inf is not to be had; where too few are, choices end
+ * in -1 with shares of 0.  A NaN counts as +inf, and makes the shares NaN that it enters.  The sum of sigmoids is taken so that it is not 0 where all of them are below fp32's range. */
+CATCOC_API void catcoc_route(void *stream, const void *logits, const float *bias, int32_t *choice, float *share, const CatcocRouting *how, uint32_t tokens,
+                             uint32_t experts, uint32_t top, uint32_t dataType);
+/* The gradient of the logits (of dataType, all of them written) from that of the shares; the choice is taken as given (outside [0, experts): none), groups play no part. */
+CATCOC_API void catcoc_route_backward(void *stream, const float *dshare, const void *logits, const int32_t *choice, void *dlogits, const CatcocRouting *how,
+                                      uint32_t tokens, uint32_t experts, uint32_t top, uint32_t dataType);
+
+/* The plan of the choices [rows] (of choiceBits 32 or 64): order lists the rows by expert, in ascending order within one, those outside [0, experts) (at most 1024) behind
+ * the last; back[i] is where row i went; ends[e] is one past expert e's last place, group ends of the grouped products.  workspace:
+ * catcoc_sort_by_expert_workspace_size() bytes, of any content. */
+CATCOC_API uint64_t catcoc_sort_by_expert_workspace_size(uint32_t rows, uint32_t experts);
+CATCOC_API void catcoc_sort_by_expert(void *stream, const void *choice, int32_t *order, int32_t *back, int32_t *ends, void *workspace, uint64_t workspaceBytes,
+                                      uint32_t rows, uint32_t experts, uint32_t choiceBits);
+
+/* Every token's row at its choices' places: out[back[t,j]] = x[t], x [tokens,cols] of valueBytes (1, 2, 4) each, back [tokens,top], out [tokens*top,cols]; with e4m3 codes their
+ * scale [ceil(cols/128), tokens] to outScale [ceil(cols/128), tokens*top] (NULL: none).  Places outside the rows are left out; rows that no choice has stay as they were. */
+CATCOC_API void catcoc_spread_rows(void *stream, const void *x, const float *scale, const int32_t *back, void *out, float *outScale, uint32_t tokens,
+                                   uint32_t top, uint32_t cols, uint32_t valueBytes);
+/* The rows back at their tokens: out[t] = sum over j of share[t,j] y[back[t,j]], in the order of j; share NULL: ones (the gradient of catcoc_spread_rows). */
+CATCOC_API void catcoc_gather_rows(void *stream, const void *y, const int32_t *back, const float *share, void *out, uint32_t tokens, uint32_t top, uint32_t cols,
+                                   uint32_t dataType);
+/* Its gradients: dy[back[t,j]] = share[t,j] dout[t], dshare[t,j] = <dout[t], y[back[t,j]]> (0 for a place outside the rows). */
+CATCOC_API void catcoc_gather_rows_backward(void *stream, const void *dout, const void *y, const int32_t *back, const float *share, void *dy, float *dshare,
+                                            uint32_t tokens, uint32_t top, uint32_t cols, uint32_t dataType);
+
 /* The reference's accuracy gate (examples/utils/verify_result.py:26-43,88-117 with the tolerances of
  * examples/utils/utils.py:44-52) on host arrays: every element |out - gold| <= rtol * max(1, |gold|) with
  * rtol = 2^-8 (fp16) / 2^-7 (bf16) for computeTimes < 2048 and twice that otherwise, and

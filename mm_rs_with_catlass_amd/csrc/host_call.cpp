@@ -8,11 +8,15 @@
 #include <Python.h>
 
 #include <ATen/ops/empty.h>
+#include <c10/hip/HIPFunctions.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/Dtype.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <string.h>
+
+#include <initializer_list>
+#include <optional>
 
 #include "catcoc_hip.h"
 
@@ -452,12 +456,352 @@ PyObject *fp8Grouped(PyObject *, PyObject *const *v, Py_ssize_t n)   // x, w, sc
     });
 }
 
+// ---- operators around a layer of experts: rms_norm() and those below it in ops.py, of the same kind.
+decltype(&catcoc_rms_norm) rmsNorm;
+decltype(&catcoc_rms_norm_backward) rmsNormBackward;
+decltype(&catcoc_rms_norm_backward_workspace_size) rmsNormWorkspace;
+decltype(&catcoc_route) routeTo;
+decltype(&catcoc_route_backward) routeBackward;
+decltype(&catcoc_sort_by_expert) sortByExpert;
+decltype(&catcoc_sort_by_expert_workspace_size) sortWorkspace;
+decltype(&catcoc_spread_rows) spreadRows;
+decltype(&catcoc_gather_rows) gatherRows;
+decltype(&catcoc_gather_rows_backward) gatherBackward;
+
+PyObject *attachLayer(PyObject *, PyObject *const *v, Py_ssize_t n)
+{
+    if (n != 10) return PyErr_Format(PyExc_TypeError, "attach_layer takes ten addresses");
+    void *p[10];
+    for (int i = 0; i < 10; ++i) {
+        p[i] = PyLong_AsVoidPtr(v[i]);
+        if (p[i] == nullptr) return PyErr_Occurred() ? nullptr : PyErr_Format(PyExc_ValueError, "address %d is null", i);
+    }
+    rmsNorm = (decltype(rmsNorm))p[0];
+    rmsNormBackward = (decltype(rmsNormBackward))p[1];
+    rmsNormWorkspace = (decltype(rmsNormWorkspace))p[2];
+    routeTo = (decltype(routeTo))p[3];
+    routeBackward = (decltype(routeBackward))p[4];
+    sortByExpert = (decltype(sortByExpert))p[5];
+    sortWorkspace = (decltype(sortWorkspace))p[6];
+    spreadRows = (decltype(spreadRows))p[7];
+    gatherRows = (decltype(gatherRows))p[8];
+    gatherBackward = (decltype(gatherBackward))p[9];
+    Py_RETURN_NONE;
+}
+
+// Tensors on the current device, whose stream the call goes to.
+struct Here {
+    const c10::DeviceIndex device = c10::hip::current_device();
+
+    const at::Tensor &any(PyObject *o, int64_t dims) const
+    {
+        const at::Tensor &t = tensor(o, at::ScalarType::Undefined, dims);
+        if (t.get_device() != device) throw Other{};
+        return t;
+    }
+    const at::Tensor &of(PyObject *o, at::ScalarType type, at::IntArrayRef shape) const
+    {
+        const at::Tensor &t = shaped(o, type, shape);
+        if (t.get_device() != device) throw Other{};
+        return t;
+    }
+    uint8_t *maybe(PyObject *o, at::ScalarType type, at::IntArrayRef shape) const { return o == Py_None ? nullptr : address(of(o, type, shape)); }
+    void check(const Result &r) const
+    {
+        if (r.t->get_device() != device) throw Other{};
+    }
+};
+
+// The type of an operand that is of type `own` or fp32.
+at::ScalarType likeOrWide(PyObject *o, at::ScalarType own)
+{
+    if (!THPVariable_CheckExact(o)) throw Other{};
+    const at::ScalarType t = THPVariable_Unpack(o).scalar_type();
+    if (t != own && t != at::kFloat) throw Other{};
+    return t;
+}
+
+double real(PyObject *o)
+{
+    if (!PyFloat_CheckExact(o)) throw Other{};
+    return PyFloat_AS_DOUBLE(o);
+}
+
+template <typename F>
+PyObject *guardedLayer(const char *name, Py_ssize_t n, Py_ssize_t wanted, F &&body)
+{
+    if (gatherBackward == nullptr) return PyErr_Format(PyExc_TypeError, "%s comes after attach_layer", name);
+    return guarded(name, n, wanted, body);
+}
+
+PyObject *tupleOf(std::initializer_list<Result *> results)
+{
+    PyObject *all = PyTuple_New((Py_ssize_t)results.size());
+    Py_ssize_t i = 0;
+    for (Result *r : results) {
+        PyObject *o = all ? r->object() : nullptr;
+        if (o == nullptr) {
+            Py_XDECREF(all);
+            return nullptr;
+        }
+        PyTuple_SET_ITEM(all, i++, o);
+    }
+    return all;
+}
+
+// Both norms: x, weight, residual, eps, then for the first out, residual_out; for the second keep, out, scale, kept, residual_out.
+PyObject *norm(PyObject *const *v, bool fp8)
+{
+    const Here here;
+    const at::Tensor &x = here.any(v[0], 2);
+    const int64_t rows = x.size(0), cols = x.size(1);
+    const at::ScalarType type = x.scalar_type(), weightType = likeOrWide(v[1], type);
+    const uint32_t typeCode = code(type, true);
+    if (rows > MOST || cols > MOST) throw Other{};
+    const int64_t sizes[2] = {rows, cols};
+    const at::IntArrayRef shape(sizes, 2);
+    const at::Tensor &weight = here.of(v[1], weightType, {cols});
+    const bool summed = v[2] != Py_None, keep = !fp8 || number(v[4], 1) != 0;
+    PyObject *const out = v[fp8 ? 7 : 4], *const sumOut = v[fp8 ? 8 : 5];
+    if ((!summed && sumOut != Py_None) || (!keep && out != Py_None)) throw Other{};
+    const at::ScalarType sumType = summed ? likeOrWide(v[2], type) : type;
+    uint8_t *const residual = here.maybe(v[2], sumType, shape);
+    const float eps = (float)real(v[3]);
+    std::optional<Result> y, sum, q, scale;
+    if (keep) here.check(y.emplace(out, type, shape, x));
+    if (summed) here.check(sum.emplace(sumOut, sumType, shape, x));
+    if (fp8) {
+        here.check(q.emplace(v[5], F8, shape, x));
+        here.check(scale.emplace(v[6], at::kFloat, at::IntArrayRef({blocks(cols), rows}), x));
+    }
+    uint8_t *const px = address(x), *const pw = address(weight), *const py = y ? y->at_() : nullptr, *const ps = sum ? sum->at_() : nullptr;
+    uint8_t *const pq = q ? q->at_() : nullptr;
+    float *const pscale = scale ? (float *)scale->at_() : nullptr;
+    const uint32_t sumCode = code(sumType, true), weightCode = code(weightType, true);
+    void *const s = stream();
+    Py_BEGIN_ALLOW_THREADS
+    rmsNorm(s, px, residual, pw, py, ps, pq, pscale, (uint32_t)rows, (uint32_t)cols, eps, typeCode, sumCode, weightCode);
+    Py_END_ALLOW_THREADS
+    if (!accepted()) return nullptr;
+    if (!fp8) return summed ? tupleOf({&*y, &*sum}) : y->object();
+    if (keep) return summed ? tupleOf({&*q, &*scale, &*y, &*sum}) : tupleOf({&*q, &*scale, &*y});
+    return summed ? tupleOf({&*q, &*scale, &*sum}) : tupleOf({&*q, &*scale});
+}
+
+PyObject *norm16(PyObject *, PyObject *const *v, Py_ssize_t n)   // x, weight, residual, eps, out, residual_out
+{
+    return guardedLayer("rms_norm", n, 6, [&] { return norm(v, false); });
+}
+
+PyObject *normFp8(PyObject *, PyObject *const *v, Py_ssize_t n)   // x, weight, residual, eps, keep, out, scale, kept, residual_out
+{
+    return guardedLayer("rms_norm_fp8", n, 9, [&] { return norm(v, true); });
+}
+
+PyObject *normBackward(PyObject *, PyObject *const *v, Py_ssize_t n)   // dy, x, weight, dsum, eps, dx, dw
+{
+    return guardedLayer("rms_norm_backward", n, 7, [&]() -> PyObject * {
+        const Here here;
+        const at::Tensor &dy = here.any(v[0], 2);
+        const int64_t rows = dy.size(0), cols = dy.size(1);
+        const at::ScalarType type = dy.scalar_type(), sumType = likeOrWide(v[1], type), weightType = likeOrWide(v[2], type);
+        const uint32_t typeCode = code(type, true), sumCode = code(sumType, true), weightCode = code(weightType, true);
+        if (rows > MOST || cols > MOST) throw Other{};
+        const int64_t sizes[2] = {rows, cols};
+        const at::IntArrayRef shape(sizes, 2);
+        const at::Tensor &x = here.of(v[1], sumType, shape), &weight = here.of(v[2], weightType, {cols});
+        uint8_t *const dsum = here.maybe(v[3], sumType, shape);
+        const float eps = (float)real(v[4]);
+        Result dx(v[5], sumType, shape, x), dw(v[6], weightType, {cols}, x);
+        here.check(dx);
+        here.check(dw);
+        const uint64_t bytes = rmsNormWorkspace((uint32_t)rows, (uint32_t)cols);
+        const at::Tensor work = at::empty({(int64_t)bytes}, x.options().dtype(at::kByte));
+        uint8_t *const pd = address(dy), *const px = address(x), *const pw = address(weight), *const pdx = dx.at_(), *const pdw = dw.at_(), *const pwork = address(work);
+        void *const s = stream();
+        Py_BEGIN_ALLOW_THREADS
+        rmsNormBackward(s, pd, px, pw, dsum, pdx, pdw, pwork, bytes, (uint32_t)rows, (uint32_t)cols, eps, typeCode, sumCode, weightCode);
+        Py_END_ALLOW_THREADS
+        return accepted() ? tupleOf({&dx, &dw}) : nullptr;
+    });
+}
+
+uint32_t score(PyObject *o)
+{
+    if (!PyUnicode_CheckExact(o)) throw Other{};
+    if (PyUnicode_CompareWithASCIIString(o, "softmax") == 0) return CATCOC_SCORE_SOFTMAX;
+    if (PyUnicode_CompareWithASCIIString(o, "sigmoid") == 0) return CATCOC_SCORE_SIGMOID;
+    throw Other{};
+}
+
+uint32_t positive(PyObject *o)
+{
+    const int64_t v = number(o, MOST);
+    if (v < 1) throw Other{};
+    return (uint32_t)v;
+}
+
+PyObject *route(PyObject *, PyObject *const *v, Py_ssize_t n)   // logits, top, score, bias, groups, top_groups, group_top, renormalize, scale, choice, share
+{
+    return guardedLayer("route", n, 11, [&]() -> PyObject * {
+        const Here here;
+        const at::Tensor &logits = here.any(v[0], 2);
+        const int64_t tokens = logits.size(0), experts = logits.size(1), top = positive(v[1]);
+        const uint32_t type = code(logits.scalar_type(), true);
+        if (tokens > MOST || experts > MOST || top > experts) throw Other{};
+        CatcocRouting how{score(v[2]), positive(v[4]), positive(v[5]), positive(v[6]), (uint32_t)number(v[7], 1), (float)real(v[8])};
+        const float *const bias = (const float *)here.maybe(v[3], at::kFloat, {experts});
+        Result choice(v[9], at::kInt, {tokens, top}, logits), share(v[10], at::kFloat, {tokens, top}, logits);
+        here.check(choice);
+        here.check(share);
+        uint8_t *const px = address(logits);
+        int32_t *const pc = (int32_t *)choice.at_();
+        float *const ps = (float *)share.at_();
+        void *const s = stream();
+        Py_BEGIN_ALLOW_THREADS
+        routeTo(s, px, bias, pc, ps, &how, (uint32_t)tokens, (uint32_t)experts, (uint32_t)top, type);
+        Py_END_ALLOW_THREADS
+        return accepted() ? tupleOf({&choice, &share}) : nullptr;
+    });
+}
+
+PyObject *routeGradient(PyObject *, PyObject *const *v, Py_ssize_t n)   // dshare, logits, choice, score, renormalize, scale, out
+{
+    return guardedLayer("route_backward", n, 7, [&]() -> PyObject * {
+        const Here here;
+        const at::Tensor &logits = here.any(v[1], 2), &choice = here.any(v[2], 2);
+        const int64_t tokens = logits.size(0), experts = logits.size(1), top = choice.size(1);
+        const uint32_t type = code(logits.scalar_type(), true);
+        if (choice.scalar_type() != at::kInt || choice.size(0) != tokens || tokens > MOST || experts > MOST || top > experts) throw Other{};
+        const at::Tensor &dshare = here.of(v[0], at::kFloat, {tokens, top});
+        CatcocRouting how{score(v[3]), 1, 1, 1, (uint32_t)number(v[4], 1), (float)real(v[5])};
+        Result out(v[6], logits.scalar_type(), {tokens, experts}, logits);
+        here.check(out);
+        uint8_t *const px = address(logits), *const po = out.at_();
+        const float *const pd = (const float *)address(dshare);
+        const int32_t *const pc = (const int32_t *)address(choice);
+        void *const s = stream();
+        Py_BEGIN_ALLOW_THREADS
+        routeBackward(s, pd, px, pc, po, &how, (uint32_t)tokens, (uint32_t)experts, (uint32_t)top, type);
+        Py_END_ALLOW_THREADS
+        return accepted() ? out.object() : nullptr;
+    });
+}
+
+PyObject *sortChoices(PyObject *, PyObject *const *v, Py_ssize_t n)   // choice, experts, order, back, ends
+{
+    return guardedLayer("sort_by_expert", n, 5, [&]() -> PyObject * {
+        const Here here;
+        const at::Tensor &choice = here.any(v[0], 2);
+        const int64_t rows = choice.numel(), experts = positive(v[1]);
+        const bool wide = choice.scalar_type() == at::kLong;
+        if ((!wide && choice.scalar_type() != at::kInt) || rows > MOST || experts > 1024) throw Other{};
+        Result order(v[2], at::kInt, {rows}, choice), back(v[3], at::kInt, choice.sizes(), choice), ends(v[4], at::kInt, {experts}, choice);
+        here.check(order);
+        here.check(back);
+        here.check(ends);
+        const uint64_t bytes = sortWorkspace((uint32_t)rows, (uint32_t)experts);
+        at::Tensor work;
+        if (bytes) work = at::empty({(int64_t)bytes}, choice.options().dtype(at::kByte));
+        uint8_t *const pc = address(choice), *const pwork = bytes ? address(work) : nullptr;
+        int32_t *const po = (int32_t *)order.at_(), *const pb = (int32_t *)back.at_(), *const pe = (int32_t *)ends.at_();
+        void *const s = stream();
+        Py_BEGIN_ALLOW_THREADS
+        sortByExpert(s, pc, po, pb, pe, pwork, bytes, (uint32_t)rows, (uint32_t)experts, wide ? 64 : 32);
+        Py_END_ALLOW_THREADS
+        return accepted() ? tupleOf({&order, &back, &ends}) : nullptr;
+    });
+}
+
+PyObject *spread(PyObject *, PyObject *const *v, Py_ssize_t n)   // x, back, scale, out, out_scale
+{
+    return guardedLayer("spread_rows", n, 5, [&]() -> PyObject * {
+        const Here here;
+        const at::Tensor &x = here.any(v[0], 2), &back = here.any(v[1], 2);
+        const int64_t tokens = x.size(0), cols = x.size(1), top = back.size(1);
+        if (x.scalar_type() != F8) code(x.scalar_type(), true);
+        if (back.scalar_type() != at::kInt || back.size(0) != tokens || back.numel() > MOST || tokens > MOST || top > MOST || cols > MOST) throw Other{};
+        const bool scaled = v[2] != Py_None;
+        if (!scaled && v[4] != Py_None) throw Other{};
+        const float *const scale = (const float *)here.maybe(v[2], at::kFloat, {blocks(cols), tokens});
+        Result out(v[3], x.scalar_type(), {tokens * top, cols}, x);
+        here.check(out);
+        std::optional<Result> outScale;
+        if (scaled) here.check(outScale.emplace(v[4], at::kFloat, at::IntArrayRef({blocks(cols), tokens * top}), x));
+        uint8_t *const px = address(x), *const po = out.at_();
+        const int32_t *const pb = (const int32_t *)address(back);
+        float *const ps = scaled ? (float *)outScale->at_() : nullptr;
+        const uint32_t size = (uint32_t)x.element_size();
+        void *const s = stream();
+        Py_BEGIN_ALLOW_THREADS
+        spreadRows(s, px, scale, pb, po, ps, (uint32_t)tokens, (uint32_t)top, (uint32_t)cols, size);
+        Py_END_ALLOW_THREADS
+        if (!accepted()) return nullptr;
+        return scaled ? tupleOf({&out, &*outScale}) : out.object();
+    });
+}
+
+PyObject *gather(PyObject *, PyObject *const *v, Py_ssize_t n)   // y, back, share, out
+{
+    return guardedLayer("gather_rows", n, 4, [&]() -> PyObject * {
+        const Here here;
+        const at::Tensor &y = here.any(v[0], 2), &back = here.any(v[1], 2);
+        const int64_t tokens = back.size(0), top = back.size(1), cols = y.size(1);
+        const uint32_t type = code(y.scalar_type(), true);
+        if (back.scalar_type() != at::kInt || y.size(0) != back.numel() || y.size(0) > MOST || tokens > MOST || top > MOST || cols > MOST) throw Other{};
+        const float *const share = (const float *)here.maybe(v[2], at::kFloat, {tokens, top});
+        Result out(v[3], y.scalar_type(), {tokens, cols}, y);
+        here.check(out);
+        uint8_t *const py = address(y), *const po = out.at_();
+        const int32_t *const pb = (const int32_t *)address(back);
+        void *const s = stream();
+        Py_BEGIN_ALLOW_THREADS
+        gatherRows(s, py, pb, share, po, (uint32_t)tokens, (uint32_t)top, (uint32_t)cols, type);
+        Py_END_ALLOW_THREADS
+        return accepted() ? out.object() : nullptr;
+    });
+}
+
+PyObject *gatherGradient(PyObject *, PyObject *const *v, Py_ssize_t n)   // dout, y, back, share, dy, dshare
+{
+    return guardedLayer("gather_rows_backward", n, 6, [&]() -> PyObject * {
+        const Here here;
+        const at::Tensor &y = here.any(v[1], 2), &back = here.any(v[2], 2);
+        const int64_t tokens = back.size(0), top = back.size(1), cols = y.size(1);
+        const uint32_t type = code(y.scalar_type(), true);
+        if (back.scalar_type() != at::kInt || y.size(0) != back.numel() || y.size(0) > MOST || tokens > MOST || top > MOST || cols > MOST) throw Other{};
+        const at::Tensor &dout = here.of(v[0], y.scalar_type(), {tokens, cols}), &share = here.of(v[3], at::kFloat, {tokens, top});
+        Result dy(v[4], y.scalar_type(), y.sizes(), y), dshare(v[5], at::kFloat, {tokens, top}, y);
+        here.check(dy);
+        here.check(dshare);
+        uint8_t *const pd = address(dout), *const py = address(y), *const po = dy.at_();
+        const int32_t *const pb = (const int32_t *)address(back);
+        const float *const ps = (const float *)address(share);
+        float *const pds = (float *)dshare.at_();
+        void *const s = stream();
+        Py_BEGIN_ALLOW_THREADS
+        gatherBackward(s, pd, py, pb, ps, po, pds, (uint32_t)tokens, (uint32_t)top, (uint32_t)cols, type);
+        Py_END_ALLOW_THREADS
+        return accepted() ? tupleOf({&dy, &dshare}) : nullptr;
+    });
+}
+
 PyMethodDef methods[] = {{"attach_ragged", (PyCFunction)(void *)attachRagged, METH_FASTCALL, "addresses of the e4m3 and grouped operators' functions"},
                          {"quantize_fp8", (PyCFunction)(void *)quantize, METH_FASTCALL, "one call: (codes, scale), or None for the Python path"},
                          {"fp8_matmul_allreduce", (PyCFunction)(void *)fp8, METH_FASTCALL, "one call: the output, or None for the Python path"},
                          {"grouped_matmul", (PyCFunction)(void *)grouped, METH_FASTCALL, "one call: the output, or None for the Python path"},
                          {"grouped_matmul_dw", (PyCFunction)(void *)dw, METH_FASTCALL, "one call: the output, or None for the Python path"},
                          {"grouped_fp8_matmul", (PyCFunction)(void *)fp8Grouped, METH_FASTCALL, "one call: the output, or None for the Python path"},
+                         {"attach_layer", (PyCFunction)(void *)attachLayer, METH_FASTCALL, "addresses of the functions around a layer of experts"},
+                         {"rms_norm", (PyCFunction)(void *)norm16, METH_FASTCALL, "one call: the output or outputs, or None for the Python path"},
+                         {"rms_norm_fp8", (PyCFunction)(void *)normFp8, METH_FASTCALL, "one call: the outputs, or None for the Python path"},
+                         {"rms_norm_backward", (PyCFunction)(void *)normBackward, METH_FASTCALL, "one call: (dx, dw), or None for the Python path"},
+                         {"route", (PyCFunction)(void *)route, METH_FASTCALL, "one call: (choice, share), or None for the Python path"},
+                         {"route_backward", (PyCFunction)(void *)routeGradient, METH_FASTCALL, "one call: the output, or None for the Python path"},
+                         {"sort_by_expert", (PyCFunction)(void *)sortChoices, METH_FASTCALL, "one call: (order, back, ends), or None for the Python path"},
+                         {"spread_rows", (PyCFunction)(void *)spread, METH_FASTCALL, "one call: the output or outputs, or None for the Python path"},
+                         {"gather_rows", (PyCFunction)(void *)gather, METH_FASTCALL, "one call: the output, or None for the Python path"},
+                         {"gather_rows_backward", (PyCFunction)(void *)gatherGradient, METH_FASTCALL, "one call: (dy, dshare), or None for the Python path"},
                          {"attach", (PyCFunction)(void *)attach, METH_FASTCALL, "addresses of the library's functions, CatcocError, CocTilingParams"},
                          {"call", (PyCFunction)(void *)call, METH_FASTCALL, "one operator call: the output, or None for the Python path"},
                          {nullptr, nullptr, 0, nullptr}};

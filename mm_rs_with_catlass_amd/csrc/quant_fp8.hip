@@ -9,51 +9,11 @@
 // 4096x4096 bf16 10.4 us; 16 rows of 1024 5.6 us, the launch.
 #include <hip/hip_runtime.h>
 
-#include "ragged.h"
+#include "rows_device.h"
 
 namespace catcoc {
 
 namespace {
-
-struct Eight {
-    float v[8];
-};
-
-// Values [at, at + 8) of a row of `size`; zeros past its end.
-template <uint32_t DT>
-__device__ __forceinline__ Eight load8(const void *x, size_t row, uint32_t pitch, uint32_t at, uint32_t size)
-{
-    constexpr uint32_t ES = DT == 0 ? 4u : 2u;
-    const unsigned char *p = (const unsigned char *)x + (row * pitch + at) * ES;
-    uint32_t raw[ES * 2];
-    if (at + 8u <= size) {
-        __builtin_memcpy(raw, p, sizeof raw);
-    } else {
-#pragma unroll
-        for (uint32_t i = 0; i < ES * 2u; ++i) raw[i] = 0;
-#pragma unroll
-        for (uint32_t i = 0; i < 7u; ++i) {
-            if (at + i >= size) continue;
-            if constexpr (DT == 0) __builtin_memcpy(&raw[i], p + 4u * i, 4);
-            else {
-                unsigned short h;
-                __builtin_memcpy(&h, p + 2u * i, 2);
-                raw[i >> 1] |= (uint32_t)h << (16u * (i & 1u));
-            }
-        }
-    }
-    Eight e;
-#pragma unroll
-    for (uint32_t i = 0; i < 8u; ++i) {
-        if constexpr (DT == 0) e.v[i] = __builtin_bit_cast(float, raw[i]);
-        else {
-            const uint32_t h = (raw[i >> 1] >> (16u * (i & 1u))) & 0xffffu;
-            if constexpr (DT == DT_BF16) e.v[i] = __builtin_bit_cast(float, h << 16);
-            else e.v[i] = (float)__builtin_bit_cast(_Float16, (unsigned short)h);
-        }
-    }
-    return e;
-}
 
 // silu(g) * u = g / (1 + e^-g) * u, where e^-g and its reciprocal are far inside fp32's range.  e^-g = 2^t e^r, t = -g log2 e and r what its rounding leaves: it would
 // else cost the result 2^-18.
@@ -86,57 +46,6 @@ __device__ __forceinline__ void silu_times8(Eight &g, const Eight &u)
 #pragma unroll
         for (int i = 0; i < 8; ++i) g.v[i] = silu_times_far(g.v[i], u.v[i]);
     }
-}
-
-__device__ __forceinline__ uint32_t magnitude(float v) { return __builtin_bit_cast(uint32_t, v) & 0x7fffffffu; }   // (as an integer: a NaN is the largest)
-
-__device__ __forceinline__ float scale_of(uint32_t top)
-{
-    const float t = __builtin_bit_cast(float, top);
-    return (t < kScaleFloor ? kScaleFloor : t) / kE4m3Top;   // (NaN stays)
-}
-
-__device__ __forceinline__ v2i codes8(const Eight &e, float scale)
-{
-    float q[8];
-    const float r = 1.f / scale;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        const float t = e.v[i] * r;
-        q[i] = __builtin_fmaf(__builtin_fmaf(-t, scale, e.v[i]), r, t);
-    }
-    if (!__builtin_isfinite(scale)) {   // (zeros and NaN)
-#pragma unroll
-        for (int i = 0; i < 8; ++i) q[i] = e.v[i] / scale;
-    }
-    int a = 0, b = 0;
-    a = __builtin_amdgcn_cvt_pk_fp8_f32(q[0], q[1], a, false);
-    a = __builtin_amdgcn_cvt_pk_fp8_f32(q[2], q[3], a, true);
-    b = __builtin_amdgcn_cvt_pk_fp8_f32(q[4], q[5], b, false);
-    b = __builtin_amdgcn_cvt_pk_fp8_f32(q[6], q[7], b, true);
-    return v2i{a, b};
-}
-
-__device__ __forceinline__ void store8(unsigned char *q, size_t row, uint32_t pitch, uint32_t at, uint32_t size, v2i v)
-{
-    unsigned char *p = q + row * pitch + at;
-    if (at + 8u <= size) {
-        __builtin_memcpy(p, &v, 8);
-    } else {
-#pragma unroll
-        for (uint32_t i = 0; i < 7u; ++i)
-            if (at + i < size) p[i] = (unsigned char)((uint32_t)v[i >> 2] >> (8u * (i & 3u)));
-    }
-}
-
-// The largest of 16 consecutive lanes' values, in all of them.
-__device__ __forceinline__ uint32_t max16(uint32_t v)
-{
-    v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x128, 0xf, 0xf, false));   // row_ror:8, 4, 2, 1
-    v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x124, 0xf, 0xf, false));
-    v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x122, 0xf, 0xf, false));
-    v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x121, 0xf, 0xf, false));
-    return v;
 }
 
 }  // namespace

@@ -9,19 +9,11 @@
 
 #include "gemm_dma_kernel.h"
 #include "ragged_args.h"
+#include "rows_device.h"
 
 namespace catcoc {
 
 typedef int v8i __attribute__((ext_vector_type(8)));
-
-// One dimension of a launch holds fewer than 2^32 threads: workgroups past that go on in the second one, in rows of kGridRow.  Those past the last one asked for
-// have to find nothing to do.  For the checked kernel and the quantizer; in the small tiles' kernel the second index costs a call of 18.5 us 0.46 of them.
-constexpr uint32_t kGridRowLog = 22, kGridRow = 1u << kGridRowLog;
-inline dim3 grid_of(uint64_t wgs, uint32_t threads)
-{
-    return wgs * threads < (1ull << 32) ? dim3((uint32_t)wgs) : dim3(kGridRow, (uint32_t)((wgs + kGridRow - 1u) >> kGridRowLog));
-}
-__device__ __forceinline__ uint32_t workgroup() { return (blockIdx.y << kGridRowLog) + blockIdx.x; }
 
 // A read of 16 bytes at any address.
 __device__ __forceinline__ v4i load16_any(const unsigned char *p)

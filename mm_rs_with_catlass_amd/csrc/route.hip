@@ -1,0 +1,538 @@
+// The router: which experts a token goes to, with what shares, the shares' gradient, and the rows' order by expert.
+//
+// A token's experts lie on 16 or 64 lanes, a group of them on a power of two of those, up to 32 a lane.  An expert's rank is one 64-bit number, its key: a double whose last ten bits
+// are the expert's index, counted so that of equal scores the lower index is the larger key.  Maxima of doubles then order scores and ties alike.  Where the
+// order is that of the logits (no bias, no sums of scores) a key holds all of a logit's bits; else it is the score in 64 bits, whose first 42 bits count: which of two
+// experts is ahead is a matter of more bits than fp32 has, as one of a prompt's 10^5 choices is decided by less than 2^-24 now and then.
+// Every lane sorts its keys once (odd-even merge sort: Batcher, AFIPS 1968); then the largest of the lanes' first keys is taken `top` times.
+#include <hip/hip_runtime.h>
+
+#include "layer_args.h"
+#include "rows_device.h"
+
+namespace catcoc {
+
+namespace {
+
+constexpr double kNone = -__builtin_huge_val();   // a key that is none: below all others
+constexpr double kMostKey = 0x1p1000;             // infinity and NaN count as this
+constexpr uint64_t kIndexBits = 1023;
+
+// An exchange between lanes of a row of 16.
+template <int CTRL>
+__device__ __forceinline__ float lane_turn(float v)
+{
+    return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTRL, 0xf, 0xf, false));
+}
+
+template <int CTRL>
+__device__ __forceinline__ double lane_turn(double v)
+{
+    const uint64_t b = __builtin_bit_cast(uint64_t, v);
+    const uint32_t lo = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)b, CTRL, 0xf, 0xf, false);
+    const uint32_t hi = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)(b >> 32), CTRL, 0xf, 0xf, false);
+    return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+}
+
+// f over the values of LANES lanes, in all of them, in an order that is always the same.
+template <int LANES, typename T, typename F>
+__device__ __forceinline__ T over_lanes(T v, F f)
+{
+    v = f(v, lane_turn<0x128>(v));   // row_ror:8, 4, 2, 1
+    v = f(v, lane_turn<0x124>(v));
+    v = f(v, lane_turn<0x122>(v));
+    v = f(v, lane_turn<0x121>(v));
+    if constexpr (LANES == 64) {
+        v = f(v, __shfl_xor(v, 16));
+        v = f(v, __shfl_xor(v, 32));
+    }
+    return v;
+}
+
+template <int LANES, typename T>
+__device__ __forceinline__ T lanes_max(T v)
+{
+    return over_lanes<LANES>(v, [](T a, T b) { return __builtin_elementwise_max(a, b); });
+}
+
+template <int LANES, typename T>
+__device__ __forceinline__ T lanes_sum(T v)
+{
+    return over_lanes<LANES>(v, [](T a, T b) { return a + b; });
+}
+
+__device__ __forceinline__ double with_index(double k, uint32_t index)
+{
+    if (k == kNone) return k;
+    k = k <= kMostKey ? k + 0.0 : kMostKey;   // (+ 0.0: -0 is 0)
+    const uint64_t b = __builtin_bit_cast(uint64_t, k);
+    return __builtin_bit_cast(double, (b & ~kIndexBits) | (b >> 63 ? index : kIndexBits - index));
+}
+
+__device__ __forceinline__ double without_index(double k) { return __builtin_bit_cast(double, __builtin_bit_cast(uint64_t, k) & ~kIndexBits); }
+
+__device__ __forceinline__ uint32_t index_of(double k)
+{
+    const uint64_t b = __builtin_bit_cast(uint64_t, k);
+    return (uint32_t)(b >> 63 ? b & kIndexBits : kIndexBits - (b & kIndexBits));
+}
+
+__device__ __forceinline__ void in_order(double &a, double &b)
+{
+    const double hi = __builtin_elementwise_max(a, b), lo = __builtin_elementwise_min(a, b);
+    a = hi;
+    b = lo;
+}
+
+// Largest first.
+template <int V>
+__device__ __forceinline__ void sort_keys(double (&k)[V])
+{
+#pragma unroll
+    for (int p = 1; p < V; p <<= 1)
+#pragma unroll
+        for (int q = p; q > 0; q >>= 1)
+#pragma unroll
+            for (int j = q % p; j + q < V; j += 2 * q)
+#pragma unroll
+                for (int i = 0; i < q; ++i)
+                    if (i + j + q < V && (i + j) / (2 * p) == (i + j + q) / (2 * p)) in_order(k[i + j], k[i + j + q]);
+}
+
+__device__ __forceinline__ float widen1(uint32_t h, uint32_t type)
+{
+    return type == DT_BF16 ? __builtin_bit_cast(float, h << 16) : (float)__builtin_bit_cast(_Float16, (unsigned short)h);
+}
+
+__device__ __forceinline__ float logit_at(const void *x, size_t at, uint32_t type)
+{
+    return type == 0 ? ((const float *)x)[at] : widen1(((const unsigned short *)x)[at], type);
+}
+
+// Logits [at, at + count) of up to V, -inf behind them.
+template <int V>
+__device__ __forceinline__ void load_logits(const void *x, size_t at, uint32_t count, uint32_t type, float (&v)[V])
+{
+    if (type == 0) {
+        const float *p = (const float *)x + at;
+        if (count == V) __builtin_memcpy(v, p, sizeof v);
+        else {
+#pragma unroll
+            for (uint32_t i = 0; i < V; ++i) v[i] = i < count ? p[i] : -__builtin_huge_valf();
+        }
+    } else {
+        const unsigned short *p = (const unsigned short *)x + at;
+        unsigned short h[V];
+        if (count == V) __builtin_memcpy(h, p, sizeof h);
+        else {
+#pragma unroll
+            for (uint32_t i = 0; i < V; ++i) h[i] = i < count ? p[i] : 0;
+        }
+#pragma unroll
+        for (uint32_t i = 0; i < V; ++i) v[i] = i < count ? widen1(h[i], type) : -__builtin_huge_valf();
+    }
+}
+
+// What an expert's share is made of, from its logit: of the softmax e^(l - most), of the sigmoid s(l), where it is only to be compared with that of the largest logit,
+// `most`, and that is not positive, e^(l - most) / (1 + e^l) in its place: s(l) itself could be 0 for all of them.
+__device__ __forceinline__ float weight_of(float l, float most, bool sigmoid, bool compared)
+{
+    if (!sigmoid) return expf(l - most);
+    return compared && most <= 0.f ? expf(l - most) / (1.f + expf(l)) : 1.f / (1.f + expf(-l));
+}
+
+}  // namespace
+
+template <int LANES, int V>
+__global__ void __launch_bounds__(256) route_kernel(const RouteArgs args)
+{
+    const uint32_t lane = threadIdx.x & 63u, l = lane % LANES;
+    const uint64_t at = ((uint64_t)workgroup() * 4u + (threadIdx.x >> 6)) * (64 / LANES) + lane / LANES;
+    if (at - lane / LANES >= args.tokens) return;   // (a wave without tokens)
+    const size_t token = at < args.tokens ? at : args.tokens - 1u;   // (the last one once more, for nothing)
+    const uint32_t slot = l / args.groupLanes, part = l % args.groupLanes, size = args.experts / args.groups, in = part * args.perLane;
+    const uint32_t first = slot * size + in, count = slot < args.groups && in < size ? umin(args.perLane, size - in) : 0u;
+    float v[V];
+    load_logits<V>(args.logits, token * args.experts + (count ? first : 0u), count, args.type, v);
+
+    float most = 0.f;
+    if (!args.sigmoid) {
+        most = v[0];
+#pragma unroll
+        for (int i = 1; i < V; ++i) most = __builtin_elementwise_max(most, v[i]);
+        most = lanes_max<LANES>(most);
+    }
+    double k[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) k[i] = v[i];
+    float total = 0.f;   // of the softmax
+    if (args.bias != nullptr || args.groupTop == 2) {
+        double p[V], sum = 0.0;
+        if (args.sigmoid) {
+#pragma unroll
+            for (int i = 0; i < V; ++i) p[i] = 1.0 / (1.0 + exp(-(double)v[i]));
+        } else {
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                p[i] = exp((double)v[i] - (double)most);
+                sum += p[i];
+            }
+            sum = lanes_sum<LANES>(sum);
+            total = (float)sum;
+            const double r = 1.0 / sum;
+#pragma unroll
+            for (int i = 0; i < V; ++i) p[i] *= r;
+        }
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            if (k[i] == kNone) continue;
+            k[i] = p[i];
+            if (args.bias != nullptr) k[i] += args.bias[first + i];   // (an expert that there is: its logit is more than -inf)
+        }
+    } else if (!args.sigmoid && !args.renormalize) {
+#pragma unroll
+        for (int i = 0; i < V; ++i) total += v[i] == -__builtin_huge_valf() ? 0.f : expf(v[i] - most);
+        total = lanes_sum<LANES>(total);
+    }
+#pragma unroll
+    for (int i = 0; i < V; ++i) k[i] = with_index(k[i], first + i);
+    sort_keys<V>(k);
+
+    if (args.topGroups < args.groups) {
+        double a = k[0], b = V > 1 ? k[V > 1 ? 1 : 0] : kNone;   // the group's best two
+        for (uint32_t by = 1; by < args.groupLanes; by <<= 1) {
+            const double c = __shfl_xor(a, (int)by), d = __shfl_xor(b, (int)by);
+            b = __builtin_elementwise_max(__builtin_elementwise_min(a, c), __builtin_elementwise_max(b, d));
+            a = __builtin_elementwise_max(a, c);
+        }
+        double best = without_index(a);
+        if (args.groupTop == 2 && b != kNone) best += without_index(b);
+        best = with_index(best, slot);
+        uint32_t ahead = 0;
+        for (uint32_t g = 0; g < args.groups; ++g) ahead += __shfl(best, (int)(g * args.groupLanes), LANES) > best ? 1u : 0u;
+        if (ahead >= args.topGroups) {
+#pragma unroll
+            for (int i = 0; i < V; ++i) k[i] = kNone;
+        }
+    }
+
+    double mine = kNone;   // lane j: the j-th choice
+    for (uint32_t j = 0; j < args.top; ++j) {
+        const double next = lanes_max<LANES>(k[0]);
+        if (l == j) mine = next;
+        const bool taken = k[0] == next;
+#pragma unroll
+        for (int i = 0; i + 1 < V; ++i) k[i] = taken ? k[i + 1] : k[i];
+        k[V - 1] = taken ? kNone : k[V - 1];
+    }
+    const bool on = mine != kNone;
+    const uint32_t expert = on ? index_of(mine) : 0u;
+    const float logit = on ? logit_at(args.logits, token * args.experts + expert, args.type) : -__builtin_huge_valf();
+    if (args.renormalize) most = lanes_max<LANES>(logit);
+    float share = on ? weight_of(logit, most, args.sigmoid, args.renormalize) : 0.f;
+    const bool spoilt = total != total;   // a softmax with a NaN or an infinity in it has no other scores either
+    if (args.renormalize) total = spoilt ? total : lanes_sum<LANES>(share);
+    if (args.renormalize || !args.sigmoid) share /= total;
+    if (l >= args.top || at >= args.tokens) return;
+    args.choice[token * args.top + l] = on ? (int32_t)expert : -1;
+    args.share[token * args.top + l] = on ? share * args.scale : 0.f;
+}
+
+// With w the shares without scale: dl_c = scale w_c (1 - s(l_c) where sigmoid) (g_c - sum of w g where they are shares of a sum); the softmax of all experts: dl_e = scale p_e (g_e - sum of p g).
+template <int LANES, int V>
+__global__ void __launch_bounds__(256) route_backward_kernel(const RouteArgs args)
+{
+    const uint32_t lane = threadIdx.x & 63u, l = lane % LANES;
+    const uint64_t at = ((uint64_t)workgroup() * 4u + (threadIdx.x >> 6)) * (64 / LANES) + lane / LANES;
+    if (at - lane / LANES >= args.tokens) return;
+    const size_t token = at < args.tokens ? at : args.tokens - 1u;
+    const uint32_t first = l * args.perLane, count = first < args.experts ? umin(args.perLane, args.experts - first) : 0u;
+    const bool all = !args.sigmoid && !args.renormalize;   // every expert's logit moves the shares
+    float v[V], most = 0.f, total = 1.f;
+    if (all) {
+        load_logits<V>(args.logits, token * args.experts + (count ? first : 0u), count, args.type, v);
+        most = v[0];
+#pragma unroll
+        for (int i = 1; i < V; ++i) most = __builtin_elementwise_max(most, v[i]);
+        most = lanes_max<LANES>(most);
+        total = 0.f;
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            v[i] = v[i] == -__builtin_huge_valf() ? 0.f : expf(v[i] - most);
+            total += v[i];
+        }
+        total = lanes_sum<LANES>(total);
+    }
+    const int32_t chosen = l < args.top ? args.chosen[token * args.top + l] : -1;
+    const bool on = (uint32_t)chosen < args.experts;
+    const float g = on ? args.dshare[token * args.top + l] * args.scale : 0.f;
+    const float logit = on ? logit_at(args.logits, token * args.experts + (uint32_t)chosen, args.type) : -__builtin_huge_valf();
+    if (args.renormalize) most = lanes_max<LANES>(logit);
+    float w = on && logit != -__builtin_huge_valf() ? weight_of(logit, most, args.sigmoid, args.renormalize) : 0.f;
+    if (args.renormalize) total = lanes_sum<LANES>(w);
+    if ((args.renormalize || !args.sigmoid) && total > 0.f) w /= total;   // (no sum: no expert)
+    const float sum = args.renormalize || all ? lanes_sum<LANES>(w * g) : 0.f;
+    float d = w * (g - (all ? 0.f : sum));
+    if (args.sigmoid) d *= 1.f / (1.f + expf(logit));
+    if (all) {
+        const float r = total > 0.f ? -sum / total : 0.f;
+#pragma unroll
+        for (int i = 0; i < V; ++i) v[i] *= r;
+    } else {
+#pragma unroll
+        for (int i = 0; i < V; ++i) v[i] = 0.f;
+    }
+    for (uint32_t j = 0; j < args.top; ++j) {   // (an expert that is chosen twice gets both)
+        const uint32_t to = (uint32_t)__shfl(chosen, (int)j, LANES) - first;
+        const float more = __shfl(d, (int)j, LANES);
+#pragma unroll
+        for (uint32_t i = 0; i < V; ++i) v[i] += to == i ? more : 0.f;
+    }
+    if (at >= args.tokens || count == 0) return;
+    const size_t to = token * args.experts + first;
+    if (args.type == 0) {
+        float *p = (float *)args.dlogits + to;
+        if (count == V) __builtin_memcpy(p, v, sizeof v);
+        else {
+#pragma unroll
+            for (uint32_t i = 0; i < V; ++i)
+                if (i < count) p[i] = v[i];
+        }
+    } else {
+        unsigned short h[V], *p = (unsigned short *)args.dlogits + to;
+#pragma unroll
+        for (uint32_t i = 0; i < V; ++i)
+            h[i] = args.type == DT_BF16 ? __builtin_bit_cast(unsigned short, (__bf16)v[i]) : __builtin_bit_cast(unsigned short, (_Float16)v[i]);
+        if (count == V) __builtin_memcpy(p, h, sizeof h);
+        else {
+#pragma unroll
+            for (uint32_t i = 0; i < V; ++i)
+                if (i < count) p[i] = h[i];
+        }
+    }
+}
+
+template <int LANES, int V, bool BACKWARD>
+static int launch_route_kernel(const RouteArgs &a, hipStream_t stream)
+{
+    const uint64_t waves = (a.tokens + (uint64_t)(64 / LANES) - 1u) / (64 / LANES);
+    const dim3 grid = grid_of((waves + 3) / 4, 256);
+    if constexpr (BACKWARD) hipLaunchKernelGGL((route_backward_kernel<LANES, V>), grid, dim3(256), 0, stream, a);
+    else hipLaunchKernelGGL((route_kernel<LANES, V>), grid, dim3(256), 0, stream, a);
+    return (int)hipGetLastError();
+}
+
+// Lanes of a token, and of a group in it, for `groups` groups of experts: 16 lanes where they hold it in 16 values each, else 64.
+static uint32_t route_lanes(RouteArgs &a, uint32_t groups)
+{
+    uint32_t slots = 1;
+    while (slots < groups) slots *= 2;
+    const uint32_t size = a.experts / groups;
+    for (uint32_t lanes = 16; lanes <= 64; lanes *= 4) {
+        if (slots > lanes || a.top > lanes) continue;
+        a.groupLanes = lanes / slots;
+        a.perLane = (size + a.groupLanes - 1) / a.groupLanes;
+        if (a.perLane <= (lanes == 16 ? 16u : 32u)) return lanes;
+    }
+    return 0;
+}
+
+template <bool BACKWARD>
+static int launch_route_shape(RouteArgs a, hipStream_t stream)
+{
+    const uint32_t lanes = route_lanes(a, BACKWARD ? 1u : a.groups), n = a.perLane;
+    if (lanes == 16) {
+        if (n <= 1) return launch_route_kernel<16, 1, BACKWARD>(a, stream);
+        if (n <= 2) return launch_route_kernel<16, 2, BACKWARD>(a, stream);
+        if (n <= 4) return launch_route_kernel<16, 4, BACKWARD>(a, stream);
+        if (n <= 8) return launch_route_kernel<16, 8, BACKWARD>(a, stream);
+        return launch_route_kernel<16, 16, BACKWARD>(a, stream);
+    }
+    if (n <= 2) return launch_route_kernel<64, 2, BACKWARD>(a, stream);
+    if (n <= 8) return launch_route_kernel<64, 8, BACKWARD>(a, stream);
+    if (n <= 16) return launch_route_kernel<64, 16, BACKWARD>(a, stream);
+    if constexpr (!BACKWARD) return launch_route_kernel<64, 32, false>(a, stream);   // (groups in a number that is no power of two)
+    return -1;
+}
+
+// Groups that the kernel can lay out: at most 64 of them.
+bool can_route(uint32_t experts, uint32_t top, uint32_t groups)
+{
+    RouteArgs a{};
+    a.experts = experts;
+    a.top = top;
+    return route_lanes(a, groups) != 0;
+}
+
+int launch_route(const RouteArgs &a, void *stream) { return launch_route_shape<false>(a, (hipStream_t)stream); }
+int launch_route_backward(const RouteArgs &a, void *stream) { return launch_route_shape<true>(a, (hipStream_t)stream); }
+
+// ---- rows by expert -----------------------------------------------------------------------------------------------------------------------
+// A counting sort, stable: a wave counts how many of its consecutive rows go to each expert, the counts' sums over waves, blocks and experts are where its first
+// row of each goes, and the rows follow in 64s, a row's place among them by how many lanes before it have the same expert.
+
+namespace {
+
+constexpr uint32_t kSortWaves = 16;
+
+// The expert of a row; `experts` for one that is none's.
+template <typename I>
+__device__ __forceinline__ uint32_t expert_of(const SortArgs &args, uint32_t row)
+{
+    const I c = ((const I *)args.choice)[row];
+    return c >= 0 && c < (I)args.experts ? (uint32_t)c : args.experts;
+}
+
+template <typename I, uint32_t MOST>
+__device__ __forceinline__ void count_rows(const SortArgs &args, uint32_t (&count)[kSortWaves][MOST + 1], uint32_t begin, uint32_t end)
+{
+    for (uint32_t i = threadIdx.x; i < kSortWaves * (MOST + 1u); i += 64u * kSortWaves) (&count[0][0])[i] = 0;
+    __syncthreads();
+    const uint32_t wave = threadIdx.x >> 6;
+    for (uint32_t row = begin + (threadIdx.x & 63u); row < end; row += 64u) atomicAdd(&count[wave][expert_of<I>(args, row)], 1u);
+    __syncthreads();
+}
+
+__device__ __forceinline__ void wave_rows(const SortArgs &args, uint32_t &begin, uint32_t &end)
+{
+    const uint32_t each = args.perBlock / kSortWaves;
+    const uint64_t from = (uint64_t)blockIdx.x * args.perBlock + (threadIdx.x >> 6) * each;
+    begin = (uint32_t)(from < args.rows ? from : args.rows);
+    end = (uint32_t)(from + each < args.rows ? from + each : args.rows);
+}
+
+}  // namespace
+
+template <typename I, uint32_t MOST>
+__global__ void __launch_bounds__(64 * kSortWaves) count_by_expert_kernel(const SortArgs args)
+{
+    __shared__ uint32_t count[kSortWaves][MOST + 1];
+    uint32_t begin, end;
+    wave_rows(args, begin, end);
+    count_rows<I, MOST>(args, count, begin, end);
+    for (uint32_t e = threadIdx.x; e <= args.experts; e += 64u * kSortWaves) {
+        uint32_t n = 0;
+        for (uint32_t w = 0; w < kSortWaves; ++w) n += count[w][e];
+        args.part[(size_t)blockIdx.x * (args.experts + 1u) + e] = n;
+    }
+}
+
+template <typename I, uint32_t MOST>
+__global__ void __launch_bounds__(64 * kSortWaves) sort_by_expert_kernel(const SortArgs args)
+{
+    constexpr uint32_t THREADS = 64 * kSortWaves, SLICES = MOST < 512 ? 4 : 1, WIDE = THREADS / SLICES;
+    __shared__ uint32_t count[kSortWaves][MOST + 1];
+    __shared__ uint32_t totals[SLICES][MOST + 1], before[SLICES][MOST + 1], sums[kSortWaves];
+    uint32_t begin, end;
+    wave_rows(args, begin, end);
+    count_rows<I, MOST>(args, count, begin, end);
+    // ---- each expert's rows: of all blocks, and of those before this one
+    const uint32_t slice = threadIdx.x / WIDE;
+    for (uint32_t e = threadIdx.x % WIDE; e <= args.experts; e += WIDE) {
+        uint32_t all = 0, those = 0;
+        if (args.part == nullptr) {
+            if (slice == 0) {
+#pragma unroll
+                for (uint32_t w = 0; w < kSortWaves; ++w) all += count[w][e];
+            }
+        } else {
+#pragma unroll 8
+            for (uint32_t b = slice; b < args.blocks; b += SLICES) {
+                const uint32_t n = args.part[(size_t)b * (args.experts + 1u) + e];
+                all += n;
+                those += b < blockIdx.x ? n : 0u;
+            }
+        }
+        totals[slice][e] = all;
+        before[slice][e] = those;
+    }
+    __syncthreads();
+    // ---- where an expert's rows begin
+    uint32_t n = 0, upTo;
+    if (threadIdx.x < args.experts) {
+#pragma unroll
+        for (uint32_t s = 0; s < SLICES; ++s) n += totals[s][threadIdx.x];
+    }
+    upTo = n;
+#pragma unroll
+    for (uint32_t by = 1; by < 64; by <<= 1) {
+        const uint32_t less = __shfl_up(upTo, by);
+        if ((threadIdx.x & 63u) >= by) upTo += less;
+    }
+    if ((threadIdx.x & 63u) == 63u) sums[threadIdx.x >> 6] = upTo;
+    __syncthreads();
+    uint32_t every = 0;
+#pragma unroll
+    for (uint32_t w = 0; w < kSortWaves; ++w) {
+        upTo += w < threadIdx.x >> 6 ? sums[w] : 0u;
+        every += sums[w];
+    }
+    if (blockIdx.x == 0 && threadIdx.x < args.experts) args.ends[threadIdx.x] = (int32_t)upTo;
+    // ---- where a wave's first row of each expert goes (behind the last expert's: the rows of none)
+    auto spread = [&](uint32_t e, uint32_t at) {
+#pragma unroll
+        for (uint32_t s = 0; s < SLICES; ++s) at += before[s][e];
+        for (uint32_t w = 0; w < kSortWaves; ++w) {
+            const uint32_t c = count[w][e];
+            count[w][e] = at;
+            at += c;
+        }
+    };
+    if (threadIdx.x < args.experts) spread(threadIdx.x, upTo - n);
+    if (threadIdx.x == THREADS - 1u) spread(args.experts, every);
+    __syncthreads();
+    const uint32_t wave = threadIdx.x >> 6, lane = threadIdx.x & 63u, bits = 32u - (uint32_t)__builtin_clz(args.experts);
+    for (uint32_t first = begin; first < end; first += 64u) {
+        const uint32_t row = first + lane;
+        const bool on = row < end;
+        const uint32_t e = on ? expert_of<I>(args, row) : 0u;
+        uint64_t same = __ballot(on);
+        for (uint32_t b = 0; b < bits; ++b) {
+            const bool set = (e >> b) & 1u;
+            const uint64_t those = __ballot(set);
+            same &= set ? those : ~those;
+        }
+        const uint32_t rank = (uint32_t)__builtin_popcountll(same & ((1ull << lane) - 1ull));
+        if (on) {
+            volatile uint32_t *const next = &count[wave][e];   // (a wave's own: its accesses stay in order)
+            const uint32_t at = *next + rank;
+            if (rank == 0) *next = at + (uint32_t)__builtin_popcountll(same);
+            args.back[row] = (int32_t)at;
+            if (at < args.rows) args.order[at] = (int32_t)row;   // (it is, unless the choices change meanwhile)
+        }
+    }
+}
+
+// Blocks of a sort: one, in one launch, where that is all there is to do; then the blocks' counts are summed by every block.
+constexpr uint32_t kSortAlone = 8192, kSortBlock = 1024, kMostSortBlocks = 256;
+
+uint32_t sort_blocks(uint32_t rows)
+{
+    if (rows <= kSortAlone) return 1;
+    const uint32_t blocks = rows / kSortBlock + (rows % kSortBlock != 0);
+    return blocks < kMostSortBlocks ? blocks : kMostSortBlocks;
+}
+
+template <typename I, uint32_t MOST>
+static int launch_sort_type(const SortArgs &a, hipStream_t stream)
+{
+    if (a.blocks > 1) {
+        hipLaunchKernelGGL((count_by_expert_kernel<I, MOST>), dim3(a.blocks), dim3(64 * kSortWaves), 0, stream, a);
+        const int e = (int)hipGetLastError();
+        if (e) return e;
+    }
+    hipLaunchKernelGGL((sort_by_expert_kernel<I, MOST>), dim3(a.blocks), dim3(64 * kSortWaves), 0, stream, a);
+    return (int)hipGetLastError();
+}
+
+int launch_sort(uint32_t choiceBits, SortArgs a, void *stream)
+{
+    a.blocks = sort_blocks(a.rows);
+    const uint64_t each = (a.rows + (uint64_t)a.blocks - 1u) / a.blocks;
+    a.perBlock = (uint32_t)((each + kSortBlock - 1u) / kSortBlock * kSortBlock);
+    if (a.blocks == 1) a.part = nullptr;
+    if (choiceBits == 32) return a.experts <= 256 ? launch_sort_type<int32_t, 256>(a, (hipStream_t)stream) : launch_sort_type<int32_t, 1024>(a, (hipStream_t)stream);
+    return a.experts <= 256 ? launch_sort_type<int64_t, 256>(a, (hipStream_t)stream) : launch_sort_type<int64_t, 1024>(a, (hipStream_t)stream);
+}
+
+}  // namespace catcoc

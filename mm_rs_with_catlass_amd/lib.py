@@ -56,6 +56,14 @@ class CatcocSymmetricDesc(C.Structure):
 KERNEL_GENERAL, KERNEL_ALIGNED, KERNEL_FLEXIBLE, KERNEL_SMALL, KERNEL_STREAMING, KERNEL_RAGGED, KERNEL_RAGGED_CHECKED = 1, 2, 3, 4, 5, 6, 7
 
 
+SCORES = {"softmax": 0, "sigmoid": 1}
+
+
+class CatcocRouting(C.Structure):
+    _fields_ = [("score", C.c_uint32), ("groups", C.c_uint32), ("topGroups", C.c_uint32), ("groupTop", C.c_uint32), ("renormalize", C.c_uint32),
+                ("scale", C.c_float)]
+
+
 class CatcocLaunchInfo(C.Structure):
     _fields_ = [(n, C.c_uint32) for n in ("kernel", "tileRows", "tileCols", "kSlices", "dealt", "largeTiles")]
 
@@ -94,7 +102,12 @@ EXPORTS = [
     "catcoc_verify", "catcoc_comm_block_idx_ex", "catcoc_comm_core_loop", "catcoc_task_tiles",
     "catcoc_pipelined_plan_create", "catcoc_pipelined_plan_destroy", "catcoc_pipelined_round_count",
     "catcoc_quantize_fp8", "catcoc_fp8_matmul_allreduce", "catcoc_grouped_matmul", "catcoc_grouped_matmul_dw", "catcoc_grouped_fp8_matmul",
+    "catcoc_rms_norm", "catcoc_rms_norm_backward", "catcoc_rms_norm_backward_workspace_size", "catcoc_route", "catcoc_route_backward",
+    "catcoc_sort_by_expert", "catcoc_sort_by_expert_workspace_size", "catcoc_spread_rows", "catcoc_gather_rows", "catcoc_gather_rows_backward",
 ]
+
+LAYER_OPS = ("catcoc_rms_norm", "catcoc_rms_norm_backward", "catcoc_route", "catcoc_route_backward", "catcoc_sort_by_expert", "catcoc_spread_rows",
+             "catcoc_gather_rows", "catcoc_gather_rows_backward")
 
 _lib = None
 
@@ -223,6 +236,20 @@ def load():
     L.catcoc_grouped_fp8_matmul.argtypes = [vp] * 7 + [u32] * 5 + [vp]
     for n in ("catcoc_quantize_fp8", "catcoc_fp8_matmul_allreduce", "catcoc_grouped_matmul", "catcoc_grouped_matmul_dw", "catcoc_grouped_fp8_matmul"):
         getattr(L, n).restype = None
+    u64 = C.c_uint64
+    L.catcoc_rms_norm.argtypes = [vp] * 8 + [u32, u32, C.c_float, u32, u32, u32]
+    L.catcoc_rms_norm_backward.argtypes = [vp] * 8 + [u64, u32, u32, C.c_float, u32, u32, u32]
+    L.catcoc_route.argtypes = [vp] * 5 + [C.POINTER(CatcocRouting), u32, u32, u32, u32]
+    L.catcoc_route_backward.argtypes = [vp] * 5 + [C.POINTER(CatcocRouting), u32, u32, u32, u32]
+    L.catcoc_sort_by_expert.argtypes = [vp] * 6 + [u64, u32, u32, u32]
+    L.catcoc_spread_rows.argtypes = [vp] * 6 + [u32] * 4
+    L.catcoc_gather_rows.argtypes = [vp] * 5 + [u32] * 4
+    L.catcoc_gather_rows_backward.argtypes = [vp] * 7 + [u32] * 4
+    for n in LAYER_OPS:
+        getattr(L, n).restype = None
+    for n in ("catcoc_rms_norm_backward_workspace_size", "catcoc_sort_by_expert_workspace_size"):
+        getattr(L, n).argtypes = [u32, u32]
+        getattr(L, n).restype = u64
     _lib = L
     return L
 
@@ -239,6 +266,9 @@ def load_host():
         CatcocError, CocTilingParams)
     _host.attach_ragged(*(C.cast(getattr(L, n), C.c_void_p).value for n in (
         "catcoc_quantize_fp8", "catcoc_fp8_matmul_allreduce", "catcoc_grouped_matmul", "catcoc_grouped_matmul_dw", "catcoc_grouped_fp8_matmul")))
+    _host.attach_layer(*(C.cast(getattr(L, n), C.c_void_p).value for n in (
+        "catcoc_rms_norm", "catcoc_rms_norm_backward", "catcoc_rms_norm_backward_workspace_size", "catcoc_route", "catcoc_route_backward", "catcoc_sort_by_expert",
+        "catcoc_sort_by_expert_workspace_size", "catcoc_spread_rows", "catcoc_gather_rows", "catcoc_gather_rows_backward")))
     return _host
 
 

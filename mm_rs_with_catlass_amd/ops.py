@@ -745,6 +745,313 @@ def grouped_fp8_matmul(x, w, scale_x, scale_w, group_ends, out_dtype=torch.bfloa
     return out
 
 
+MOST_EXPERTS, MOST_TOP = 1024, 64   # experts of the router and of the sort by expert; choices of a token
+
+
+def _check_here(*ts):
+    """Operands of the operators below: on the current device, whose stream the call goes to."""
+    _check_dev(*ts)
+    here = torch.cuda.current_device()
+    for t in ts:
+        if t is not None and t.device.index != here:
+            _fail("operands must live on the current device %d (got a tensor on %s)", here, t.device)
+
+
+def _float_type(t, name):
+    if t.dtype is torch.float32:
+        return 0
+    if t.dtype not in _TORCH_TO_DT:
+        _fail("%s must be float16, bfloat16 or float32 (got %s)", name, t.dtype)
+    return _TORCH_TO_DT[t.dtype]
+
+
+def _like_or_wide(t, dtype, name):
+    """The code of an operand that is of the given type or fp32."""
+    _want(t, name, (dtype, torch.float32))
+    return _float_type(t, name)
+
+
+def _norm_operands(x, weight, residual, residual_out):
+    _want(x, "x", None, 2)
+    rows, cols = x.shape
+    types = _float_type(x, "x"), 0 if residual is None else _like_or_wide(residual, x.dtype, "residual"), _like_or_wide(weight, x.dtype, "weight")
+    _fits("x", rows=rows, columns=cols)
+    _want(weight, "weight", None, 1, None, (cols,))
+    _want(residual, "residual", None, 2, None, (rows, cols))
+    if residual is None and residual_out is not None:
+        _fail("residual_out without a residual")
+    if residual is not None:
+        _want(residual_out, "residual_out", residual.dtype, 2, None, (rows, cols))
+    return types
+
+
+def _rms_norm(x, weight, residual, eps, types, out, residual_out, codes, scale):
+    t, rt, wt = types
+    _l.load().catcoc_rms_norm(_stream(), x.data_ptr(), _ptr(residual), weight.data_ptr(), _ptr(out), _ptr(residual_out), _ptr(codes), _ptr(scale),
+                              x.shape[0], x.shape[1], eps, t, rt, wt)
+    _l.check()
+
+
+def rms_norm(x, weight, residual=None, eps=1e-6, out=None, residual_out=None):
+    """s = x + residual, y = s / sqrt(mean(s^2) + eps) * weight over each row (catcoc_rms_norm).
+
+    x [rows,cols] fp16, bf16 or fp32, at most 16384 columns; weight [cols] and residual [rows,cols] of x's type or fp32.  Returns y in x's type; with a residual
+    (y, s), s in the residual's type and what y is the norm of.  out may be x, residual_out residual."""
+    done = (_host or _compiled()).rms_norm(x, weight, residual, eps, out, residual_out)
+    if done is not None:
+        return done
+    types = _norm_operands(x, weight, residual, residual_out)
+    _want(out, "out", x.dtype, 2, None, tuple(x.shape))
+    _check_here(x, weight, residual, out, residual_out)
+    if out is None:
+        out = torch.empty_like(x)
+    if residual is not None and residual_out is None:
+        residual_out = torch.empty_like(residual)
+    _rms_norm(x, weight, residual, eps, types, out, residual_out, None, None)
+    return out if residual is None else (out, residual_out)
+
+
+def rms_norm_fp8(x, weight, residual=None, eps=1e-6, keep=False, out=None, scale=None, kept=None, residual_out=None):
+    """rms_norm() with y in e4m3: (codes [rows,cols], scale [ceil(cols/128), rows]), as quantize_fp8() makes them of y before its rounding; then, with keep, y in x's
+    type too, and, with a residual, s.  out, scale, kept, residual_out: tensors for the results."""
+    done = (_host or _compiled()).rms_norm_fp8(x, weight, residual, eps, keep, out, scale, kept, residual_out)
+    if done is not None:
+        return done
+    types = _norm_operands(x, weight, residual, residual_out)
+    rows, cols = x.shape
+    _want(out, "out", torch.float8_e4m3fn, 2, None, (rows, cols))
+    _want(scale, "scale", torch.float32, 2, None, (_blocks(cols), rows))
+    if kept is not None and not keep:
+        _fail("kept without keep")
+    _want(kept, "kept", x.dtype, 2, None, (rows, cols))
+    _check_here(x, weight, residual, out, scale, kept, residual_out)
+    if out is None:
+        out = torch.empty((rows, cols), dtype=torch.float8_e4m3fn, device=x.device)
+    if scale is None:
+        scale = torch.empty((_blocks(cols), rows), dtype=torch.float32, device=x.device)
+    if keep and kept is None:
+        kept = torch.empty_like(x)
+    if residual is not None and residual_out is None:
+        residual_out = torch.empty_like(residual)
+    _rms_norm(x, weight, residual, eps, types, kept, residual_out, out, scale)
+    return (out, scale) + ((kept,) if keep else ()) + ((residual_out,) if residual is not None else ())
+
+
+def rms_norm_backward(dy, x, weight, dsum=None, eps=1e-6, dx=None, dw=None):
+    """The gradients of rms_norm() (catcoc_rms_norm_backward): (dx, dw).
+
+    dy [rows,cols] of y's type; x what was normalised (with a residual: s), of that type or fp32, as dsum: what else flows into s; dx, of x's type, is the gradient of
+    the residual too.  weight, dw [cols] of dy's type or fp32.  dx may be dsum."""
+    done = (_host or _compiled()).rms_norm_backward(dy, x, weight, dsum, eps, dx, dw)
+    if done is not None:
+        return done
+    _want(dy, "dy", None, 2)
+    rows, cols = dy.shape
+    t, st, wt = _float_type(dy, "dy"), _like_or_wide(x, dy.dtype, "x"), _like_or_wide(weight, dy.dtype, "weight")
+    _fits("dy", rows=rows, columns=cols)
+    _want(x, "x", None, 2, None, (rows, cols))
+    _want(weight, "weight", None, 1, None, (cols,))
+    _want(dsum, "dsum", x.dtype, 2, None, (rows, cols))
+    _want(dx, "dx", x.dtype, 2, None, (rows, cols))
+    _want(dw, "dw", weight.dtype, 1, None, (cols,))
+    _check_here(dy, x, weight, dsum, dx, dw)
+    if dx is None:
+        dx = torch.empty_like(x)
+    if dw is None:
+        dw = torch.empty_like(weight)
+    so = _l.load()
+    work = torch.empty(int(so.catcoc_rms_norm_backward_workspace_size(rows, cols)), dtype=torch.uint8, device=x.device)
+    so.catcoc_rms_norm_backward(_stream(), dy.data_ptr(), x.data_ptr(), weight.data_ptr(), _ptr(dsum), dx.data_ptr(), dw.data_ptr(), work.data_ptr(), work.numel(),
+                                rows, cols, eps, t, st, wt)
+    _l.check()
+    return dx, dw
+
+
+def _routing(score, groups, top_groups, group_top, renormalize, scale):
+    if score not in _l.SCORES:
+        _fail("score must be one of %s (got %r)", ", ".join(sorted(_l.SCORES)), score)
+    for name, v in (("groups", groups), ("top_groups", top_groups), ("group_top", group_top)):
+        if not isinstance(v, int) or not 1 <= v < 2 ** 31:
+            _fail("%s must be a positive number (got %r)", name, v)
+    return _l.CatcocRouting(_l.SCORES[score], groups, top_groups, group_top, bool(renormalize), scale)
+
+
+def _want_top(top):
+    if not isinstance(top, int) or not 1 <= top < 2 ** 31:
+        _fail("top must be a positive number (got %r)", top)
+
+
+def route(logits, top, score="softmax", bias=None, groups=1, top_groups=1, group_top=1, renormalize=True, scale=1.0, choice=None, share=None):
+    """Each token's `top` best experts and their shares (catcoc_route): (choice int32 [tokens,top], share fp32 [tokens,top]).
+
+    logits [tokens,experts] fp16, bf16 or fp32, at most 1024 experts.  score: "softmax" or "sigmoid" of the logits.  bias [experts] fp32: added to the scores for the choice, not for
+    the shares.  groups: experts come in so many groups of consecutive ones (at most 64), and are chosen from the `top_groups` of them whose `group_top` (1 or 2) best
+    sum to most.  Ties go to the lowest index.  share: the scores, of their sum where renormalised, times scale.  Logits of -inf (and biases): experts that are not to be
+    had; where too few are left the choice is -1, no expert, and its share 0."""
+    done = (_host or _compiled()).route(logits, top, score, bias, groups, top_groups, group_top, renormalize, scale, choice, share)
+    if done is not None:
+        return done
+    _want(logits, "logits", None, 2)
+    tokens, experts = logits.shape
+    t = _float_type(logits, "logits")
+    _fits("logits", rows=tokens, columns=experts)
+    _want_top(top)
+    how = _routing(score, groups, top_groups, group_top, renormalize, scale)
+    _want(bias, "bias", torch.float32, 1, None, (experts,))
+    _want(choice, "choice", torch.int32, 2, None, (tokens, top))
+    _want(share, "share", torch.float32, 2, None, (tokens, top))
+    _check_here(logits, bias, choice, share)
+    if choice is None:
+        choice = torch.empty((tokens, top), dtype=torch.int32, device=logits.device)
+    if share is None:
+        share = torch.empty((tokens, top), dtype=torch.float32, device=logits.device)
+    _l.load().catcoc_route(_stream(), logits.data_ptr(), _ptr(bias), choice.data_ptr(), share.data_ptr(), C.byref(how), tokens, experts, top, t)
+    _l.check()
+    return choice, share
+
+
+def route_backward(dshare, logits, choice, score="softmax", renormalize=True, scale=1.0, out=None):
+    """The gradient of route()'s logits from that of its shares, for the choice that it made (catcoc_route_backward); score, renormalize and scale as there."""
+    done = (_host or _compiled()).route_backward(dshare, logits, choice, score, renormalize, scale, out)
+    if done is not None:
+        return done
+    _want(logits, "logits", None, 2)
+    tokens, experts = logits.shape
+    t = _float_type(logits, "logits")
+    _fits("logits", rows=tokens, columns=experts)
+    _want(choice, "choice", torch.int32, 2)
+    if choice.shape[0] != tokens:
+        _fail("choice has %d rows, logits have %d", choice.shape[0], tokens)
+    top = choice.shape[1]
+    _want(dshare, "dshare", torch.float32, 2, None, (tokens, top))
+    _want(out, "out", logits.dtype, 2, None, (tokens, experts))
+    how = _routing(score, 1, 1, 1, renormalize, scale)
+    _check_here(dshare, logits, choice, out)
+    if out is None:
+        out = torch.empty_like(logits)
+    _l.load().catcoc_route_backward(_stream(), dshare.data_ptr(), logits.data_ptr(), choice.data_ptr(), out.data_ptr(), C.byref(how), tokens, experts, top, t)
+    _l.check()
+    return out
+
+
+def sort_by_expert(choice, experts, order=None, back=None, ends=None):
+    """The choices' rows by expert (catcoc_sort_by_expert): (order, back, ends), all int32.
+
+    choice [tokens,top] int32 or int64.  order [tokens*top]: row i of the sorted rows is choice order[i] of the flattened ones, in ascending order within an expert; back, of
+    choice's shape: where each choice's row is; ends [experts]: one past each expert's last row, group_ends of the grouped operators.  Choices of no expert (-1, or
+    past the last one) are sorted behind the last one's.  At most 1024 experts.  Nothing is read back to the host."""
+    done = (_host or _compiled()).sort_by_expert(choice, experts, order, back, ends)
+    if done is not None:
+        return done
+    _want(choice, "choice", (torch.int32, torch.int64), 2)
+    rows = choice.numel()
+    _fits("choice", rows=rows)
+    if not isinstance(experts, int) or not 1 <= experts <= MOST_EXPERTS:
+        _fail("experts must be a number in 1..%d (got %r)", MOST_EXPERTS, experts)
+    _want(order, "order", torch.int32, 1, None, (rows,))
+    _want(back, "back", torch.int32, 2, None, tuple(choice.shape))
+    _want(ends, "ends", torch.int32, 1, None, (experts,))
+    _check_here(choice, order, back, ends)
+    if order is None:
+        order = torch.empty(rows, dtype=torch.int32, device=choice.device)
+    if back is None:
+        back = torch.empty(choice.shape, dtype=torch.int32, device=choice.device)
+    if ends is None:
+        ends = torch.empty(experts, dtype=torch.int32, device=choice.device)
+    so = _l.load()
+    work = torch.empty(int(so.catcoc_sort_by_expert_workspace_size(rows, experts)), dtype=torch.uint8, device=choice.device)
+    so.catcoc_sort_by_expert(_stream(), choice.data_ptr(), order.data_ptr(), back.data_ptr(), ends.data_ptr(), work.data_ptr(), work.numel(), rows, experts,
+                             64 if choice.dtype == torch.int64 else 32)
+    _l.check()
+    return order, back, ends
+
+
+def _want_back(back, tokens=None):
+    """(tokens, choices of each)"""
+    _want(back, "back", torch.int32, 2)
+    if tokens is not None and back.shape[0] != tokens:
+        _fail("back has %d rows, there are %d tokens", back.shape[0], tokens)
+    _fits("back", rows=back.numel())
+    return tuple(back.shape)
+
+
+def spread_rows(x, back, scale=None, out=None, out_scale=None):
+    """Every token's row at the places of its choices (catcoc_spread_rows): out[back[t,j]] = x[t].
+
+    x [tokens,cols] fp16, bf16, fp32 or e4m3; back [tokens,top] int32 from sort_by_expert().  Returns [tokens*top,cols]; with scale [ceil(cols/128), tokens] of e4m3 rows
+    (out, scale [ceil(cols/128), tokens*top]).  Places outside the rows (-1) are left out, rows that no choice has stay as they were.  The gradient is gather_rows()."""
+    done = (_host or _compiled()).spread_rows(x, back, scale, out, out_scale)
+    if done is not None:
+        return done
+    _want(x, "x", (torch.float8_e4m3fn, torch.float16, torch.bfloat16, torch.float32), 2)
+    tokens, cols = x.shape
+    _fits("x", rows=tokens, columns=cols)
+    _, top = _want_back(back, tokens)
+    if scale is None and out_scale is not None:
+        _fail("out_scale without scale")
+    _want(scale, "scale", torch.float32, 2, None, (_blocks(cols), tokens))
+    _want(out, "out", x.dtype, 2, None, (tokens * top, cols))
+    _want(out_scale, "out_scale", torch.float32, 2, None, (_blocks(cols), tokens * top))
+    _check_here(x, back, scale, out, out_scale)
+    if out is None:
+        out = torch.empty((tokens * top, cols), dtype=x.dtype, device=x.device)
+    if scale is not None and out_scale is None:
+        out_scale = torch.empty((_blocks(cols), tokens * top), dtype=torch.float32, device=x.device)
+    _l.load().catcoc_spread_rows(_stream(), x.data_ptr(), _ptr(scale), back.data_ptr(), out.data_ptr(), _ptr(out_scale), tokens, top, cols, x.element_size())
+    _l.check()
+    return out if scale is None else (out, out_scale)
+
+
+def gather_rows(y, back, share=None, out=None):
+    """The choices' rows summed at their tokens (catcoc_gather_rows): out[t] = sum over j of share[t,j] y[back[t,j]], in fp32 and rounded once.
+
+    y [tokens*top,cols] fp16, bf16 or fp32; back [tokens,top] int32; share [tokens,top] fp32 (None: ones).  Returns [tokens,cols]."""
+    done = (_host or _compiled()).gather_rows(y, back, share, out)
+    if done is not None:
+        return done
+    tokens, top = _want_back(back)
+    _want(y, "y", None, 2)
+    t = _float_type(y, "y")
+    cols = y.shape[1]
+    _fits("y", columns=cols)
+    _want(y, "y", None, 2, None, (tokens * top, cols))
+    _want(share, "share", torch.float32, 2, None, (tokens, top))
+    _want(out, "out", y.dtype, 2, None, (tokens, cols))
+    _check_here(y, back, share, out)
+    if out is None:
+        out = torch.empty((tokens, cols), dtype=y.dtype, device=y.device)
+    _l.load().catcoc_gather_rows(_stream(), y.data_ptr(), back.data_ptr(), _ptr(share), out.data_ptr(), tokens, top, cols, t)
+    _l.check()
+    return out
+
+
+def gather_rows_backward(dout, y, back, share, dy=None, dshare=None):
+    """The gradients of gather_rows() with shares (catcoc_gather_rows_backward): (dy, of y's type, dshare fp32).  Rows of dy that no choice has stay as they were."""
+    done = (_host or _compiled()).gather_rows_backward(dout, y, back, share, dy, dshare)
+    if done is not None:
+        return done
+    tokens, top = _want_back(back)
+    _want(y, "y", None, 2)
+    t = _float_type(y, "y")
+    cols = y.shape[1]
+    _fits("y", columns=cols)
+    _want(y, "y", None, 2, None, (tokens * top, cols))
+    _want(dout, "dout", y.dtype, 2, None, (tokens, cols))
+    if not isinstance(share, torch.Tensor):
+        _fail("share must be a tensor (got %s)", type(share).__name__)
+    _want(share, "share", torch.float32, 2, None, (tokens, top))
+    _want(dy, "dy", y.dtype, 2, None, tuple(y.shape))
+    _want(dshare, "dshare", torch.float32, 2, None, (tokens, top))
+    _check_here(dout, y, back, share, dy, dshare)
+    if dy is None:
+        dy = torch.empty_like(y)
+    if dshare is None:
+        dshare = torch.empty((tokens, top), dtype=torch.float32, device=y.device)
+    _l.load().catcoc_gather_rows_backward(_stream(), dout.data_ptr(), y.data_ptr(), back.data_ptr(), share.data_ptr(), dy.data_ptr(), dshare.data_ptr(), tokens, top, cols, t)
+    _l.check()
+    return dy, dshare
+
+
 def verify(out, gold, dtype, compute_times):
     """The reference's accuracy gate on host data (float32 numpy arrays or CPU tensors).  -> (passed, n_bad, mean_rel_err)."""
     import numpy as np
