@@ -1,8 +1,11 @@
-"""A feed-forward layer of experts on the grouped and e4m3 operators: how they are called together.
+"""A feed-forward layer of experts on the grouped and e4m3 operators, and the block around it: how they are called together.
 
 `experts()` is the layer in 16 bits with its backward pass, `ServedExperts` the same layer on e4m3 weights, with an expert that every token
 takes (its down projection split over ranks: one rank's all-reduce share).  An expert is w_down (silu(w_gate x) * (w_up x)); gate and up are
 one matrix [2 inter, hidden], weights lie as [out, in].
+
+`block()` goes from the residual stream to what is added to it next: norm, router, experts; `ServedBlock` is the same on e4m3 weights, its rows
+quantized by the norm.  `rms_norm()` and `route()` are the operators of ops.py with their gradients.
 
     python -m mm_rs_with_catlass_amd.experts      # a few training steps, then the trained weights served in e4m3
 """
@@ -75,14 +78,154 @@ def gather(y, share, back):
     return (y[back].view(*share.shape, y.shape[1]).float() * share.float().unsqueeze(-1)).sum(1).to(y.dtype)
 
 
+class Spread(torch.autograd.Function):
+    """Every token's row at its choices' places (ops.spread_rows)."""
+
+    @staticmethod
+    def forward(ctx, x, back):
+        ctx.save_for_backward(back)
+        return ops.spread_rows(x.contiguous(), back)
+
+    @staticmethod
+    def backward(ctx, d):
+        back, = ctx.saved_tensors
+        return Gather.apply(d, back, None), None
+
+
+class Gather(torch.autograd.Function):
+    """The choices' rows summed at their tokens, by share where there is one (ops.gather_rows)."""
+
+    @staticmethod
+    def forward(ctx, y, back, share):
+        ctx.save_for_backward(y if share is not None else None, back, share)
+        return ops.gather_rows(y.contiguous(), back, share)
+
+    @staticmethod
+    def backward(ctx, dout):
+        y, back, share = ctx.saved_tensors
+        if share is None:
+            return Spread.apply(dout, back), None, None
+        if torch.is_grad_enabled():     # (gradients of gradients: from operators that have them)
+            d, at = Spread.apply(dout, back).float(), back.reshape(-1).long()
+            sorted_share = share.new_zeros(at.numel()).index_put((at,), share.reshape(-1))
+            return (d * sorted_share.unsqueeze(-1)).to(y.dtype), None, (d * y.float()).sum(1)[at].view(share.shape)
+        dy, dshare = ops.gather_rows_backward(dout.contiguous(), y.contiguous(), back, share)
+        return dy, None, dshare
+
+
+class _Plan:
+    """Where the rows of a call's choices lie.  Tensors on the GPU go through the operators, those on the host, and more experts or choices than the operators
+    take, through torch."""
+
+    def __init__(self, choice, experts):
+        self.top, self.kernels = choice.shape[1], choice.is_cuda and experts <= ops.MOST_EXPERTS and 1 <= choice.shape[1] <= ops.MOST_TOP
+        if self.kernels:
+            choice = choice if choice.dtype in (torch.int32, torch.int64) else choice.int()
+            self.order, self.back, self.ends = ops.sort_by_expert(choice.contiguous(), experts)
+        else:
+            self.order, self.back, self.ends = sort_by_expert(choice, experts)
+
+    def spread(self, x):
+        return Spread.apply(x, self.back) if self.kernels else spread(x, self.top, self.order)
+
+    def spread_fp8(self, x, scale):
+        """e4m3 rows and their scales."""
+        if self.kernels:
+            return ops.spread_rows(x, self.back, scale)
+        token = torch.div(self.order, self.top, rounding_mode="floor")
+        return x.view(torch.uint8)[token].view(x.dtype), scale[:, token]
+
+    def gather(self, y, share):
+        return Gather.apply(y, self.back, share.float().contiguous()) if self.kernels else gather(y, share, self.back)
+
+
 def experts(x, w_gate_up, w_down, choice, share):
     """x [tokens, hidden] fp16 or bf16, w_gate_up [experts, 2 inter, hidden], w_down [experts, hidden, inter], choice and share [tokens, top]:
     each token's experts (none: -1) and their weights.  Returns [tokens, hidden]; differentiable in x, both weights and share."""
-    order, back, ends = sort_by_expert(choice, w_gate_up.shape[0])
-    h = GroupedLinear.apply(spread(x, choice.shape[1], order), w_gate_up, ends)
+    plan = _Plan(choice, w_gate_up.shape[0])
+    h = GroupedLinear.apply(plan.spread(x), w_gate_up, plan.ends)
     gate, up = h.float().chunk(2, 1)
-    y = GroupedLinear.apply((torch.nn.functional.silu(gate) * up).to(x.dtype), w_down, ends)
-    return gather(y, share, back)
+    y = GroupedLinear.apply((torch.nn.functional.silu(gate) * up).to(x.dtype), w_down, plan.ends)
+    return plan.gather(y, share)
+
+
+class RmsNorm(torch.autograd.Function):
+    """ops.rms_norm with its gradients; without a residual the sum is None."""
+
+    @staticmethod
+    def forward(ctx, x, weight, residual, eps):
+        y, s = (ops.rms_norm(x, weight, eps=eps), None) if residual is None else ops.rms_norm(x, weight, residual, eps=eps)
+        ctx.save_for_backward(x if s is None else s, weight)
+        ctx.eps, ctx.types = eps, (x.dtype, None if residual is None else residual.dtype)
+        ctx.set_materialize_grads(False)
+        return y, s
+
+    @staticmethod
+    def backward(ctx, dy, dsum):
+        s, weight = ctx.saved_tensors
+        x_type, residual_type = ctx.types
+        if dy is None:
+            ds, dw = dsum, None
+        elif torch.is_grad_enabled():   # (gradients of gradients: the formula in torch)
+            v, w, d = s.float(), weight.float(), dy.float()
+            r = (v.square().mean(1, keepdim=True) + ctx.eps).rsqrt()
+            n, g = v * r, d * w
+            ds = r * (g - n * (g * n).mean(1, keepdim=True)) + (0 if dsum is None else dsum.float())
+            ds, dw = ds.to(s.dtype), (d * n).sum(0).to(weight.dtype)
+        else:
+            ds, dw = ops.rms_norm_backward(dy.contiguous(), s, weight, None if dsum is None else dsum.contiguous(), eps=ctx.eps)
+        return ds if ds is None else ds.to(x_type), dw, ds if residual_type is not None else None, None
+
+
+def rms_norm(x, weight, residual=None, eps=1e-6):
+    """ops.rms_norm(), differentiable in x, weight and residual: y, or (y, x + residual)."""
+    y, s = RmsNorm.apply(x, weight, residual, eps)
+    return y if residual is None else (y, s)
+
+
+class Route(torch.autograd.Function):
+    """ops.route with the shares' gradient; how: its arguments by name."""
+
+    @staticmethod
+    def forward(ctx, logits, top, bias, how):
+        choice, share = ops.route(logits, top, bias=bias, **how)
+        ctx.save_for_backward(logits, choice)
+        ctx.score, ctx.renormalize, ctx.scale = how.get("score", "softmax"), how.get("renormalize", True), how.get("scale", 1.0)
+        ctx.mark_non_differentiable(choice)
+        return choice, share
+
+    @staticmethod
+    def backward(ctx, _, dshare):
+        logits, choice = ctx.saved_tensors
+        if not torch.is_grad_enabled():
+            return ops.route_backward(dshare.contiguous(), logits, choice, score=ctx.score, renormalize=ctx.renormalize, scale=ctx.scale), None, None, None
+        # (gradients of gradients: the formula in torch)
+        on, at = choice >= 0, choice.long().clamp_min(0)
+        v = torch.where(logits > -torch.inf, logits.float(), torch.finfo(torch.float32).min)
+        p = torch.sigmoid(v) if ctx.score == "sigmoid" else torch.softmax(v, 1)
+        w, g = torch.where(on, p.gather(1, at), 0.0), torch.where(on, dshare * ctx.scale, 0.0)
+        if ctx.renormalize:
+            total = w.sum(1, keepdim=True)
+            w = w / torch.where(total > 0, total, 1.0)
+        d = w * (g - (w * g).sum(1, keepdim=True)) if ctx.renormalize else w * g
+        if ctx.score == "sigmoid":
+            d = d * (1 - p.gather(1, at))
+        out = torch.zeros_like(p) if ctx.renormalize or ctx.score == "sigmoid" else -p * (w * g).sum(1, keepdim=True)
+        return out.scatter_add(1, at, torch.where(on, d, 0.0)).to(logits.dtype), None, None, None
+
+
+def route(logits, top, bias=None, **how):
+    """ops.route(), its shares differentiable in logits: (choice, share)."""
+    return Route.apply(logits, top, bias, how)
+
+
+def block(x, residual, norm, router, w_gate_up, w_down, top, bias=None, eps=1e-6, **how):
+    """From the residual stream to what is added to it next: x [tokens, hidden] fp16 or bf16, the last layer's output; residual [tokens, hidden] of its type or fp32, what it is
+    added to; norm [hidden], router [experts, hidden]; top, bias and how: of route().  Returns the experts' output and the sum x + residual; differentiable in all
+    floating operands but bias."""
+    y, s = rms_norm(x, norm, residual, eps)
+    choice, share = route(y.float() @ router.float().t(), top, bias, **how)
+    return experts(y, w_gate_up, w_down, choice, share), s
 
 
 def _quantize_each(w):
@@ -104,34 +247,47 @@ class ServedExperts:
         self.gate_up, self.down = _quantize_each(w_gate_up), _quantize_each(w_down)
         self.shared = None if shared_gate_up is None else [ops.quantize_fp8(w, block_rows=128) for w in (shared_gate_up, shared_down)]
 
-    def __call__(self, x, choice, share, peers=(), rank=0):
-        """peers: the other ranks' fp32 partials [tokens, hidden] of the shared expert."""
-        order, back, ends = sort_by_expert(choice, self.experts)
-        rows, scale = ops.quantize_fp8(spread(x, choice.shape[1], order))
-        h = ops.grouped_fp8_matmul(rows, self.gate_up[0], scale, self.gate_up[1], ends, out_dtype=x.dtype)
+    def __call__(self, x, choice, share, peers=(), rank=0, codes=None):
+        """peers: the other ranks' fp32 partials [tokens, hidden] of the shared expert; codes: x in e4m3 with its scales, where it was quantized before."""
+        plan = _Plan(choice, self.experts)
+        codes = ops.quantize_fp8(x.contiguous()) if codes is None else codes
+        rows, scale = plan.spread_fp8(*codes)    # (a row's codes are the same before and after)
+        h = ops.grouped_fp8_matmul(rows, self.gate_up[0], scale, self.gate_up[1], plan.ends, out_dtype=x.dtype)
         rows, scale = ops.quantize_fp8(h, gated=True)
-        out = gather(ops.grouped_fp8_matmul(rows, self.down[0], scale, self.down[1], ends, out_dtype=x.dtype), share, back)
+        out = plan.gather(ops.grouped_fp8_matmul(rows, self.down[0], scale, self.down[1], plan.ends, out_dtype=x.dtype), share)
         if self.shared is None:
             return out
         (gate_up, gate_up_scale), (down, down_scale) = self.shared
-        rows, scale = ops.quantize_fp8(x)
+        rows, scale = codes
         h = ops.fp8_matmul_allreduce(rows, gate_up, scale, gate_up_scale, out_dtype=x.dtype)
         rows, scale = ops.quantize_fp8(h, gated=True)
         return out + ops.fp8_matmul_allreduce(rows, down, scale, down_scale, peers, rank, len(peers) + 1, out_dtype=x.dtype)
 
 
+class ServedBlock:
+    """block() on e4m3 weights: the norm's rows leave it in 16 bits for the router and in e4m3 for the experts, the shared one too."""
+
+    def __init__(self, norm, router, w_gate_up, w_down, top, shared_gate_up=None, shared_down=None, bias=None, eps=1e-6, **how):
+        self.norm, self.router, self.eps, self.top, self.bias, self.how = norm, router.float().t().contiguous(), eps, top, bias, how
+        self.experts = ServedExperts(w_gate_up, w_down, shared_gate_up, shared_down)
+
+    def __call__(self, x, residual, peers=(), rank=0):
+        q, scale, y, s = ops.rms_norm_fp8(x, self.norm, residual, eps=self.eps, keep=True)
+        choice, share = ops.route(y.float() @ self.router, self.top, bias=self.bias, **self.how)
+        return self.experts(y, choice, share, peers, rank, codes=(q, scale)), s
+
+
 def main():
     torch.manual_seed(0)
     tokens, hidden, inter, count, top, dev = 512, 1024, 512, 8, 2, "cuda"
-    x = torch.randn(tokens, hidden, device=dev, dtype=torch.bfloat16)
+    x, residual = torch.randn(tokens, hidden, device=dev, dtype=torch.bfloat16), torch.randn(tokens, hidden, device=dev)
     aim = torch.randn(tokens, hidden, device=dev)
-    router = torch.randn(hidden, count, device=dev) / hidden ** 0.5
-    masters = [torch.randn(count, 2 * inter, hidden, device=dev) / hidden ** 0.5, torch.randn(count, hidden, inter, device=dev) / inter ** 0.5]
-    share, choice = (x.float() @ router).softmax(1).topk(top)
+    masters = [torch.ones(hidden, device=dev), torch.randn(count, hidden, device=dev) / hidden ** 0.5, torch.randn(count, 2 * inter, hidden, device=dev) / hidden ** 0.5,
+               torch.randn(count, hidden, inter, device=dev) / inter ** 0.5]
     optimizer = torch.optim.Adam(masters, lr=3e-3)
     for step in range(20):
         weights = [m.to(torch.bfloat16).requires_grad_() for m in masters]
-        loss = (experts(x, *weights, choice, share).float() - aim).square().mean()
+        loss = (block(x, residual, *weights, top, renormalize=False)[0].float() - aim).square().mean()
         loss.backward()
         for m, w in zip(masters, weights):
             m.grad = w.grad.float()
@@ -139,7 +295,8 @@ def main():
         if step % 5 == 4:
             print("step %d  loss %.4f" % (step + 1, loss.item()), flush=True)
     weights = [m.to(torch.bfloat16) for m in masters]
-    trained, served = experts(x, *weights, choice, share).float(), ServedExperts(*weights)(x, choice, share).float()
+    trained = block(x, residual, *weights, top, renormalize=False)[0].float()
+    served = ServedBlock(*weights, top, renormalize=False)(x, residual)[0].float()
     print("served in e4m3: %.1f %% from the 16-bit layer" % (100 * ((served - trained).norm() / trained.norm()).item()))
 
 
