@@ -14,23 +14,23 @@ namespace catcoc {
 
 namespace {
 
-constexpr double kNone = -__builtin_huge_val();   // a key that is none: below all others
-constexpr double kMostKey = 0x1p1000;             // infinity and NaN count as this
-constexpr uint64_t kIndexBits = 1023;
+constexpr double kMostKey = 0x1p1000;     // infinity and NaN count as this,
+constexpr double kNone = -0x1p1000;       // and what is not to be had as this, or less by its index
+constexpr uint32_t kIndexBits = 1023;
 
 // An exchange between lanes of a row of 16.
 template <int CTRL>
 __device__ __forceinline__ float lane_turn(float v)
 {
-    return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTRL, 0xf, 0xf, false));
+    return __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, v), CTRL, 0xf, 0xf, false));
 }
 
 template <int CTRL>
 __device__ __forceinline__ double lane_turn(double v)
 {
     const uint64_t b = __builtin_bit_cast(uint64_t, v);
-    const uint32_t lo = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)b, CTRL, 0xf, 0xf, false);
-    const uint32_t hi = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)(b >> 32), CTRL, 0xf, 0xf, false);
+    const uint32_t lo = (uint32_t)__builtin_amdgcn_mov_dpp((int)(uint32_t)b, CTRL, 0xf, 0xf, false);
+    const uint32_t hi = (uint32_t)__builtin_amdgcn_mov_dpp((int)(uint32_t)(b >> 32), CTRL, 0xf, 0xf, false);
     return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
 }
 
@@ -61,20 +61,20 @@ __device__ __forceinline__ T lanes_sum(T v)
     return over_lanes<LANES>(v, [](T a, T b) { return a + b; });
 }
 
+// (A NaN is no operand of a minimum: what is left is the other one.  + 0.0: -0 is 0.)
 __device__ __forceinline__ double with_index(double k, uint32_t index)
 {
-    if (k == kNone) return k;
-    k = k <= kMostKey ? k + 0.0 : kMostKey;   // (+ 0.0: -0 is 0)
-    const uint64_t b = __builtin_bit_cast(uint64_t, k);
-    return __builtin_bit_cast(double, (b & ~kIndexBits) | (b >> 63 ? index : kIndexBits - index));
+    const uint64_t b = __builtin_bit_cast(uint64_t, __builtin_elementwise_max(__builtin_elementwise_min(k, kMostKey), kNone) + 0.0);
+    const uint32_t hi = (uint32_t)(b >> 32), counted = index ^ (~(uint32_t)((int32_t)hi >> 31) & kIndexBits);   // down from 1023, below zero up from 0
+    return __builtin_bit_cast(double, (uint64_t)hi << 32 | ((uint32_t)b & ~kIndexBits) | (counted & kIndexBits));
 }
 
-__device__ __forceinline__ double without_index(double k) { return __builtin_bit_cast(double, __builtin_bit_cast(uint64_t, k) & ~kIndexBits); }
+__device__ __forceinline__ double without_index(double k) { return __builtin_bit_cast(double, __builtin_bit_cast(uint64_t, k) & ~(uint64_t)kIndexBits); }
 
 __device__ __forceinline__ uint32_t index_of(double k)
 {
     const uint64_t b = __builtin_bit_cast(uint64_t, k);
-    return (uint32_t)(b >> 63 ? b & kIndexBits : kIndexBits - (b & kIndexBits));
+    return ((uint32_t)b ^ ~(uint32_t)((int32_t)(b >> 32) >> 31)) & kIndexBits;
 }
 
 __device__ __forceinline__ void in_order(double &a, double &b)
@@ -133,6 +133,30 @@ __device__ __forceinline__ void load_logits(const void *x, size_t at, uint32_t c
     }
 }
 
+// e^x to 2^-45 of it: 2^n e^r with |r| <= ln 2 / 2 and e^r as the polynomial that meets it at ten Chebyshev nodes (2^-45.6); 0 from -800 down, infinity from 800 up.
+__device__ __forceinline__ double exp64(double x)
+{
+    const double t = __builtin_elementwise_min(__builtin_elementwise_max(x, -800.0), 800.0), n = __builtin_rint(t * 0x1.71547652b82fep+0), r = __builtin_fma(n, -0x1.62e42fefa39efp-1, t);
+    double p = 0x1.72e107c874de9p-19;
+    p = __builtin_fma(p, r, 0x1.a17df0d914d6cp-16);
+    p = __builtin_fma(p, r, 0x1.a01994c849582p-13);
+    p = __builtin_fma(p, r, 0x1.6c162bb7d965cp-10);
+    p = __builtin_fma(p, r, 0x1.11111123bf154p-7);
+    p = __builtin_fma(p, r, 0x1.55555588b8403p-5);
+    p = __builtin_fma(p, r, 0x1.5555555550d88p-3);
+    p = __builtin_fma(p, r, 0x1.ffffffffe74f1p-2);
+    p = __builtin_fma(p, r, 0x1.0000000000006p+0);
+    p = __builtin_fma(p, r, 0x1.000000000003dp+0);
+    return __builtin_amdgcn_ldexp(p, (int)n);
+}
+
+// 1 / d to 2^-47 of it, for 1 <= d below 2^1000: the instruction's 2^-24 and a step of Newton's; 0 above.
+__device__ __forceinline__ double reciprocal(double d)
+{
+    const double c = __builtin_elementwise_min(d, 0x1p1000), r = __builtin_amdgcn_rcp(c);
+    return __builtin_fma(__builtin_fma(-c, r, 1.0), r, r);
+}
+
 // What an expert's share is made of, from its logit: of the softmax e^(l - most), of the sigmoid s(l), where it is only to be compared with that of the largest logit,
 // `most`, and that is not positive, e^(l - most) / (1 + e^l) in its place: s(l) itself could be 0 for all of them.
 __device__ __forceinline__ float weight_of(float l, float most, bool sigmoid, bool compared)
@@ -154,6 +178,10 @@ __global__ void __launch_bounds__(256) route_kernel(const RouteArgs args)
     const uint32_t first = slot * size + in, count = slot < args.groups && in < size ? umin(args.perLane, size - in) : 0u;
     float v[V];
     load_logits<V>(args.logits, token * args.experts + (count ? first : 0u), count, args.type, v);
+    float b[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) b[i] = 0.f;
+    if (args.bias != nullptr) load_logits<V>(args.bias, count ? first : 0u, count, 0, b);
 
     float most = 0.f;
     if (!args.sigmoid) {
@@ -163,36 +191,35 @@ __global__ void __launch_bounds__(256) route_kernel(const RouteArgs args)
         most = lanes_max<LANES>(most);
     }
     double k[V];
-#pragma unroll
-    for (int i = 0; i < V; ++i) k[i] = v[i];
     float total = 0.f;   // of the softmax
     if (args.bias != nullptr || args.groupTop == 2) {
-        double p[V], sum = 0.0;
+        double r = 1.0;
         if (args.sigmoid) {
 #pragma unroll
-            for (int i = 0; i < V; ++i) p[i] = 1.0 / (1.0 + exp(-(double)v[i]));
+            for (int i = 0; i < V; ++i) k[i] = reciprocal(1.0 + exp64(-(double)v[i]));
         } else {
+            double sum = 0.0;
+            bool odd = !(most < __builtin_huge_valf());
 #pragma unroll
             for (int i = 0; i < V; ++i) {
-                p[i] = exp((double)v[i] - (double)most);
-                sum += p[i];
+                k[i] = exp64((double)v[i] - (double)most);
+                sum += k[i];
+                odd |= v[i] != v[i];
             }
-            sum = lanes_sum<LANES>(sum);
+            sum = lanes_sum<LANES>(odd ? (double)__builtin_nanf("") : sum);   // (of values none of which is finite: no score)
             total = (float)sum;
-            const double r = 1.0 / sum;
-#pragma unroll
-            for (int i = 0; i < V; ++i) p[i] *= r;
+            r = 1.0 / sum;
         }
 #pragma unroll
-        for (int i = 0; i < V; ++i) {
-            if (k[i] == kNone) continue;
-            k[i] = p[i];
-            if (args.bias != nullptr) k[i] += args.bias[first + i];   // (an expert that there is: its logit is more than -inf)
-        }
+        for (int i = 0; i < V; ++i) k[i] = v[i] > -__builtin_huge_valf() ? __builtin_fma(k[i], r, (double)b[i]) : (double)v[i];   // (as it is: a NaN, or not to be had)
     } else if (!args.sigmoid && !args.renormalize) {
 #pragma unroll
         for (int i = 0; i < V; ++i) total += v[i] == -__builtin_huge_valf() ? 0.f : expf(v[i] - most);
         total = lanes_sum<LANES>(total);
+    }
+    if (args.bias == nullptr && args.groupTop == 1) {
+#pragma unroll
+        for (int i = 0; i < V; ++i) k[i] = v[i];
     }
 #pragma unroll
     for (int i = 0; i < V; ++i) k[i] = with_index(k[i], first + i);
@@ -206,7 +233,7 @@ __global__ void __launch_bounds__(256) route_kernel(const RouteArgs args)
             a = __builtin_elementwise_max(a, c);
         }
         double best = without_index(a);
-        if (args.groupTop == 2 && b != kNone) best += without_index(b);
+        if (args.groupTop == 2 && b > kNone) best += without_index(b);
         best = with_index(best, slot);
         uint32_t ahead = 0;
         for (uint32_t g = 0; g < args.groups; ++g) ahead += __shfl(best, (int)(g * args.groupLanes), LANES) > best ? 1u : 0u;
@@ -221,11 +248,13 @@ __global__ void __launch_bounds__(256) route_kernel(const RouteArgs args)
         const double next = lanes_max<LANES>(k[0]);
         if (l == j) mine = next;
         const bool taken = k[0] == next;
+        if (taken) {   // (a branch: as selects, the compiler makes an index of them and looks for it among all keys)
 #pragma unroll
-        for (int i = 0; i + 1 < V; ++i) k[i] = taken ? k[i + 1] : k[i];
-        k[V - 1] = taken ? kNone : k[V - 1];
+            for (int i = 0; i + 1 < V; ++i) k[i] = k[i + 1];
+            k[V - 1] = kNone;
+        }
     }
-    const bool on = mine != kNone;
+    const bool on = mine > kNone;
     const uint32_t expert = on ? index_of(mine) : 0u;
     const float logit = on ? logit_at(args.logits, token * args.experts + expert, args.type) : -__builtin_huge_valf();
     if (args.renormalize) most = lanes_max<LANES>(logit);
