@@ -7,6 +7,8 @@
 // Every lane sorts its keys once (odd-even merge sort: Batcher, AFIPS 1968); then the largest of the lanes' first keys is taken `top` times.
 #include <hip/hip_runtime.h>
 
+#include <utility>
+
 #include "layer_args.h"
 #include "rows_device.h"
 
@@ -32,6 +34,19 @@ __device__ __forceinline__ double lane_turn(double v)
     const uint32_t lo = (uint32_t)__builtin_amdgcn_mov_dpp((int)(uint32_t)b, CTRL, 0xf, 0xf, false);
     const uint32_t hi = (uint32_t)__builtin_amdgcn_mov_dpp((int)(uint32_t)(b >> 32), CTRL, 0xf, 0xf, false);
     return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+}
+
+template <typename F, int... I>
+__device__ __forceinline__ void turns(F f, std::integer_sequence<int, I...>)
+{
+    (f(std::integral_constant<int, 0x121 + I>{}), ...);   // row_ror:1 to 15
+}
+
+// f with each of the 15 turns of a row of 16 lanes.
+template <typename F>
+__device__ __forceinline__ void each_other_lane(F f)
+{
+    turns(f, std::make_integer_sequence<int, 15>{});
 }
 
 // f over the values of LANES lanes, in all of them, in an order that is always the same.
@@ -61,12 +76,12 @@ __device__ __forceinline__ T lanes_sum(T v)
     return over_lanes<LANES>(v, [](T a, T b) { return a + b; });
 }
 
-// (A NaN is no operand of a minimum: what is left is the other one.  + 0.0: -0 is 0.)
+// (A NaN is no operand of a minimum: what is left is the other one.)
 __device__ __forceinline__ double with_index(double k, uint32_t index)
 {
-    const uint64_t b = __builtin_bit_cast(uint64_t, __builtin_elementwise_max(__builtin_elementwise_min(k, kMostKey), kNone) + 0.0);
-    const uint32_t hi = (uint32_t)(b >> 32), counted = index ^ (~(uint32_t)((int32_t)hi >> 31) & kIndexBits);   // down from 1023, below zero up from 0
-    return __builtin_bit_cast(double, (uint64_t)hi << 32 | ((uint32_t)b & ~kIndexBits) | (counted & kIndexBits));
+    const uint64_t b = __builtin_bit_cast(uint64_t, __builtin_elementwise_max(__builtin_elementwise_min(k, kMostKey), kNone));
+    const uint32_t hi = (uint32_t)(b >> 32), counted = ~(index ^ (uint32_t)((int32_t)hi >> 31));   // down from 1023, below zero up from 0
+    return __builtin_bit_cast(double, (uint64_t)hi << 32 | (((uint32_t)b & ~kIndexBits) | (counted & kIndexBits)));
 }
 
 __device__ __forceinline__ double without_index(double k) { return __builtin_bit_cast(double, __builtin_bit_cast(uint64_t, k) & ~(uint64_t)kIndexBits); }
@@ -133,10 +148,11 @@ __device__ __forceinline__ void load_logits(const void *x, size_t at, uint32_t c
     }
 }
 
-// e^x to 2^-45 of it: 2^n e^r with |r| <= ln 2 / 2 and e^r as the polynomial that meets it at ten Chebyshev nodes (2^-45.6); 0 from -800 down, infinity from 800 up.
+// e^x to 2^-45 of it, |x| <= 700: 2^n e^r with |r| <= ln 2 / 2 and e^r as the polynomial that meets it at ten Chebyshev nodes (2^-45.6).  Beside 1.5 2^52 a number is
+// a whole one, n the last bits of the sum.
 __device__ __forceinline__ double exp64(double x)
 {
-    const double t = __builtin_elementwise_min(__builtin_elementwise_max(x, -800.0), 800.0), n = __builtin_rint(t * 0x1.71547652b82fep+0), r = __builtin_fma(n, -0x1.62e42fefa39efp-1, t);
+    const double t = __builtin_fma(x, 0x1.71547652b82fep+0, 0x1.8p52), n = t - 0x1.8p52, r = __builtin_fma(n, -0x1.62e42fefa39efp-1, x);
     double p = 0x1.72e107c874de9p-19;
     p = __builtin_fma(p, r, 0x1.a17df0d914d6cp-16);
     p = __builtin_fma(p, r, 0x1.a01994c849582p-13);
@@ -147,14 +163,14 @@ __device__ __forceinline__ double exp64(double x)
     p = __builtin_fma(p, r, 0x1.ffffffffe74f1p-2);
     p = __builtin_fma(p, r, 0x1.0000000000006p+0);
     p = __builtin_fma(p, r, 0x1.000000000003dp+0);
-    return __builtin_amdgcn_ldexp(p, (int)n);
+    return __builtin_bit_cast(double, __builtin_bit_cast(uint64_t, p) + (__builtin_bit_cast(uint64_t, t) << 52));
 }
 
-// 1 / d to 2^-47 of it, for 1 <= d below 2^1000: the instruction's 2^-24 and a step of Newton's; 0 above.
-__device__ __forceinline__ double reciprocal(double d)
+// The sigmoid to 2^-44 of it; logits further than 700 from zero count as that.  A reciprocal is the instruction's, 2^-24 off, and a step of Newton's.
+__device__ __forceinline__ double sigmoid64(float x)
 {
-    const double c = __builtin_elementwise_min(d, 0x1p1000), r = __builtin_amdgcn_rcp(c);
-    return __builtin_fma(__builtin_fma(-c, r, 1.0), r, r);
+    const double d = 1.0 + exp64(-(double)__builtin_amdgcn_fmed3f(x, -700.f, 700.f)), r = __builtin_amdgcn_rcp(d);
+    return __builtin_fma(__builtin_fma(-d, r, 1.0), r, r);
 }
 
 // What an expert's share is made of, from its logit: of the softmax e^(l - most), of the sigmoid s(l), where it is only to be compared with that of the largest logit,
@@ -168,7 +184,7 @@ __device__ __forceinline__ float weight_of(float l, float most, bool sigmoid, bo
 }  // namespace
 
 template <int LANES, int V>
-__global__ void __launch_bounds__(256) route_kernel(const RouteArgs args)
+__global__ void __launch_bounds__(256, LANES == 16 ? 4 : V <= 16 ? 3 : 2) route_kernel(const RouteArgs args)
 {
     const uint32_t lane = threadIdx.x & 63u, l = lane % LANES;
     const uint64_t at = ((uint64_t)workgroup() * 4u + (threadIdx.x >> 6)) * (64 / LANES) + lane / LANES;
@@ -193,38 +209,49 @@ __global__ void __launch_bounds__(256) route_kernel(const RouteArgs args)
     double k[V];
     float total = 0.f;   // of the softmax
     if (args.bias != nullptr || args.groupTop == 2) {
+        bool odd = false;   // NaN, or not to be had
+#pragma unroll
+        for (int i = 0; i < V; ++i) odd |= !(v[i] > -__builtin_huge_valf());
         double r = 1.0;
         if (args.sigmoid) {
 #pragma unroll
-            for (int i = 0; i < V; ++i) k[i] = reciprocal(1.0 + exp64(-(double)v[i]));
+            for (int i = 0; i < V; ++i) k[i] = sigmoid64(v[i]);
         } else {
             double sum = 0.0;
-            bool odd = !(most < __builtin_huge_valf());
 #pragma unroll
             for (int i = 0; i < V; ++i) {
-                k[i] = exp64((double)v[i] - (double)most);
+                k[i] = exp64(__builtin_elementwise_max((double)v[i] - (double)most, -700.0));
                 sum += k[i];
-                odd |= v[i] != v[i];
             }
-            sum = lanes_sum<LANES>(odd ? (double)__builtin_nanf("") : sum);   // (of values none of which is finite: no score)
+            bool spoilt = !(most < __builtin_huge_valf());
+            if (__any(odd)) {
+#pragma unroll
+                for (int i = 0; i < V; ++i) spoilt |= v[i] != v[i];
+            }
+            sum = lanes_sum<LANES>(spoilt ? (double)__builtin_nanf("") : sum);   // (of values not all of which are numbers: no score)
             total = (float)sum;
             r = 1.0 / sum;
         }
 #pragma unroll
-        for (int i = 0; i < V; ++i) k[i] = v[i] > -__builtin_huge_valf() ? __builtin_fma(k[i], r, (double)b[i]) : (double)v[i];   // (as it is: a NaN, or not to be had)
-    } else if (!args.sigmoid && !args.renormalize) {
+        for (int i = 0; i < V; ++i) k[i] = __builtin_fma(k[i], r, (double)b[i]);
+        if (__any(odd)) {
 #pragma unroll
-        for (int i = 0; i < V; ++i) total += v[i] == -__builtin_huge_valf() ? 0.f : expf(v[i] - most);
-        total = lanes_sum<LANES>(total);
-    }
-    if (args.bias == nullptr && args.groupTop == 1) {
+            for (int i = 0; i < V; ++i) k[i] = v[i] > -__builtin_huge_valf() ? k[i] : (double)v[i];
+        }
+    } else {
+        if (!args.sigmoid && !args.renormalize) {
 #pragma unroll
-        for (int i = 0; i < V; ++i) k[i] = v[i];
+            for (int i = 0; i < V; ++i) total += v[i] == -__builtin_huge_valf() ? 0.f : expf(v[i] - most);
+            total = lanes_sum<LANES>(total);
+        }
+#pragma unroll
+        for (int i = 0; i < V; ++i) k[i] = v[i] + 0.f;   // (-0 is 0)
     }
 #pragma unroll
     for (int i = 0; i < V; ++i) k[i] = with_index(k[i], first + i);
     sort_keys<V>(k);
 
+    bool out = false;   // of the groups that are chosen from
     if (args.topGroups < args.groups) {
         double a = k[0], b = V > 1 ? k[V > 1 ? 1 : 0] : kNone;   // the group's best two
         for (uint32_t by = 1; by < args.groupLanes; by <<= 1) {
@@ -235,23 +262,48 @@ __global__ void __launch_bounds__(256) route_kernel(const RouteArgs args)
         double best = without_index(a);
         if (args.groupTop == 2 && b > kNone) best += without_index(b);
         best = with_index(best, slot);
-        uint32_t ahead = 0;
-        for (uint32_t g = 0; g < args.groups; ++g) ahead += __shfl(best, (int)(g * args.groupLanes), LANES) > best ? 1u : 0u;
-        if (ahead >= args.topGroups) {
-#pragma unroll
-            for (int i = 0; i < V; ++i) k[i] = kNone;
+        uint32_t ahead = 0;   // how many groups are
+        if constexpr (LANES == 16) {
+            each_other_lane([&](auto turn) { ahead += lane_turn<decltype(turn)::value>(best) > best ? 1u : 0u; });   // (a group counts once for each of its lanes)
+            out = ahead >= args.topGroups * args.groupLanes;
+        } else {
+            for (uint32_t g = 0; g < args.groups; ++g) ahead += __shfl(best, (int)(g * args.groupLanes), LANES) > best ? 1u : 0u;
+            out = ahead >= args.topGroups;
         }
     }
 
     double mine = kNone;   // lane j: the j-th choice
-    for (uint32_t j = 0; j < args.top; ++j) {
-        const double next = lanes_max<LANES>(k[0]);
-        if (l == j) mine = next;
-        const bool taken = k[0] == next;
-        if (taken) {   // (a branch: as selects, the compiler makes an index of them and looks for it among all keys)
+    if constexpr (V <= 4) {
+        if (out) {
 #pragma unroll
-            for (int i = 0; i + 1 < V; ++i) k[i] = k[i + 1];
-            k[V - 1] = kNone;
+            for (int i = 0; i < V; ++i) k[i] = kNone;
+        }
+        for (uint32_t j = 0; j < args.top; ++j) {
+            const double next = lanes_max<LANES>(k[0]);
+            if (l == j) mine = next;
+            if (k[0] == next) {   // (a branch: as selects, the compiler makes an index of them and looks for it among all keys)
+#pragma unroll
+                for (int i = 0; i + 1 < V; ++i) k[i] = k[i + 1];
+                k[V - 1] = kNone;
+            }
+        }
+    } else {
+        // A lane's first two keys are in registers, the others wait in LDS: moving 15 of them up in registers at each turn took a third of the kernel's instructions.
+        __shared__ double keys[V + 1][256];
+#pragma unroll
+        for (int i = 2; i < V; ++i)
+            if ((uint32_t)i <= args.top) keys[i][threadIdx.x] = k[i];
+        keys[V][threadIdx.x] = kNone;
+        double first_key = out ? kNone : k[0], second = out ? kNone : k[1];
+        uint32_t at_key = out ? (uint32_t)V : 2u;   // the one behind the second
+        for (uint32_t j = 0; j < args.top; ++j) {
+            const double next = lanes_max<LANES>(first_key);
+            if (l == j) mine = next;
+            const bool taken = first_key == next;
+            const double third = keys[at_key][threadIdx.x];
+            first_key = taken ? second : first_key;
+            second = taken ? third : second;
+            at_key = umin(at_key + (taken ? 1u : 0u), (uint32_t)V);
         }
     }
     const bool on = mine > kNone;
@@ -259,8 +311,7 @@ __global__ void __launch_bounds__(256) route_kernel(const RouteArgs args)
     const float logit = on ? logit_at(args.logits, token * args.experts + expert, args.type) : -__builtin_huge_valf();
     if (args.renormalize) most = lanes_max<LANES>(logit);
     float share = on ? weight_of(logit, most, args.sigmoid, args.renormalize) : 0.f;
-    const bool spoilt = total != total;   // a softmax with a NaN or an infinity in it has no other scores either
-    if (args.renormalize) total = spoilt ? total : lanes_sum<LANES>(share);
+    if (args.renormalize) total = total == total ? lanes_sum<LANES>(share) : total;   // (a softmax with a NaN or an infinity in it has no other scores either)
     if (args.renormalize || !args.sigmoid) share /= total;
     if (l >= args.top || at >= args.tokens) return;
     args.choice[token * args.top + l] = on ? (int32_t)expert : -1;
@@ -402,23 +453,36 @@ int launch_route_backward(const RouteArgs &a, void *stream) { return launch_rout
 
 namespace {
 
-constexpr uint32_t kSortWaves = 16;
+constexpr uint32_t kSortWaves = 16, kSortThreads = 64 * kSortWaves;
 
-// The expert of a row; `experts` for one that is none's.
+constexpr uint32_t kSortTurns = 4;   // times 64 rows that a wave asks for together
+constexpr uint32_t kNoRow = 0xffffffffu;
+
+// The experts of a wave's rows [first, first + 256) that are before `end`.
 template <typename I>
-__device__ __forceinline__ uint32_t expert_of(const SortArgs &args, uint32_t row)
+__device__ __forceinline__ void load_experts(const SortArgs &args, uint32_t first, uint32_t end, uint32_t (&expert)[kSortTurns])
 {
-    const I c = ((const I *)args.choice)[row];
-    return c >= 0 && c < (I)args.experts ? (uint32_t)c : args.experts;
+    I c[kSortTurns];
+    const uint32_t at = first + (threadIdx.x & 63u);   // (below 2^31 + 2^8)
+#pragma unroll
+    for (uint32_t i = 0; i < kSortTurns; ++i) c[i] = ((const I *)args.choice)[umin(at + 64u * i, end - 1u)];
+#pragma unroll
+    for (uint32_t i = 0; i < kSortTurns; ++i) expert[i] = at + 64u * i >= end ? kNoRow : c[i] >= 0 && c[i] < (I)args.experts ? (uint32_t)c[i] : args.experts;
 }
 
+// How many of each wave's rows go to each expert.  `expert`: of its first 256 rows on the way in, of its last ones on the way out.
 template <typename I, uint32_t MOST>
-__device__ __forceinline__ void count_rows(const SortArgs &args, uint32_t (&count)[kSortWaves][MOST + 1], uint32_t begin, uint32_t end)
+__device__ __forceinline__ void count_rows(const SortArgs &args, uint32_t (&count)[kSortWaves][MOST + 1], uint32_t begin, uint32_t end, uint32_t (&expert)[kSortTurns])
 {
-    for (uint32_t i = threadIdx.x; i < kSortWaves * (MOST + 1u); i += 64u * kSortWaves) (&count[0][0])[i] = 0;
+    for (uint32_t i = threadIdx.x; i < kSortWaves * (MOST + 1u); i += kSortThreads) (&count[0][0])[i] = 0;
     __syncthreads();
-    const uint32_t wave = threadIdx.x >> 6;
-    for (uint32_t row = begin + (threadIdx.x & 63u); row < end; row += 64u) atomicAdd(&count[wave][expert_of<I>(args, row)], 1u);
+    uint32_t *const mine = count[threadIdx.x >> 6];
+    for (uint32_t first = begin; first < end; first += 64u * kSortTurns) {
+        if (first != begin) load_experts<I>(args, first, end, expert);
+#pragma unroll
+        for (uint32_t i = 0; i < kSortTurns; ++i)
+            if (expert[i] != kNoRow) atomicAdd(&mine[expert[i]], 1u);
+    }
     __syncthreads();
 }
 
@@ -433,112 +497,129 @@ __device__ __forceinline__ void wave_rows(const SortArgs &args, uint32_t &begin,
 }  // namespace
 
 template <typename I, uint32_t MOST>
-__global__ void __launch_bounds__(64 * kSortWaves) count_by_expert_kernel(const SortArgs args)
+__global__ void __launch_bounds__(kSortThreads) count_by_expert_kernel(const SortArgs args)
 {
     __shared__ uint32_t count[kSortWaves][MOST + 1];
-    uint32_t begin, end;
+    uint32_t begin, end, expert[kSortTurns];
     wave_rows(args, begin, end);
-    count_rows<I, MOST>(args, count, begin, end);
-    for (uint32_t e = threadIdx.x; e <= args.experts; e += 64u * kSortWaves) {
+    if (begin < end) load_experts<I>(args, begin, end, expert);
+    count_rows<I, MOST>(args, count, begin, end, expert);
+    if (threadIdx.x < args.experts) {
         uint32_t n = 0;
-        for (uint32_t w = 0; w < kSortWaves; ++w) n += count[w][e];
-        args.part[(size_t)blockIdx.x * (args.experts + 1u) + e] = n;
+#pragma unroll
+        for (uint32_t w = 0; w < kSortWaves; ++w) n += count[w][threadIdx.x];
+        args.part[(size_t)blockIdx.x * args.experts + threadIdx.x] = n;
     }
 }
 
 template <typename I, uint32_t MOST>
-__global__ void __launch_bounds__(64 * kSortWaves) sort_by_expert_kernel(const SortArgs args)
+__global__ void __launch_bounds__(kSortThreads) sort_by_expert_kernel(const SortArgs args)
 {
-    constexpr uint32_t THREADS = 64 * kSortWaves, SLICES = MOST < 512 ? 4 : 1, WIDE = THREADS / SLICES;
     __shared__ uint32_t count[kSortWaves][MOST + 1];
-    __shared__ uint32_t totals[SLICES][MOST + 1], before[SLICES][MOST + 1], sums[kSortWaves];
-    uint32_t begin, end;
+    __shared__ uint32_t totals[kSortThreads], before[kSortThreads], sums[2][kSortWaves];
+    const uint32_t wave = threadIdx.x >> 6, lane = threadIdx.x & 63u;
+    uint32_t begin, end, n = 0, those = 0, expert[kSortTurns];
     wave_rows(args, begin, end);
-    count_rows<I, MOST>(args, count, begin, end);
-    // ---- each expert's rows: of all blocks, and of those before this one
-    const uint32_t slice = threadIdx.x / WIDE;
-    for (uint32_t e = threadIdx.x % WIDE; e <= args.experts; e += WIDE) {
-        uint32_t all = 0, those = 0;
-        if (args.part == nullptr) {
-            if (slice == 0) {
-#pragma unroll
-                for (uint32_t w = 0; w < kSortWaves; ++w) all += count[w][e];
-            }
-        } else {
-#pragma unroll 8
-            for (uint32_t b = slice; b < args.blocks; b += SLICES) {
-                const uint32_t n = args.part[(size_t)b * (args.experts + 1u) + e];
-                all += n;
-                those += b < blockIdx.x ? n : 0u;
+    if (begin < end) load_experts<I>(args, begin, end, expert);
+    // ---- thread e: rows of expert e, of all blocks (n) and of those before this one; the blocks' counts are read by as many threads an expert as there are
+    const uint32_t wide = args.experts <= 64u ? 6u : 32u - (uint32_t)__builtin_clz(args.experts - 1u);
+    if (args.part != nullptr) {
+        const uint32_t e = threadIdx.x & ((1u << wide) - 1u);
+        uint32_t all = 0, some = 0;
+        if (e < args.experts) {
+#pragma unroll 16
+            for (uint32_t i = threadIdx.x >> wide; i < args.blocks; i += kSortThreads >> wide) {
+                const uint32_t b = i + blockIdx.x < args.blocks ? i + blockIdx.x : i + blockIdx.x - args.blocks;   // (each block from another one on: an L2's channels share the work)
+                const uint32_t c = args.part[(size_t)b * args.experts + e];
+                all += c;
+                some += b < blockIdx.x ? c : 0u;
             }
         }
-        totals[slice][e] = all;
-        before[slice][e] = those;
+        totals[threadIdx.x] = all;
+        before[threadIdx.x] = some;
     }
-    __syncthreads();
-    // ---- where an expert's rows begin
-    uint32_t n = 0, upTo;
+    count_rows<I, MOST>(args, count, begin, end, expert);
     if (threadIdx.x < args.experts) {
+        if (args.part != nullptr) {
+            for (uint32_t i = threadIdx.x; i < kSortThreads; i += 1u << wide) {
+                n += totals[i];
+                those += before[i];
+            }
+        } else {
 #pragma unroll
-        for (uint32_t s = 0; s < SLICES; ++s) n += totals[s][threadIdx.x];
+            for (uint32_t w = 0; w < kSortWaves; ++w) n += count[w][threadIdx.x];
+        }
     }
-    upTo = n;
+    // ---- where an expert's rows begin
+    uint32_t upTo = n, past = those;
 #pragma unroll
     for (uint32_t by = 1; by < 64; by <<= 1) {
-        const uint32_t less = __shfl_up(upTo, by);
-        if ((threadIdx.x & 63u) >= by) upTo += less;
+        const uint32_t less = __shfl_up(upTo, by), more = __shfl_xor(past, by);
+        if (lane >= by) upTo += less;
+        past += more;
     }
-    if ((threadIdx.x & 63u) == 63u) sums[threadIdx.x >> 6] = upTo;
+    if (lane == 63u) sums[0][wave] = upTo, sums[1][wave] = past;
     __syncthreads();
     uint32_t every = 0;
+    past = 0;
 #pragma unroll
     for (uint32_t w = 0; w < kSortWaves; ++w) {
-        upTo += w < threadIdx.x >> 6 ? sums[w] : 0u;
-        every += sums[w];
+        upTo += w < wave ? sums[0][w] : 0u;
+        every += sums[0][w];
+        past += sums[1][w];
     }
     if (blockIdx.x == 0 && threadIdx.x < args.experts) args.ends[threadIdx.x] = (int32_t)upTo;
-    // ---- where a wave's first row of each expert goes (behind the last expert's: the rows of none)
+    // ---- where a wave's first row of each expert goes (behind the last expert's: the rows of none, of which as many are before this block as its other rows leave)
     auto spread = [&](uint32_t e, uint32_t at) {
 #pragma unroll
-        for (uint32_t s = 0; s < SLICES; ++s) at += before[s][e];
         for (uint32_t w = 0; w < kSortWaves; ++w) {
             const uint32_t c = count[w][e];
             count[w][e] = at;
             at += c;
         }
     };
-    if (threadIdx.x < args.experts) spread(threadIdx.x, upTo - n);
-    if (threadIdx.x == THREADS - 1u) spread(args.experts, every);
+    if (threadIdx.x < args.experts) spread(threadIdx.x, upTo - n + those);
+    if (threadIdx.x == kSortThreads - 1u) {
+        const uint64_t from = (uint64_t)blockIdx.x * args.perBlock;
+        spread(args.experts, every + (uint32_t)(from < args.rows ? from : args.rows) - past);
+    }
     __syncthreads();
-    const uint32_t wave = threadIdx.x >> 6, lane = threadIdx.x & 63u, bits = 32u - (uint32_t)__builtin_clz(args.experts);
-    for (uint32_t first = begin; first < end; first += 64u) {
-        const uint32_t row = first + lane;
-        const bool on = row < end;
-        const uint32_t e = on ? expert_of<I>(args, row) : 0u;
-        uint64_t same = __ballot(on);
-        for (uint32_t b = 0; b < bits; ++b) {
-            const bool set = (e >> b) & 1u;
-            const uint64_t those = __ballot(set);
-            same &= set ? those : ~those;
-        }
-        const uint32_t rank = (uint32_t)__builtin_popcountll(same & ((1ull << lane) - 1ull));
-        if (on) {
-            volatile uint32_t *const next = &count[wave][e];   // (a wave's own: its accesses stay in order)
-            const uint32_t at = *next + rank;
-            if (rank == 0) *next = at + (uint32_t)__builtin_popcountll(same);
-            args.back[row] = (int32_t)at;
-            if (at < args.rows) args.order[at] = (int32_t)row;   // (it is, unless the choices change meanwhile)
+    const uint32_t bits = 32u - (uint32_t)__builtin_clz(args.experts);
+    for (uint32_t first = begin; first < end; first += 64u * kSortTurns) {
+        if (end - begin > 64u * kSortTurns) load_experts<I>(args, first, end, expert);
+#pragma unroll
+        for (uint32_t i = 0; i < kSortTurns; ++i) {
+            const uint32_t row = first + 64u * i + lane, e = expert[i];
+            const bool on = e != kNoRow;
+            uint64_t same = __ballot(on);
+            if (same == 0) break;
+            for (uint32_t b = 0; b < bits; ++b) {
+                const bool set = (e >> b) & 1u;
+                const uint64_t those_set = __ballot(set);
+                same &= set ? those_set : ~those_set;
+            }
+            const uint32_t rank = (uint32_t)__builtin_popcountll(same & ((1ull << lane) - 1ull));
+            if (on) {
+                volatile uint32_t *const next = &count[wave][e];   // (a wave's own: its accesses stay in order)
+                const uint32_t at = *next + rank;
+                if (rank == 0) *next = at + (uint32_t)__builtin_popcountll(same);
+                args.back[row] = (int32_t)at;
+                if (at < args.rows) args.order[at] = (int32_t)row;   // (it is, unless the choices change meanwhile)
+            }
         }
     }
 }
 
-// Blocks of a sort: one, in one launch, where that is all there is to do; then the blocks' counts are summed by every block.
-constexpr uint32_t kSortAlone = 8192, kSortBlock = 1024, kMostSortBlocks = 256;
+// Blocks of a sort.  Up to 4096 rows one, which needs no counts of others (us, 128 experts, one launch / two: 2048 rows 5.0 / 7.1, 4096 6.3 / 7.4, 8192 9.7 / 7.5); then
+// of 1024 rows or more, as every block sums all blocks' counts (blocks of 1024 / 2048 / 4096: 16384 rows to 128 experts 7.8 / 8.1 / 9.1, 131072 to 128 10.5 / 9.6 / 10.2, 131072 to
+// 1024 31 / 21 / 19).
+constexpr uint32_t kSortAlone = 4096, kSortBlock = 1024, kMostSortBlocks = 256;
 
-uint32_t sort_blocks(uint32_t rows)
+uint32_t sort_blocks(uint32_t rows, uint32_t experts)
 {
     if (rows <= kSortAlone) return 1;
-    const uint32_t blocks = rows / kSortBlock + (rows % kSortBlock != 0);
+    const uint64_t counts = (uint64_t)rows * experts;
+    const uint32_t block = kSortBlock << (counts > (1u << 25) ? 2 : counts > (1u << 22) ? 1 : 0), blocks = rows / block + (rows % block != 0);
     return blocks < kMostSortBlocks ? blocks : kMostSortBlocks;
 }
 
@@ -546,17 +627,17 @@ template <typename I, uint32_t MOST>
 static int launch_sort_type(const SortArgs &a, hipStream_t stream)
 {
     if (a.blocks > 1) {
-        hipLaunchKernelGGL((count_by_expert_kernel<I, MOST>), dim3(a.blocks), dim3(64 * kSortWaves), 0, stream, a);
+        hipLaunchKernelGGL((count_by_expert_kernel<I, MOST>), dim3(a.blocks), dim3(kSortThreads), 0, stream, a);
         const int e = (int)hipGetLastError();
         if (e) return e;
     }
-    hipLaunchKernelGGL((sort_by_expert_kernel<I, MOST>), dim3(a.blocks), dim3(64 * kSortWaves), 0, stream, a);
+    hipLaunchKernelGGL((sort_by_expert_kernel<I, MOST>), dim3(a.blocks), dim3(kSortThreads), 0, stream, a);
     return (int)hipGetLastError();
 }
 
 int launch_sort(uint32_t choiceBits, SortArgs a, void *stream)
 {
-    a.blocks = sort_blocks(a.rows);
+    a.blocks = sort_blocks(a.rows, a.experts);
     const uint64_t each = (a.rows + (uint64_t)a.blocks - 1u) / a.blocks;
     a.perBlock = (uint32_t)((each + kSortBlock - 1u) / kSortBlock * kSortBlock);
     if (a.blocks == 1) a.part = nullptr;
