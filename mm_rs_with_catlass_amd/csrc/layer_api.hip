@@ -82,7 +82,7 @@ void catcoc_rms_norm(void *stream, const void *x, const void *residual, const vo
     if (!residual != !sum) { api_fail(E_NULL, "residual and sum come together"); return; }
     if (!x || !weight) { api_fail(E_NULL, "x and weight must be non-NULL"); return; }
     if ((cols <= 1024 ? (rows + 3ull) / 4 : rows) > 2 * kMaxWgs) { api_fail(E_SHAPE, "%u rows of %u columns are more than one launch holds", rows, cols); return; }
-    NormArgs a{x, residual, weight, out, sum, q, scale, rows, cols, eps, weightType};
+    NormArgs a{x, residual, weight, out, sum, q, scale, rows, cols, eps, weightType, 0};
     api_launched(launch_norm(dataType, residual ? residualType : DT_NONE, a, stream));
 }
 

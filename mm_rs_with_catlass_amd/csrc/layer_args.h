@@ -19,6 +19,7 @@ struct NormArgs {
     uint32_t rows, cols;
     float eps;
     uint32_t weightType;         // 0 (fp32), or the type of x
+    uint32_t runs;               // workgroups are dealt out in runs (run_place)
 };
 
 struct NormBackwardArgs {

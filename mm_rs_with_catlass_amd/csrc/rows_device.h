@@ -99,13 +99,20 @@ __device__ __forceinline__ Raw8<DT> round8(const Eight &e)
     return raw;
 }
 
-template <uint32_t DT>
+// LATER: past the caches, for what is not read again soon.
+template <uint32_t DT, bool LATER = false>
 __device__ __forceinline__ void store_raw8(void *x, size_t row, uint32_t pitch, uint32_t at, uint32_t size, const Raw8<DT> &raw)
 {
     constexpr uint32_t ES = DT == 0 ? 4u : 2u;
     unsigned char *p = (unsigned char *)x + (row * pitch + at) * ES;
     if (at + 8u <= size) {
-        __builtin_memcpy(p, raw.w, sizeof raw.w);
+        if constexpr (LATER) {
+            typedef uint32_t v4u __attribute__((ext_vector_type(4), aligned(2)));
+#pragma unroll
+            for (uint32_t i = 0; i < ES * 2u; i += 4u) __builtin_nontemporal_store(v4u{raw.w[i], raw.w[i + 1u], raw.w[i + 2u], raw.w[i + 3u]}, (v4u *)(p + 4u * i));
+        } else {
+            __builtin_memcpy(p, raw.w, sizeof raw.w);
+        }
     } else {
 #pragma unroll
         for (uint32_t i = 0; i < 7u; ++i) {
