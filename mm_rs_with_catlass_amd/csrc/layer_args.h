@@ -62,6 +62,7 @@ struct RowsArgs {
     float *outScale;             // spread: [column blocks, tokens * top]
     float *dshare;               // backward: [tokens, top]
     uint32_t tokens, top, cols;
+    uint32_t scaleWgs;           // spread: how many workgroups are the scales'
 };
 
 }  // namespace catcoc

@@ -263,23 +263,32 @@ int launch_norm(uint32_t type, uint32_t residualType, const NormArgs &a, void *s
     return launch_norm_type<0>(a, residualType, (hipStream_t)stream);
 }
 
-// How many workgroups share the rows, each with a part of dw of its own.
-uint32_t norm_backward_parts(uint32_t rows, uint32_t cols)
+// Threads of a row and of a workgroup, and how many workgroups share the rows, each with a part of dw of its own: 512 of 512 threads, two to a CU; 256 of 1024, whose rows'
+// sums meet in LDS before they are a part, where there are many long rows (us: 8192 rows of 8192 110 / 106, 16384 of 4096 107 / 104; 32 of 4096 6.3 / 7.6, 8192 of 2048 31 / 33).
+struct BackwardShape {
+    uint32_t row, wg, parts;
+};
+static BackwardShape backward_shape(uint32_t rows, uint32_t cols)
 {
-    const uint32_t group = cols <= 1024 ? 8u : cols <= 2048 ? 4u : cols <= 4096 ? 2u : 1u;   // rows at a time
-    const uint32_t turns = rows / group + (rows % group != 0);
-    return turns < 512u ? turns : 512u;
+    const uint32_t row = cols <= 1024 ? 64u : cols <= 2048 ? 128u : cols <= 4096 ? 256u : cols <= 8192 ? 512u : 1024u;
+    const uint32_t wg = cols > 8192 || (cols > 2048 && rows >= 2048) ? 1024u : 512u, each = wg / row, most = 262144u / wg, turns = rows / each + (rows % each != 0);
+    return {row, wg, turns < most ? turns : most};
 }
+
+uint32_t norm_backward_parts(uint32_t rows, uint32_t cols) { return backward_shape(rows, cols).parts; }
 
 template <uint32_t DT, uint32_t ST>
 static int launch_backward_types(const NormBackwardArgs &a, hipStream_t stream)
 {
     if (a.parts) {
         auto go = [&](auto kernel, uint32_t threads) { hipLaunchKernelGGL(kernel, dim3(a.parts), dim3(threads), 0, stream, a); };
-        if (a.cols <= 1024) go(rms_norm_backward_kernel<DT, ST, 64, 512>, 512);
-        else if (a.cols <= 2048) go(rms_norm_backward_kernel<DT, ST, 128, 512>, 512);
-        else if (a.cols <= 4096) go(rms_norm_backward_kernel<DT, ST, 256, 512>, 512);
-        else if (a.cols <= 8192) go(rms_norm_backward_kernel<DT, ST, 512, 512>, 512);
+        const BackwardShape s = backward_shape(a.rows, a.cols);
+        if (s.row == 64) go(rms_norm_backward_kernel<DT, ST, 64, 512>, 512);
+        else if (s.row == 128) go(rms_norm_backward_kernel<DT, ST, 128, 512>, 512);
+        else if (s.row == 256 && s.wg == 512) go(rms_norm_backward_kernel<DT, ST, 256, 512>, 512);
+        else if (s.row == 256) go(rms_norm_backward_kernel<DT, ST, 256, 1024>, 1024);
+        else if (s.row == 512 && s.wg == 512) go(rms_norm_backward_kernel<DT, ST, 512, 512>, 512);
+        else if (s.row == 512) go(rms_norm_backward_kernel<DT, ST, 512, 1024>, 1024);
         else go(rms_norm_backward_kernel<DT, ST, 1024, 1024>, 1024);
         const int e = (int)hipGetLastError();
         if (e) return e;

@@ -59,145 +59,145 @@ __device__ __forceinline__ void store16(unsigned char *row, uint64_t at, uint64_
 
 __device__ __forceinline__ uint32_t uniform(uint32_t v) { return (uint32_t)__builtin_amdgcn_readfirstlane((int)v); }
 
-// A wave takes SEG KiB of a token's row.  ES: bytes of a value.
-template <uint32_t ES, int SEG>
+// A wave takes a KiB of a token's row (four were slower: 8192 tokens' 4096 e4m3 values to eight places 81.6 us, 76.8 with one; 16384 rows of 256 values to two 13 and 7.3).
+// Scales, if any, are the first `scaleWgs` workgroups': a thread takes a choice's of up to eight blocks, all asked for before the first is stored (2048 tokens of 4096 to
+// eight places 18.1 us, 20.4 with a row's scales behind its values, 15.7 without scales; one token 3.6 and 4.8).  ES: bytes of a value.
+constexpr uint32_t kScaleRows = 256, kScaleBlocks = 8;
+
+template <uint32_t ES>
 __global__ void __launch_bounds__(256) spread_rows_kernel(const RowsArgs args)
 {
-    const uint64_t size = (uint64_t)args.cols * ES, rows = (uint64_t)args.tokens * args.top;
-    const uint32_t segs = (uint32_t)((size + SEG * 1024u - 1u) / (SEG * 1024u)), lane = threadIdx.x & 63u;
-    const uint32_t wave = uniform(workgroup() * 4u + (threadIdx.x >> 6));
-    const uint32_t token = wave / segs, seg = wave - token * segs;
-    if (token >= args.tokens) return;
-    const unsigned char *const from = (const unsigned char *)args.x + token * size;
-    const uint64_t at = (uint64_t)seg * SEG * 1024u + lane * 16u;
-    v4i v[SEG];
+    const uint64_t rows = (uint64_t)args.tokens * args.top;
+    uint32_t wg = workgroup();
+    if constexpr (ES == 1) {
+        if (wg < args.scaleWgs) {
+            const uint32_t blocks = (args.cols + kScaleBlock - 1u) / kScaleBlock, parts = (blocks + kScaleBlocks - 1u) / kScaleBlocks;
+            const uint32_t group = wg / parts, first = (wg - group * parts) * kScaleBlocks;
+            const uint64_t at = (uint64_t)group * kScaleRows + threadIdx.x;
+            if (at >= rows) return;
+            const uint32_t to = (uint32_t)args.back[at], token = (uint32_t)at / args.top;
+            if (to >= rows) return;
+            float s[kScaleBlocks];
 #pragma unroll
-    for (int i = 0; i < SEG; ++i) v[i] = load16<ES>(from, at + i * 1024u, size);
+            for (uint32_t i = 0; i < kScaleBlocks; ++i) s[i] = args.scale[(uint64_t)umin(first + i, blocks - 1u) * args.tokens + token];
+#pragma unroll
+            for (uint32_t i = 0; i < kScaleBlocks; ++i)
+                if (first + i < blocks) args.outScale[(first + i) * rows + to] = s[i];
+            return;
+        }
+        wg -= args.scaleWgs;
+    }
+    const uint64_t size = (uint64_t)args.cols * ES;
+    const uint32_t segs = (uint32_t)((size + 1023u) / 1024u), lane = threadIdx.x & 63u;
+    const uint32_t wave = uniform(wg * 4u + (threadIdx.x >> 6));
+    const uint32_t token = wave / segs;
+    if (token >= args.tokens) return;
+    const uint64_t at = (uint64_t)(wave - token * segs) * 1024u + lane * 16u;
+    if (at >= size) return;
+    const v4i v = load16<ES>((const unsigned char *)args.x + token * size, at, size);
     const int32_t *const back = args.back + (uint64_t)token * args.top;
     for (uint32_t j = 0; j < args.top; ++j) {
         const uint32_t to = uniform((uint32_t)back[j]);
-        if (to >= rows) continue;
-        unsigned char *const row = (unsigned char *)args.out + to * size;
-#pragma unroll
-        for (int i = 0; i < SEG; ++i)
-            if (at + i * 1024u < size) store16<ES>(row, at + i * 1024u, size, v[i]);
-    }
-    if (args.scale != nullptr && seg == 0) {
-        const uint32_t blocks = (args.cols + kScaleBlock - 1u) / kScaleBlock;
-        for (uint32_t b = lane; b < blocks; b += 64u) {
-            const float s = args.scale[(uint64_t)b * args.tokens + token];
-            for (uint32_t j = 0; j < args.top; ++j) {
-                const uint32_t to = uniform((uint32_t)back[j]);
-                if (to < rows) args.outScale[b * rows + to] = s;
-            }
-        }
+        if (to < rows) store16<ES>((unsigned char *)args.out + to * size, at, size, v);
     }
 }
 
-// A wave takes SEG times 512 values of a token's sum; four choices' rows are asked for together.
-template <uint32_t DT, int SEG>
+// A wave takes 512 values of a token's sum (1024 were slower: 2048 tokens of eight rows of 4096 37.1 us, 34.9 with 512); eight choices' rows are asked for together.
+template <uint32_t DT>
 __global__ void __launch_bounds__(256) gather_rows_kernel(const RowsArgs args)
 {
     const uint64_t rows = (uint64_t)args.tokens * args.top;
-    const uint32_t segs = (args.cols + SEG * 512u - 1u) / (SEG * 512u), lane = threadIdx.x & 63u;
+    const uint32_t segs = (args.cols + 511u) / 512u, lane = threadIdx.x & 63u;
     const uint32_t wave = uniform(workgroup() * 4u + (threadIdx.x >> 6));
-    const uint32_t token = wave / segs, col = (wave - token * segs) * SEG * 512u + lane * 8u;
+    const uint32_t token = wave / segs, col = (wave - token * segs) * 512u + lane * 8u;
     if (token >= args.tokens) return;
     const int32_t *const back = args.back + (uint64_t)token * args.top;
     const float *const share = args.share ? args.share + (uint64_t)token * args.top : nullptr;
-    Eight sum[SEG] = {};
-    constexpr int BATCH = SEG > 1 ? 4 : 8;
+    Eight sum = {};
+    constexpr uint32_t BATCH = 8;
     for (uint32_t first = 0; first < args.top; first += BATCH) {
-        Raw8<DT> raw[BATCH][SEG];
+        Raw8<DT> raw[BATCH];
         bool on[BATCH];
 #pragma unroll
-        for (uint32_t j = 0; j < (uint32_t)BATCH; ++j) {
+        for (uint32_t j = 0; j < BATCH; ++j) {
             const uint32_t at = first + j < args.top ? uniform((uint32_t)back[first + j]) : 0xffffffffu;
             on[j] = at < rows;
-            if (!on[j]) continue;
-#pragma unroll
-            for (int i = 0; i < SEG; ++i) raw[j][i] = load_raw8<DT>(args.y, at, args.cols, col + i * 512u, args.cols);
+            if (on[j]) raw[j] = load_raw8<DT>(args.y, at, args.cols, col, args.cols);
         }
 #pragma unroll
-        for (uint32_t j = 0; j < (uint32_t)BATCH; ++j) {
+        for (uint32_t j = 0; j < BATCH; ++j) {
             if (!on[j]) continue;
             const float s = share ? share[first + j] : 1.f;
+            const Eight v = widen8<DT>(raw[j]);
 #pragma unroll
-            for (int i = 0; i < SEG; ++i) {
-                const Eight v = widen8<DT>(raw[j][i]);
-#pragma unroll
-                for (int k = 0; k < 8; ++k) sum[i].v[k] = __builtin_fmaf(s, v.v[k], sum[i].v[k]);
-            }
+            for (int k = 0; k < 8; ++k) sum.v[k] = __builtin_fmaf(s, v.v[k], sum.v[k]);
         }
     }
-#pragma unroll
-    for (int i = 0; i < SEG; ++i)
-        if (col + i * 512u < args.cols) store_raw8<DT>(args.out, token, args.cols, col + i * 512u, args.cols, round8<DT>(sum[i]));
+    if (col < args.cols) store_raw8<DT>(args.out, token, args.cols, col, args.cols, round8<DT>(sum));
 }
 
-// T threads take a choice's row, one after the other a token's.
+// T threads take a choice's row.  The choices of a token follow each other on one XCD, whose L2 then has the token's gradient for all but the first (us, with one workgroup
+// for all of a token's choices / with these: 2048 tokens of eight rows of 4096 64 / 56, 32 of them 8.6 / 3.2).
 template <uint32_t DT, int T>
 __global__ void __launch_bounds__(256) gather_rows_backward_kernel(const RowsArgs args)
 {
-    constexpr uint32_t W = T / 64;
-    __shared__ float parts[2][W];
+    constexpr uint32_t W = T / 64, EACH = 256 / T;
+    __shared__ float parts[W];
     const uint64_t rows = (uint64_t)args.tokens * args.top;
-    const uint32_t t = threadIdx.x % T;
-    const uint64_t token = T < 256 ? (uint64_t)workgroup() * (256u / T) + uniform(threadIdx.x / T) : workgroup();
-    if (token >= args.tokens) return;
-    for (uint32_t j = 0; j < args.top; ++j) {
-        const uint64_t i = token * args.top + j;
-        const uint32_t at = uniform((uint32_t)args.back[i]);
+    const uint32_t t = threadIdx.x % T, wg = workgroup(), turn = wg >> 3;
+    const uint64_t token = ((uint64_t)(turn / args.top) * 8u + (wg & 7u)) * EACH + uniform(threadIdx.x / T);
+    if (token >= args.tokens) return;   // (a wave's or a workgroup's)
+    const uint64_t i = token * args.top + turn % args.top;
+    const uint32_t at = uniform((uint32_t)args.back[i]);
+    float dot = 0.f;
+    if (at < rows) {
         const float share = args.share[i];
-        float dot = 0.f;
-        if (at < rows) {
-            for (uint32_t col = t * 8u; col < args.cols; col += T * 16u) {
-                const uint32_t next = col + T * 8u;   // (two pieces of both rows are asked for together)
-                const Raw8<DT> rd = load_raw8<DT>(args.x, token, args.cols, col, args.cols), ry = load_raw8<DT>(args.y, at, args.cols, col, args.cols);
-                Raw8<DT> rd2 = {}, ry2 = {};
-                if (next < args.cols) {
-                    rd2 = load_raw8<DT>(args.x, token, args.cols, next, args.cols);
-                    ry2 = load_raw8<DT>(args.y, at, args.cols, next, args.cols);
-                }
-                Eight d = widen8<DT>(rd), y = widen8<DT>(ry);
+        for (uint32_t col = t * 8u; col < args.cols; col += T * 16u) {
+            const uint32_t next = col + T * 8u;   // (two pieces of both rows are asked for together)
+            const Raw8<DT> rd = load_raw8<DT>(args.x, token, args.cols, col, args.cols), ry = load_raw8<DT>(args.y, at, args.cols, col, args.cols);
+            Raw8<DT> rd2 = {}, ry2 = {};
+            if (next < args.cols) {
+                rd2 = load_raw8<DT>(args.x, token, args.cols, next, args.cols);
+                ry2 = load_raw8<DT>(args.y, at, args.cols, next, args.cols);
+            }
+            Eight d = widen8<DT>(rd), y = widen8<DT>(ry);
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                dot = __builtin_fmaf(d.v[k], y.v[k], dot);
+                d.v[k] *= share;
+            }
+            store_raw8<DT>(args.out, at, args.cols, col, args.cols, round8<DT>(d));
+            if (next < args.cols) {
+                d = widen8<DT>(rd2), y = widen8<DT>(ry2);
 #pragma unroll
                 for (int k = 0; k < 8; ++k) {
                     dot = __builtin_fmaf(d.v[k], y.v[k], dot);
                     d.v[k] *= share;
                 }
-                store_raw8<DT>(args.out, at, args.cols, col, args.cols, round8<DT>(d));
-                if (next < args.cols) {
-                    d = widen8<DT>(rd2), y = widen8<DT>(ry2);
-#pragma unroll
-                    for (int k = 0; k < 8; ++k) {
-                        dot = __builtin_fmaf(d.v[k], y.v[k], dot);
-                        d.v[k] *= share;
-                    }
-                    store_raw8<DT>(args.out, at, args.cols, next, args.cols, round8<DT>(d));
-                }
+                store_raw8<DT>(args.out, at, args.cols, next, args.cols, round8<DT>(d));
             }
         }
-        dot = wave_sum(dot);
-        if constexpr (W > 1) {
-            if ((t & 63u) == 0) parts[j & 1u][t >> 6] = dot;
-            __syncthreads();
-            dot = parts[j & 1u][0];
-#pragma unroll
-            for (uint32_t k = 1; k < W; ++k) dot += parts[j & 1u][k];
-        }
-        if (t == 0) args.dshare[i] = dot;
     }
+    dot = wave_sum(dot);
+    if constexpr (W > 1) {
+        if ((t & 63u) == 0) parts[t >> 6] = dot;
+        __syncthreads();
+        dot = parts[0];
+#pragma unroll
+        for (uint32_t k = 1; k < W; ++k) dot += parts[k];
+    }
+    if (t == 0) args.dshare[i] = dot;
 }
 
-// Fewer segments a wave where there would else be fewer than 16 waves a CU.
-constexpr uint64_t kManyWaves = 4096;
-
 template <uint32_t ES>
-static int launch_spread_size(const RowsArgs &a, hipStream_t stream)
+static int launch_spread_size(RowsArgs a, hipStream_t stream)
 {
-    const uint64_t size = (uint64_t)a.cols * ES, fours = a.tokens * ((size + 4095) / 4096), ones = a.tokens * ((size + 1023) / 1024);
-    if (fours >= kManyWaves) hipLaunchKernelGGL((spread_rows_kernel<ES, 4>), grid_of((fours + 3) / 4, 256), dim3(256), 0, stream, a);
-    else hipLaunchKernelGGL((spread_rows_kernel<ES, 1>), grid_of((ones + 3) / 4, 256), dim3(256), 0, stream, a);
+    const uint64_t waves = a.tokens * (((uint64_t)a.cols * ES + 1023) / 1024);
+    if (a.scale != nullptr) {
+        const uint64_t blocks = (a.cols + kScaleBlock - 1u) / kScaleBlock, rows = (uint64_t)a.tokens * a.top;
+        a.scaleWgs = (uint32_t)((rows + kScaleRows - 1) / kScaleRows * ((blocks + kScaleBlocks - 1) / kScaleBlocks));
+    }
+    hipLaunchKernelGGL((spread_rows_kernel<ES>), grid_of(a.scaleWgs + (waves + 3) / 4, 256), dim3(256), 0, stream, a);
     return (int)hipGetLastError();
 }
 
@@ -211,9 +211,8 @@ int launch_spread_rows(uint32_t valueBytes, const RowsArgs &a, void *stream)
 template <uint32_t DT>
 static int launch_gather_type(const RowsArgs &a, hipStream_t stream)
 {
-    const uint64_t twos = a.tokens * (uint64_t)((a.cols + 1023u) / 1024u), ones = a.tokens * (uint64_t)((a.cols + 511u) / 512u);
-    if (twos >= kManyWaves) hipLaunchKernelGGL((gather_rows_kernel<DT, 2>), grid_of((twos + 3) / 4, 256), dim3(256), 0, stream, a);
-    else hipLaunchKernelGGL((gather_rows_kernel<DT, 1>), grid_of((ones + 3) / 4, 256), dim3(256), 0, stream, a);
+    const uint64_t waves = a.tokens * (uint64_t)((a.cols + 511u) / 512u);
+    hipLaunchKernelGGL((gather_rows_kernel<DT>), grid_of((waves + 3) / 4, 256), dim3(256), 0, stream, a);
     return (int)hipGetLastError();
 }
 
@@ -227,8 +226,10 @@ int launch_gather_rows(uint32_t type, const RowsArgs &a, void *stream)
 template <uint32_t DT>
 static int launch_gather_backward_type(const RowsArgs &a, hipStream_t stream)
 {
-    if (a.cols <= 1024) hipLaunchKernelGGL((gather_rows_backward_kernel<DT, 64>), grid_of((a.tokens + 3ull) / 4, 256), dim3(256), 0, stream, a);
-    else hipLaunchKernelGGL((gather_rows_backward_kernel<DT, 256>), grid_of(a.tokens, 256), dim3(256), 0, stream, a);
+    const uint32_t each = a.cols <= 1024 ? 4 : 1;   // tokens a workgroup
+    const uint64_t wgs = (a.tokens + 8ull * each - 1) / (8ull * each) * 8 * a.top;
+    if (each == 4) hipLaunchKernelGGL((gather_rows_backward_kernel<DT, 64>), grid_of(wgs, 256), dim3(256), 0, stream, a);
+    else hipLaunchKernelGGL((gather_rows_backward_kernel<DT, 256>), grid_of(wgs, 256), dim3(256), 0, stream, a);
     return (int)hipGetLastError();
 }
 
