@@ -23,18 +23,6 @@ __device__ __forceinline__ v4i load16_any(const unsigned char *p)
     return v;
 }
 
-// Inclusive sums over the lanes of a wave.
-__device__ __forceinline__ uint32_t wave_prefix(uint32_t v)
-{
-    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x111, 0xf, 0xf, false);   // row_shr:1, 2, 4, 8
-    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x112, 0xf, 0xf, false);
-    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x114, 0xf, 0xf, false);
-    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x118, 0xf, 0xf, false);
-    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x142, 0xa, 0xf, false);   // row_bcast:15 and 31
-    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x143, 0xc, 0xf, false);
-    return v;
-}
-
 // Position `wg` of a launch of `total` tiles that go round-robin to the eight XCDs: each of them gets a run of consecutive tiles, which share rows and
 // matrices in its L2.  Returns total or more past the end.
 __device__ __forceinline__ uint32_t xcd_run(uint32_t wg, uint32_t total)

@@ -551,13 +551,7 @@ __global__ void __launch_bounds__(kSortThreads) sort_by_expert_kernel(const Sort
         }
     }
     // ---- where an expert's rows begin
-    uint32_t upTo = n, past = those;
-#pragma unroll
-    for (uint32_t by = 1; by < 64; by <<= 1) {
-        const uint32_t less = __shfl_up(upTo, by), more = __shfl_xor(past, by);
-        if (lane >= by) upTo += less;
-        past += more;
-    }
+    uint32_t upTo = wave_prefix(n), past = wave_prefix(those);
     if (lane == 63u) sums[0][wave] = upTo, sums[1][wave] = past;
     __syncthreads();
     uint32_t every = 0;
