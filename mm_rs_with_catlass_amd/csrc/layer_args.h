@@ -42,7 +42,7 @@ struct RouteArgs {
     uint32_t tokens, experts, top, type;
     uint32_t sigmoid, groups, topGroups, groupTop, renormalize;
     float scale;
-    uint32_t groupLanes, perLane;   // lanes of a group's experts (a power of two), experts a lane
+    uint32_t groupLanes;         // lanes of a group's experts, a power of two
 };
 
 struct SortArgs {

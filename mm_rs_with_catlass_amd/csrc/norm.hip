@@ -10,6 +10,9 @@
 // y is what the next operator reads, the sum is read after a whole layer: it is stored past the caches, which leaves them to y (us, a norm and a quantizer of its y, without /
 // with it: 3000 rows of 4096 26.3 / 23.7, 16384 140 / 128; where the sum is read at once 37.3 / 40.1 and 185 / 185).  Loops of resident workgroups with the next row's loads ahead
 // were slower (16384 rows 102-105 us, 95 without), as were loads past the caches.
+//
+// 16384 rows of 4096 in bf16 with a residual 91 us, 5.9 TB/s (a copy of as many bytes 104); 4099 rows of 1808 to e4m3 with an fp32 residual 15.8, 5.2 TB/s; 16 rows 3.5.  The
+// backward pass of 8192 rows of 4096 54 us, 5.0 TB/s: 47 its rows, 4 the sum of the weight gradient's parts.
 #include <hip/hip_runtime.h>
 
 #include "layer_args.h"

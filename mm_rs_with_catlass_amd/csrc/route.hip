@@ -1,10 +1,16 @@
 // The router: which experts a token goes to, with what shares, the shares' gradient, and the rows' order by expert.
 //
-// A token's experts lie on 16 or 64 lanes, a group of them on a power of two of those, up to 32 a lane.  An expert's rank is one 64-bit number, its key: a double whose last ten bits
-// are the expert's index, counted so that of equal scores the lower index is the larger key.  Maxima of doubles then order scores and ties alike.  Where the
-// order is that of the logits (no bias, no sums of scores) a key holds all of a logit's bits; else it is the score in 64 bits, whose first 42 bits count: which of two
-// experts is ahead is a matter of more bits than fp32 has, as one of a prompt's 10^5 choices is decided by less than 2^-24 now and then.
+//   score p_e = softmax(l)_e or s(l_e); the `top` largest of p_e + b_e, in the topGroups groups whose best one or two sum to most; share = scale p_c (/ sum of the chosen p).
+//
+// A token's experts lie on 16 or 64 lanes, a group of them on a power of two of those, up to 32 a lane: four tokens a wave where 16 lanes hold them (16384 tokens
+// of 256 experts, biased, 12.3 us; 24.7 with a wave for each token).  An expert's rank is one 64-bit number, its key: a double whose last ten bits are the expert's index, counted so that of equal scores
+// the lower index is the larger key.  Maxima of doubles, as fast here as those of floats, then order scores and ties alike, and nothing has to be carried along with a
+// score.  Where the order is that of the logits (no bias, no sums of scores) a key holds all of a logit's bits; else it is the score in 64 bits, whose first 42 bits count: which of
+// two experts is ahead is a matter of more bits than fp32 has, as one of a prompt's 10^5 choices is decided by less than 2^-24 now and then.
 // Every lane sorts its keys once (odd-even merge sort: Batcher, AFIPS 1968); then the largest of the lanes' first keys is taken `top` times.
+//
+// Bound by its 64-bit instructions where there are many tokens: 16384 of 256 experts in groups, biased, 12 us (1200 instructions a wave, 70 % of the time; the logits alone
+// would take 3.5), and 50 us with the library's exponential and division, a load for each bias and the compiler's way of moving up a sorted list; 32 tokens of 64 experts 3.1 us.
 #include <hip/hip_runtime.h>
 
 #include <utility>
@@ -124,27 +130,40 @@ __device__ __forceinline__ float logit_at(const void *x, size_t at, uint32_t typ
     return type == 0 ? ((const float *)x)[at] : widen1(((const unsigned short *)x)[at], type);
 }
 
-// Logits [at, at + count) of up to V, -inf behind them.
-template <int V>
-__device__ __forceinline__ void load_logits(const void *x, size_t at, uint32_t count, uint32_t type, float (&v)[V])
+// Value i of a lane that is `part` of a group's lanes is the group's expert place_in_group(): consecutive lanes hold consecutive pieces of P.  Pieces of four, with which a
+// wave's accesses lie beside each other, where there is little but them (gradients of 16384 tokens of 256 experts 10.7 us, 14.5 with a lane's values in one piece), one
+// piece where there are few registers left (the choice of the same 13.0 us, 16.0 with pieces of four).
+template <int P>
+__device__ __forceinline__ uint32_t place_in_group(uint32_t part, uint32_t lanes, int i)
 {
-    if (type == 0) {
-        const float *p = (const float *)x + at;
-        if (count == V) __builtin_memcpy(v, p, sizeof v);
-        else {
+    return ((uint32_t)(i / P) * lanes + part) * P + (uint32_t)(i % P);
+}
+
+// A lane's logits of a group of `size` that begins at `at`, -inf for those there are not.
+template <int P, int V>
+__device__ __forceinline__ void load_logits(const void *x, size_t at, uint32_t part, uint32_t lanes, uint32_t size, uint32_t type, float (&v)[V])
+{
 #pragma unroll
-            for (uint32_t i = 0; i < V; ++i) v[i] = i < count ? p[i] : -__builtin_huge_valf();
+    for (int c = 0; c < V / P; ++c) {
+        const uint32_t o = place_in_group<P>(part, lanes, c * P);
+        if (type == 0) {
+            const float *p = (const float *)x + at + o;
+            if (o + P <= size) __builtin_memcpy(&v[c * P], p, P * 4);
+            else {
+#pragma unroll
+                for (uint32_t i = 0; i < (uint32_t)P; ++i) v[c * P + i] = o + i < size ? p[i] : -__builtin_huge_valf();
+            }
+        } else {
+            const unsigned short *p = (const unsigned short *)x + at + o;
+            unsigned short h[P];
+            if (o + P <= size) __builtin_memcpy(h, p, P * 2);
+            else {
+#pragma unroll
+                for (uint32_t i = 0; i < (uint32_t)P; ++i) h[i] = o + i < size ? p[i] : 0;
+            }
+#pragma unroll
+            for (uint32_t i = 0; i < (uint32_t)P; ++i) v[c * P + i] = o + i < size ? widen1(h[i], type) : -__builtin_huge_valf();
         }
-    } else {
-        const unsigned short *p = (const unsigned short *)x + at;
-        unsigned short h[V];
-        if (count == V) __builtin_memcpy(h, p, sizeof h);
-        else {
-#pragma unroll
-            for (uint32_t i = 0; i < V; ++i) h[i] = i < count ? p[i] : 0;
-        }
-#pragma unroll
-        for (uint32_t i = 0; i < V; ++i) v[i] = i < count ? widen1(h[i], type) : -__builtin_huge_valf();
     }
 }
 
@@ -190,14 +209,10 @@ __global__ void __launch_bounds__(256, LANES == 16 ? 4 : V <= 16 ? 3 : 2) route_
     const uint64_t at = ((uint64_t)workgroup() * 4u + (threadIdx.x >> 6)) * (64 / LANES) + lane / LANES;
     if (at - lane / LANES >= args.tokens) return;   // (a wave without tokens)
     const size_t token = at < args.tokens ? at : args.tokens - 1u;   // (the last one once more, for nothing)
-    const uint32_t slot = l / args.groupLanes, part = l % args.groupLanes, size = args.experts / args.groups, in = part * args.perLane;
-    const uint32_t first = slot * size + in, count = slot < args.groups && in < size ? umin(args.perLane, size - in) : 0u;
+    const uint32_t each = args.experts / args.groups, slot = l / args.groupLanes, part = l % args.groupLanes;
+    const uint32_t size = slot < args.groups ? each : 0u, first = size ? slot * each : 0u;   // the group's
     float v[V];
-    load_logits<V>(args.logits, token * args.experts + (count ? first : 0u), count, args.type, v);
-    float b[V];
-#pragma unroll
-    for (int i = 0; i < V; ++i) b[i] = 0.f;
-    if (args.bias != nullptr) load_logits<V>(args.bias, count ? first : 0u, count, 0, b);
+    load_logits<V, V>(args.logits, token * args.experts + first, part, args.groupLanes, size, args.type, v);
 
     float most = 0.f;
     if (!args.sigmoid) {
@@ -232,6 +247,10 @@ __global__ void __launch_bounds__(256, LANES == 16 ? 4 : V <= 16 ? 3 : 2) route_
             total = (float)sum;
             r = 1.0 / sum;
         }
+        float b[V];
+#pragma unroll
+        for (int i = 0; i < V; ++i) b[i] = 0.f;
+        if (args.bias != nullptr) load_logits<V, V>(args.bias, first, part, args.groupLanes, size, 0, b);
 #pragma unroll
         for (int i = 0; i < V; ++i) k[i] = __builtin_fma(k[i], r, (double)b[i]);
         if (__any(odd)) {
@@ -248,7 +267,7 @@ __global__ void __launch_bounds__(256, LANES == 16 ? 4 : V <= 16 ? 3 : 2) route_
         for (int i = 0; i < V; ++i) k[i] = v[i] + 0.f;   // (-0 is 0)
     }
 #pragma unroll
-    for (int i = 0; i < V; ++i) k[i] = with_index(k[i], first + i);
+    for (int i = 0; i < V; ++i) k[i] = with_index(k[i], first + part * V + i);
     sort_keys<V>(k);
 
     bool out = false;   // of the groups that are chosen from
@@ -318,19 +337,22 @@ __global__ void __launch_bounds__(256, LANES == 16 ? 4 : V <= 16 ? 3 : 2) route_
     args.share[token * args.top + l] = on ? share * args.scale : 0.f;
 }
 
+// Between a wave's writes to LDS and its reads of other lanes' (LDS keeps a wave's accesses in order, the compiler knows of one lane's only).
+__device__ __forceinline__ void wave_turn() { asm volatile("" ::: "memory"); }
+
 // With w the shares without scale: dl_c = scale w_c (1 - s(l_c) where sigmoid) (g_c - sum of w g where they are shares of a sum); the softmax of all experts: dl_e = scale p_e (g_e - sum of p g).
 template <int LANES, int V>
 __global__ void __launch_bounds__(256) route_backward_kernel(const RouteArgs args)
 {
+    constexpr int P = V < 4 ? V : 4;
     const uint32_t lane = threadIdx.x & 63u, l = lane % LANES;
     const uint64_t at = ((uint64_t)workgroup() * 4u + (threadIdx.x >> 6)) * (64 / LANES) + lane / LANES;
     if (at - lane / LANES >= args.tokens) return;
     const size_t token = at < args.tokens ? at : args.tokens - 1u;
-    const uint32_t first = l * args.perLane, count = first < args.experts ? umin(args.perLane, args.experts - first) : 0u;
     const bool all = !args.sigmoid && !args.renormalize;   // every expert's logit moves the shares
     float v[V], most = 0.f, total = 1.f;
     if (all) {
-        load_logits<V>(args.logits, token * args.experts + (count ? first : 0u), count, args.type, v);
+        load_logits<P, V>(args.logits, token * args.experts, l, LANES, args.experts, args.type, v);
         most = v[0];
 #pragma unroll
         for (int i = 1; i < V; ++i) most = __builtin_elementwise_max(most, v[i]);
@@ -362,32 +384,59 @@ __global__ void __launch_bounds__(256) route_backward_kernel(const RouteArgs arg
 #pragma unroll
         for (int i = 0; i < V; ++i) v[i] = 0.f;
     }
-    for (uint32_t j = 0; j < args.top; ++j) {   // (an expert that is chosen twice gets both)
-        const uint32_t to = (uint32_t)__shfl(chosen, (int)j, LANES) - first;
-        const float more = __shfl(d, (int)j, LANES);
+    if constexpr (V <= 4) {
+        for (uint32_t j = 0; j < args.top; ++j) {   // (an expert that is chosen twice gets both)
+            const uint32_t to = (uint32_t)__shfl(chosen, (int)j, LANES) - l * V;
+            const float more = __shfl(d, (int)j, LANES);
 #pragma unroll
-        for (uint32_t i = 0; i < V; ++i) v[i] += to == i ? more : 0.f;
-    }
-    if (at >= args.tokens || count == 0) return;
-    const size_t to = token * args.experts + first;
-    if (args.type == 0) {
-        float *p = (float *)args.dlogits + to;
-        if (count == V) __builtin_memcpy(p, v, sizeof v);
-        else {
-#pragma unroll
-            for (uint32_t i = 0; i < V; ++i)
-                if (i < count) p[i] = v[i];
+            for (uint32_t i = 0; i < V; ++i) v[i] += to == i ? more : 0.f;
         }
     } else {
-        unsigned short h[V], *p = (unsigned short *)args.dlogits + to;
+        // Through LDS, where a choice finds its expert's place; an expert that is chosen twice gets both from each of its choices.
+        __shared__ float rows[256 * V];
+        float *const row = rows + (threadIdx.x - l) * V;
+        float more = 0.f;
+        for (uint32_t j = 0; j < args.top; ++j) {
+            const int32_t other = __shfl(chosen, (int)j, LANES);
+            const float part = __shfl(d, (int)j, LANES);
+            more += other == chosen ? part : 0.f;
+        }
 #pragma unroll
-        for (uint32_t i = 0; i < V; ++i)
-            h[i] = args.type == DT_BF16 ? __builtin_bit_cast(unsigned short, (__bf16)v[i]) : __builtin_bit_cast(unsigned short, (_Float16)v[i]);
-        if (count == V) __builtin_memcpy(p, h, sizeof h);
-        else {
+        for (int i = 0; i < V; ++i) row[place_in_group<P>(l, LANES, i)] = v[i];
+        wave_turn();
+        const uint32_t place = on ? (uint32_t)chosen : 0u;
+        const float there = row[place] + more;
+        wave_turn();
+        if (on) row[place] = there;
+        wave_turn();
 #pragma unroll
-            for (uint32_t i = 0; i < V; ++i)
-                if (i < count) p[i] = h[i];
+        for (int i = 0; i < V; ++i) v[i] = row[place_in_group<P>(l, LANES, i)];
+    }
+    if (at >= args.tokens) return;
+#pragma unroll
+    for (int c = 0; c < V / P; ++c) {
+        const uint32_t o = place_in_group<P>(l, LANES, c * P);
+        if (o >= args.experts) continue;
+        const size_t to = token * args.experts + o;
+        if (args.type == 0) {
+            float *p = (float *)args.dlogits + to;
+            if (o + P <= args.experts) __builtin_memcpy(p, &v[c * P], P * 4);
+            else {
+#pragma unroll
+                for (uint32_t i = 0; i < (uint32_t)P; ++i)
+                    if (o + i < args.experts) p[i] = v[c * P + i];
+            }
+        } else {
+            unsigned short h[P], *p = (unsigned short *)args.dlogits + to;
+#pragma unroll
+            for (int i = 0; i < P; ++i)
+                h[i] = args.type == DT_BF16 ? __builtin_bit_cast(unsigned short, (__bf16)v[c * P + i]) : __builtin_bit_cast(unsigned short, (_Float16)v[c * P + i]);
+            if (o + P <= args.experts) __builtin_memcpy(p, h, P * 2);
+            else {
+#pragma unroll
+                for (uint32_t i = 0; i < (uint32_t)P; ++i)
+                    if (o + i < args.experts) p[i] = h[i];
+            }
         }
     }
 }
@@ -402,26 +451,30 @@ static int launch_route_kernel(const RouteArgs &a, hipStream_t stream)
     return (int)hipGetLastError();
 }
 
-// Lanes of a token, and of a group in it, for `groups` groups of experts: 16 lanes where they hold it in 16 values each, else 64.
-static uint32_t route_lanes(RouteArgs &a, uint32_t groups)
+// Lanes of a token, of a group in it, and values a lane, for `groups` groups of experts: 16 lanes where they hold it in 16 values each, else 64.  0 lanes: not on these.
+struct RouteShape {
+    uint32_t lanes, groupLanes, perLane;
+};
+static RouteShape route_shape(uint32_t experts, uint32_t top, uint32_t groups)
 {
     uint32_t slots = 1;
     while (slots < groups) slots *= 2;
-    const uint32_t size = a.experts / groups;
+    const uint32_t size = experts / groups;
     for (uint32_t lanes = 16; lanes <= 64; lanes *= 4) {
-        if (slots > lanes || a.top > lanes) continue;
-        a.groupLanes = lanes / slots;
-        a.perLane = (size + a.groupLanes - 1) / a.groupLanes;
-        if (a.perLane <= (lanes == 16 ? 16u : 32u)) return lanes;
+        if (slots > lanes || top > lanes) continue;
+        const uint32_t of = lanes / slots, n = (size + of - 1) / of;
+        if (n <= (lanes == 16 ? 16u : 32u)) return {lanes, of, n};
     }
-    return 0;
+    return {0, 0, 0};
 }
 
 template <bool BACKWARD>
 static int launch_route_shape(RouteArgs a, hipStream_t stream)
 {
-    const uint32_t lanes = route_lanes(a, BACKWARD ? 1u : a.groups), n = a.perLane;
-    if (lanes == 16) {
+    const RouteShape s = route_shape(a.experts, a.top, BACKWARD ? 1u : a.groups);
+    const uint32_t n = s.perLane;
+    a.groupLanes = s.groupLanes;
+    if (s.lanes == 16) {
         if (n <= 1) return launch_route_kernel<16, 1, BACKWARD>(a, stream);
         if (n <= 2) return launch_route_kernel<16, 2, BACKWARD>(a, stream);
         if (n <= 4) return launch_route_kernel<16, 4, BACKWARD>(a, stream);
@@ -438,10 +491,7 @@ static int launch_route_shape(RouteArgs a, hipStream_t stream)
 // Groups that the kernel can lay out: at most 64 of them.
 bool can_route(uint32_t experts, uint32_t top, uint32_t groups)
 {
-    RouteArgs a{};
-    a.experts = experts;
-    a.top = top;
-    return route_lanes(a, groups) != 0;
+    return route_shape(experts, top, groups).lanes != 0;
 }
 
 int launch_route(const RouteArgs &a, void *stream) { return launch_route_shape<false>(a, (hipStream_t)stream); }
@@ -449,7 +499,8 @@ int launch_route_backward(const RouteArgs &a, void *stream) { return launch_rout
 
 // ---- rows by expert -----------------------------------------------------------------------------------------------------------------------
 // A counting sort, stable: a wave counts how many of its consecutive rows go to each expert, the counts' sums over waves, blocks and experts are where its first
-// row of each goes, and the rows follow in 64s, a row's place among them by how many lanes before it have the same expert.
+// row of each goes, and the rows follow in 64s, a row's place among them by how many lanes before it have the same expert.  Latencies bound it: 256 rows 3.3 us, 131072 rows to 128
+// experts 9.2 (two launches of 2.9 and 6.5; the bytes would take 0.3).
 
 namespace {
 

