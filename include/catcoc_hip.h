@@ -379,8 +379,8 @@ CATCOC_API uint64_t catcoc_sort_by_expert_workspace_size(uint32_t rows, uint32_t
 CATCOC_API void catcoc_sort_by_expert(void *stream, const void *choice, int32_t *order, int32_t *back, int32_t *ends, void *workspace, uint64_t workspaceBytes,
                                       uint32_t rows, uint32_t experts, uint32_t choiceBits);
 
-/* Every token's row at its choices' places: out[back[t,j]] = x[t], x [tokens,cols] of valueBytes (1, 2, 4) each, back [tokens,top], out [tokens*top,cols]; with e4m3 codes their
- * scale [ceil(cols/128), tokens] to outScale [ceil(cols/128), tokens*top] (NULL: none).  Places outside the rows are left out; rows that no choice has stay as they were. */
+/* Every token's row at its choices' places: out[back[t,j]] = x[t], x [tokens,cols] of valueBytes (1, 2, 4) each, back [tokens,top], out [tokens*top,cols]; with e4m3 codes
+ * (valueBytes 1) their scale [ceil(cols/128), tokens] to outScale [ceil(cols/128), tokens*top] (NULL: none).  Places outside the rows are left out; rows that no choice has stay as they were. */
 CATCOC_API void catcoc_spread_rows(void *stream, const void *x, const float *scale, const int32_t *back, void *out, float *outScale, uint32_t tokens,
                                    uint32_t top, uint32_t cols, uint32_t valueBytes);
 /* The rows back at their tokens: out[t] = sum over j of share[t,j] y[back[t,j]], in the order of j; share NULL: ones (the gradient of catcoc_spread_rows). */

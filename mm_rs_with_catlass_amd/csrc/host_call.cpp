@@ -722,7 +722,7 @@ PyObject *spread(PyObject *, PyObject *const *v, Py_ssize_t n)   // x, back, sca
         if (x.scalar_type() != F8) code(x.scalar_type(), true);
         if (back.scalar_type() != at::kInt || back.size(0) != tokens || back.numel() > MOST || tokens > MOST || top > MOST || cols > MOST) throw Other{};
         const bool scaled = v[2] != Py_None;
-        if (!scaled && v[4] != Py_None) throw Other{};
+        if (scaled ? x.scalar_type() != F8 : v[4] != Py_None) throw Other{};
         const float *const scale = (const float *)here.maybe(v[2], at::kFloat, {blocks(cols), tokens});
         Result out(v[3], x.scalar_type(), {tokens * top, cols}, x);
         here.check(out);

@@ -196,6 +196,7 @@ void catcoc_spread_rows(void *stream, const void *x, const float *scale, const i
     if (check_rows(tokens, top, cols) || check_pieces(tokens, (uint64_t)cols * valueBytes)) return;
     if (tokens == 0) { api_launched(0); return; }
     if (!scale != !outScale) { api_fail(E_NULL, "scale and outScale come together"); return; }
+    if (scale && valueBytes != 1) { api_fail(E_DTYPE, "scales come with values of 1 byte (got %u)", valueBytes); return; }
     if (!x || !back || !out) { api_fail(E_NULL, "x, back and out must be non-NULL"); return; }
     RowsArgs a{};
     a.x = x;

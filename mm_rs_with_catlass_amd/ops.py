@@ -989,6 +989,8 @@ def spread_rows(x, back, scale=None, out=None, out_scale=None):
     _, top = _want_back(back, tokens)
     if scale is None and out_scale is not None:
         _fail("out_scale without scale")
+    if scale is not None:
+        _want(x, "x with scale", torch.float8_e4m3fn)
     _want(scale, "scale", torch.float32, 2, None, (_blocks(cols), tokens))
     _want(out, "out", x.dtype, 2, None, (tokens * top, cols))
     _want(out_scale, "out_scale", torch.float32, 2, None, (_blocks(cols), tokens * top))

@@ -81,7 +81,8 @@ def codes_are_near(q, scale, y, slack):
     assert ((q.double() - t).abs() <= step / 2 + (slack + 4 * u) * t.abs()).all()
 
 
-NORMS = [(1, 1), (1, 128), (3, 127), (5, 512), (7, 513), (64, 1000), (130, 1024), (33, 1025), (16, 2048), (9, 2050), (257, 1808), (5, 4096), (6, 4097), (3, 8192), (4, 7777), (3, 8193), (2, 16384)]
+NORMS = [(1, 1), (1, 128), (3, 127), (5, 512), (7, 513), (64, 1000), (130, 1024), (33, 1025), (16, 2048), (9, 2050), (257, 1808), (5, 4096), (6, 4097), (3, 8192), (4, 7777), (3, 8193), (2, 16384),
+         (1030, 1500), (4110, 300), (1025, 4100), (4099, 1000)]
 TYPES = [(BF16, None, BF16), (BF16, BF16, F32), (BF16, F32, BF16), (F16, F16, F16), (F16, F32, F32), (F32, None, F32), (F32, F32, F32)]
 
 
@@ -152,7 +153,7 @@ def test_norm_of_zeros_and_of_values_that_are_not_finite():
     assert (ops.rms_norm(x[:1], w, eps=0.0).isnan()).all()                # (0 / 0)
 
 
-@pytest.mark.parametrize("rows,cols", [(0, 64), (1, 1), (1, 300), (7, 513), (8, 1024), (600, 1000), (1025, 2048), (37, 1999), (1500, 4096), (130, 4100), (515, 8192), (20, 8200), (5, 16384), (5000, 256)])
+@pytest.mark.parametrize("rows,cols", [(0, 64), (1, 1), (1, 300), (7, 513), (8, 1024), (600, 1000), (1025, 2048), (37, 1999), (1500, 4096), (130, 4100), (515, 8192), (20, 8200), (5, 16384), (5000, 256), (2050, 2100), (2049, 4100), (300, 16000)])
 @pytest.mark.parametrize("dtype,stype,wtype", [(BF16, BF16, BF16), (BF16, F32, F32), (F16, F16, F32), (F16, F32, F16), (F32, F32, F32)])
 @pytest.mark.parametrize("more", [False, True])
 def test_norm_backward(rows, cols, dtype, stype, wtype, more):
@@ -401,7 +402,8 @@ def plain_sort(choice, experts):
 
 
 SORTS = [(0, 2, 5), (1, 1, 1), (1, 8, 64), (63, 1, 7), (64, 1, 7), (65, 2, 8), (300, 3, 60), (1024, 1, 256), (1025, 7, 255), (4096, 2, 256), (4097, 2, 257), (8192, 1, 128), (8193, 1, 128),
-         (9000, 4, 1024), (16384, 8, 128), (40000, 8, 160), (300001, 1, 31), (70000, 6, 1000)]
+         (9000, 4, 1024), (16384, 8, 128), (40000, 8, 160), (300001, 1, 31), (70000, 6, 1000), (600001, 1, 8), (1200003, 1, 5),
+         (150000, 8, 64)]
 
 
 @pytest.mark.parametrize("tokens,top,experts", SORTS)
@@ -520,6 +522,24 @@ def test_rows_past_4_gib():
     dy, dshare = ops.gather_rows_backward(x, rows, back, share)
     assert torch.equal(dy[-8:], (rows[-8:].float() * 0.25).to(BF16)) and not dy[-12:-8].any()
     near(dshare[-2:], (x[-2:].double() ** 2).sum(1, keepdim=True).expand(-1, top), (cols + 1) * u * (x[-2:].double() ** 2).sum(1, keepdim=True))
+    del rows, dy
+    q, scale = ops.quantize_fp8(x)
+    many = torch.arange(tokens * 8, dtype=torch.int32, device=DEV).view(tokens, 8)
+    rows, scales = ops.spread_rows(q, many, scale)
+    assert torch.equal(bits(rows[-8:]), bits(q[-1:]).expand(8, -1)) and torch.equal(scales[:, -8:], scale[:, -1:].expand(-1, 8))
+
+
+def test_logits_past_4_gib():
+    tokens, experts = 4_200_000, 260
+    g = gen(12)
+    logits = torch.zeros((tokens, experts), device=DEV)
+    logits[-5:] = randn(g, 5, experts)
+    choice, share = ops.route(logits, 4, renormalize=False)
+    want = ops.route(logits[-5:], 4, renormalize=False)
+    assert torch.equal(choice[-5:], want[0]) and torch.equal(share[-5:], want[1]) and torch.equal(choice[:3].cpu(), torch.arange(4, dtype=torch.int32).expand(3, 4))
+    dshare = randn(g, tokens, 4)
+    got = ops.route_backward(dshare, logits, choice, renormalize=False)
+    assert torch.equal(got[-5:], ops.route_backward(dshare[-5:], logits[-5:], want[0], renormalize=False))
 
 
 # ---- together, on streams, in graphs ----------------------------------------------------------------------------------------------------
@@ -579,6 +599,21 @@ def test_behind_their_stream():
         got = [t.clone() for t in e.run()]
     side.synchronize()
     assert same(got, want)
+
+
+def test_calls_on_two_streams_at_once():
+    a, b = Everything(25), Everything(26)
+    want = [[t.clone() for t in e.run()] for e in (a, b)]
+    torch.cuda.synchronize()
+    sides = [torch.cuda.Stream() for _ in range(2)]
+    got = [[], []]
+    for _ in range(5):
+        for i, (e, side) in enumerate(zip((a, b), sides)):
+            with torch.cuda.stream(side):
+                got[i].append(e.run())
+    torch.cuda.synchronize()
+    for runs, w in zip(got, want):
+        assert all(same(r, w) for r in runs)
 
 
 def test_two_graphs_replayed_in_turn():
@@ -653,7 +688,7 @@ def test_the_compiled_call_and_the_python_path_answer_alike(monkeypatch):
                       (t, (logits, 4, "softmax", bias.half()), {}), (t, (logits, 4), {"groups": 3}), (t, (logits, 4), {"groups": 8, "top_groups": 1}), (t, (logits, 4), {"group_top": 3}),
                       (t, (logits, 4), {"scale": float("nan")}), (t, (torch.zeros((2, 1025), device=DEV), 4), {}), (tb, (share, logits, choice.long()), {}),
                       (tb, (share[:, 1:], logits, choice), {}), (s, (choice, 0), {}), (s, (choice, 1025), {}), (s, (choice.short(), 16), {}), (p, (x, back[1:]), {}),
-                      (p, (x, back.cpu()), {}), (p, (x, back[:, :0]), {}), (c, (rows[1:], back), {}), (c, (rows, back, share.half()), {}), (cb, (x, rows, back, None), {}),
+                      (p, (x, back.cpu()), {}), (p, (x, back, scale), {}), (p, (x, back[:, :0]), {}), (c, (rows[1:], back), {}), (c, (rows, back, share.half()), {}), (cb, (x, rows, back, None), {}),
                       (cb, (x.float(), rows, back, share), {})):
         assert not alike(fn, *a, **kw), (fn.__name__, kw)
 

@@ -91,6 +91,7 @@ def test_rows_refuse():
     refuses("back must be", p, x, choice.long())
     refuses("back has 4 rows", p, x, choice[1:])
     refuses("scale must have shape", p, x.to(F8), choice, torch.zeros((5, 3)))
+    refuses("x with scale must be", p, x, choice, torch.zeros((3, 5)))
     refuses("out_scale without scale", p, x, choice, out_scale=torch.zeros((3, 10)))
     refuses("out_scale must have shape", p, x.to(F8), choice, torch.zeros((3, 5)), out_scale=torch.zeros((3, 5)))
     refuses("out must have shape", p, x, choice, out=x)
@@ -180,6 +181,7 @@ def test_c_abi_refuses():
     says("choices each", p, 16, None, 16, 16, None, 1 << 30, 2, 8, 2)
     says("scale and outScale", p, 16, 16, 16, 16, None, 4, 2, 8, 1)
     says("non-NULL", p, 16, None, None, 16, None, 4, 2, 8, 1)
+    says("values of 1 byte", p, 16, 16, 16, 16, 16, 4, 2, 8, 2)
     says("more than one launch holds", p, 16, None, 16, 16, None, 1 << 30, 1, 1 << 21, 2)
     says("dataType", g, 16, 16, None, 16, 4, 2, 8, L.INT8)
     says("non-NULL", g, 16, None, None, 16, 4, 2, 8, L.BF16)
