@@ -50,7 +50,7 @@ def build(verbose=False, extra=(), jobs=8):
                "-D_GLIBCXX_USE_CXX11_ABI=%d" % torch._C._GLIBCXX_USE_CXX11_ABI, "-I", os.path.join(ROOT, "include"),
                "-I", os.path.join(os.environ.get("ROCM_PATH", "/opt/rocm"), "include"), "-I", os.path.join(t, "include"),
                "-I", os.path.join(t, "include", "torch", "csrc", "api", "include"), "-I", sysconfig.get_paths()["include"],
-               os.path.join(PKG, "csrc", "host_call.cpp"), "-o", HOST_CALL, "-L", os.path.join(t, "lib"), "-lc10", "-lc10_hip", "-ltorch_cpu", "-ltorch_python"]
+               os.path.join(PKG, "csrc", "host_call.cpp"), "-o", HOST_CALL, "-L", os.path.join(t, "lib"), "-lc10", "-lc10_hip", "-ltorch_cpu", "-ltorch_hip", "-ltorch_python"]
         if verbose:
             print(" ".join(cmd), flush=True)
         r = subprocess.run(cmd, capture_output=True, text=True)

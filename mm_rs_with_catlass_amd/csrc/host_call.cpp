@@ -7,7 +7,7 @@
 // that path, which also says what is wrong.
 #include <Python.h>
 
-#include <ATen/ops/empty.h>
+#include <ATen/hip/EmptyTensor.h>
 #include <c10/hip/HIPFunctions.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/Dtype.h>
@@ -82,6 +82,12 @@ const at::Tensor &tensor(PyObject *o, at::ScalarType type, int64_t dims, int64_t
 }
 
 uint8_t *address(const at::Tensor &t) { return (uint8_t *)t.mutable_data_ptr(); }
+
+// A new tensor, made without the dispatcher's two turns (0.25 us of a call's 4 to 6.4 for each output).
+at::Tensor fresh(at::IntArrayRef shape, at::ScalarType type, const at::Tensor &like)
+{
+    return at::Tensor(at::detail::empty_cuda(shape, type, like.device(), std::nullopt));
+}
 
 uint8_t *optional(PyObject *o, at::ScalarType type, int64_t dims, int64_t atLeast) { return o == Py_None ? nullptr : address(tensor(o, type, dims, atLeast)); }
 
@@ -202,7 +208,7 @@ PyObject *launch(PyObject *const *v)
             type = ((THPDtype *)v[OUT_DTYPE])->scalar_type;
             if (type != at::kHalf && type != at::kBFloat16) throw Other{};
         }
-        made = at::empty({rows, n}, a.options().dtype(type));
+        made = fresh({rows, n}, type, a);
     }
     uint8_t *const pa = address(a), *const pb = address(b), *const po = address(*out);
     const uint32_t outType = out->scalar_type() == at::kHalf ? FP16 : BF16;
@@ -271,7 +277,7 @@ struct Result {
     Result(PyObject *o, at::ScalarType type, at::IntArrayRef shape, const at::Tensor &like)
     {
         if (o == Py_None) {
-            made = at::empty(shape, like.options().dtype(type));
+            made = fresh(shape, type, like);
             return;
         }
         t = &tensor(o, type, (int64_t)shape.size());
@@ -616,7 +622,7 @@ PyObject *normBackward(PyObject *, PyObject *const *v, Py_ssize_t n)   // dy, x,
         here.check(dx);
         here.check(dw);
         const uint64_t bytes = rmsNormWorkspace((uint32_t)rows, (uint32_t)cols);
-        const at::Tensor work = at::empty({(int64_t)bytes}, x.options().dtype(at::kByte));
+        const at::Tensor work = fresh({(int64_t)bytes}, at::kByte, x);
         uint8_t *const pd = address(dy), *const px = address(x), *const pw = address(weight), *const pdx = dx.at_(), *const pdw = dw.at_(), *const pwork = address(work);
         void *const s = stream();
         Py_BEGIN_ALLOW_THREADS
@@ -702,7 +708,7 @@ PyObject *sortChoices(PyObject *, PyObject *const *v, Py_ssize_t n)   // choice,
         here.check(ends);
         const uint64_t bytes = sortWorkspace((uint32_t)rows, (uint32_t)experts);
         at::Tensor work;
-        if (bytes) work = at::empty({(int64_t)bytes}, choice.options().dtype(at::kByte));
+        if (bytes) work = fresh({(int64_t)bytes}, at::kByte, choice);
         uint8_t *const pc = address(choice), *const pwork = bytes ? address(work) : nullptr;
         int32_t *const po = (int32_t *)order.at_(), *const pb = (int32_t *)back.at_(), *const pe = (int32_t *)ends.at_();
         void *const s = stream();

@@ -693,6 +693,16 @@ def test_the_compiled_call_and_the_python_path_answer_alike(monkeypatch):
         assert not alike(fn, *a, **kw), (fn.__name__, kw)
 
 
+def test_results_are_those_of_their_mode():
+    x, w = randn(gen(32), 4, 256, dtype=BF16), torch.ones(256, dtype=BF16, device=DEV)
+    with torch.inference_mode():
+        got = [ops.rms_norm(x, w), *ops.quantize_fp8(x), *ops.route(x, 2)]
+        assert all(t.is_inference() and not t.requires_grad for t in got)
+    got = [ops.rms_norm(x, w), *ops.quantize_fp8(x), *ops.route(x, 2)]
+    assert not any(t.is_inference() or t.requires_grad for t in got) and all(t.device == x.device and t.is_contiguous() for t in got)
+    assert got[0].clone().requires_grad_().sum().backward() is None
+
+
 def test_launches_of_more_rows_than_one_dimension_holds():
     """2^24 rows of 256 threads: workgroups go on in the launch's second dimension."""
     rows = 2 ** 24 + 5
