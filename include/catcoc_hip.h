@@ -374,7 +374,7 @@ CATCOC_API void catcoc_route_backward(void *stream, const float *dshare, const v
 
 /* The plan of the choices [rows] (of choiceBits 32 or 64): order lists the rows by expert, in ascending order within one, those outside [0, experts) (at most 1024) behind
  * the last; back[i] is where row i went; ends[e] is one past expert e's last place, group ends of the grouped products.  workspace:
- * catcoc_sort_by_expert_workspace_size() bytes, of any content. */
+ * catcoc_sort_by_expert_workspace_size() bytes, of any content.  No output of this call or of the three below lies in the memory of the rows or choices it is made from. */
 CATCOC_API uint64_t catcoc_sort_by_expert_workspace_size(uint32_t rows, uint32_t experts);
 CATCOC_API void catcoc_sort_by_expert(void *stream, const void *choice, int32_t *order, int32_t *back, int32_t *ends, void *workspace, uint64_t workspaceBytes,
                                       uint32_t rows, uint32_t experts, uint32_t choiceBits);

@@ -60,6 +60,14 @@ int check_rows(uint32_t tokens, uint32_t top, uint32_t cols)
     return 0;
 }
 
+// Other waves read what this one writes: their memory must not be the same.
+int check_apart(const char *out, const void *a, uint64_t aBytes, const char *in, const void *b, uint64_t bBytes)
+{
+    const uintptr_t x = (uintptr_t)a, y = (uintptr_t)b;
+    if (aBytes && bBytes && x < y + bBytes && y < x + aBytes) return api_fail(E_SHAPE, "%s lies in the memory of %s", out, in);
+    return 0;
+}
+
 // The most workgroups that a launch can have: a wave for each KiB of a row.
 int check_pieces(uint32_t tokens, uint64_t rowBytes)
 {
@@ -178,6 +186,10 @@ void catcoc_sort_by_expert(void *stream, const void *choice, int32_t *order, int
         return;
     }
     if ((uintptr_t)workspace % 4 != 0) { api_fail(E_WORKSPACE, "workspace must be 4-byte aligned"); return; }
+    const uint64_t choiceBytes = (uint64_t)rows * (choiceBits / 8u);
+    if (check_apart("order", order, rows * 4ull, "choice", choice, choiceBytes) || check_apart("back", back, rows * 4ull, "choice", choice, choiceBytes) ||
+        check_apart("ends", ends, experts * 4ull, "choice", choice, choiceBytes))
+        return;
     SortArgs a{};
     a.choice = choice;
     a.order = order;
@@ -198,6 +210,8 @@ void catcoc_spread_rows(void *stream, const void *x, const float *scale, const i
     if (!scale != !outScale) { api_fail(E_NULL, "scale and outScale come together"); return; }
     if (scale && valueBytes != 1) { api_fail(E_DTYPE, "scales come with values of 1 byte (got %u)", valueBytes); return; }
     if (!x || !back || !out) { api_fail(E_NULL, "x, back and out must be non-NULL"); return; }
+    if (check_apart("out", out, (uint64_t)tokens * top * cols * valueBytes, "x", x, (uint64_t)tokens * cols * valueBytes)) return;
+    if (scale && check_apart("outScale", outScale, (uint64_t)tokens * top * ((cols + 127u) / 128u) * 4u, "scale", scale, (uint64_t)tokens * ((cols + 127u) / 128u) * 4u)) return;
     RowsArgs a{};
     a.x = x;
     a.scale = scale;
@@ -217,6 +231,7 @@ void catcoc_gather_rows(void *stream, const void *y, const int32_t *back, const 
     if (check_rows(tokens, top, cols) || check_pieces(tokens, cols * 2ull)) return;
     if (tokens == 0) { api_launched(0); return; }
     if (!y || !back || !out) { api_fail(E_NULL, "y, back and out must be non-NULL"); return; }
+    if (check_apart("out", out, (uint64_t)tokens * cols * (dataType ? 2u : 4u), "y", y, (uint64_t)tokens * top * cols * (dataType ? 2u : 4u))) return;
     RowsArgs a{};
     a.y = y;
     a.back = back;
@@ -235,6 +250,7 @@ void catcoc_gather_rows_backward(void *stream, const void *dout, const void *y, 
     if (check_rows(tokens, top, cols) || check_pieces(tokens, 1024)) return;
     if (tokens == 0) { api_launched(0); return; }
     if (!dout || !y || !back || !share || !dy || !dshare) { api_fail(E_NULL, "dout, y, back, share, dy and dshare must be non-NULL"); return; }
+    if (check_apart("dy", dy, (uint64_t)tokens * top * cols * (dataType ? 2u : 4u), "dout", dout, (uint64_t)tokens * cols * (dataType ? 2u : 4u))) return;
     RowsArgs a{};
     a.x = dout;
     a.y = y;

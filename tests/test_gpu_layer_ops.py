@@ -509,6 +509,19 @@ def test_places_outside_the_rows_are_left_out():
     assert torch.equal(dy, want) and dshare[0, 1] == 0 and not dshare[2].any() and dshare.isfinite().all()
 
 
+def test_outputs_on_their_rows_are_refused():
+    g = gen(17)
+    choice = torch.randint(0, 5, (40, 1), device=DEV, dtype=torch.int32, generator=g)
+    x, back = randn(g, 40, 64, dtype=BF16), torch.randperm(40, device=DEV, generator=g).int()[:, None].contiguous()
+    kept = choice.clone(), x.clone()
+    for match, fn, a, kw in [("back lies", ops.sort_by_expert, (choice, 5), {"back": choice}), ("order lies", ops.sort_by_expert, (choice, 5), {"order": choice.view(-1)}),
+                             ("out lies", ops.spread_rows, (x, back), {"out": x}), ("out lies", ops.gather_rows, (x, back), {"out": x}),
+                             ("dy lies", ops.gather_rows_backward, (x, x.clone(), back, torch.ones(40, 1, device=DEV)), {"dy": x})]:
+        with pytest.raises(L.CatcocError, match=match):
+            fn(*a, **kw)
+    assert torch.equal(choice, kept[0]) and torch.equal(x, kept[1])
+
+
 def test_rows_past_4_gib():
     tokens, top, cols = 70000, 4, 8192
     g = gen(11)

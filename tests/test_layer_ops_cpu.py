@@ -187,6 +187,18 @@ def test_c_abi_refuses():
     says("non-NULL", g, 16, None, None, 16, 4, 2, 8, L.BF16)
     says("dataType", gb, 16, 16, 16, 16, 16, 16, 4, 2, 8, L.INT8)
     says("non-NULL", gb, 16, 16, 16, None, 16, 16, 4, 2, 8, L.BF16)
+    # outputs in the memory of what other waves still read: the last and the first value of an overlap
+    for shift in (0, 399, -399):
+        says("order lies in the memory of choice", s, 4096, 4096 + shift, 8192, 16384, None, 0, 100, 8, 32)
+        says("back lies in the memory of choice", s, 4096, 8192, 4096 + shift, 16384, None, 0, 100, 8, 32)
+    says("back lies in the memory of choice", s, 4096, 8192, 4096 + 799, 16384, None, 0, 100, 8, 64)
+    says("ends lies in the memory of choice", s, 4096, 8192, 16384, 4096 - 31, None, 0, 100, 8, 32)
+    says("out lies in the memory of x", p, 4096, None, 16, 4096 + 63, None, 4, 2, 8, 2)
+    says("out lies in the memory of x", p, 4096, None, 16, 4096 - 127, None, 4, 2, 8, 2)
+    says("outScale lies in the memory of scale", p, 4096, 16384, 16, 8192, 16384, 4, 2, 8, 1)
+    says("out lies in the memory of y", g, 4096, 16, None, 4096 + 127, 4, 2, 8, L.BF16)
+    says("out lies in the memory of y", g, 4096, 16, None, 4096 - 127, 4, 2, 8, 0)
+    says("dy lies in the memory of dout", gb, 4096, 8192, 16, 16, 4096 - 127, 16, 4, 2, 8, L.BF16)
     # nothing to do: accepted, nothing launched
     for fn, a in ((n, (None, None, None, 16, None, None, None, 0, 128, 1e-6, 0, 0, 0)), (r, (None, None, None, None, how(), 0, 8, 2, 0)),
                   (p, (None, None, None, None, None, 0, 2, 8, 2)), (g, (None, None, None, None, 0, 2, 8, 0)), (gb, (None,) * 6 + (0, 2, 8, 0))):
