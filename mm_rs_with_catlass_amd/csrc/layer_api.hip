@@ -13,6 +13,7 @@ int launch_norm_backward(uint32_t type, bool wide, const NormBackwardArgs &a, vo
 bool can_route(uint32_t experts, uint32_t top, uint32_t groups);
 int launch_route(const RouteArgs &a, void *stream);
 int launch_route_backward(const RouteArgs &a, void *stream);
+bool sort_counts_first(uint32_t rows, uint32_t experts);
 uint32_t sort_blocks(uint32_t rows, uint32_t experts);
 int launch_sort(uint32_t choiceBits, SortArgs a, void *stream);
 int launch_spread_rows(uint32_t valueBytes, const RowsArgs &a, void *stream);
@@ -169,8 +170,7 @@ void catcoc_route_backward(void *stream, const float *dshare, const void *logits
 
 uint64_t catcoc_sort_by_expert_workspace_size(uint32_t rows, uint32_t experts)
 {
-    const uint32_t blocks = sort_blocks(rows, experts);
-    return blocks > 1 ? (uint64_t)blocks * experts * 4u : 0u;
+    return sort_counts_first(rows, experts) ? (uint64_t)sort_blocks(rows, experts) * experts * 4u : 0u;
 }
 
 void catcoc_sort_by_expert(void *stream, const void *choice, int32_t *order, int32_t *back, int32_t *ends, void *workspace, uint64_t workspaceBytes, uint32_t rows,

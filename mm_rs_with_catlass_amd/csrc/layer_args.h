@@ -48,7 +48,7 @@ struct RouteArgs {
 struct SortArgs {
     const void *choice;          // [rows], 32 or 64 bits
     int32_t *order, *back, *ends;
-    uint32_t *part;              // [blocks, experts] how many rows of a block go to each expert; NULL: one block
+    uint32_t *part;              // [blocks, experts] how many rows of a block go to each expert; NULL: each block counts for itself
     uint32_t rows, experts, blocks, perBlock;
 };
 

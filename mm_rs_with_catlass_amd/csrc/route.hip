@@ -499,8 +499,8 @@ int launch_route_backward(const RouteArgs &a, void *stream) { return launch_rout
 
 // ---- rows by expert -----------------------------------------------------------------------------------------------------------------------
 // A counting sort, stable: a wave counts how many of its consecutive rows go to each expert, the counts' sums over waves, blocks and experts are where its first
-// row of each goes, and the rows follow in 64s, a row's place among them by how many lanes before it have the same expert.  Latencies bound it: 256 rows 3.3 us, 131072 rows to 128
-// experts 9.2 (two launches of 2.9 and 6.5; the bytes would take 0.3).
+// row of each goes, and the rows follow in 64s, a row's place among them by how many lanes before it have the same expert.  Latencies bound it: 256 rows 3.4 us, 8192 to 128
+// experts 5.4, 131072 9.2 (two launches of 2.9 and 6.5; the bytes would take 0.3).
 
 namespace {
 
@@ -535,6 +535,20 @@ __device__ __forceinline__ void count_rows(const SortArgs &args, uint32_t (&coun
             if (expert[i] != kNoRow) atomicAdd(&mine[expert[i]], 1u);
     }
     __syncthreads();
+}
+
+// How many of the rows [begin, end) go to each expert, added to `hist`.
+template <typename I>
+__device__ __forceinline__ void count_others(const SortArgs &args, uint32_t *hist, uint32_t begin, uint32_t end)
+{
+#pragma unroll 4
+    for (uint32_t first = begin + (threadIdx.x >> 6) * 64u * kSortTurns; first < end; first += kSortThreads * kSortTurns) {
+        uint32_t expert[kSortTurns];
+        load_experts<I>(args, first, end, expert);
+#pragma unroll
+        for (uint32_t i = 0; i < kSortTurns; ++i)
+            if (expert[i] < args.experts) atomicAdd(&hist[expert[i]], 1u);
+    }
 }
 
 __device__ __forceinline__ void wave_rows(const SortArgs &args, uint32_t &begin, uint32_t &end)
@@ -588,6 +602,12 @@ __global__ void __launch_bounds__(kSortThreads) sort_by_expert_kernel(const Sort
         }
         totals[threadIdx.x] = all;
         before[threadIdx.x] = some;
+    } else if (args.blocks > 1u) {
+        totals[threadIdx.x] = before[threadIdx.x] = 0;
+        __syncthreads();
+        const uint32_t from = blockIdx.x * args.perBlock, to = from + args.perBlock;   // (of few rows)
+        count_others<I>(args, before, 0u, from);
+        count_others<I>(args, totals, to, args.rows);
     }
     count_rows<I, MOST>(args, count, begin, end, expert);
     if (threadIdx.x < args.experts) {
@@ -597,6 +617,10 @@ __global__ void __launch_bounds__(kSortThreads) sort_by_expert_kernel(const Sort
                 those += before[i];
             }
         } else {
+            if (args.blocks > 1u) {
+                those = before[threadIdx.x];
+                n = those + totals[threadIdx.x];
+            }
 #pragma unroll
             for (uint32_t w = 0; w < kSortWaves; ++w) n += count[w][threadIdx.x];
         }
@@ -655,23 +679,26 @@ __global__ void __launch_bounds__(kSortThreads) sort_by_expert_kernel(const Sort
     }
 }
 
-// Blocks of a sort.  Up to 4096 rows one, which needs no counts of others (us, 128 experts, one launch / two: 2048 rows 5.0 / 7.1, 4096 6.3 / 7.4, 8192 9.7 / 7.5); then
-// of 1024 rows or more, as every block sums all blocks' counts (blocks of 1024 / 2048 / 4096: 16384 rows to 128 experts 7.8 / 8.1 / 9.1, 131072 to 128 10.5 / 9.6 / 10.2, 131072 to
-// 1024 31 / 21 / 19).
-constexpr uint32_t kSortAlone = 4096, kSortBlock = 1024, kMostSortBlocks = 256;
+// Blocks of a sort.  Up to 32768 rows of 1024 each, in one launch, every block counting the others' rows itself (us, one launch / two, 128 experts: 4096 rows 5.0 / 7.0, 16384 6.0 /
+// 7.5, 32768 7.5 / 7.9, 49152 9.1 / 8.3; half as many rows where few experts share LDS's atomics, 16 of them: 16384 6.5 / 7.1, 32768 9.0 / 7.4, 32 of them: 32768 7.5 / 7.4; and a second launch is 3 us on the
+// host); then of 1024 rows or more, whose counts come from a first launch and are summed by every block (blocks of 1024 / 2048 / 4096: 131072 rows to 128
+// experts 10.5 / 9.6 / 10.2, to 1024 31 / 21 / 19).
+constexpr uint32_t kSortRecount = 32768, kSortBlock = 1024, kMostSortBlocks = 256;
+
+bool sort_counts_first(uint32_t rows, uint32_t experts) { return rows > (experts < 32 ? kSortRecount / 2 : kSortRecount); }
 
 uint32_t sort_blocks(uint32_t rows, uint32_t experts)
 {
-    if (rows <= kSortAlone) return 1;
     const uint64_t counts = (uint64_t)rows * experts;
-    const uint32_t block = kSortBlock << (counts > (1u << 25) ? 2 : counts > (1u << 22) ? 1 : 0), blocks = rows / block + (rows % block != 0);
-    return blocks < kMostSortBlocks ? blocks : kMostSortBlocks;
+    const uint32_t block = kSortBlock << (!sort_counts_first(rows, experts) ? 0 : counts > (1u << 25) ? 2 : counts > (1u << 22) ? 1 : 0);
+    const uint32_t blocks = rows / block + (rows % block != 0);
+    return rows == 0 ? 1 : blocks < kMostSortBlocks ? blocks : kMostSortBlocks;
 }
 
 template <typename I, uint32_t MOST>
 static int launch_sort_type(const SortArgs &a, hipStream_t stream)
 {
-    if (a.blocks > 1) {
+    if (a.part != nullptr) {
         hipLaunchKernelGGL((count_by_expert_kernel<I, MOST>), dim3(a.blocks), dim3(kSortThreads), 0, stream, a);
         const int e = (int)hipGetLastError();
         if (e) return e;
@@ -685,7 +712,7 @@ int launch_sort(uint32_t choiceBits, SortArgs a, void *stream)
     a.blocks = sort_blocks(a.rows, a.experts);
     const uint64_t each = (a.rows + (uint64_t)a.blocks - 1u) / a.blocks;
     a.perBlock = (uint32_t)((each + kSortBlock - 1u) / kSortBlock * kSortBlock);
-    if (a.blocks == 1) a.part = nullptr;
+    if (!sort_counts_first(a.rows, a.experts)) a.part = nullptr;
     if (choiceBits == 32) return a.experts <= 256 ? launch_sort_type<int32_t, 256>(a, (hipStream_t)stream) : launch_sort_type<int32_t, 1024>(a, (hipStream_t)stream);
     return a.experts <= 256 ? launch_sort_type<int64_t, 256>(a, (hipStream_t)stream) : launch_sort_type<int64_t, 1024>(a, (hipStream_t)stream);
 }

@@ -402,7 +402,7 @@ def plain_sort(choice, experts):
 
 
 SORTS = [(0, 2, 5), (1, 1, 1), (1, 8, 64), (63, 1, 7), (64, 1, 7), (65, 2, 8), (300, 3, 60), (1024, 1, 256), (1025, 7, 255), (4096, 2, 256), (4097, 2, 257), (8192, 1, 128), (8193, 1, 128),
-         (9000, 4, 1024), (16384, 8, 128), (40000, 8, 160), (300001, 1, 31), (70000, 6, 1000), (600001, 1, 8), (1200003, 1, 5),
+         (9000, 4, 1024), (16384, 8, 128), (40000, 8, 160), (300001, 1, 31), (70000, 6, 1000), (600001, 1, 8), (1200003, 1, 5), (16384, 1, 9), (16385, 1, 9), (4096, 8, 100), (4097, 8, 100), (5000, 3, 3),
          (150000, 8, 64)]
 
 
@@ -565,7 +565,7 @@ class Everything:
         self.tokens, self.cols, self.experts, self.top = 300, 1100, 24, 3
         self.x, self.r, self.w = stream(g, self.tokens, self.cols, BF16), stream(g, self.tokens, self.cols, F32), 1 + 0.1 * randn(g, self.cols)
         self.logits, self.bias = randn(g, self.tokens, self.experts), 0.1 * randn(g, self.experts)
-        self.many = torch.randint(-1, 200, (5000, 4), device=DEV, generator=g)
+        self.many = torch.randint(-1, 200, (9000, 4), device=DEV, generator=g)
 
     def inputs(self):
         return [self.x, self.r, self.w, self.logits, self.bias, self.many]
@@ -662,7 +662,7 @@ class Nothing:
 def test_the_compiled_call_and_the_python_path_answer_alike(monkeypatch):
     g = gen(31)
     x, w, r = stream(g, 20, 300, BF16), randn(g, 300, dtype=BF16), stream(g, 20, 300, F32)
-    logits, bias, many = randn(g, 20, 16), randn(g, 16), torch.randint(0, 9, (5000, 2), device=DEV, generator=g)
+    logits, bias, many = randn(g, 20, 16), randn(g, 16), torch.randint(0, 9, (9000, 2), device=DEV, generator=g)
     choice, share = ops.route(logits, 4)
     order, back, ends = ops.sort_by_expert(choice, 16)
     rows, (q, scale) = ops.spread_rows(x, back), ops.quantize_fp8(x)
