@@ -224,9 +224,9 @@ __global__ void __launch_bounds__(256, LANES == 16 ? 4 : V <= 16 ? 3 : 2) route_
     double k[V];
     float total = 0.f;   // of the softmax
     if (args.bias != nullptr || args.groupTop == 2) {
-        bool odd = false;   // NaN, or not to be had
+        bool odd = false;   // NaN, infinite, or not to be had
 #pragma unroll
-        for (int i = 0; i < V; ++i) odd |= !(v[i] > -__builtin_huge_valf());
+        for (int i = 0; i < V; ++i) odd |= !(__builtin_fabsf(v[i]) < __builtin_huge_valf());
         double r = 1.0;
         if (args.sigmoid) {
 #pragma unroll
@@ -255,7 +255,7 @@ __global__ void __launch_bounds__(256, LANES == 16 ? 4 : V <= 16 ? 3 : 2) route_
         for (int i = 0; i < V; ++i) k[i] = __builtin_fma(k[i], r, (double)b[i]);
         if (__any(odd)) {
 #pragma unroll
-            for (int i = 0; i < V; ++i) k[i] = v[i] > -__builtin_huge_valf() ? k[i] : (double)v[i];
+            for (int i = 0; i < V; ++i) k[i] = b[i] == -__builtin_huge_valf() ? kNone : v[i] > -__builtin_huge_valf() ? k[i] : (double)v[i];   // (a bias masks a score that is NaN)
         }
     } else {
         if (!args.sigmoid && !args.renormalize) {

@@ -730,3 +730,31 @@ def test_launches_of_more_rows_than_one_dimension_holds():
     assert torch.equal(ops.gather_rows(x, back)[-6:], last)
     dy, dshare = ops.gather_rows_backward(x, x, back, torch.ones((rows, 1), device=DEV))
     assert torch.equal(dy[-6:], last) and not dshare[:-6].any()
+
+
+@pytest.mark.parametrize("experts,top,how", [(12, 8, {}), (60, 8, {}), (256, 8, {}), (300, 20, {}), (1024, 8, {}), (64, 6, dict(groups=8, top_groups=4, group_top=2)),
+                                             (256, 8, dict(groups=8, top_groups=4))])
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("renormalize", [False, True])
+def test_biases_mask_rows_that_are_not_finite_too(experts, top, how, score, renormalize):
+    """A bias of -inf stands whatever a row's logits are: NaN or infinite ones, its own among them, and those that make every score of a softmax NaN."""
+    g = gen(experts + top)
+    logits, bias = randn(g, 9, experts), 0.1 * randn(g, experts)
+    gone = torch.arange(0, experts, 3, device=DEV)
+    bias[gone] = -float("inf")
+    nan, inf = float("nan"), float("inf")
+    logits[1, 4], logits[2, 4], logits[3, 3], logits[4, 3] = nan, inf, nan, inf     # (3 is masked, 4 is not)
+    logits[5, 3], logits[5, 4], logits[6, gone], logits[7] = nan, inf, nan, nan
+    logits[8, 1:] = -inf
+    choice, share = ops.route(logits, top, score=score, bias=bias, renormalize=renormalize, **how)
+    assert not (torch.isin(choice, gone.int())).any() and (choice[8] < 0).all() and (share[8] == 0).all()
+    want = plain_route(logits[:1], top, score, bias, renormalize=renormalize, **how)
+    assert torch.equal(choice[:1], want[0])
+    for line in choice.tolist():
+        got = [c for c in line if c >= 0]
+        assert len(set(got)) == len(got) and all(c < experts for c in got)
+    assert (share[choice < 0] == 0).all() and not share[0].isnan().any()
+    if score == "softmax":
+        assert share[1:8][choice[1:8] >= 0].isnan().all()
+    else:
+        assert (choice[1, 0] == 4 and share[1, 0].isnan() and share[3:5].isfinite().all() and share[6].isfinite().all())
