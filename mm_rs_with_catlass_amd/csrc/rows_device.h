@@ -6,18 +6,20 @@
 
 #include <type_traits>
 
+#include "launch_grid.h"
 #include "ragged_args.h"
 
 namespace catcoc {
 
 typedef int v2i __attribute__((ext_vector_type(2)));
 
-// One dimension of a launch holds fewer than 2^32 threads: workgroups past that go on in the second one, in rows of kGridRow.  Those past the last one asked for
-// have to find nothing to do.  For the checked kernel and the quantizer; in the small tiles' kernel the second index costs a call of 18.5 us 0.46 of them.
-constexpr uint32_t kGridRowLog = 22, kGridRow = 1u << kGridRowLog;
+// One dimension of a launch holds fewer than 2^32 threads: workgroups past that go on in the second one, in rows of kGridRow (launch_grid.h).  Those past the last one
+// asked for have to find nothing to do.  For the checked kernel, the quantizer, norms, router and rows; in the small tiles' kernel the second index costs a call of 18.5 us
+// 0.46 of them.
 inline dim3 grid_of(uint64_t wgs, uint32_t threads)
 {
-    return wgs * threads < (1ull << 32) ? dim3((uint32_t)wgs) : dim3(kGridRow, (uint32_t)((wgs + kGridRow - 1u) >> kGridRowLog));
+    const LaunchGrid g = launch_grid(wgs, threads);
+    return dim3(g.x, g.y);
 }
 __device__ __forceinline__ uint32_t workgroup() { return (blockIdx.y << kGridRowLog) + blockIdx.x; }
 

@@ -758,3 +758,18 @@ def test_biases_mask_rows_that_are_not_finite_too(experts, top, how, score, reno
         assert share[1:8][choice[1:8] >= 0].isnan().all()
     else:
         assert (choice[1, 0] == 4 and share[1, 0].isnan() and share[3:5].isfinite().all() and share[6].isfinite().all())
+
+
+def test_launches_of_more_long_rows_than_one_dimension_holds():
+    """2^22 rows of 1024 threads, in place (69 GB)."""
+    rows, cols = 2 ** 22 + 3, 8200
+    x = torch.zeros((rows, cols), dtype=BF16, device=DEV)
+    w = torch.ones(cols, dtype=BF16, device=DEV)
+    ends = stream(gen(34), 5, cols, BF16)
+    x[-5:], x[:5], x[2 ** 20 - 2:2 ** 20 + 3] = ends, ends, ends
+    want = ops.rms_norm(ends, w)
+    ops.rms_norm(x, w, out=x)
+    assert torch.equal(x[-5:], want) and torch.equal(x[:5], want) and torch.equal(x[2 ** 20 - 2:2 ** 20 + 3], want)
+    assert not x[5:100].any() and not x[-100:-5].any()
+    del x
+    torch.cuda.empty_cache()

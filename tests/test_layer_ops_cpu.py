@@ -226,3 +226,33 @@ def test_sizes_past_32_bits_are_refused():
     refuses("back has 4294967301 rows", ops.gather_rows, wide(far, 1), wide(far, 1, dtype=i32))
     refuses("y has 4294967301 columns", ops.gather_rows, wide(4, far), wide(4, 1, dtype=i32))
     refuses("y has 4294967301 columns", ops.gather_rows_backward, wide(4, far), wide(4, far), wide(4, 1, dtype=i32), wide(4, 1, dtype=torch.float32))
+
+
+def test_grids_hold_every_workgroup_and_fewer_than_2_32_threads_a_dimension(tmp_path):
+    """The arithmetic of launches in two dimensions, compiled for the host: every block size, from one workgroup to 2^31."""
+    import os
+    import subprocess
+    csrc = os.path.join(os.path.dirname(os.path.abspath(L.__file__)), "csrc")
+    source, program = tmp_path / "grid.cpp", tmp_path / "grid"
+    source.write_text(r"""
+#include <stdio.h>
+#include <initializer_list>
+#include "launch_grid.h"
+int main()
+{
+    for (uint32_t threads = 64; threads <= 1024; threads *= 2)
+        for (uint64_t wgs : {1ull, 4099ull, (1ull << 22) - 1, 1ull << 22, (1ull << 22) + 5, (1ull << 32) / threads - 1, (1ull << 32) / threads, (1ull << 32) / threads + 1, 1ull << 29, 1ull << 30, 1ull << 31}) {
+            const catcoc::LaunchGrid g = catcoc::launch_grid(wgs, threads);
+            printf("%u %llu %u %u\n", threads, (unsigned long long)wgs, g.x, g.y);
+        }
+}
+""")
+    subprocess.run([os.environ.get("CXX", "g++"), "-std=c++17", "-I", csrc, str(source), "-o", str(program)], check=True)
+    lines = subprocess.run([str(program)], check=True, capture_output=True, text=True).stdout.split("\n")[:-1]
+    assert len(lines) == 5 * 11
+    for line in lines:
+        threads, wgs, x, y = map(int, line.split())
+        assert 0 < x * threads < 2 ** 32 and 0 < y <= 65535 and x * y >= wgs and (y == 1 or x * (y - 1) < wgs), line
+        assert y == 1 or x & (x - 1) == 0
+        if wgs * threads < 2 ** 32:
+            assert (x, y) == (wgs, 1)
