@@ -120,3 +120,39 @@ def test_leaves_the_others_to_the_python_path(op, name, monkeypatch):
             assert a == b
         else:
             assert all(torch.equal(x, y) for x, y in zip(a, b))
+
+
+def test_outputs_are_made_as_torch_makes_them(monkeypatch):
+    """Compiled calls and the Python path: torch's deterministic mode fills new tensors, dispatch modes see them."""
+    from torch.utils._python_dispatch import TorchDispatchMode
+
+    class Seen(TorchDispatchMode):
+        def __init__(self):
+            super().__init__()
+            self.names = []
+
+        def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+            self.names.append(func.name())
+            return func(*args, **(kwargs or {}))
+    g = torch.Generator(device="cuda:0").manual_seed(5)
+    x, w = torch.randn((6, 256), device="cuda:0", generator=g).bfloat16(), torch.ones(256, device="cuda:0", dtype=torch.bfloat16)
+    a, b = torch.randn((6, 256), device="cuda:0", generator=g).bfloat16(), torch.randn((64, 256), device="cuda:0", generator=g).bfloat16()
+    back = torch.tensor([[0, -1], [5, 3], [6, 11], [2, 2], [1, 4], [-1, 7]], dtype=torch.int32, device="cuda:0")
+    compiled = ops._host or ops._compiled()
+
+    class Python:
+        def __getattr__(self, name):
+            return lambda *args: None
+    for host in (compiled, Python()):
+        monkeypatch.setattr(ops, "_host", host)
+        torch.use_deterministic_algorithms(True)
+        try:
+            rows = ops.spread_rows(x, back)
+        finally:
+            torch.use_deterministic_algorithms(False)
+        left = [8, 9, 10]
+        assert rows[left].isnan().all() and torch.equal(rows[3], x[1])
+        for call, outputs in ((lambda: ops.quantize_fp8(x), 2), (lambda: ops.rms_norm(x, w), 1), (lambda: ops.matmul_allreduce(a, b, [], 0, 1, trans_b=True), 1)):
+            with Seen() as seen:
+                call()
+            assert sum(n.startswith("aten::empty") for n in seen.names) >= outputs, seen.names
