@@ -386,7 +386,7 @@ CATCOC_API void catcoc_spread_rows(void *stream, const void *x, const float *sca
 /* The rows back at their tokens: out[t] = sum over j of share[t,j] y[back[t,j]], in the order of j; share NULL: ones (the gradient of catcoc_spread_rows). */
 CATCOC_API void catcoc_gather_rows(void *stream, const void *y, const int32_t *back, const float *share, void *out, uint32_t tokens, uint32_t top, uint32_t cols,
                                    uint32_t dataType);
-/* Its gradients: dy[back[t,j]] = share[t,j] dout[t], dshare[t,j] = <dout[t], y[back[t,j]]> (0 for a place outside the rows). */
+/* Its gradients: dy[back[t,j]] = share[t,j] dout[t], dshare[t,j] = <dout[t], y[back[t,j]]> (0 for a place outside the rows).  dy NULL, or y and dshare NULL: not wanted. */
 CATCOC_API void catcoc_gather_rows_backward(void *stream, const void *dout, const void *y, const int32_t *back, const float *share, void *dy, float *dshare,
                                             uint32_t tokens, uint32_t top, uint32_t cols, uint32_t dataType);
 

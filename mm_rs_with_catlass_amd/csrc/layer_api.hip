@@ -249,8 +249,10 @@ void catcoc_gather_rows_backward(void *stream, const void *dout, const void *y, 
     if (!is_float(dataType)) { api_fail(E_DTYPE, "dataType %u must be 0 (fp32), FP16 or BF16", dataType); return; }
     if (check_rows(tokens, top, cols) || check_pieces(tokens, 1024)) return;
     if (tokens == 0) { api_launched(0); return; }
-    if (!dout || !y || !back || !share || !dy || !dshare) { api_fail(E_NULL, "dout, y, back, share, dy and dshare must be non-NULL"); return; }
-    if (check_apart("dy", dy, (uint64_t)tokens * top * cols * (dataType ? 2u : 4u), "dout", dout, (uint64_t)tokens * cols * (dataType ? 2u : 4u))) return;
+    if (!dout || !back || !share) { api_fail(E_NULL, "dout, back and share must be non-NULL"); return; }
+    if (!dy && !dshare) { api_fail(E_NULL, "dy or dshare must be non-NULL"); return; }
+    if (!y != !dshare) { api_fail(E_NULL, "y and dshare come together"); return; }
+    if (dy && check_apart("dy", dy, (uint64_t)tokens * top * cols * (dataType ? 2u : 4u), "dout", dout, (uint64_t)tokens * cols * (dataType ? 2u : 4u))) return;
     RowsArgs a{};
     a.x = dout;
     a.y = y;

@@ -54,13 +54,13 @@ struct SortArgs {
 
 struct RowsArgs {
     const void *x;               // [tokens, cols]; backward: the gradient that comes in
-    const void *y;               // [tokens * top, cols]
+    const void *y;               // [tokens * top, cols]; backward: NULL without dshare
     const float *scale;          // spread: [column blocks, tokens] or NULL
     const float *share;          // [tokens, top] or NULL (ones)
     const int32_t *back;         // [tokens, top]
-    void *out;                   // spread, backward: [tokens * top, cols]; gather: [tokens, cols]
+    void *out;                   // spread, backward: [tokens * top, cols], backward NULL where it is not wanted; gather: [tokens, cols]
     float *outScale;             // spread: [column blocks, tokens * top]
-    float *dshare;               // backward: [tokens, top]
+    float *dshare;               // backward: [tokens, top], NULL where it is not wanted
     uint32_t tokens, top, cols;
     uint32_t scaleWgs;           // spread: how many workgroups are the scales'
 };

@@ -140,7 +140,8 @@ __global__ void __launch_bounds__(256) gather_rows_kernel(const RowsArgs args)
 
 // T threads take a choice's row.  The choices of a token follow each other on one XCD, whose L2 then has the token's gradient for all but the first (us, with one workgroup
 // for all of a token's choices / with these: 2048 tokens of eight rows of 4096 64 / 56, 32 of them 8.6 / 3.2).
-template <uint32_t DT, int T>
+// DY, DSHARE: which of the two gradients is wanted; y is not read for dy alone.
+template <uint32_t DT, int T, bool DY, bool DSHARE>
 __global__ void __launch_bounds__(256) gather_rows_backward_kernel(const RowsArgs args)
 {
     constexpr uint32_t W = T / 64, EACH = 256 / T;
@@ -153,42 +154,44 @@ __global__ void __launch_bounds__(256) gather_rows_backward_kernel(const RowsArg
     const uint32_t at = uniform((uint32_t)args.back[i]);
     float dot = 0.f;
     if (at < rows) {
-        const float share = args.share[i];
+        const float share = DY ? args.share[i] : 0.f;
+        auto piece = [&](uint32_t col, Raw8<DT> &d, Raw8<DT> &y) {
+            d = load_raw8<DT>(args.x, token, args.cols, col, args.cols);
+            if constexpr (DSHARE) y = load_raw8<DT>(args.y, at, args.cols, col, args.cols);
+        };
+        auto done = [&](uint32_t col, const Raw8<DT> &rd, const Raw8<DT> &ry) {
+            Eight d = widen8<DT>(rd);
+            if constexpr (DSHARE) {
+                const Eight y = widen8<DT>(ry);
+#pragma unroll
+                for (int k = 0; k < 8; ++k) dot = __builtin_fmaf(d.v[k], y.v[k], dot);
+            }
+            if constexpr (DY) {
+#pragma unroll
+                for (int k = 0; k < 8; ++k) d.v[k] *= share;
+                store_raw8<DT>(args.out, at, args.cols, col, args.cols, round8<DT>(d));
+            }
+        };
         for (uint32_t col = t * 8u; col < args.cols; col += T * 16u) {
             const uint32_t next = col + T * 8u;   // (two pieces of both rows are asked for together)
-            const Raw8<DT> rd = load_raw8<DT>(args.x, token, args.cols, col, args.cols), ry = load_raw8<DT>(args.y, at, args.cols, col, args.cols);
-            Raw8<DT> rd2 = {}, ry2 = {};
-            if (next < args.cols) {
-                rd2 = load_raw8<DT>(args.x, token, args.cols, next, args.cols);
-                ry2 = load_raw8<DT>(args.y, at, args.cols, next, args.cols);
-            }
-            Eight d = widen8<DT>(rd), y = widen8<DT>(ry);
-#pragma unroll
-            for (int k = 0; k < 8; ++k) {
-                dot = __builtin_fmaf(d.v[k], y.v[k], dot);
-                d.v[k] *= share;
-            }
-            store_raw8<DT>(args.out, at, args.cols, col, args.cols, round8<DT>(d));
-            if (next < args.cols) {
-                d = widen8<DT>(rd2), y = widen8<DT>(ry2);
-#pragma unroll
-                for (int k = 0; k < 8; ++k) {
-                    dot = __builtin_fmaf(d.v[k], y.v[k], dot);
-                    d.v[k] *= share;
-                }
-                store_raw8<DT>(args.out, at, args.cols, next, args.cols, round8<DT>(d));
-            }
+            Raw8<DT> d = {}, y = {}, d2 = {}, y2 = {};
+            piece(col, d, y);
+            if (next < args.cols) piece(next, d2, y2);
+            done(col, d, y);
+            if (next < args.cols) done(next, d2, y2);
         }
     }
-    dot = wave_sum(dot);
-    if constexpr (W > 1) {
-        if ((t & 63u) == 0) parts[t >> 6] = dot;
-        __syncthreads();
-        dot = parts[0];
+    if constexpr (DSHARE) {
+        dot = wave_sum(dot);
+        if constexpr (W > 1) {
+            if ((t & 63u) == 0) parts[t >> 6] = dot;
+            __syncthreads();
+            dot = parts[0];
 #pragma unroll
-        for (uint32_t k = 1; k < W; ++k) dot += parts[k];
+            for (uint32_t k = 1; k < W; ++k) dot += parts[k];
+        }
+        if (t == 0) args.dshare[i] = dot;
     }
-    if (t == 0) args.dshare[i] = dot;
 }
 
 template <uint32_t ES>
@@ -230,9 +233,13 @@ static int launch_gather_backward_type(const RowsArgs &a, hipStream_t stream)
 {
     const uint32_t each = a.cols <= 1024 ? 4 : 1;   // tokens a workgroup
     const uint64_t wgs = (a.tokens + 8ull * each - 1) / (8ull * each) * 8 * a.top;
-    if (each == 4) hipLaunchKernelGGL((gather_rows_backward_kernel<DT, 64>), grid_of(wgs, 256), dim3(256), 0, stream, a);
-    else hipLaunchKernelGGL((gather_rows_backward_kernel<DT, 256>), grid_of(wgs, 256), dim3(256), 0, stream, a);
-    return (int)hipGetLastError();
+    auto go = [&](auto kernel) {
+        hipLaunchKernelGGL(kernel, grid_of(wgs, 256), dim3(256), 0, stream, a);
+        return (int)hipGetLastError();
+    };
+    if (a.dshare == nullptr) return each == 4 ? go(gather_rows_backward_kernel<DT, 64, true, false>) : go(gather_rows_backward_kernel<DT, 256, true, false>);
+    if (a.out == nullptr) return each == 4 ? go(gather_rows_backward_kernel<DT, 64, false, true>) : go(gather_rows_backward_kernel<DT, 256, false, true>);
+    return each == 4 ? go(gather_rows_backward_kernel<DT, 64, true, true>) : go(gather_rows_backward_kernel<DT, 256, true, true>);
 }
 
 int launch_gather_rows_backward(uint32_t type, const RowsArgs &a, void *stream)

@@ -93,11 +93,12 @@ class Spread(torch.autograd.Function):
 
 
 class Gather(torch.autograd.Function):
-    """The choices' rows summed at their tokens, by share where there is one (ops.gather_rows)."""
+    """The choices' rows summed at their tokens, by share where there is one (ops.gather_rows).  The rows are kept for the shares' gradient, where that is wanted."""
 
     @staticmethod
     def forward(ctx, y, back, share):
-        ctx.save_for_backward(y if share is not None else None, back, share)
+        ctx.save_for_backward(y if ctx.needs_input_grad[2] else None, back, share)
+        ctx.rows, ctx.dtype = ctx.needs_input_grad[0], y.dtype
         return ops.gather_rows(y.contiguous(), back, share)
 
     @staticmethod
@@ -108,8 +109,9 @@ class Gather(torch.autograd.Function):
         if torch.is_grad_enabled():     # (gradients of gradients: from operators that have them)
             d, at = Spread.apply(dout, back).float(), back.reshape(-1).long()
             sorted_share = share.new_zeros(at.numel()).index_put((at,), share.reshape(-1))
-            return (d * sorted_share.unsqueeze(-1)).to(y.dtype), None, (d * y.float()).sum(1)[at].view(share.shape)
-        dy, dshare = ops.gather_rows_backward(dout.contiguous(), y.contiguous(), back, share)
+            return ((d * sorted_share.unsqueeze(-1)).to(ctx.dtype) if ctx.rows else None, None,
+                    None if y is None else (d * y.float()).sum(1)[at].view(share.shape))
+        dy, dshare = ops.gather_rows_backward(dout.contiguous(), None if y is None else y.contiguous(), back, share, rows=ctx.rows)
         return dy, None, dshare
 
 
@@ -174,7 +176,7 @@ class RmsNorm(torch.autograd.Function):
             ds, dw = ds.to(s.dtype), (d * n).sum(0).to(weight.dtype)
         else:
             ds, dw = ops.rms_norm_backward(dy.contiguous(), s, weight, None if dsum is None else dsum.contiguous(), eps=ctx.eps)
-        return ds if ds is None else ds.to(x_type), dw, ds if residual_type is not None else None, None
+        return ds.to(x_type) if ds is not None and ctx.needs_input_grad[0] else None, dw, ds if residual_type is not None else None, None
 
 
 def rms_norm(x, weight, residual=None, eps=1e-6):

@@ -1027,29 +1027,36 @@ def gather_rows(y, back, share=None, out=None):
     return out
 
 
-def gather_rows_backward(dout, y, back, share, dy=None, dshare=None):
-    """The gradients of gather_rows() with shares (catcoc_gather_rows_backward): (dy, of y's type, dshare fp32).  Rows of dy that no choice has stay as they were."""
-    done = (_host or _compiled()).gather_rows_backward(dout, y, back, share, dy, dshare)
+def gather_rows_backward(dout, y, back, share, dy=None, dshare=None, rows=True):
+    """The gradients of gather_rows() with shares (catcoc_gather_rows_backward): (dy, of y's type, dshare fp32).  Rows of dy that no choice has stay as they were.
+
+    y None: dshare is not wanted, y is not read, and dy is of dout's type.  rows False: dy is not wanted.  What is not wanted is None."""
+    done = (_host or _compiled()).gather_rows_backward(dout, y, back, share, dy, dshare) if rows and y is not None else None
     if done is not None:
         return done
     tokens, top = _want_back(back)
-    _want(y, "y", None, 2)
-    t = _float_type(y, "y")
-    cols = y.shape[1]
-    _fits("y", columns=cols)
+    given, name = (dout, "dout") if y is None else (y, "y")
+    _want(given, name, None, 2)
+    t = _float_type(given, name)
+    cols = given.shape[1]
+    _fits(name, columns=cols)
+    if y is None and dshare is not None:
+        _fail("dshare without y")
+    if not rows and (y is None or dy is not None):
+        _fail("no gradient is wanted" if y is None else "dy without rows")
     _want(y, "y", None, 2, None, (tokens * top, cols))
-    _want(dout, "dout", y.dtype, 2, None, (tokens, cols))
+    _want(dout, "dout", given.dtype, 2, None, (tokens, cols))
     if not isinstance(share, torch.Tensor):
         _fail("share must be a tensor (got %s)", type(share).__name__)
     _want(share, "share", torch.float32, 2, None, (tokens, top))
-    _want(dy, "dy", y.dtype, 2, None, tuple(y.shape))
+    _want(dy, "dy", given.dtype, 2, None, (tokens * top, cols))
     _want(dshare, "dshare", torch.float32, 2, None, (tokens, top))
     _check_here(dout, y, back, share, dy, dshare)
-    if dy is None:
-        dy = torch.empty_like(y)
-    if dshare is None:
-        dshare = torch.empty((tokens, top), dtype=torch.float32, device=y.device)
-    _l.load().catcoc_gather_rows_backward(_stream(), dout.data_ptr(), y.data_ptr(), back.data_ptr(), share.data_ptr(), dy.data_ptr(), dshare.data_ptr(), tokens, top, cols, t)
+    if rows and dy is None:
+        dy = torch.empty((tokens * top, cols), dtype=given.dtype, device=dout.device)
+    if y is not None and dshare is None:
+        dshare = torch.empty((tokens, top), dtype=torch.float32, device=dout.device)
+    _l.load().catcoc_gather_rows_backward(_stream(), dout.data_ptr(), _ptr(y), back.data_ptr(), share.data_ptr(), _ptr(dy), _ptr(dshare), tokens, top, cols, t)
     _l.check()
     return dy, dshare
 

@@ -228,3 +228,24 @@ def test_experts_past_what_the_operators_take():
     halves = [served(x[:5], wide[:, i:i + 35], weights[:, i:i + 35]) for i in (0, 35)]
     assert not E._Plan(wide, 60).kernels
     assert ((served(x[:5], wide, weights).double() - sum(h.double() for h in halves)).abs() <= 4 * 2.0 ** -8 * sum(h.double().abs().amax() for h in halves)).all()
+
+
+def test_gathers_make_the_gradients_that_are_wanted():
+    """Rows are kept for the shares' gradient alone, and not read for the other; both as where both are wanted, first and second."""
+    from mm_rs_with_catlass_amd.experts import Gather
+    g = gen(40)
+    back = torch.randperm(24, device=DEV, generator=g).to(torch.int32).view(8, 3)
+    y, share, d = randn(g, 24, 40), randn(g, 8, 3), randn(g, 8, 40)
+    a, s = y.clone().requires_grad_(), share.clone().requires_grad_()
+    want = torch.autograd.grad(Gather.apply(a, back, s), (a, s), d)
+    for graph in (False, True):
+        out = Gather.apply(a, back, share)
+        assert out.grad_fn.saved_tensors[0] is None
+        assert torch.equal(torch.autograd.grad(out, a, d, create_graph=graph)[0], want[0])
+        out = Gather.apply(y, back, s)
+        got, = torch.autograd.grad(out, s, d, create_graph=graph)
+        # (with a graph torch adds up the dot products of 40 values in another order)
+        assert torch.equal(got, want[1]) if not graph else ((got - want[1]).abs() <= 2 * 40 * u * (d.abs()[:, None, :] * y.abs()[back.long()]).sum(2)).all()
+    at = back.long()
+    alike(lambda v: (Gather.apply(v, back, share),), lambda v: ((v[at] * share.to(v.dtype)[:, :, None]).sum(1),), [y], 41, 2.0 ** -18)
+    alike(lambda v: (Gather.apply(y, back, v),), lambda v: ((y.to(v.dtype)[at] * v[:, :, None]).sum(1),), [share], 42, 2.0 ** -18)

@@ -773,3 +773,22 @@ def test_launches_of_more_long_rows_than_one_dimension_holds():
     assert not x[5:100].any() and not x[-100:-5].any()
     del x
     torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize("tokens,top,cols", [(0, 2, 64), (1, 8, 4096), (3, 2, 7), (37, 3, 129), (9, 2, 1025), (600, 2, 1808), (5, 3, 9000)])
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+def test_one_gradient_of_gathered_rows(tokens, top, cols, dtype):
+    """What is wanted alone is what both together give; places outside the rows as there."""
+    g = gen(tokens + cols)
+    back, share = places(g, tokens, top), torch.rand((tokens, top), device=DEV, generator=g)
+    if tokens > 2:
+        back[1, 0], back[2, 1] = -1, tokens * top
+    x, y = stream(g, tokens, cols, dtype), stream(g, tokens * top, cols, dtype)
+    mark = torch.full_like(y, 3.0)
+    dy, dshare = ops.gather_rows_backward(x, y, back, share, dy=mark.clone())
+    only, none = ops.gather_rows_backward(x, None, back, share, dy=mark.clone())
+    assert none is None and torch.equal(only, dy)
+    none, only = ops.gather_rows_backward(x, y, back, share, rows=False)
+    assert none is None and torch.equal(only, dshare)
+    only, none = ops.gather_rows_backward(x, None, back, share)
+    assert only.dtype == dtype and only.shape == y.shape

@@ -256,3 +256,22 @@ int main()
         assert y == 1 or x & (x - 1) == 0
         if wgs * threads < 2 ** 32:
             assert (x, y) == (wgs, 1)
+
+
+def test_one_gradient_of_gathered_rows_refuses():
+    choice, share, x, y = torch.zeros((5, 2), dtype=torch.int32), torch.zeros((5, 2)), torch.zeros((5, 300), dtype=torch.half), torch.zeros((10, 300), dtype=torch.half)
+    b = ops.gather_rows_backward
+    refuses("dshare without y", b, x, None, choice, share, dshare=share)
+    refuses("no gradient is wanted", b, x, None, choice, share, rows=False)
+    refuses("dy without rows", b, x, y, choice, share, dy=y, rows=False)
+    refuses("dout must have shape", b, x[1:], None, choice, share)
+    refuses("dout must be float16", b, x.int(), None, choice, share)
+    refuses("dy must be", b, x, None, choice, share, dy=y.float())
+    refuses("dy must have shape", b, x, None, choice, share, dy=x)
+    refuses("must live on the GPU", b, x, None, choice, share)
+    refuses("must live on the GPU", b, x, y, choice, share, rows=False)
+    so = L.load()
+    for match, a in [("dy or dshare", (16, 16, 16, 16, None, None)), ("y and dshare come", (16, None, 16, 16, 16, 16)), ("y and dshare come", (16, 16, 16, 16, 16, None)),
+                     ("non-NULL", (None, 16, 16, 16, 16, 16)), ("non-NULL", (16, 16, None, 16, 16, 16)), ("non-NULL", (16, 16, 16, None, 16, 16))]:
+        so.catcoc_gather_rows_backward(None, *a, 4, 2, 8, L.BF16)
+        assert so.catcoc_last_status() != 0 and match in L.last_error(), L.last_error()
