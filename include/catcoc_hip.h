@@ -336,16 +336,18 @@ CATCOC_API void catcoc_grouped_fp8_matmul(void *stream, const uint8_t *x, const 
 
 /* No counterpart in the reference; beside the e4m3 and grouped operators.  Any alignment of the element type serves.  A call without rows or tokens is accepted and
  * writes nothing (dw, ends: zeros).  Sums are held in fp32 and rounded once, in an order that the sizes alone decide; nothing is added by atomics that come out in
- * another order on another run.  dataType: FP16, BF16 or 0 (fp32); other types of a call are that or 0.
+ * another order on another run.  dataType: FP16, BF16 or 0 (fp32); other types of a call are that or 0.  Outputs lie apart from each other and from all operands, or the
+ * call is refused, but for these, which may take an operand's place where values of both are of one size: a norm's out and sum that of x or residual, dx that of dy, x or dsum, dw that of
+ * weight, dlogits that of logits, dy that of y, dshare that of share.
  *
- * Root-mean-square norm of rows: s = x + residual, rounded to residualType and kept in `sum` (which may be `residual`), y = s / sqrt(mean(s^2) + eps) * weight of what is
- * kept.  residual and sum NULL: s = x.  y goes to out (which may be x) in x's type, and, or, to e4m3 codes q with scale [ceil(cols/128), rows] as catcoc_quantize_fp8 makes
+ * Root-mean-square norm of rows: s = x + residual, rounded to residualType and kept in `sum`, y = s / sqrt(mean(s^2) + eps) * weight of what is
+ * kept.  residual and sum NULL: s = x.  y goes to out in x's type, and, or, to e4m3 codes q with scale [ceil(cols/128), rows] as catcoc_quantize_fp8 makes
  * them, each rounded from fp32 by itself; NULL: not wanted.  x, residual, sum, out, q [rows,cols], at most 16384 columns; weight [cols]. */
 CATCOC_API void catcoc_rms_norm(void *stream, const void *x, const void *residual, const void *weight, void *out, void *sum, uint8_t *q, float *scale,
                                 uint32_t rows, uint32_t cols, float eps, uint32_t dataType, uint32_t residualType, uint32_t weightType);
 
 /* Its gradients, from dy (dataType) and what was normalised: x (`sum` where there was a residual), sumType.  With r = 1 / sqrt(mean(x^2) + eps), n = x r, g = dy weight:
- * dx = r (g - n mean(g n)) + dsum, in sumType; it is the gradient of the residual too.  dsum: NULL or what else flows into the sum, sumType (dx may be dsum).  dw [cols] =
+ * dx = r (g - n mean(g n)) + dsum, in sumType; it is the gradient of the residual too.  dsum: NULL or what else flows into the sum, sumType.  dw [cols] =
  * sum over the rows of dy n, in weightType.  workspace: catcoc_rms_norm_backward_workspace_size() bytes, of any content. */
 CATCOC_API uint64_t catcoc_rms_norm_backward_workspace_size(uint32_t rows, uint32_t cols);
 CATCOC_API void catcoc_rms_norm_backward(void *stream, const void *dy, const void *x, const void *weight, const void *dsum, void *dx, void *dw, void *workspace,
@@ -374,7 +376,7 @@ CATCOC_API void catcoc_route_backward(void *stream, const float *dshare, const v
 
 /* The plan of the choices [rows] (of choiceBits 32 or 64): order lists the rows by expert, in ascending order within one, those outside [0, experts) (at most 1024) behind
  * the last; back[i] is where row i went; ends[e] is one past expert e's last place, group ends of the grouped products.  workspace:
- * catcoc_sort_by_expert_workspace_size() bytes, of any content.  No output of this call or of the three below lies in the memory of the rows or choices it is made from. */
+ * catcoc_sort_by_expert_workspace_size() bytes, of any content. */
 CATCOC_API uint64_t catcoc_sort_by_expert_workspace_size(uint32_t rows, uint32_t experts);
 CATCOC_API void catcoc_sort_by_expert(void *stream, const void *choice, int32_t *order, int32_t *back, int32_t *ends, void *workspace, uint64_t workspaceBytes,
                                       uint32_t rows, uint32_t experts, uint32_t choiceBits);

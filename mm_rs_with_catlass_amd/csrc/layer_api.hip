@@ -3,6 +3,8 @@
 
 #include <math.h>
 
+#include <initializer_list>
+
 #include "api_status.h"
 #include "layer_args.h"
 
@@ -61,13 +63,30 @@ int check_rows(uint32_t tokens, uint32_t top, uint32_t cols)
     return 0;
 }
 
-// Other waves read what this one writes: their memory must not be the same.
-int check_apart(const char *out, const void *a, uint64_t aBytes, const char *in, const void *b, uint64_t bBytes)
+// An operand's memory.
+struct Memory {
+    const char *name;
+    const void *at;
+    uint64_t bytes;
+    int like = 0;   // an output may take the place of an operand that has this number too, the same rows of values of one size: who writes a row has read it before, and nobody else does
+};
+
+int check_apart(std::initializer_list<Memory> outs, std::initializer_list<Memory> ins)
 {
-    const uintptr_t x = (uintptr_t)a, y = (uintptr_t)b;
-    if (aBytes && bBytes && x < y + bBytes && y < x + aBytes) return api_fail(E_SHAPE, "%s lies in the memory of %s", out, in);
+    auto overlap = [](const Memory &a, const Memory &b) {
+        const uintptr_t x = (uintptr_t)a.at, y = (uintptr_t)b.at;
+        return a.at && b.at && a.bytes && b.bytes && x < y + b.bytes && y < x + a.bytes;
+    };
+    for (const Memory *o = outs.begin(); o != outs.end(); ++o) {
+        for (const Memory &i : ins)
+            if (overlap(*o, i) && !(o->like && o->like == i.like && o->at == i.at && o->bytes == i.bytes)) return api_fail(E_SHAPE, "%s lies in the memory of %s", o->name, i.name);
+        for (const Memory *p = outs.begin(); p != o; ++p)
+            if (overlap(*o, *p)) return api_fail(E_SHAPE, "%s lies in the memory of %s", o->name, p->name);
+    }
     return 0;
 }
+
+uint64_t bytes_of(uint32_t dt) { return dt ? 2u : 4u; }
 
 // The most workgroups that a launch can have: a wave for each KiB of a row.
 int check_pieces(uint32_t tokens, uint64_t rowBytes)
@@ -91,6 +110,10 @@ void catcoc_rms_norm(void *stream, const void *x, const void *residual, const vo
     if (!residual != !sum) { api_fail(E_NULL, "residual and sum come together"); return; }
     if (!x || !weight) { api_fail(E_NULL, "x and weight must be non-NULL"); return; }
     if ((cols <= 1024 ? (rows + 3ull) / 4 : rows) > 2 * kMaxWgs) { api_fail(E_SHAPE, "%u rows of %u columns are more than one launch holds", rows, cols); return; }
+    const uint64_t values = (uint64_t)rows * cols;
+    if (check_apart({{"out", out, values * bytes_of(dataType), 1}, {"sum", sum, values * bytes_of(residualType), 1}, {"q", q, values}, {"scale", scale, (cols + 127ull) / 128u * rows * 4u}},
+                    {{"x", x, values * bytes_of(dataType), 1}, {"residual", residual, values * bytes_of(residualType), 1}, {"weight", weight, cols * bytes_of(weightType)}}))
+        return;
     NormArgs a{x, residual, weight, out, sum, q, scale, rows, cols, eps, weightType, 0};
     api_launched(launch_norm(dataType, residual ? residualType : DT_NONE, a, stream));
 }
@@ -112,6 +135,11 @@ void catcoc_rms_norm_backward(void *stream, const void *dy, const void *x, const
         return;
     }
     if ((uintptr_t)workspace % 4 != 0) { api_fail(E_WORKSPACE, "workspace must be 4-byte aligned"); return; }
+    const uint64_t values = (uint64_t)rows * cols;
+    if (check_apart({{"dx", dx, values * bytes_of(sumType), 1}, {"dw", dw, cols * bytes_of(weightType), 2}, {"workspace", workspace, catcoc_rms_norm_backward_workspace_size(rows, cols)}},
+                    {{"dy", dy, values * bytes_of(dataType), 1}, {"x", x, values * bytes_of(sumType), 1}, {"weight", weight, cols * bytes_of(weightType), 2},
+                     {"dsum", dsum, values * bytes_of(sumType), 1}}))
+        return;
     NormBackwardArgs a{dy, x, weight, dsum, dx, dw, (float *)workspace, rows, cols, norm_backward_parts(rows, cols), eps, weightType};
     api_launched(launch_norm_backward(dataType, sumType == 0, a, stream));
 }
@@ -129,6 +157,8 @@ void catcoc_route(void *stream, const void *logits, const float *bias, int32_t *
     if (!can_route(experts, top, laid)) { api_fail(E_SHAPE, "%u groups: at most 64 are supported", groups); return; }
     if (tokens == 0) { api_launched(0); return; }
     if (!logits || !choice || !share) { api_fail(E_NULL, "logits, choice and share must be non-NULL"); return; }
+    const uint64_t scores = (uint64_t)tokens * experts, choices = (uint64_t)tokens * top;
+    if (check_apart({{"choice", choice, choices * 4u}, {"share", share, choices * 4u}}, {{"logits", logits, scores * bytes_of(dataType)}, {"bias", bias, experts * 4ull}})) return;
     RouteArgs a{};
     a.logits = logits;
     a.bias = bias;
@@ -153,6 +183,8 @@ void catcoc_route_backward(void *stream, const float *dshare, const void *logits
     if (check_route(how, tokens, experts, top, dataType)) return;
     if (tokens == 0) { api_launched(0); return; }
     if (!dshare || !logits || !choice || !dlogits) { api_fail(E_NULL, "dshare, logits, choice and dlogits must be non-NULL"); return; }
+    const uint64_t bytes = (uint64_t)tokens * experts * bytes_of(dataType), choices = (uint64_t)tokens * top;
+    if (check_apart({{"dlogits", dlogits, bytes, 1}}, {{"logits", logits, bytes, 1}, {"dshare", dshare, choices * 4u}, {"choice", choice, choices * 4u}})) return;
     RouteArgs a{};
     a.logits = logits;
     a.dshare = dshare;
@@ -186,9 +218,8 @@ void catcoc_sort_by_expert(void *stream, const void *choice, int32_t *order, int
         return;
     }
     if ((uintptr_t)workspace % 4 != 0) { api_fail(E_WORKSPACE, "workspace must be 4-byte aligned"); return; }
-    const uint64_t choiceBytes = (uint64_t)rows * (choiceBits / 8u);
-    if (check_apart("order", order, rows * 4ull, "choice", choice, choiceBytes) || check_apart("back", back, rows * 4ull, "choice", choice, choiceBytes) ||
-        check_apart("ends", ends, experts * 4ull, "choice", choice, choiceBytes))
+    if (check_apart({{"order", order, rows * 4ull}, {"back", back, rows * 4ull}, {"ends", ends, experts * 4ull}, {"workspace", workspace, need}},
+                    {{"choice", choice, (uint64_t)rows * (choiceBits / 8u)}}))
         return;
     SortArgs a{};
     a.choice = choice;
@@ -210,8 +241,10 @@ void catcoc_spread_rows(void *stream, const void *x, const float *scale, const i
     if (!scale != !outScale) { api_fail(E_NULL, "scale and outScale come together"); return; }
     if (scale && valueBytes != 1) { api_fail(E_DTYPE, "scales come with values of 1 byte (got %u)", valueBytes); return; }
     if (!x || !back || !out) { api_fail(E_NULL, "x, back and out must be non-NULL"); return; }
-    if (check_apart("out", out, (uint64_t)tokens * top * cols * valueBytes, "x", x, (uint64_t)tokens * cols * valueBytes)) return;
-    if (scale && check_apart("outScale", outScale, (uint64_t)tokens * top * ((cols + 127u) / 128u) * 4u, "scale", scale, (uint64_t)tokens * ((cols + 127u) / 128u) * 4u)) return;
+    const uint64_t rows = (uint64_t)tokens * top, blocks = (cols + 127u) / 128u;
+    if (check_apart({{"out", out, rows * cols * valueBytes}, {"outScale", outScale, rows * blocks * 4u}},
+                    {{"x", x, (uint64_t)tokens * cols * valueBytes}, {"scale", scale, tokens * blocks * 4u}, {"back", back, rows * 4u}}))
+        return;
     RowsArgs a{};
     a.x = x;
     a.scale = scale;
@@ -231,7 +264,8 @@ void catcoc_gather_rows(void *stream, const void *y, const int32_t *back, const 
     if (check_rows(tokens, top, cols) || check_pieces(tokens, cols * 2ull)) return;
     if (tokens == 0) { api_launched(0); return; }
     if (!y || !back || !out) { api_fail(E_NULL, "y, back and out must be non-NULL"); return; }
-    if (check_apart("out", out, (uint64_t)tokens * cols * (dataType ? 2u : 4u), "y", y, (uint64_t)tokens * top * cols * (dataType ? 2u : 4u))) return;
+    const uint64_t rows = (uint64_t)tokens * top;
+    if (check_apart({{"out", out, (uint64_t)tokens * cols * bytes_of(dataType)}}, {{"y", y, rows * cols * bytes_of(dataType)}, {"back", back, rows * 4u}, {"share", share, rows * 4u}})) return;
     RowsArgs a{};
     a.y = y;
     a.back = back;
@@ -252,7 +286,10 @@ void catcoc_gather_rows_backward(void *stream, const void *dout, const void *y, 
     if (!dout || !back || !share) { api_fail(E_NULL, "dout, back and share must be non-NULL"); return; }
     if (!dy && !dshare) { api_fail(E_NULL, "dy or dshare must be non-NULL"); return; }
     if (!y != !dshare) { api_fail(E_NULL, "y and dshare come together"); return; }
-    if (dy && check_apart("dy", dy, (uint64_t)tokens * top * cols * (dataType ? 2u : 4u), "dout", dout, (uint64_t)tokens * cols * (dataType ? 2u : 4u))) return;
+    const uint64_t rows = (uint64_t)tokens * top;
+    if (check_apart({{"dy", dy, rows * cols * bytes_of(dataType), 1}, {"dshare", dshare, rows * 4u, 2}},
+                    {{"dout", dout, (uint64_t)tokens * cols * bytes_of(dataType)}, {"y", y, rows * cols * bytes_of(dataType), 1}, {"back", back, rows * 4u}, {"share", share, rows * 4u, 2}}))
+        return;
     RowsArgs a{};
     a.x = dout;
     a.y = y;

@@ -796,7 +796,7 @@ def rms_norm(x, weight, residual=None, eps=1e-6, out=None, residual_out=None):
     """s = x + residual, y = s / sqrt(mean(s^2) + eps) * weight over each row (catcoc_rms_norm).
 
     x [rows,cols] fp16, bf16 or fp32, at most 16384 columns; weight [cols] and residual [rows,cols] of x's type or fp32.  Returns y in x's type; with a residual
-    (y, s), s in the residual's type and what y is the norm of.  out may be x, residual_out residual."""
+    (y, s), s in the residual's type and what y is the norm of.  out and residual_out may be x or residual, of their types."""
     done = (_host or _compiled()).rms_norm(x, weight, residual, eps, out, residual_out)
     if done is not None:
         return done
@@ -841,7 +841,7 @@ def rms_norm_backward(dy, x, weight, dsum=None, eps=1e-6, dx=None, dw=None):
     """The gradients of rms_norm() (catcoc_rms_norm_backward): (dx, dw).
 
     dy [rows,cols] of y's type; x what was normalised (with a residual: s), of that type or fp32, as dsum: what else flows into s; dx, of x's type, is the gradient of
-    the residual too.  weight, dw [cols] of dy's type or fp32.  dx may be dsum."""
+    the residual too.  weight, dw [cols] of dy's type or fp32.  dx may be dy (of its type), x or dsum, dw may be weight."""
     done = (_host or _compiled()).rms_norm_backward(dy, x, weight, dsum, eps, dx, dw)
     if done is not None:
         return done
@@ -911,7 +911,8 @@ def route(logits, top, score="softmax", bias=None, groups=1, top_groups=1, group
 
 
 def route_backward(dshare, logits, choice, score="softmax", renormalize=True, scale=1.0, out=None):
-    """The gradient of route()'s logits from that of its shares, for the choice that it made (catcoc_route_backward); score, renormalize and scale as there."""
+    """The gradient of route()'s logits from that of its shares, for the choice that it made (catcoc_route_backward); score, renormalize and scale as there.
+    out may be logits."""
     done = (_host or _compiled()).route_backward(dshare, logits, choice, score, renormalize, scale, out)
     if done is not None:
         return done
@@ -1030,7 +1031,7 @@ def gather_rows(y, back, share=None, out=None):
 def gather_rows_backward(dout, y, back, share, dy=None, dshare=None, rows=True):
     """The gradients of gather_rows() with shares (catcoc_gather_rows_backward): (dy, of y's type, dshare fp32).  Rows of dy that no choice has stay as they were.
 
-    y None: dshare is not wanted, y is not read, and dy is of dout's type.  rows False: dy is not wanted.  What is not wanted is None."""
+    y None: dshare is not wanted, y is not read, and dy is of dout's type.  rows False: dy is not wanted.  What is not wanted is None.  dy may be y, dshare share."""
     done = (_host or _compiled()).gather_rows_backward(dout, y, back, share, dy, dshare) if rows and y is not None else None
     if done is not None:
         return done

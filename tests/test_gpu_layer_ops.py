@@ -792,3 +792,53 @@ def test_one_gradient_of_gathered_rows(tokens, top, cols, dtype):
     assert none is None and torch.equal(only, dshare)
     only, none = ops.gather_rows_backward(x, None, back, share)
     assert only.dtype == dtype and only.shape == y.shape
+
+
+@pytest.mark.parametrize("cols", [40, 700, 1500, 4096, 9000])
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_outputs_in_the_place_of_operands(cols, dtype):
+    """Every output that may take an operand's place, against one of its own."""
+    g = gen(cols)
+    x, r, w, dy, more = stream(g, 77, cols, dtype), stream(g, 77, cols, dtype), 1 + 0.1 * randn(g, cols, dtype=dtype), stream(g, 77, cols, dtype), stream(g, 77, cols, dtype)
+    want = ops.rms_norm(x, w, r)
+    for out, kept in ((0, 1), (1, 0), (0, None), (1, None), (None, 0), (None, 1)):
+        own = x.clone(), r.clone()
+        got = ops.rms_norm(own[0], w, own[1], out=None if out is None else own[out], residual_out=None if kept is None else own[kept])
+        assert same(got, want)
+    want = ops.rms_norm_fp8(x, w, r, keep=True)
+    own = x.clone(), r.clone()
+    assert same([bits(t) for t in ops.rms_norm_fp8(own[0], w, own[1], keep=True, kept=own[1], residual_out=own[0])], [bits(t) for t in want])
+    want = ops.rms_norm_backward(dy, x, w, more)
+    for place in range(3):
+        own = dy.clone(), x.clone(), more.clone()
+        weight = w.clone()
+        assert same(ops.rms_norm_backward(own[0], own[1], weight, own[2], dx=own[place], dw=weight), want)
+    back, share, y = places(g, 77, 3), randn(g, 77, 3), stream(g, 231, cols, dtype)
+    want = ops.gather_rows_backward(x, y, back, share)
+    own, parts = y.clone(), share.clone()
+    assert same(ops.gather_rows_backward(x, own, back, parts, dy=own, dshare=parts), want)
+    experts = min(cols, 1000)
+    for renormalize in (True, False):
+        logits = x[:, :experts].contiguous()
+        choice, _ = ops.route(logits, 3, score="sigmoid")
+        for score in ("softmax", "sigmoid"):
+            want = ops.route_backward(share, logits, choice, score=score, renormalize=renormalize)
+            own = logits.clone()
+            assert torch.equal(ops.route_backward(share, own, choice, score=score, renormalize=renormalize, out=own), want)
+
+
+def test_outputs_a_row_off_their_operands_are_refused():
+    g = gen(50)
+    room = randn(g, 9, 64, dtype=BF16)
+    w, x, off = torch.ones(64, dtype=BF16, device=DEV), room[:8], room[1:]
+    kept = room.clone()
+    back, share, logits = torch.randperm(8, device=DEV, generator=g).int()[:, None].contiguous(), torch.ones(8, 1, device=DEV), room[:8]
+    for match, fn, a, kw in [("out lies in the memory of x", ops.rms_norm, (x, w), {"out": off}), ("sum lies in the memory of residual", ops.rms_norm, (x.clone(), w, x), {"residual_out": off}),
+                             ("sum lies in the memory of out", ops.rms_norm, (x.clone(), w, x.clone()), {"out": x, "residual_out": x}),
+                             ("q lies in the memory of x", ops.rms_norm_fp8, (x, w), {"out": room.view(-1)[:256].view(F8).view(8, 64)}),
+                             ("dx lies in the memory of dy", ops.rms_norm_backward, (x, x.clone(), w), {"dx": off}), ("dx lies in the memory of x", ops.rms_norm_backward, (x.clone(), x, w), {"dx": off}),
+                             ("dy lies in the memory of y", ops.gather_rows_backward, (x.clone(), x, back, share), {"dy": off}),
+                             ("dlogits lies in the memory of logits", ops.route_backward, (share, logits, back), {"out": off})]:
+        with pytest.raises(L.CatcocError, match=match):
+            fn(*a, **kw)
+    assert torch.equal(room, kept)

@@ -275,3 +275,63 @@ def test_one_gradient_of_gathered_rows_refuses():
                      ("non-NULL", (None, 16, 16, 16, 16, 16)), ("non-NULL", (16, 16, None, 16, 16, 16)), ("non-NULL", (16, 16, 16, None, 16, 16))]:
         so.catcoc_gather_rows_backward(None, *a, 4, 2, 8, L.BF16)
         assert so.catcoc_last_status() != 0 and match in L.last_error(), L.last_error()
+
+
+def test_outputs_in_the_memory_of_operands_are_refused():
+    """Every pair of an output and an operand or another output: one byte of them in common, at either end; and the outputs that may take an operand's place, a row off it."""
+    so = L.load()
+    how = C.byref(L.CatcocRouting(0, 1, 1, 1, 1, 1.0))
+    T = 32                                                      # tokens or rows, of 256 values; two choices each
+    need = so.catcoc_rms_norm_backward_workspace_size(T, 256)
+    sorted_rows = 1 << 20
+    sort_need = so.catcoc_sort_by_expert_workspace_size(sorted_rows, 8)
+    values, wide, choices, scales = T * 256 * 2, T * 512 * 2, T * 2 * 4, T * 2 * 4
+    calls = [
+        (so.catcoc_rms_norm, [("x", values), ("residual", 2 * values), ("weight", 512), ("out", values), ("sum", 2 * values), ("q", values // 2), ("scale", scales)],
+         (T, 256, 1e-6, L.BF16, 0, L.BF16), ["out", "sum", "q", "scale"]),
+        (so.catcoc_rms_norm, [("x", values), ("residual", values), ("weight", 1024), ("out", values), ("sum", values), ("q", values // 2), ("scale", scales)],
+         (T, 256, 1e-6, L.BF16, L.BF16, 0), ["out", "sum", "q", "scale"]),
+        (so.catcoc_rms_norm_backward, [("dy", values), ("x", 2 * values), ("weight", 512), ("dsum", 2 * values), ("dx", 2 * values), ("dw", 512), ("workspace", need)],
+         (need, T, 256, 1e-6, L.FP16, 0, L.FP16), ["dx", "dw", "workspace"]),
+        (so.catcoc_route, [("logits", values), ("bias", 1024), ("choice", choices), ("share", choices)], (how, T, 256, 2, L.BF16), ["choice", "share"]),
+        (so.catcoc_route_backward, [("dshare", choices), ("logits", values), ("choice", choices), ("dlogits", values)], (how, T, 256, 2, L.BF16), ["dlogits"]),
+        (so.catcoc_sort_by_expert, [("choice", sorted_rows * 8), ("order", sorted_rows * 4), ("back", sorted_rows * 4), ("ends", 32), ("workspace", sort_need)],
+         (sort_need, sorted_rows, 8, 64), ["order", "back", "ends", "workspace"]),
+        (so.catcoc_spread_rows, [("x", values // 2), ("scale", scales), ("back", choices), ("out", wide // 2), ("outScale", 2 * scales)], (T, 2, 256, 1), ["out", "outScale"]),
+        (so.catcoc_gather_rows, [("y", wide), ("back", choices), ("share", choices), ("out", values)], (T, 2, 256, L.BF16), ["out"]),
+        (so.catcoc_gather_rows_backward, [("dout", values), ("y", wide), ("back", choices), ("share", choices), ("dy", wide), ("dshare", choices)],
+         (T, 2, 256, L.BF16), ["dy", "dshare"]),
+        # (values of one column: as many bytes as the shares, but not in their order)
+        (so.catcoc_gather_rows_backward, [("dout", T * 4), ("y", choices), ("back", choices), ("share", choices), ("dy", choices), ("dshare", choices)], (T, 2, 1, 0), ["dy", "dshare"]),
+    ]
+    seen = 0
+    for fn, operands, tail, outs in calls:
+        size = dict(operands)
+        apart = {name: (i + 1) << 32 for i, name in enumerate(size)}
+        for out in outs:
+            for other in size:
+                if other == out:
+                    continue
+                # (addresses of floats and indexes may be any here: nothing is launched; the workspaces' are multiples of four)
+                for shift in (size[other] - 4, 4 - size[out], 4 if size[other] > 4 else -4):
+                    at = dict(apart)
+                    at[out] = apart[other] + shift
+                    fn(None, *at.values(), *tail)
+                    said = L.last_error()
+                    assert so.catcoc_last_status() != 0 and set(said.split(" lies in the memory of ")) == {out, other}, (fn.__name__, out, other, shift, said)
+                    seen += 1
+    assert seen > 100
+    # in an operand's very place, but not of its rows: dy in share's, dshare in y's (one column)
+    fn, operands, tail, _ = calls[-1]
+    for out, other in (("dy", "share"), ("dshare", "y"), ("dy", "back"), ("dshare", "dout")):
+        at = {name: (i + 1) << 32 for i, (name, _) in enumerate(operands)}
+        at[out] = at[other]
+        fn(None, *at.values(), *tail)
+        assert so.catcoc_last_status() != 0 and "%s lies in the memory of %s" % (out, other) in L.last_error()
+    # and of values of another size
+    fn, operands, tail, _ = calls[0]
+    for out, other in (("out", "residual"), ("sum", "x"), ("q", "x")):
+        at = {name: (i + 1) << 32 for i, (name, _) in enumerate(operands)}
+        at[out] = at[other]
+        fn(None, *at.values(), *tail)
+        assert so.catcoc_last_status() != 0 and "%s lies in the memory of %s" % (out, other) in L.last_error()
