@@ -201,19 +201,30 @@ class Route(torch.autograd.Function):
         logits, choice = ctx.saved_tensors
         if not torch.is_grad_enabled():
             return ops.route_backward(dshare.contiguous(), logits, choice, score=ctx.score, renormalize=ctx.renormalize, scale=ctx.scale), None, None, None
-        # (gradients of gradients: the formula in torch)
-        on, at = choice >= 0, choice.long().clamp_min(0)
-        v = torch.where(logits > -torch.inf, logits.float(), torch.finfo(torch.float32).min)
-        p = torch.sigmoid(v) if ctx.score == "sigmoid" else torch.softmax(v, 1)
-        w, g = torch.where(on, p.gather(1, at), 0.0), torch.where(on, dshare * ctx.scale, 0.0)
-        if ctx.renormalize:
-            total = w.sum(1, keepdim=True)
-            w = w / torch.where(total > 0, total, 1.0)
-        d = w * (g - (w * g).sum(1, keepdim=True)) if ctx.renormalize else w * g
-        if ctx.score == "sigmoid":
-            d = d * (1 - p.gather(1, at))
-        out = torch.zeros_like(p) if ctx.renormalize or ctx.score == "sigmoid" else -p * (w * g).sum(1, keepdim=True)
-        return out.scatter_add(1, at, torch.where(on, d, 0.0)).to(logits.dtype), None, None, None
+        return _route_gradient(dshare, logits, choice, ctx.score, ctx.renormalize, ctx.scale), None, None, None
+
+
+def _route_gradient(dshare, logits, choice, score, renormalize, scale):
+    """ops.route_backward()'s formula in torch, for gradients of gradients."""
+    at = choice.long().clamp_min(0)
+    l = logits.float().gather(1, at)
+    on = (choice >= 0) & (l != -torch.inf)
+    l, g = torch.where(on, l, 0.0), torch.where(on, dshare * scale, 0.0)
+    if renormalize:     # (shares from logarithms: the scores of experts that are all far down are nothing in fp32)
+        u = torch.where(on, torch.nn.functional.logsigmoid(l) if score == "sigmoid" else l, -torch.inf)
+        w = torch.where(on, torch.softmax(torch.where(on.any(1, keepdim=True), u, 0.0), 1), 0.0)
+        d = w * (g - (w * g).sum(1, keepdim=True))
+        rest = torch.zeros_like(logits, dtype=torch.float32)
+    elif score == "sigmoid":
+        d, rest = torch.sigmoid(l) * g, torch.zeros_like(logits, dtype=torch.float32)
+    else:               # every expert's logit moves the shares
+        v = logits.float()
+        p = torch.softmax(torch.where((v != -torch.inf).any(1, keepdim=True), v, 0.0), 1)
+        d = torch.where(on, p.gather(1, at), 0.0) * g
+        rest = -p * d.sum(1, keepdim=True)
+    if score == "sigmoid":
+        d = d * torch.sigmoid(-l)
+    return rest.scatter_add(1, at, torch.where(on, d, 0.0)).to(logits.dtype)
 
 
 def route(logits, top, bias=None, **how):

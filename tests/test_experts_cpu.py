@@ -105,3 +105,49 @@ def test_no_tokens():
     assert out.shape == (0, 6)
     for grad, leaf in zip(torch.autograd.grad(out.sum(), leaves), leaves):
         assert grad.shape == leaf.shape and not grad.any()
+
+
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("renormalize", [False, True])
+@pytest.mark.parametrize("down", [0.0, -60.0, -120.0, -2000.0])
+def test_gradient_of_the_router_with_a_graph_of_its_own(score, renormalize, down):
+    """The formula behind second gradients, where the chosen experts' scores are as far down as they may be: against autograd in 64 bits of shares made from logarithms."""
+    from types import SimpleNamespace
+
+    from mm_rs_with_catlass_amd.experts import Route
+    g = torch.Generator().manual_seed(3)
+    logits, dshare, t = torch.randn((7, 12), generator=g), torch.randn((7, 4), generator=g), torch.randn((7, 12), generator=g)
+    choice = torch.stack([torch.randperm(6, generator=g)[:4] for _ in range(7)]).int()
+    logits[:, :6] += down                       # (the choices', by a bias)
+    if score == "sigmoid":
+        logits[3:, 6:] += down
+    logits[1, choice[1, 3].long()] = -float("inf")
+    choice[1, 3], choice[2] = -1, -1
+    logits[4, 8:] = -float("inf")
+
+    def gradients(l, d, along):
+        l, d = l.clone().requires_grad_(), d.clone().requires_grad_()
+        ctx = SimpleNamespace(saved_tensors=(l, choice), score=score, renormalize=renormalize, scale=1.5)
+        with torch.enable_grad():
+            first = Route.backward(ctx, None, d)[0]
+            return [first, *torch.autograd.grad((first * along).sum(), (l, d))]
+
+    def exact(l, d, along):
+        l, d = l.double().requires_grad_(), d.double().requires_grad_()
+        on, at = choice >= 0, choice.long().clamp_min(0)
+        u = torch.nn.functional.logsigmoid(l) if score == "sigmoid" else torch.log_softmax(l, 1)
+        u = torch.where(on, u.gather(1, at), -float("inf"))
+        if renormalize:
+            u = torch.where(on, u - torch.where(on.any(1, keepdim=True), u, 0.0).logsumexp(1, keepdim=True), -float("inf"))
+        share = torch.where(on, torch.exp(torch.where(on, u, 0.0)), 0.0) * 1.5
+        first, = torch.autograd.grad(share, l, d, create_graph=True)
+        return [first, *torch.autograd.grad((first * along.double()).sum(), (l, d))]
+    got, want = gradients(logits, dshare, t), exact(logits, dshare, t)
+    assert not got[0][2].any()
+    for a, b in zip(got, want):
+        b = torch.where(torch.isnan(b), 0.0, b)     # (a gradient through -inf)
+        # differences of products of shares (at most 1), |dshare| and |t| (at most 4 each), whose logarithms move by 2^-24 of logits and sums of some hundreds at most where the shares are
+        # taken relative to each other, and of |down| where they are not and not below fp32
+        assert a.isfinite().all() and (a.double() - b).abs().max() <= 1.5 * 4 * 4 * 200 * 2.0 ** -24
+    if renormalize:
+        assert got[0].abs().amax(1)[[0, 1, 3, 4, 5, 6]].min() > 1e-3

@@ -249,3 +249,31 @@ def test_gathers_make_the_gradients_that_are_wanted():
     at = back.long()
     alike(lambda v: (Gather.apply(v, back, share),), lambda v: ((v[at] * share.to(v.dtype)[:, :, None]).sum(1),), [y], 41, 2.0 ** -18)
     alike(lambda v: (Gather.apply(y, back, v),), lambda v: ((y.to(v.dtype)[at] * v[:, :, None]).sum(1),), [share], 42, 2.0 ** -18)
+
+
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("renormalize", [False, True])
+def test_gradient_of_far_logits_with_a_graph_of_its_own(score, renormalize):
+    """Chosen experts far below the others, or all far below zero: the gradient that keeps a graph is the operator's."""
+    from mm_rs_with_catlass_amd.experts import route
+    logits = randn(gen(30), 8, 12)
+    logits[1] -= 120.0
+    logits[2] -= 300.0
+    logits[3, 4:] += 110.0
+    logits[4] = -float("inf")
+    logits[5, 2:] = -float("inf")
+    logits[6, 1:] = torch.finfo(F32).min
+    bias = torch.zeros(12, device=DEV)
+    bias[4:] = -2.0                                 # (the far ones are chosen)
+    d = randn(gen(31), 8, 4)
+    grads = []
+    for graph in (False, True):
+        v = logits.clone().requires_grad_()
+        _, share = route(v, 4, bias=bias, score=score, renormalize=renormalize)
+        got, = torch.autograd.grad(share, v, d, create_graph=graph)
+        grads.append(got.detach())
+    # two evaluations in fp32 of w (g - sum w g): each within 110 half steps of max |g| times the shares' sum
+    size = 4 * d.abs().amax(1, keepdim=True) if not renormalize else d.abs().amax(1, keepdim=True)
+    assert grads[0].isfinite().all() and ((grads[0] - grads[1]).abs() <= 2 * 2 * 110 * u * size).all()
+    if renormalize:
+        assert grads[1][1:4].abs().amax(1).min() > 1e-3
