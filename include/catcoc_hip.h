@@ -359,7 +359,7 @@ typedef struct CatcocRouting {
     uint32_t score;              /* CATCOC_SCORE_*: what a logit becomes */
     uint32_t groups;             /* experts come in so many groups of consecutive ones (0: 1) ... */
     uint32_t topGroups;          /* ... of which so many are chosen from (0: all) ... */
-    uint32_t groupTop;           /* ... by the sum of the best one or two of a group (0: 1) */
+    uint32_t groupTop;           /* ... by the sum of the best one or two of a group (0: 1) that are to be had: the one alone where only one is */
     uint32_t renormalize;        /* shares of the chosen scores' sum, not the scores themselves */
     float scale;                 /* of the shares */
 } CatcocRouting;

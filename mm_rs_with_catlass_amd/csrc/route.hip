@@ -279,7 +279,7 @@ __global__ void __launch_bounds__(256, LANES == 16 ? 4 : V <= 16 ? 3 : 2) route_
             a = __builtin_elementwise_max(a, c);
         }
         double best = without_index(a);
-        if (args.groupTop == 2 && b > kNone) best += without_index(b);
+        if (args.groupTop == 2 && b > kNone) best += without_index(b);   // (a group with one expert left goes by that one, as a group of one does)
         best = with_index(best, slot);
         uint32_t ahead = 0;   // how many groups are
         if constexpr (LANES == 16) {

@@ -886,7 +886,7 @@ def route(logits, top, score="softmax", bias=None, groups=1, top_groups=1, group
 
     logits [tokens,experts] fp16, bf16 or fp32, at most 1024 experts.  score: "softmax" or "sigmoid" of the logits.  bias [experts] fp32: added to the scores for the choice, not for
     the shares.  groups: experts come in so many groups of consecutive ones (at most 64), and are chosen from the `top_groups` of them whose `group_top` (1 or 2) best
-    sum to most.  Ties go to the lowest index.  share: the scores, of their sum where renormalised, times scale.  Logits of -inf (and biases): experts that are not to be
+    that are to be had sum to most (where there is one such expert in a group, that one alone).  Ties go to the lowest index.  share: the scores, of their sum where renormalised, times scale.  Logits of -inf (and biases): experts that are not to be
     had; where too few are left the choice is -1, no expert, and its share 0."""
     done = (_host or _compiled()).route(logits, top, score, bias, groups, top_groups, group_top, renormalize, scale, choice, share)
     if done is not None:

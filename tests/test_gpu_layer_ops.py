@@ -842,3 +842,24 @@ def test_outputs_a_row_off_their_operands_are_refused():
         with pytest.raises(L.CatcocError, match=match):
             fn(*a, **kw)
     assert torch.equal(room, kept)
+
+
+@pytest.mark.parametrize("tokens,experts,top,groups,top_groups", [(60, 8, 2, 4, 2), (60, 16, 4, 4, 2), (50, 60, 4, 4, 2), (40, 256, 8, 8, 4), (20, 160, 6, 8, 3), (20, 96, 4, 6, 2), (15, 640, 8, 10, 4),
+                                                                  (30, 64, 4, 64, 9)])
+@pytest.mark.parametrize("score,biased", [("softmax", False), ("softmax", True), ("sigmoid", False), ("sigmoid", True)])
+def test_groups_with_one_expert_left(tokens, experts, top, groups, top_groups, score, biased):
+    """A group's score is the sum of its best two that are to be had: of one where one is left, whose group may still be the best."""
+    g = gen(experts + groups)
+    logits, each = randn(g, tokens, experts), experts // groups
+    gone = torch.rand((tokens, groups, each), device=DEV, generator=g) < 0.3
+    gone[:, 0] = True                                                   # one left in the first group,
+    gone[:, 0, each // 2] = False
+    gone[::3, 1 % groups] = True                                        # none in the second
+    logits[:, each // 2] += torch.where(torch.arange(tokens, device=DEV) % 2 == 0, 12.0, -2.0)
+    logits[gone.view(tokens, experts)] = -float("inf")
+    bias = 0.1 * randn(g, experts) if biased else None
+    how = dict(groups=groups, top_groups=top_groups, group_top=2)
+    choice, share = ops.route(logits, top, score=score, bias=bias, **how)
+    want = plain_route(logits, top, score, bias, **how)
+    assert torch.equal(choice, want[0]) and (score == "sigmoid" or (choice[::2, 0] == each // 2).all())
+    shares_are_near(share, want[1], logits)
