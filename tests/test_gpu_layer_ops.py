@@ -863,3 +863,41 @@ def test_groups_with_one_expert_left(tokens, experts, top, groups, top_groups, s
     want = plain_route(logits, top, score, bias, **how)
     assert torch.equal(choice, want[0]) and (score == "sigmoid" or (choice[::2, 0] == each // 2).all())
     shares_are_near(share, want[1], logits)
+
+
+@pytest.mark.parametrize("tokens,experts,top", [(21, 128, 8), (13, 100, 6), (6, 128, 40), (4, 64, 64), (17, 65, 3), (9, 250, 16), (7, 300, 12), (5, 600, 33), (3, 512, 64)])
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("dtype,renormalize,scale", [(F32, True, 1.0), (BF16, False, 2.5), (F16, True, 0.5), (F32, False, 1.0)])
+def test_route_backward_in_every_shape(tokens, experts, top, score, dtype, renormalize, scale):
+    test_route_backward(tokens, experts, top, score, dtype, renormalize, scale)
+
+
+@pytest.mark.parametrize("experts", [6, 30, 64, 100, 128, 250, 300, 500, 1000])
+@pytest.mark.parametrize("top", [3, 5, 16, 20])
+def test_route_backward_of_none_and_doubled_choices_in_every_shape(experts, top):
+    if top > experts:
+        pytest.skip("more choices than experts are refused")
+    g = gen(experts + top)
+    logits, dshare = randn(g, 9, experts), randn(g, 9, top)
+    choice = torch.randint(0, experts, (9, top), device=DEV, generator=g, dtype=torch.int32)
+    choice[1, 1:] = choice[1, :1]                               # one expert, always
+    choice[2, ::2], choice[2, 1::2] = experts - 1, 0            # two, in turn
+    choice[3, 0], choice[3, -1] = -1, experts                   # none
+    choice[4] = -5
+    choice[5], choice[5, 1] = 2 ** 31 - 1, experts - 1
+    choice[6, :2] = 0
+    choice[7], choice[7, 0], choice[7, -1] = -2 ** 31, experts // 2, experts // 2
+    for score in ("softmax", "sigmoid"):
+        for renormalize in (False, True):
+            got = ops.route_backward(dshare, logits, choice, score=score, renormalize=renormalize)
+            assert got.isfinite().all() and not got[4].any()
+            v = logits.double().requires_grad_()
+            p = torch.softmax(v, 1) if score == "softmax" else torch.sigmoid(v)
+            on = (choice >= 0) & (choice < experts)
+            p = torch.where(on, p.gather(1, choice.long().clamp(0, experts - 1)), 0.0)
+            share = p / p.sum(1, keepdim=True) if renormalize else p
+            keep = [0, 1, 2, 3, 5, 6, 7, 8]
+            want, = torch.autograd.grad(share[keep], v, dshare.double()[keep])
+            # as test_route_backward; an expert that is chosen `top` times gets as many gradients, each within its share's bound
+            size = share.detach()[keep].sum(1, keepdim=True) * dshare.double().abs().amax(1, keepdim=True)[keep]
+            near(got[keep], want[keep], 2 * (110 + top) * u * size)
