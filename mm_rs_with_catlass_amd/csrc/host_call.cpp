@@ -775,27 +775,46 @@ PyObject *gather(PyObject *, PyObject *const *v, Py_ssize_t n)   // y, back, sha
     });
 }
 
-PyObject *gatherGradient(PyObject *, PyObject *const *v, Py_ssize_t n)   // dout, y, back, share, dy, dshare
+PyObject *gatherGradient(PyObject *, PyObject *const *v, Py_ssize_t n)   // dout, y, back, share, dy, dshare, rows
 {
-    return guardedLayer("gather_rows_backward", n, 6, [&]() -> PyObject * {
+    return guardedLayer("gather_rows_backward", n, 7, [&]() -> PyObject * {
         const Here here;
-        const at::Tensor &y = here.any(v[1], 2), &back = here.any(v[2], 2);
-        const int64_t tokens = back.size(0), top = back.size(1), cols = y.size(1);
-        const uint32_t type = code(y.scalar_type(), true);
-        if (back.scalar_type() != at::kInt || y.size(0) != back.numel() || y.size(0) > MOST || tokens > MOST || top > MOST || cols > MOST) throw Other{};
-        const at::Tensor &dout = here.of(v[0], y.scalar_type(), {tokens, cols}), &share = here.of(v[3], at::kFloat, {tokens, top});
-        Result dy(v[4], y.scalar_type(), y.sizes(), y), dshare(v[5], at::kFloat, {tokens, top}, y);
-        here.check(dy);
-        here.check(dshare);
-        uint8_t *const pd = address(dout), *const py = address(y), *const po = dy.at_();
+        const bool rows = number(v[6], 1) != 0, shares = v[1] != Py_None;
+        if ((!rows && (!shares || v[4] != Py_None)) || (!shares && v[5] != Py_None)) throw Other{};
+        const at::Tensor &dout = here.any(v[0], 2), &back = here.any(v[2], 2);
+        const int64_t tokens = back.size(0), top = back.size(1), cols = dout.size(1);
+        const at::ScalarType type = dout.scalar_type();
+        const uint32_t typeCode = code(type, true);
+        if (back.scalar_type() != at::kInt || dout.size(0) != tokens || back.numel() > MOST || tokens > MOST || top > MOST || cols > MOST) throw Other{};
+        const int64_t sizes[2] = {tokens * top, cols};
+        const at::IntArrayRef spread(sizes, 2);
+        const at::Tensor &share = here.of(v[3], at::kFloat, {tokens, top});
+        uint8_t *const py = here.maybe(v[1], type, spread);
+        std::optional<Result> dy, dshare;
+        if (rows) here.check(dy.emplace(v[4], type, spread, dout));
+        if (shares) here.check(dshare.emplace(v[5], at::kFloat, at::IntArrayRef({tokens, top}), dout));
+        uint8_t *const pd = address(dout), *const po = dy ? dy->at_() : nullptr;
         const int32_t *const pb = (const int32_t *)address(back);
         const float *const ps = (const float *)address(share);
-        float *const pds = (float *)dshare.at_();
+        float *const pds = dshare ? (float *)dshare->at_() : nullptr;
         void *const s = stream();
         Py_BEGIN_ALLOW_THREADS
-        gatherBackward(s, pd, py, pb, ps, po, pds, (uint32_t)tokens, (uint32_t)top, (uint32_t)cols, type);
+        gatherBackward(s, pd, py, pb, ps, po, pds, (uint32_t)tokens, (uint32_t)top, (uint32_t)cols, typeCode);
         Py_END_ALLOW_THREADS
-        return accepted() ? tupleOf({&dy, &dshare}) : nullptr;
+        if (!accepted()) return nullptr;
+        PyObject *const both = PyTuple_New(2);
+        if (both == nullptr) return nullptr;
+        std::optional<Result> *const made[2] = {&dy, &dshare};
+        for (int i = 0; i < 2; ++i) {
+            PyObject *o = *made[i] ? (**made[i]).object() : Py_None;
+            if (!*made[i]) Py_INCREF(o);
+            if (o == nullptr) {
+                Py_DECREF(both);
+                return nullptr;
+            }
+            PyTuple_SET_ITEM(both, i, o);
+        }
+        return both;
     });
 }
 
@@ -814,7 +833,7 @@ PyMethodDef methods[] = {{"attach_ragged", (PyCFunction)(void *)attachRagged, ME
                          {"sort_by_expert", (PyCFunction)(void *)sortChoices, METH_FASTCALL, "one call: (order, back, ends), or None for the Python path"},
                          {"spread_rows", (PyCFunction)(void *)spread, METH_FASTCALL, "one call: the output or outputs, or None for the Python path"},
                          {"gather_rows", (PyCFunction)(void *)gather, METH_FASTCALL, "one call: the output, or None for the Python path"},
-                         {"gather_rows_backward", (PyCFunction)(void *)gatherGradient, METH_FASTCALL, "one call: (dy, dshare), or None for the Python path"},
+                         {"gather_rows_backward", (PyCFunction)(void *)gatherGradient, METH_FASTCALL, "one call: (dy, dshare), None for what is not wanted, or None for the Python path"},
                          {"attach", (PyCFunction)(void *)attach, METH_FASTCALL, "addresses of the library's functions, CatcocError, CocTilingParams"},
                          {"call", (PyCFunction)(void *)call, METH_FASTCALL, "one operator call: the output, or None for the Python path"},
                          {nullptr, nullptr, 0, nullptr}};

@@ -1032,7 +1032,7 @@ def gather_rows_backward(dout, y, back, share, dy=None, dshare=None, rows=True):
     """The gradients of gather_rows() with shares (catcoc_gather_rows_backward): (dy, of y's type, dshare fp32).  Rows of dy that no choice has stay as they were.
 
     y None: dshare is not wanted, y is not read, and dy is of dout's type.  rows False: dy is not wanted.  What is not wanted is None.  dy may be y, dshare share."""
-    done = (_host or _compiled()).gather_rows_backward(dout, y, back, share, dy, dshare) if rows and y is not None else None
+    done = (_host or _compiled()).gather_rows_backward(dout, y, back, share, dy, dshare, rows)
     if done is not None:
         return done
     tokens, top = _want_back(back)

@@ -901,3 +901,21 @@ def test_route_backward_of_none_and_doubled_choices_in_every_shape(experts, top)
             # as test_route_backward; an expert that is chosen `top` times gets as many gradients, each within its share's bound
             size = share.detach()[keep].sum(1, keepdim=True) * dshare.double().abs().amax(1, keepdim=True)[keep]
             near(got[keep], want[keep], 2 * (110 + top) * u * size)
+
+
+def test_one_gradient_of_gathered_rows_from_the_compiled_call(monkeypatch):
+    g = gen(60)
+    x, y, back, share = randn(g, 12, 200, dtype=BF16), randn(g, 36, 200, dtype=BF16), places(g, 12, 3), randn(g, 12, 3)
+    compiled, given = ops._host or ops._compiled(), (torch.empty_like(y), torch.empty_like(share))
+    for a, kw in (((x, None, back, share), {}), ((x, y, back, share), {"rows": False}), ((x, None, back, share), {"dy": given[0]}), ((x, y, back, share), {"dshare": given[1], "rows": False}),
+                  ((x[:0], None, back[:0], share[:0]), {}), ((x[:0], y[:0], back[:0], share[:0]), {"rows": False})):
+        host = compiled.gather_rows_backward(*a, kw.get("dy"), kw.get("dshare"), kw.get("rows", True))
+        assert host is not None
+        host = [None if t is None else t.clone() for t in host]
+        with monkeypatch.context() as m:
+            m.setattr(ops, "_host", Nothing())
+            python = ops.gather_rows_backward(*a, **kw)
+        assert [t is None for t in host] == [t is None for t in python] and all(p is None or torch.equal(h, p) for h, p in zip(host, python))
+    for a in ((x, None, back, share, None, share, True), (x, None, back, share, None, None, False), (x, y, back, share, y.clone(), None, False), (x[1:], None, back, share, None, None, True),
+              (x, y[1:], back, share, None, None, False)):
+        assert compiled.gather_rows_backward(*a) is None
