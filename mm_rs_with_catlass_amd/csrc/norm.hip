@@ -4,14 +4,16 @@
 //   With n = s r and g = dy w: ds = r (g - n mean(g n)) + dsum, dw = sum over the rows of dy n.
 //
 // The sum is rounded to the residual's type, in which it is kept, and what is kept is normalised: so the backward pass, which has only that, takes the gradient of
-// what the forward pass computed.  y is rounded once, from fp32, to each of the forms it is wanted in: codes are not codes of the 16-bit y.
+// what the forward pass computed.  y is rounded once, from fp32, to each of the forms it is wanted in: codes are not codes of the 16-bit y.  A code's quotient does not depend on the
+// root, so that products of 16-bit values often lie on the very middle of two codes: there fp32's last bit decides, and of 65536 codes up to nine are a step from those of another
+// order of the same operations.
 //
 // Memory bounds both.  A row stays in the registers of the threads that share it between its one read and its writes: 64, 256 or 1024 threads with eight to 32 values each.
 // y is what the next operator reads, the sum is read after a whole layer: it is stored past the caches, which leaves them to y (us, a norm and a quantizer of its y, without /
 // with it: 3000 rows of 4096 26.3 / 23.7, 16384 140 / 128; where the sum is read at once 37.3 / 40.1 and 185 / 185).  Loops of resident workgroups with the next row's loads ahead
-// were slower (16384 rows 102-105 us, 95 without), as were loads past the caches.
+// were 7 to 10 % slower, as were loads past the caches.
 //
-// 16384 rows of 4096 in bf16 with a residual 91 us, 5.9 TB/s (a copy of as many bytes 104); 4099 rows of 1808 to e4m3 with an fp32 residual 15.8, 5.2 TB/s; 16 rows 3.5.  The
+// us a call, three or more sets of operands in turn: 16384 rows of 4096 in bf16 with a residual 91, 5.9 TB/s (a copy of as many bytes 104); 4099 rows of 1808 to e4m3 with an fp32 residual 15.8, 5.2 TB/s; 16 rows 3.6 on the GPU.  The
 // backward pass of 8192 rows of 4096 54 us, 5.0 TB/s: 47 its rows, 4 the sum of the weight gradient's parts.
 #include <hip/hip_runtime.h>
 
@@ -37,7 +39,7 @@ __device__ __forceinline__ float row_sum(float v, float *parts)
 }
 
 // Workgroup `wg` of a launch, which go round-robin to the eight XCDs, as the place of its rows: every XCD gets runs of kRun consecutive ones, whose scales lie in one
-// line (4099 rows of 1808 to e4m3 23.2 us without, 22.2 with it, 4096 of 8192 51.6 and 48.7; not where few workgroups would share few XCDs, nor without scales, where it costs up to a
+// line (4099 rows of 1808 to e4m3 with an fp32 residual 16.7 us without, 15.9 with it, 4096 of 8192 with one 42.7 and 40.8, without one 24.6 and 23.7; not where few workgroups would share few XCDs, nor without scales, where it costs up to a
 // tenth).
 constexpr uint32_t kRun = 16;
 __device__ __forceinline__ uint32_t run_place(uint32_t wg)

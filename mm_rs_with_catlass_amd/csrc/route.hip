@@ -3,14 +3,15 @@
 //   score p_e = softmax(l)_e or s(l_e); the `top` largest of p_e + b_e, in the topGroups groups whose best one or two sum to most; share = scale p_c (/ sum of the chosen p).
 //
 // A token's experts lie on 16 or 64 lanes, a group of them on a power of two of those, up to 32 a lane: four tokens a wave where 16 lanes hold them (16384 tokens
-// of 256 experts, biased, 12.3 us; 24.7 with a wave for each token).  An expert's rank is one 64-bit number, its key: a double whose last ten bits are the expert's index, counted so that of equal scores
+// of 256 experts, biased, 12 us; twice that with a wave for each token).  An expert's rank is one 64-bit number, its key: a double whose last ten bits are the expert's index, counted so that of equal scores
 // the lower index is the larger key.  Maxima of doubles, as fast here as those of floats, then order scores and ties alike, and nothing has to be carried along with a
 // score.  Where the order is that of the logits (no bias, no sums of scores) a key holds all of a logit's bits; else it is the score in 64 bits, whose first 42 bits count: which of
 // two experts is ahead is a matter of more bits than fp32 has, as one of a prompt's 10^5 choices is decided by less than 2^-24 now and then.
 // Every lane sorts its keys once (odd-even merge sort: Batcher, AFIPS 1968); then the largest of the lanes' first keys is taken `top` times.
 //
-// Bound by its 64-bit instructions where there are many tokens: 16384 of 256 experts in groups, biased, 12 us (1200 instructions a wave, 70 % of the time; the logits alone
-// would take 3.5), and 50 us with the library's exponential and division, a load for each bias and the compiler's way of moving up a sorted list; 32 tokens of 64 experts 3.1 us.
+// Bound by its 64-bit instructions where there are many tokens: us a call, three or more sets of logits in turn: 16384 of 256 experts in groups, biased, 12 (1200 instructions a wave, 74 % of the time; the logits alone
+// would take 3.5), by the logits alone 8, and 50 us with the library's exponential and division, a load for each bias and the compiler's way of moving up a sorted list; 32 tokens of 64 experts 3.0 us on the GPU.  512
+// experts, top 10: 19 us, in groups and biased 27.
 #include <hip/hip_runtime.h>
 
 #include <utility>
@@ -131,8 +132,8 @@ __device__ __forceinline__ float logit_at(const void *x, size_t at, uint32_t typ
 }
 
 // Value i of a lane that is `part` of a group's lanes is the group's expert place_in_group(): consecutive lanes hold consecutive pieces of P.  Pieces of four, with which a
-// wave's accesses lie beside each other, where there is little but them (gradients of 16384 tokens of 256 experts 10.7 us, 14.5 with a lane's values in one piece), one
-// piece where there are few registers left (the choice of the same 13.0 us, 16.0 with pieces of four).
+// wave's accesses lie beside each other, where there is little but them (gradients of 16384 tokens of 256 experts 10 us, a third more with a lane's values in one piece), one
+// piece where there are few registers left (the choice of the same a quarter more with pieces of four).
 template <int P>
 __device__ __forceinline__ uint32_t place_in_group(uint32_t part, uint32_t lanes, int i)
 {
@@ -167,7 +168,8 @@ __device__ __forceinline__ void load_logits(const void *x, size_t at, uint32_t p
     }
 }
 
-// e^x to 2^-45 of it, |x| <= 700: 2^n e^r with |r| <= ln 2 / 2 and e^r as the polynomial that meets it at ten Chebyshev nodes (2^-45.6).  Beside 1.5 2^52 a number is
+// e^x to 2^-44.4 of it, |x| <= 700 (2^-45.3 to 100: the one constant for ln 2 is off by 2^-54 of it, n times over): 2^n e^r with |r| <= ln 2 / 2 and e^r as the polynomial
+// that meets it at ten Chebyshev nodes (2^-45.6).  Beside 1.5 2^52 a number is
 // a whole one, n the last bits of the sum.
 __device__ __forceinline__ double exp64(double x)
 {
@@ -499,7 +501,7 @@ int launch_route_backward(const RouteArgs &a, void *stream) { return launch_rout
 
 // ---- rows by expert -----------------------------------------------------------------------------------------------------------------------
 // A counting sort, stable: a wave counts how many of its consecutive rows go to each expert, the counts' sums over waves, blocks and experts are where its first
-// row of each goes, and the rows follow in 64s, a row's place among them by how many lanes before it have the same expert.  Latencies bound it: 256 rows 3.4 us, 8192 to 128
+// row of each goes, and the rows follow in 64s, a row's place among them by how many lanes before it have the same expert.  Latencies bound it: 256 rows 3.2 us, 8192 to 128
 // experts 5.4, 131072 9.2 (two launches of 2.9 and 6.5; the bytes would take 0.3).
 
 namespace {

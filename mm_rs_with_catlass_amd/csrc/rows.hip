@@ -7,7 +7,8 @@
 // Memory bounds all three.  Work is cut by token, not by place: a token's row is read once for all of its choices.  A place outside the rows (a choice without a row: -1)
 // is neither read nor written.
 //
-// 2048 tokens of 4096 values with eight places each: spread 30.8 us, 4.9 TB/s (e4m3 with scales 18.1, 4.4), gather 34.6, 4.4, backward 56, 5.1; 32 tokens 3.7, 3.9 and 3.2 us.
+// us a call, six sets of operands and results in turn, so that they come from memory: 2048 tokens of 4096 bf16 values with eight places each: spread 30.5, 4.9 TB/s (e4m3 with
+// scales 17.4, 4.5; 14.5 where every call's results go to one place, half of which the 256 MB cache holds), gather 33.5, 4.5, backward 57, 5.0, its rows alone 40; 32 tokens 3.6, 3.8 and 3.6.
 #include <hip/hip_runtime.h>
 
 #include "layer_args.h"
@@ -63,7 +64,7 @@ __device__ __forceinline__ uint32_t uniform(uint32_t v) { return (uint32_t)__bui
 
 // A wave takes a KiB of a token's row (four were slower: 8192 tokens' 4096 e4m3 values to eight places 81.6 us, 76.8 with one; 16384 rows of 256 values to two 13 and 7.3).
 // Scales, if any, are the first `scaleWgs` workgroups': a thread takes a choice's of up to eight blocks, all asked for before the first is stored (2048 tokens of 4096 to
-// eight places 18.1 us, 20.4 with a row's scales behind its values, 15.7 without scales; one token 3.6 and 4.8).  ES: bytes of a value.
+// eight places 17.4 us, 15.2 without scales; with a row's scales behind its values 2.3 more, one token 1.2 more).  ES: bytes of a value.
 constexpr uint32_t kScaleRows = 256, kScaleBlocks = 8;
 
 template <uint32_t ES>
@@ -139,7 +140,7 @@ __global__ void __launch_bounds__(256) gather_rows_kernel(const RowsArgs args)
 }
 
 // T threads take a choice's row.  The choices of a token follow each other on one XCD, whose L2 then has the token's gradient for all but the first (us, with one workgroup
-// for all of a token's choices / with these: 2048 tokens of eight rows of 4096 64 / 56, 32 of them 8.6 / 3.2).
+// for all of a token's choices / with these: 2048 tokens of eight rows of 4096 64 / 57, 32 of them 8.6 / 3.6).
 // DY, DSHARE: which of the two gradients is wanted; y is not read for dy alone.
 template <uint32_t DT, int T, bool DY, bool DSHARE>
 __global__ void __launch_bounds__(256) gather_rows_backward_kernel(const RowsArgs args)
